@@ -8,6 +8,8 @@ and their cos/sin are bit-identical to ``RotaryEmbedding.cos_cached/sin_cached``
 
 from __future__ import annotations
 
+from weakref import WeakKeyDictionary
+
 import torch
 from torch import Tensor
 
@@ -30,7 +32,14 @@ class RotaryEmbedding:
         self.sin_cached = emb.sin()
 
 
-_table_cache: dict[tuple, tuple[Tensor, Tensor]] = {}
+# per rope object (while it lives) and device: the tensors the tables were made from, their
+# versions, and the tables.  Holding the source tensors keeps "is" meaningful: neither an object
+# nor a tensor whose address was reused can match.
+_table_cache: WeakKeyDictionary = WeakKeyDictionary()
+
+
+def _version(t: Tensor) -> int:
+    return 0 if t.is_inference() else t._version
 
 
 def half_tables(rope, device: torch.device) -> tuple[Tensor, Tensor]:
@@ -43,16 +52,20 @@ def half_tables(rope, device: torch.device) -> tuple[Tensor, Tensor]:
         c, s = rope
         return c.to(device=device, dtype=torch.float32).contiguous(), s.to(device=device, dtype=torch.float32).contiguous()
     cos_full, sin_full = rope.cos_cached, rope.sin_cached
-    key = (id(rope), cos_full.data_ptr(), str(device))
-    hit = _table_cache.get(key)
-    if hit is not None:
-        return hit
+    try:
+        made = _table_cache.setdefault(rope, {})
+    except TypeError:  # an object without hash or weak references: made anew each call
+        made = {}
+    source = (cos_full, sin_full, _version(cos_full), _version(sin_full))
+    hit = made.get(str(device))
+    if hit is not None and all(x is y for x, y in zip(hit[0][:2], source[:2])) and hit[0][2:] == source[2:]:
+        return hit[1]
     hd = cos_full.shape[-1]
     out = (
         cos_full[:, : hd // 2].to(device=device, dtype=torch.float32).contiguous(),
         sin_full[:, : hd // 2].to(device=device, dtype=torch.float32).contiguous(),
     )
-    _table_cache[key] = out
+    made[str(device)] = (source, out)
     return out
 
 
