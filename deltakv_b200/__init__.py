@@ -14,6 +14,8 @@ deployment swaps them in (see :func:`install`):
 * ``apply_probe_to_cache`` / ``select_probes`` / ``weight_axis_scores`` / ``residual_gate``
   (deltakv.patches.probe), ``lora_activation_scores`` (deltakv.patches.exact)
 
+and what a serving loop does with the same pages between two patches (``plan_paged_step``,
+``append_into_paged``, ``paged_decode_attention``: one prefill or decode step),
 plus the fused batched forms the engine and connector use: :class:`ExactPatcher` (LoRA
 deltas) and :class:`DensePatcher` (full-rank dW of an RL step, a tensor-core GEMM).
 All computation runs in ``libdkv_b200.so``; a missing library raises (no CPU path).
@@ -23,6 +25,7 @@ from __future__ import annotations
 
 from deltakv_b200 import analytic, kivi, routes
 from deltakv_b200._lib import DkvError
+from deltakv_b200.decode import PagedStep, append_into_paged, paged_decode_attention, plan_paged_step
 from deltakv_b200.dense import DensePatcher
 from deltakv_b200.exact import (
     ExactPatcher,
@@ -57,9 +60,11 @@ __all__ = [
     "LayerDelta",
     "LowRankFactors",
     "LowRankKVPatch",
+    "PagedStep",
     "RotaryEmbedding",
     "SeqBatchTensors",
     "analytic",
+    "append_into_paged",
     "apply_layer_patches",
     "apply_layer_patches_",
     "apply_probe_to_cache",
@@ -71,6 +76,8 @@ __all__ = [
     "lora_activation_scores",
     "materialize_codes",
     "measured_error",
+    "paged_decode_attention",
+    "plan_paged_step",
     "quantize_rows",
     "replay",
     "residual_gate",

@@ -25,6 +25,7 @@ DKV_ERR_CUDA = -8
 DKV_ERR_TIMEOUT = -9
 DKV_ERR_PAGE_RANGE = -10
 DKV_ERR_WORKSPACE = -11
+DKV_ERR_NO_BLOCKS = -12
 
 # element types
 DKV_F32, DKV_F16, DKV_BF16, DKV_E4M3, DKV_I32, DKV_U8 = 0, 1, 2, 3, 4, 5
@@ -68,6 +69,10 @@ EXPORTED = (
     "dkv_subspace_correct_batched_workspace_bytes",
     "dkv_subspace_correct_batched",
     "dkv_subspace_probe_residual",
+    "dkv_plan_paged_step",
+    "dkv_append_paged",
+    "dkv_paged_decode_workspace_bytes",
+    "dkv_paged_decode_attention",
 )
 
 
@@ -267,6 +272,77 @@ class SubspaceArgs(C.Structure):
     ]
 
 
+class StepPlanArgs(C.Structure):
+    _fields_ = [
+        ("lengths", C.c_void_p),
+        ("new_lengths", C.c_void_p),
+        ("table_lens", C.c_void_p),
+        ("free_blocks", C.c_void_p),
+        ("n_free", C.c_int64),
+        ("block_tables", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("table_width", C.c_int32),
+        ("n_seqs", C.c_int32),
+        ("block_size", C.c_int32),
+        ("n_rows", C.c_int32),
+        ("cu_seqlens", C.c_void_p),
+        ("cu_new", C.c_void_p),
+        ("table_lens_out", C.c_void_p),
+        ("blocks_used", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("slots", C.c_void_p),
+        ("status", C.c_void_p),
+    ]
+
+
+class AppendArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("q", C.c_void_p),
+        ("in_dtype", C.c_int32),
+        ("n_q_heads", C.c_int32),
+        ("n_rows", C.c_int64),
+        ("k_stride_row", C.c_int64),
+        ("k_stride_head", C.c_int64),
+        ("v_stride_row", C.c_int64),
+        ("v_stride_head", C.c_int64),
+        ("q_stride_row", C.c_int64),
+        ("q_stride_head", C.c_int64),
+        ("q_out", C.c_void_p),
+        ("q_out_stride_row", C.c_int64),
+        ("q_out_stride_head", C.c_int64),
+        ("slots", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("rope_cos", C.c_void_p),
+        ("rope_sin", C.c_void_p),
+        ("rope_max_pos", C.c_int32),
+        ("k_pages", PagedCache),
+        ("v_pages", PagedCache),
+        ("status", C.c_void_p),
+    ]
+
+
+class PagedDecodeArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("q_stride_seq", C.c_int64),
+        ("q_stride_head", C.c_int64),
+        ("n_q_heads", C.c_int32),
+        ("scale", C.c_float),
+        ("seqs", SeqBatch),
+        ("k_pages", PagedCache),
+        ("v_pages", PagedCache),
+        ("out", C.c_void_p),
+        ("out_stride_seq", C.c_int64),
+        ("out_stride_head", C.c_int64),
+        ("lse", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+        ("status", C.c_void_p),
+    ]
+
+
 _lib: C.CDLL | None = None
 
 
@@ -349,6 +425,14 @@ def _declare(lib: C.CDLL) -> None:
     lib.dkv_subspace_correct_batched.argtypes = [C.POINTER(SubspaceArgs), I32, P, I64, P]
     lib.dkv_subspace_probe_residual.restype = C.c_int
     lib.dkv_subspace_probe_residual.argtypes = [P, P, I32, I64, I64, I64, I64, P, I64, P, P]
+    lib.dkv_plan_paged_step.restype = C.c_int
+    lib.dkv_plan_paged_step.argtypes = [C.POINTER(StepPlanArgs), P]
+    lib.dkv_append_paged.restype = C.c_int
+    lib.dkv_append_paged.argtypes = [C.POINTER(AppendArgs), P]
+    lib.dkv_paged_decode_workspace_bytes.restype = C.c_int
+    lib.dkv_paged_decode_workspace_bytes.argtypes = [C.POINTER(PagedDecodeArgs), C.POINTER(C.c_int64)]
+    lib.dkv_paged_decode_attention.restype = C.c_int
+    lib.dkv_paged_decode_attention.argtypes = [C.POINTER(PagedDecodeArgs), P]
 
 
 def lib() -> C.CDLL:

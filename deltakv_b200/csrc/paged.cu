@@ -298,6 +298,7 @@ extern "C" const char *dkv_status_string(int status) {
     case DKV_ERR_TIMEOUT: return "device-side wait timed out";
     case DKV_ERR_PAGE_RANGE: return "block id outside the paged cache";
     case DKV_ERR_WORKSPACE: return "workspace too small";
+    case DKV_ERR_NO_BLOCKS: return "free block list exhausted";
     default: return "unknown status";
   }
 }

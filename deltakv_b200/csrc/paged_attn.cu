@@ -1,0 +1,641 @@
+// Attention of one new token per sequence over a paged KV cache.
+//
+// For sequence b, query head h of KV head u, with s_i = scale q.K_i over its tokens i:
+//   m = max_i s_i,  l = sum_i exp(s_i - m),  O = sum_i exp(s_i - m) V_i,  out = O / l,  lse = m + ln l.
+// (m, l, O) of two disjoint parts of the tokens join exactly: with M = max(m1, m2) each part's l
+// and O are multiplied by exp(m - M) and added.  So the cache's length can be cut anywhere.
+//
+// Every K and V element is read once and used for the 1..16 query heads of its group: 2 to 16
+// flops a byte, far below the ridge, so the kernel is built as a stream of the pages.  Work is
+// cut without regard to sequences: the tokens of all sequences are laid end to end (cu_seqlens
+// is that layout), with kSeqCost virtual tokens of overhead in front of each sequence, and the
+// line is cut into equal ranges.  One warp walks one range of one KV head, so a batch of any
+// raggedness keeps all warps equally busy and the host needs no lengths.  A sequence inside
+// one range is finished by its warp; a sequence cut by a range border leaves (m, l, O) of its
+// parts in the workspace, and a second launch joins them in the order of the ranges (the
+// result does not depend on scheduling).
+#include "dkv_common.cuh"
+
+namespace dkv {
+namespace pattn {
+
+constexpr int kTile = 16;      // tokens per pipeline stage of a warp
+constexpr int kSeqCost = 16;   // virtual tokens per sequence: the cost of starting one
+constexpr int kMinRange = 32;  // tokens below which a range is not cut further
+
+struct Params {
+  const char *q;
+  int64_t q_seq, q_head;  // bytes
+  char *out;
+  int64_t out_seq, out_head;  // bytes
+  float *lse;
+  const int32_t *cu, *tables, *table_lens;
+  int64_t table_stride;
+  const char *k, *v;
+  int64_t k_block, k_slot, k_head, v_block, v_slot, v_head;  // bytes
+  int64_t num_blocks;
+  float *part_o, *part_ml;  // [range][unit][2][kGroup][head_dim], [...][kGroup][2]
+  int32_t *status;
+  float scale_log2;  // scale * log2(e): scores are kept in base 2
+  int n_seqs, n_kv, heads, group, chunks, units, ranges;
+  int hd, block_size, vec;
+};
+
+// ---------------------------------------------------------------------------------------
+// the line of tokens and its ranges
+// ---------------------------------------------------------------------------------------
+struct Line {
+  int64_t total;  // virtual tokens
+  int ranges;     // in use
+};
+__device__ __forceinline__ int64_t line_pos(const Params &p, int b) {
+  return static_cast<int64_t>(p.cu[b]) + static_cast<int64_t>(kSeqCost) * b;
+}
+__device__ __forceinline__ Line line_of(const Params &p) {
+  Line ln;
+  ln.total = line_pos(p, p.n_seqs);
+  const int64_t most = ln.total / kMinRange;
+  ln.ranges = most < 1 ? 1 : (most < p.ranges ? static_cast<int>(most) : p.ranges);
+  return ln;
+}
+__device__ __forceinline__ int64_t range_start(const Line &ln, int r) { return r * ln.total / ln.ranges; }
+// the token of sequence [at, at + len) that a range border at x falls on: a multiple of the tile
+__device__ __forceinline__ int border(int64_t x, int64_t at, int len) {
+  if (x <= at) return 0;
+  if (x >= at + len + kSeqCost) return len;
+  const int i = static_cast<int>(x - at) & ~(kTile - 1);
+  return i < len ? i : len;
+}
+// largest b with line_pos(b) <= x, 32 candidates a step (whole warp)
+__device__ __forceinline__ int seq_at(const Params &p, int64_t x, int lane) {
+  int lo = 0, hi = p.n_seqs;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int b = lo + lane * step;
+    const bool in = b < hi && line_pos(p, b) <= x;
+    const int k = __popc(__ballot_sync(0xffffffffu, in));
+    if (k > 1) lo += (k - 1) * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+// ---------------------------------------------------------------------------------------
+// a warp's walk over its range: one kTile-token tile after the other
+// ---------------------------------------------------------------------------------------
+enum { kFirst = 1, kLast = 2, kFromStart = 4, kToEnd = 8 };
+
+struct Walk {
+  int64_t x0, x1;  // the range
+  int64_t at;      // line_pos of sequence b
+  int b, next;     // sequence, its first token's index in cu terms of b + 1
+  int i, end;      // tile start and end of the piece within the sequence
+  uint32_t flags;
+  bool live;
+};
+
+// zero output of a sequence without tokens
+template <typename T>
+__device__ __forceinline__ void write_empty(const Params &p, int b, int h0, int n_h, int lane) {
+  for (int h = h0; h < h0 + n_h; ++h) {
+    T *o = reinterpret_cast<T *>(p.out + b * p.out_seq + h * p.out_head);
+    for (int d = lane; d < p.hd; d += 32) o[d] = T(0.f);
+    if (p.lse && lane == 0) p.lse[static_cast<int64_t>(b) * p.heads + h] = __int_as_float(0xff800000);
+  }
+}
+
+// moves w to the next piece of the range that has tokens, starting with sequence w.b
+template <typename T>
+__device__ __forceinline__ void walk_seq(const Params &p, Walk &w, int h0, int n_h, int lane) {
+  w.live = false;
+  while (w.b < p.n_seqs && w.at < w.x1) {
+    const int start = p.cu[w.b];
+    const int len = max(p.cu[w.b + 1] - start, 0);
+    const int i0 = border(w.x0, w.at, len), i1 = border(w.x1, w.at, len);
+    if (i1 > i0) {
+      w.i = i0, w.end = i1;
+      w.flags = kFirst | (i0 == 0 ? kFromStart : 0) | (i1 == len ? kToEnd : 0);
+      w.live = true;
+      return;
+    }
+    if (len == 0 && w.at >= w.x0) write_empty<T>(p, w.b, h0, n_h, lane);
+    ++w.b;
+    w.at += len + kSeqCost;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void walk_next(const Params &p, Walk &w, int h0, int n_h, int lane) {
+  w.i += kTile;
+  w.flags &= ~kFirst;
+  if (w.i < w.end) return;
+  w.at = line_pos(p, w.b + 1);
+  ++w.b;
+  walk_seq<T>(p, w, h0, n_h, lane);
+}
+
+// byte address of this lane's row (lanes 0-15: K of token i + lane, 16-31: V of token i + lane - 16), 0 if none
+__device__ __forceinline__ uint64_t row_address(const Params &p, const Walk &w, int u, int lane) {
+  const int i = w.i + (lane & 15);
+  if (i >= w.end) return 0;
+  const int blk = i / p.block_size, slot = i - blk * p.block_size;
+  const int64_t tlen = p.table_lens ? p.table_lens[w.b] : p.table_stride;
+  if (blk >= tlen) {
+    record_error(p.status, DKV_ERR_BLOCK_TABLE_SHORT);
+    return 0;
+  }
+  const int64_t id = p.tables[w.b * p.table_stride + blk];
+  if (id < 0 || id >= p.num_blocks) {
+    record_error(p.status, DKV_ERR_PAGE_RANGE);
+    return 0;
+  }
+  const char *a = lane < 16 ? p.k + id * p.k_block + slot * p.k_slot + u * p.k_head
+                            : p.v + id * p.v_block + slot * p.v_slot + u * p.v_head;
+  return reinterpret_cast<uint64_t>(a);
+}
+
+// four consecutive elements of a shared-memory row as floats
+__device__ __forceinline__ float4 row4(const float *r) { return *reinterpret_cast<const float4 *>(r); }
+__device__ __forceinline__ float4 row4(const __half *r) {
+  const uint2 w = *reinterpret_cast<const uint2 *>(r);
+  return make_float4(f16lo(w.x), f16hi(w.x), f16lo(w.y), f16hi(w.y));
+}
+__device__ __forceinline__ float4 row4(const __nv_bfloat16 *r) {
+  const uint2 w = *reinterpret_cast<const uint2 *>(r);
+  return make_float4(bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y));
+}
+
+// ---------------------------------------------------------------------------------------
+// the walk with fp32 arithmetic on the ordinary pipes
+// ---------------------------------------------------------------------------------------
+// HD: head_dim rounded up (columns past head_dim are zero), G: query heads of the unit (rounded
+// up), W: warps per CTA.  Scores: lane = (token, half of the head); output: lane = 4 columns,
+// the tokens dealt to 128 / HD groups of lanes where the head is shorter than 128.
+template <int DT, int HD, int G, int W>
+struct Simt {
+  using T = typename Elem<DT>::T;
+  static constexpr int kRow = HD * static_cast<int>(sizeof(T)) + 16;  // 16 B of padding: no bank conflicts
+  static constexpr int kStage = 2 * kTile * kRow;
+  static constexpr int kQRow = (HD + 8) * 4;  // two halves, 16 B apart in banks
+  static constexpr int kExtra = G * kQRow + kTile * G * 4;
+  static constexpr int kStages = 3;
+  static constexpr int kWarpBytes = kStages * kStage + kStages * 16 + kExtra;
+  static constexpr int kSmem = W * kWarpBytes;
+};
+
+template <int DT, int HD, int G, int W>
+__global__ void __launch_bounds__(W * 32) simt_kernel(Params p) {
+  using C = Simt<DT, HD, G, W>;
+  using T = typename C::T;
+  extern __shared__ __align__(16) char smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int gw = blockIdx.x * W + warp;
+  const int r = gw / p.units, unit = gw - r * p.units;
+  const Line ln = line_of(p);
+  if (r >= ln.ranges) return;
+  const int u = unit / p.chunks, chunk = unit - u * p.chunks;
+  const int n_h = min(G, p.group - chunk * G), h0 = u * p.group + chunk * G;
+
+  char *mine = smem + warp * C::kWarpBytes;
+  uint4 *meta = reinterpret_cast<uint4 *>(mine + C::kStages * C::kStage);
+  float *qs = reinterpret_cast<float *>(mine + C::kStages * C::kStage + C::kStages * 16);
+  float *ps = qs + C::kQRow / 4 * G;
+  // columns past head_dim stay zero in every stage: nothing writes them again
+  for (int i = lane; i < C::kStages * C::kStage / 16; i += 32)
+    reinterpret_cast<uint4 *>(mine)[i] = make_uint4(0, 0, 0, 0);
+  __syncwarp();
+
+  Walk w;
+  w.x0 = range_start(ln, r), w.x1 = range_start(ln, r + 1);
+  w.b = seq_at(p, w.x0, lane);
+  w.at = line_pos(p, w.b);
+  walk_seq<T>(p, w, h0, n_h, lane);
+
+  constexpr int kChunks = HD * static_cast<int>(sizeof(T)) / 16;  // 16-byte pieces of a row
+  auto fill = [&](int s) {
+    if (w.live) {
+      const uint64_t addr = row_address(p, w, u, lane);
+      const uint32_t there = __ballot_sync(0xffffffffu, addr != 0);
+      char *stage = mine + s * C::kStage;
+      if (p.vec) {
+#pragma unroll 4
+        for (int c = lane; c < 32 * kChunks; c += 32) {
+          const int row = c / kChunks, piece = c % kChunks;
+          const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
+          if (piece * 16 < p.hd * static_cast<int>(sizeof(T)))
+            cp_async16(stage + row * C::kRow + piece * 16,
+                       a ? reinterpret_cast<const char *>(a) + piece * 16 : p.k, a ? 16 : 0);
+        }
+      } else {
+        for (int row = 0; row < 32; ++row) {
+          const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
+          T *dst = reinterpret_cast<T *>(stage + row * C::kRow);
+          for (int d = lane; d < p.hd; d += 32) dst[d] = a ? reinterpret_cast<const T *>(a)[d] : T(0.f);
+        }
+      }
+      const bool last = w.i + kTile >= w.end;
+      if (lane == 0) meta[s] = make_uint4(w.b, w.flags | (last ? kLast : 0), there & 0xffffu, 0);
+      walk_next<T>(p, w, h0, n_h, lane);
+    } else if (lane == 0) {
+      meta[s] = make_uint4(0, 0, 0, 1);  // the end
+    }
+    cp_async_commit();
+  };
+
+  constexpr int kVec = HD >= 128 ? HD / 128 : 1;         // float4 columns per lane
+  constexpr int kLanes = HD >= 128 ? 32 : HD / 4;        // lanes per token in the output product
+  constexpr int kSplit = 32 / kLanes;                    // tokens handled at once there
+  float m[G], l[G], o[G][kVec][4];
+  const int key = lane & 15, half = lane >> 4;
+  const int oc = lane % kLanes, ok = lane / kLanes;
+
+  for (int s = 0; s < C::kStages; ++s) fill(s);
+  for (int s = 0;; s = s + 1 == C::kStages ? 0 : s + 1) {
+    cp_async_wait<C::kStages - 1>();
+    __syncwarp();
+    const uint4 mt = meta[s];
+    if (mt.w) break;
+    const int b = mt.x;
+    if (mt.y & kFirst) {
+      for (int i = lane; i < G * HD; i += 32) {
+        const int g = i / HD, d = i % HD;
+        float x = 0.f;
+        if (g < n_h && d < p.hd)
+          x = Elem<DT>::to_f(reinterpret_cast<const T *>(p.q + b * p.q_seq + (h0 + g) * p.q_head)[d]);
+        qs[g * (C::kQRow / 4) + d + (d >= HD / 2 ? 4 : 0)] = x;
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        m[g] = __int_as_float(0xff800000), l[g] = 0.f;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[g][j][e] = 0.f;
+      }
+      __syncwarp();
+    }
+    const T *kr = reinterpret_cast<const T *>(mine + s * C::kStage + key * C::kRow) + half * (HD / 2);
+    float acc[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) acc[g] = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < HD / 2; d += 4) {
+      const float4 x = row4(kr + d);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float4 y = *reinterpret_cast<const float4 *>(qs + g * (C::kQRow / 4) + half * (HD / 2 + 4) + d);
+        acc[g] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, acc[g]))));
+      }
+    }
+    const bool there = (mt.z >> key) & 1;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float x = acc[g] + __shfl_xor_sync(0xffffffffu, acc[g], 16);
+      x = there ? x * p.scale_log2 : __int_as_float(0xff800000);
+      float t = x;
+#pragma unroll
+      for (int k = 8; k > 0; k >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, k));
+      const float top = fmaxf(m[g], t);
+      const float base = top == __int_as_float(0xff800000) ? 0.f : top;  // nothing seen yet: any finite base
+      const float keep = exp2f(m[g] - base);
+      const float e = exp2f(x - base);
+      m[g] = top;
+      l[g] = l[g] * keep + (half == 0 ? e : 0.f);
+      if (half == 0) ps[key * G + g] = e;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[g][j][i] *= keep;
+    }
+    __syncwarp();
+#pragma unroll 4
+    for (int t = ok; t < kTile; t += kSplit) {
+      const T *vr = reinterpret_cast<const T *>(mine + s * C::kStage + (kTile + t) * C::kRow);
+      float e[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) e[g] = ps[t * G + g];
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const float4 x = row4(vr + j * 128 + oc * 4);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          o[g][j][0] = fmaf(e[g], x.x, o[g][j][0]);
+          o[g][j][1] = fmaf(e[g], x.y, o[g][j][1]);
+          o[g][j][2] = fmaf(e[g], x.z, o[g][j][2]);
+          o[g][j][3] = fmaf(e[g], x.w, o[g][j][3]);
+        }
+      }
+    }
+    if (mt.y & kLast) {
+      const bool whole = (mt.y & kFromStart) && (mt.y & kToEnd);
+      const int64_t part = (static_cast<int64_t>(r) * p.units + unit) * 2 + (mt.y & kFromStart ? 1 : 0);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float sum = l[g];
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = kLanes; k < 32; k <<= 1) o[g][j][i] += __shfl_xor_sync(0xffffffffu, o[g][j][i], k);
+        if (g < n_h && lane < kLanes) {
+          const int h = h0 + g;
+          if (whole) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + h * p.out_head);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (j * 128 + oc * 4 + i < p.hd) dst[j * 128 + oc * 4 + i] = Elem<DT>::from_f(o[g][j][i] * inv);
+            if (p.lse && lane == 0)
+              p.lse[static_cast<int64_t>(b) * p.heads + h] = (m[g] + log2f(sum)) * 0.6931471805599453f;
+          } else {
+            float *dst = p.part_o + (part * G + g) * p.hd;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (j * 128 + oc * 4 + i < p.hd) dst[j * 128 + oc * 4 + i] = o[g][j][i];
+            if (lane == 0) {
+              p.part_ml[(part * G + g) * 2] = m[g];
+              p.part_ml[(part * G + g) * 2 + 1] = sum;
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    fill(s);
+  }
+  cp_async_wait<0>();
+}
+
+// ---------------------------------------------------------------------------------------
+// join of the parts
+// ---------------------------------------------------------------------------------------
+constexpr int kJoinWarps = 8;
+
+// One CTA per (cut sequence, query head).  blockIdx.x is a sequence where by_seq, else a range
+// border (at most ranges - 1 sequences are cut); warps take every kJoinWarps-th part.
+template <int DT>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(Params p, int g_unit, int by_seq) {
+  using T = typename Elem<DT>::T;
+  __shared__ float red[kJoinWarps][256];
+  __shared__ float red_l[kJoinWarps], red_m[kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Line ln = line_of(p);
+  const int h = blockIdx.y;
+  int b, r0;
+  if (by_seq) {
+    b = blockIdx.x;
+    const int64_t at = line_pos(p, b);
+    r0 = static_cast<int>(at * ln.ranges / ln.total);
+    while (r0 > 0 && range_start(ln, r0) > at) --r0;
+    while (r0 + 1 < ln.ranges && range_start(ln, r0 + 1) <= at) ++r0;
+  } else {
+    const int rb = blockIdx.x + 1;
+    if (rb >= ln.ranges) return;
+    const int64_t x = range_start(ln, rb);
+    b = seq_at(p, x, lane);
+    const int64_t at = line_pos(p, b);
+    r0 = rb - 1;
+    if (r0 > 0 && range_start(ln, r0) >= at) return;  // an earlier border has this sequence
+  }
+  const int64_t at = line_pos(p, b);
+  const int len = max(p.cu[b + 1] - p.cu[b], 0);
+  if (len == 0) return;
+  int r1 = r0;  // last range with a part of the sequence
+  {
+    const int64_t tail = at + len + kSeqCost - 1;
+    r1 = static_cast<int>(tail * ln.ranges / ln.total);
+    r1 = min(r1, ln.ranges - 1);
+    while (r1 > 0 && range_start(ln, r1) > tail) --r1;
+    while (r1 + 1 < ln.ranges && range_start(ln, r1 + 1) <= tail) ++r1;
+  }
+  if (r1 == r0) return;  // not cut
+  const int u = h / p.group, in = h - u * p.group;
+  const int unit = u * p.chunks + in / g_unit, g = in % g_unit;
+  auto part_of = [&](int r, bool &some, bool &all) {
+    const int i0 = border(range_start(ln, r), at, len), i1 = border(range_start(ln, r + 1), at, len);
+    some = i1 > i0;
+    all = i0 == 0 && i1 == len;
+    return ((static_cast<int64_t>(r) * p.units + unit) * 2 + (i0 == 0 ? 1 : 0)) * g_unit + g;
+  };
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float top = __int_as_float(0xff800000);
+  int done = 0;
+  for (int r = r0 + threadIdx.x; r <= r1; r += kJoinWarps * 32) {
+    bool some, all;
+    const int64_t i = part_of(r, some, all);
+    done |= all;
+    if (some && !all) top = fmaxf(top, p.part_ml[i * 2]);
+  }
+  if (__syncthreads_or(done)) return;  // all its tokens fell into one range: already written
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+  if (lane == 0) red_m[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, red_m[i]);
+  const float base = top == __int_as_float(0xff800000) ? 0.f : top;
+  float acc[8], sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  for (int r = r0 + warp; r <= r1; r += kJoinWarps) {
+    bool some, all;
+    const int64_t i = part_of(r, some, all);
+    if (!some) continue;
+    const float e = exp2f(p.part_ml[i * 2] - base);
+    sum = fmaf(p.part_ml[i * 2 + 1], e, sum);
+    const float *src = p.part_o + i * p.hd;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j * 32 + lane < p.hd) acc[j] = fmaf(src[j * 32 + lane], e, acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j * 32 + lane < p.hd) red[warp][j * 32 + lane] = acc[j];
+  if (lane == 0) red_l[warp] = sum;
+  __syncthreads();
+  float total = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) total += red_l[i];
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + h * p.out_head);
+  for (int d = threadIdx.x; d < p.hd; d += kJoinWarps * 32) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) x += red[i][d];
+    dst[d] = Elem<DT>::from_f(x * inv);
+  }
+  if (p.lse && threadIdx.x == 0)
+    p.lse[static_cast<int64_t>(b) * p.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
+}
+
+// ---------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------
+struct Shape {
+  int hd_pad, g, warps;  // kernel variant
+  int chunks, units;     // chunks of a group, KV heads x chunks
+  int ranges;            // upper bound of the ranges in use
+  int64_t parts;         // part slots
+  int64_t o_bytes, bytes;
+};
+
+int sm_count(int *out) {
+  static int cached[64];
+  int dev = 0;
+  DKV_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 64 && cached[dev] > 0) {
+    *out = cached[dev];
+    return DKV_OK;
+  }
+  int n = 0;
+  DKV_CUDA_CHECK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64) cached[dev] = n;
+  *out = n;
+  return DKV_OK;
+}
+
+bool float_dtype(int dt) { return dt == DKV_F32 || dt == DKV_F16 || dt == DKV_BF16; }
+
+int check(const dkv_paged_decode_args *a) {
+  if (a == nullptr) return DKV_ERR_INVALID_ARGUMENT;
+  const dkv_paged_cache &k = a->k_pages, &v = a->v_pages;
+  if (!float_dtype(k.dtype)) return DKV_ERR_UNSUPPORTED;
+  if (k.dtype != v.dtype || k.block_size != v.block_size || k.n_heads != v.n_heads || k.head_dim != v.head_dim ||
+      k.block_size <= 0 || k.n_heads <= 0 || k.head_dim <= 0 || k.num_blocks < 0 || v.num_blocks < 0)
+    return DKV_ERR_LAYOUT;
+  if (k.head_dim > 256) return DKV_ERR_UNSUPPORTED;
+  if (a->n_q_heads <= 0 || a->n_q_heads % k.n_heads || a->n_q_heads > 65535) return DKV_ERR_UNSUPPORTED;
+  if (a->seqs.n_seqs < 0 || a->seqs.max_seq_len < 0) return DKV_ERR_INVALID_ARGUMENT;
+  if (a->seqs.n_seqs > 65535) return DKV_ERR_UNSUPPORTED;
+  return DKV_OK;
+}
+
+int shape_of(const dkv_paged_decode_args *a, Shape *s) {
+  int sms;
+  const int rc = sm_count(&sms);
+  if (rc != DKV_OK) return rc;
+  const int hd = a->k_pages.head_dim, group = a->n_q_heads / a->k_pages.n_heads;
+  s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+  s->g = group <= 4 ? 4 : 8;
+  s->warps = s->hd_pad == 256 ? 2 : 4;
+  s->chunks = (group + s->g - 1) / s->g;
+  s->units = a->k_pages.n_heads * s->chunks;
+  const int64_t most = static_cast<int64_t>(sms) * s->warps / s->units;
+  const int64_t line = static_cast<int64_t>(a->seqs.n_seqs) * (static_cast<int64_t>(a->seqs.max_seq_len) + kSeqCost);
+  const int64_t want = line / kMinRange;
+  s->ranges = static_cast<int>(most < 1 || want < 1 ? 1 : (want < most ? want : most));
+  s->parts = s->ranges > 1 ? static_cast<int64_t>(s->ranges) * s->units * 2 * s->g : 0;
+  s->o_bytes = (s->parts * hd * 4 + 15) / 16 * 16;
+  s->bytes = s->o_bytes + s->parts * 8;
+  return DKV_OK;
+}
+
+template <int DT, int HD, int G, int W>
+int launch_simt(const Params &p, int grid, cudaStream_t st) {
+  using C = Simt<DT, HD, G, W>;
+  static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
+  DKV_CUDA_CHECK(cudaFuncSetAttribute(simt_kernel<DT, HD, G, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  simt_kernel<DT, HD, G, W><<<grid, W * 32, C::kSmem, st>>>(p);
+  DKV_CUDA_CHECK(cudaGetLastError());
+  return DKV_OK;
+}
+
+template <int DT>
+int launch(const Params &p, const Shape &s, cudaStream_t st) {
+  const int64_t warps = static_cast<int64_t>(s.ranges) * s.units;
+  const int grid = static_cast<int>((warps + s.warps - 1) / s.warps);
+  int rc = DKV_ERR_UNSUPPORTED;
+#define DKV_SIMT_CASE(HD, G, W) \
+  if (s.hd_pad == HD && s.g == G && s.warps == W) rc = launch_simt<DT, HD, G, W>(p, grid, st);
+  DKV_SIMT_CASE(32, 4, 4)
+  DKV_SIMT_CASE(32, 8, 4)
+  DKV_SIMT_CASE(64, 4, 4)
+  DKV_SIMT_CASE(64, 8, 4)
+  DKV_SIMT_CASE(128, 4, 4)
+  DKV_SIMT_CASE(128, 8, 4)
+  DKV_SIMT_CASE(256, 4, 2)
+  DKV_SIMT_CASE(256, 8, 2)
+#undef DKV_SIMT_CASE
+  if (rc != DKV_OK || s.ranges == 1) return rc;
+  // the join starts as soon as every CTA of the walk is under way and waits in the kernel for its end
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  const int by_seq = p.n_seqs <= s.ranges - 1;
+  cfg.gridDim = dim3(by_seq ? p.n_seqs : s.ranges - 1, p.heads);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  DKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<DT>, p, s.g, by_seq));
+  return DKV_OK;
+}
+
+}  // namespace pattn
+}  // namespace dkv
+
+using namespace dkv;
+
+extern "C" int dkv_paged_decode_workspace_bytes(const dkv_paged_decode_args *args, int64_t *bytes) {
+  if (bytes == nullptr) return DKV_ERR_INVALID_ARGUMENT;
+  const int rc = pattn::check(args);
+  if (rc != DKV_OK) return rc;
+  pattn::Shape s;
+  const int rs = pattn::shape_of(args, &s);
+  if (rs != DKV_OK) return rs;
+  *bytes = s.bytes;
+  return DKV_OK;
+}
+
+extern "C" int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv_stream_t stream) {
+  const int rc = pattn::check(args);
+  if (rc != DKV_OK) return rc;
+  const dkv_paged_decode_args &a = *args;
+  const dkv_paged_cache &k = a.k_pages, &v = a.v_pages;
+  if (a.seqs.n_seqs == 0) return DKV_OK;
+  if (a.q == nullptr || a.out == nullptr || a.seqs.cu_seqlens == nullptr)
+    return DKV_ERR_INVALID_ARGUMENT;
+  if ((k.base == nullptr && k.num_blocks > 0) || (v.base == nullptr && v.num_blocks > 0)) return DKV_ERR_INVALID_ARGUMENT;
+  pattn::Shape s;
+  const int rs = pattn::shape_of(args, &s);
+  if (rs != DKV_OK) return rs;
+  if (s.bytes > 0 && (a.workspace == nullptr || a.workspace_bytes < s.bytes)) return DKV_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 16) return DKV_ERR_ALIGNMENT;
+  const int64_t sz = k.dtype == DKV_F32 ? 4 : 2;
+  pattn::Params p;
+  p.q = static_cast<const char *>(a.q), p.q_seq = a.q_stride_seq * sz, p.q_head = a.q_stride_head * sz;
+  p.out = static_cast<char *>(a.out), p.out_seq = a.out_stride_seq * sz, p.out_head = a.out_stride_head * sz;
+  p.lse = a.lse;
+  p.cu = a.seqs.cu_seqlens, p.tables = a.seqs.block_tables, p.table_lens = a.seqs.table_lens;
+  p.table_stride = a.seqs.table_stride;
+  if (p.tables == nullptr) p.table_lens = nullptr, p.table_stride = 0;  // tables without columns
+  p.k = static_cast<const char *>(k.base), p.v = static_cast<const char *>(v.base);
+  p.k_block = k.stride_block * sz, p.k_slot = k.stride_slot * sz, p.k_head = k.stride_head * sz;
+  p.v_block = v.stride_block * sz, p.v_slot = v.stride_slot * sz, p.v_head = v.stride_head * sz;
+  p.num_blocks = k.num_blocks < v.num_blocks ? k.num_blocks : v.num_blocks;
+  p.part_o = static_cast<float *>(a.workspace);
+  p.part_ml = s.parts ? p.part_o + s.o_bytes / 4 : nullptr;
+  p.status = a.status;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.n_seqs = a.seqs.n_seqs, p.n_kv = k.n_heads, p.heads = a.n_q_heads, p.group = a.n_q_heads / k.n_heads;
+  p.chunks = s.chunks, p.units = s.units, p.ranges = s.ranges;
+  p.hd = k.head_dim, p.block_size = k.block_size;
+  // 16-byte copies where every row of K and V starts on 16 bytes and is a multiple of 16 long
+  const int64_t all = p.k_block | p.k_slot | p.k_head | p.v_block | p.v_slot | p.v_head | (p.hd * sz) |
+                      static_cast<int64_t>(reinterpret_cast<uintptr_t>(k.base) | reinterpret_cast<uintptr_t>(v.base));
+  p.vec = all % 16 == 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (k.dtype) {
+    case DKV_F32: return pattn::launch<DKV_F32>(p, s, st);
+    case DKV_F16: return pattn::launch<DKV_F16>(p, s, st);
+    default: return pattn::launch<DKV_BF16>(p, s, st);
+  }
+}

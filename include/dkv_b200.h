@@ -52,6 +52,7 @@ typedef struct CUstream_st *dkv_stream_t;
 #define DKV_ERR_TIMEOUT (-9)           /* a bounded device-side wait gave up              */
 #define DKV_ERR_PAGE_RANGE (-10)       /* block id outside [0, num_blocks)                */
 #define DKV_ERR_WORKSPACE (-11)        /* workspace too small                             */
+#define DKV_ERR_NO_BLOCKS (-12)        /* the list of free blocks ran out                 */
 
 /* ---- element types ------------------------------------------------------ */
 #define DKV_F32 0
@@ -561,6 +562,105 @@ int dkv_subspace_probe_residual(const void *reused, const void *fresh, int32_t k
                                 int64_t reused_row_stride, int64_t fresh_row_stride,
                                 int64_t n_tokens, int64_t d, const int32_t *probe_index,
                                 int64_t n_probes, float *out, dkv_stream_t stream);
+
+/* ---- one step of a paged cache: plan, append, attend ------------------------------- */
+
+/*
+ * The bookkeeping of one prefill or decode step, from device-resident lengths (no host round
+ * trip; capturable).  lengths[b] counts the tokens of sequence b after the step, the last
+ * new_lengths[b] of them (NULL: all) being this step's rows.  Row b of block_tables holds
+ * table_lens[b] valid blocks (NULL: table_width); it is extended in place to
+ * ceil(lengths[b] / block_size) blocks from free_blocks, taken in order of b:
+ *   need_b = ceil(lengths_b / block_size), extra_b = max(0, need_b - held_b),
+ *   block_tables[b, held_b + j] = free_blocks[sum_{a<b} extra_a + j],  0 <= j < extra_b.
+ * Outputs: cu_seqlens / cu_new [n_seqs+1] = prefix sums of the lengths / new lengths,
+ * table_lens_out[b] = max(held_b, need_b), *blocks_used = sum extra_b, and for row
+ * r = cu_new[b] + i:  positions[r] = lengths_b - new_b + i,
+ *   slots[r] = block_tables[b, positions[r] / block_size] * block_size + positions[r] % block_size;
+ * rows of [cu_new[n_seqs], n_rows) get position 0 and slot -1.
+ * A negative length counts as 0 and a new length outside [0, length] is clamped to it
+ * (INVALID_ARGUMENT in *status); a sequence longer than its table row (BLOCK_TABLE_SHORT) or
+ * past the end of the free list (NO_BLOCKS) keeps the blocks that exist, its other tokens get
+ * slot -1; rows beyond n_rows are dropped and cu_new stops at n_rows (INVALID_ARGUMENT).  At most 16384 sequences.  The
+ * outputs must not overlap the inputs.
+ */
+typedef struct dkv_step_plan_args {
+  const int32_t *lengths, *new_lengths, *table_lens; /* [n_seqs]; the last two may be NULL */
+  const int32_t *free_blocks;                        /* [n_free] or NULL with n_free = 0 */
+  int64_t n_free;
+  int32_t *block_tables; /* [n_seqs, table_width], row stride table_stride */
+  int64_t table_stride;
+  int32_t table_width, n_seqs, block_size;
+  int32_t n_rows; /* capacity of positions and slots */
+  int32_t *cu_seqlens, *cu_new, *table_lens_out, *blocks_used;
+  int32_t *positions;
+  int64_t *slots;
+  int32_t *status;
+} dkv_step_plan_args;
+
+int dkv_plan_paged_step(const dkv_step_plan_args *args, dkv_stream_t stream);
+
+/*
+ * Store this step's K and V rows in their slots (slot = block * block_size + offset; a
+ * negative slot: the row stores nothing), K after rotate-half RoPE at positions[row] when the
+ * tables are given (rope.py:9-63); optionally rotate the q rows alongside (every row, padding
+ * rows included).  k, v, q: [n_rows, heads, head_dim], dtype in_dtype, row / head strides in
+ * elements; q_out has q's dtype and may be q itself.  in_dtype is the pages' dtype or F32.
+ * K and V pages share dtype, block_size, heads and head_dim.  A slot beyond the pages
+ * (PAGE_RANGE) stores nothing; a position outside [0, rope_max_pos) (ROPE_RANGE) stores
+ * nothing and leaves its q_out row alone.  Slots must be distinct: which of two rows with the
+ * same slot stays is not defined.
+ */
+typedef struct dkv_append_args {
+  const void *k, *v, *q; /* q may be NULL */
+  int32_t in_dtype;
+  int32_t n_q_heads;
+  int64_t n_rows;
+  int64_t k_stride_row, k_stride_head, v_stride_row, v_stride_head, q_stride_row, q_stride_head;
+  void *q_out;
+  int64_t q_out_stride_row, q_out_stride_head;
+  const int64_t *slots;
+  const int32_t *positions;         /* [n_rows]; NULL without RoPE */
+  const float *rope_cos, *rope_sin; /* [rope_max_pos, head_dim/2] or NULL: no rotation */
+  int32_t rope_max_pos;
+  dkv_paged_cache k_pages, v_pages;
+  int32_t *status;
+} dkv_append_args;
+
+int dkv_append_paged(const dkv_append_args *args, dkv_stream_t stream);
+
+/*
+ * Attention of one new token per sequence over its cached tokens: with i over the
+ * cu_seqlens[b+1] - cu_seqlens[b] tokens of sequence b and query head h reading KV head
+ * h / (n_q_heads / n_heads),
+ *   s_i = scale * q[b,h] . K_i,  out[b,h] = sum_i exp(s_i) V_i / sum_i exp(s_i),
+ *   lse[b,h] = ln sum_i exp(s_i)   (fp32, optional).
+ * A sequence without tokens gives out = 0 and lse = -inf.  Tokens whose block lies outside the
+ * cache (PAGE_RANGE) or beyond the table row (BLOCK_TABLE_SHORT) are left out of both sums.
+ * Slots past a sequence's length are never read into the result, whatever they hold.
+ * q, K, V and out have one dtype; scores, the running maximum and sum and the output
+ * accumulate in fp32.  head_dim <= 256, n_q_heads a multiple of the pages' n_heads.
+ * seqs.max_seq_len sizes the split of long sequences; a length above it costs speed only.
+ * workspace: dkv_paged_decode_workspace_bytes of the same args, 16-byte aligned, nothing in it
+ * needs clearing and nothing is kept in it between calls.
+ */
+typedef struct dkv_paged_decode_args {
+  const void *q; /* [n_seqs, n_q_heads, head_dim] */
+  int64_t q_stride_seq, q_stride_head;
+  int32_t n_q_heads;
+  float scale;
+  dkv_seq_batch seqs;
+  dkv_paged_cache k_pages, v_pages;
+  void *out;
+  int64_t out_stride_seq, out_stride_head;
+  float *lse; /* [n_seqs, n_q_heads] contiguous, or NULL */
+  void *workspace;
+  int64_t workspace_bytes;
+  int32_t *status;
+} dkv_paged_decode_args;
+
+int dkv_paged_decode_workspace_bytes(const dkv_paged_decode_args *args, int64_t *bytes);
+int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv_stream_t stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

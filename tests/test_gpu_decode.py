@@ -1,0 +1,667 @@
+"""One step of a paged cache (plan, append, attend) against plain implementations in 64 bits.
+
+Tolerances, derived: an output is rounded once to its type, at most eps/2 of the value.  Before
+that, fp32 arithmetic: a score is a product sum of head_dim terms, off by at most
+(head_dim + 8) 2^-23 sum |q_d k_d| scale =: ds (a tensor core may truncate, hence 2^-23); an
+error ds of the scores moves every weight by a relative 2 ds (it enters the numerator and the
+sum).  Weights enter the output product to 2^-16 (as two 16-bit terms in 16-bit types), exp and
+the running sums add 2^-20 and n 2^-24 for n tokens.  All of that is relative to
+A = sum p |v| / sum p, the output without cancellation.
+"""
+
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+import torch
+
+import deltakv_b200 as dkv
+from deltakv_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = [BF, F16, F32]
+
+
+class Cache:
+    """Random pages of a layout, tables with shuffled blocks, and the tokens they hold."""
+
+    def __init__(self, lens, n_kv, hd, block, dtype, dev, layout="kv_first", seed=0, fill=None, spare=3):
+        g = torch.Generator().manual_seed(seed)
+        need = [-(-n // block) for n in lens]
+        nb = sum(need) + spare
+        width = max(max(need, default=0), 1)
+        self.lens, self.block = lens, block
+        shape = (block, n_kv, hd)
+        if layout == "kv_first":
+            full = torch.randn(2, nb, *shape, generator=g).to(dtype)
+            k, v = full[0], full[1]
+        elif layout == "block_first":
+            full = torch.randn(nb, 2, *shape, generator=g).to(dtype)
+            k, v = full[:, 0], full[:, 1]
+        elif layout == "odd":  # every stride padded, nothing aligned
+            full = torch.randn(2, nb, block + 1, n_kv + 1, hd + 3, generator=g).to(dtype)
+            k, v = full[0, :, 1:, 1:, 1:hd + 1], full[1, :, 1:, 1:, 1:hd + 1]
+        else:  # heads before slots
+            full = torch.randn(2, nb, n_kv, block, hd, generator=g).to(dtype)
+            k, v = full[0].transpose(1, 2), full[1].transpose(1, 2)
+        order = torch.randperm(nb, generator=g)
+        tables = torch.zeros(max(len(lens), 1), width, dtype=torch.int32)
+        used = torch.zeros(nb, block, dtype=torch.bool)
+        at = 0
+        for b, n in enumerate(need):
+            tables[b, :n] = order[at:at + n]
+            for i in range(n):
+                used[order[at + i], : min(block, lens[b] - i * block)] = True
+            at += n
+        if fill is not None:  # what no token owns holds garbage
+            k[~used], v[~used] = fill, fill
+        self.used = used
+        full = full.to(dev)
+        if layout == "kv_first":
+            self.k, self.v = full[0], full[1]
+        elif layout == "block_first":
+            self.k, self.v = full[:, 0], full[:, 1]
+        elif layout == "odd":
+            self.k, self.v = full[0, :, 1:, 1:, 1:hd + 1], full[1, :, 1:, 1:, 1:hd + 1]
+        else:
+            self.k, self.v = full[0].transpose(1, 2), full[1].transpose(1, 2)
+        self.tables = tables.to(dev)
+        cu = [0]
+        for n in lens:
+            cu.append(cu[-1] + n)
+        self.cu = torch.tensor(cu, dtype=torch.int32, device=dev)
+
+    def seqs(self, **kw):
+        return dkv.SeqBatchTensors(cu_seqlens=self.cu, block_tables=self.tables, max_seq_len=max(self.lens, default=0), **kw)
+
+    def tokens(self, b):
+        n = self.lens[b]
+        ids = self.tables[b, : -(-n // self.block)].long()
+        take = lambda t: t[ids].reshape(-1, t.shape[2], t.shape[3])[:n]  # noqa: E731
+        return take(self.k), take(self.v)
+
+
+def check_attention(got, lse, q, tokens_of, scale):
+    """Every sequence's output (and lse) against the definition in fp64."""
+    n, heads, hd = q.shape
+    for b in range(n):
+        k, v = (t.double() for t in tokens_of(b))
+        if k.shape[0] == 0:
+            assert torch.all(got[b] == 0), b
+            assert lse is None or torch.all(lse[b] == -math.inf)
+            continue
+        kv = k.shape[1]
+        qb = q[b].double().view(kv, heads // kv, hd)
+        s = torch.einsum("ugd,nud->ugn", qb, k) * scale
+        ds = (hd + 8) * 2.0 ** -23 * (torch.einsum("ugd,nud->ugn", qb.abs(), k.abs()) * abs(scale)).amax(-1)
+        ref_lse = torch.logsumexp(s, -1)
+        p = torch.exp(s - ref_lse[..., None])
+        ref = torch.einsum("ugn,nud->ugd", p, v)
+        spread = torch.einsum("ugn,nud->ugd", p, v.abs())
+        tol = torch.finfo(q.dtype).eps / 2 * ref.abs() + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
+        tol = tol + spread * (2 * ds[..., None] + 2.0 ** -20 + k.shape[0] * 2.0 ** -24
+                              + (2.0 ** -16 if q.dtype != F32 else 0))
+        off = (got[b].double().view(kv, heads // kv, hd) - ref).abs()
+        assert torch.all(off <= tol), (b, k.shape[0], float((off / tol).max()))
+        if lse is not None:
+            off = (lse[b].double().view(kv, heads // kv) - ref_lse).abs()
+            tol = 2 * ds + k.shape[0] * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -22 * ref_lse.abs()
+            assert torch.all(off <= tol), (b, float((off / tol).max()))
+
+
+def run_attention(c, heads, hd, dtype, dev, seed=1, scale=None, amp=1.5):
+    g = torch.Generator().manual_seed(seed)
+    q = (amp * torch.randn(len(c.lens), heads, hd, generator=g)).to(dtype).to(dev)
+    out, lse = dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), scale=scale, return_lse=True, check=True)
+    check_attention(out, lse, q, c.tokens, hd ** -0.5 if scale is None else scale)
+    return q, out, lse
+
+
+LENS = [0, 1, 2, 15, 16, 17, 33, 100, 0, 333, 64]
+
+
+# ---------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_kv,group,hd", [(3, 3, 64), (8, 4, 128), (1, 1, 32), (2, 8, 128), (1, 16, 256), (2, 7, 80),
+                                           (1, 9, 96), (1, 33, 64), (5, 5, 64), (2, 2, 256), (3, 1, 48)])
+def test_attention_heads_and_types(cuda, dtype, n_kv, group, hd):
+    run_attention(Cache(LENS, n_kv, hd, 16, dtype, cuda), n_kv * group, hd, dtype, cuda)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [1, 2, 7, 20, 33, 72, 100, 130, 200, 255])
+def test_attention_odd_head_dims(cuda, dtype, hd):
+    run_attention(Cache([5, 0, 70], 2, hd, 16, dtype, cuda), 6, hd, dtype, cuda)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("block", [1, 3, 8, 24, 64, 256, 1000])
+def test_attention_block_sizes(cuda, dtype, block):
+    run_attention(Cache([1, 40, 0, 257, 1000], 2, 64, block, dtype, cuda), 8, 64, dtype, cuda)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["block_first", "odd", "heads_first"])
+def test_attention_layouts_and_strides(cuda, dtype, layout):
+    c = Cache([31, 0, 500, 16], 3, 64, 16, dtype, cuda, layout=layout)
+    q, out, lse = run_attention(c, 9, 64, dtype, cuda)
+    # q and out as strided views
+    wide = torch.zeros(4, 11, 70, dtype=dtype, device=cuda)
+    qs = wide[:, 1:10, 3:67]
+    qs.copy_(q)
+    into = torch.full((4, 10, 65), 7.0, dtype=dtype, device=cuda)
+    got = dkv.paged_decode_attention(qs, c.k, c.v, c.seqs(), out=into[:, 1:, 1:])
+    assert got.data_ptr() == into[:, 1:, 1:].data_ptr() and torch.equal(got, out)
+    assert torch.all(into[:, 0] == 7.0) and torch.all(into[:, :, 0] == 7.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("fill", [math.nan, math.inf, -math.inf])
+def test_attention_never_reads_what_no_token_owns(cuda, dtype, fill):
+    run_attention(Cache([1, 17, 0, 300, 15], 2, 64, 32, dtype, cuda, fill=fill), 8, 64, dtype, cuda)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens", [[20011], [9000, 1, 0, 7000], [1] * 300, [0] * 40, [3, 2049] * 20, list(range(130))])
+def test_attention_long_and_ragged(cuda, dtype, lens):
+    run_attention(Cache(lens, 2, 64, 16, dtype, cuda), 8, 64, dtype, cuda)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_many_sequences(cuda, dtype):
+    rng = random.Random(5)
+    lens = [rng.choice([0, 1, 5, rng.randrange(60)]) for _ in range(3000)]
+    c = Cache(lens, 1, 32, 8, dtype, cuda)
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(len(lens), 2, 32, generator=g).to(dtype).to(cuda)
+    out = dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), check=True)
+    for b in range(0, 3000, 37):  # one sequence alone gives the same tokens' answer
+        check_attention(out[b:b + 1], None, q[b:b + 1], lambda _, b=b: c.tokens(b), 32 ** -0.5)
+    empty = torch.tensor([n == 0 for n in lens], device=cuda)
+    assert torch.all(out[empty] == 0) and torch.all(torch.isfinite(out))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("amp,scale", [(1.5, 30.0), (60.0, None), (0.0, None), (1.5, -0.2)])
+def test_attention_extreme_scores(cuda, dtype, amp, scale):
+    """One token takes all the weight, equal scores, a negative scale."""
+    run_attention(Cache([700, 1, 90], 2, 64, 16, dtype, cuda), 4, 64, dtype, cuda, amp=amp, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_tokens_of_no_weight(cuda, dtype):
+    """K rows that score -inf weigh nothing; a sequence of only such rows has no weight at all."""
+    c = Cache([40, 20], 1, 32, 16, dtype, cuda)
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(2, 2, 32, generator=g).abs().add(0.1).to(dtype).to(cuda)
+    ids0, ids1 = c.tables[0].long(), c.tables[1].long()
+    c.k[ids0[1], 3:9] = -math.inf   # tokens 19..24 of sequence 0
+    c.k[ids1[:2]] = -math.inf       # all of sequence 1
+    out, lse = dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), return_lse=True)
+    k, v = c.tokens(0)
+    keep = torch.tensor([not 19 <= i < 25 for i in range(40)], device=cuda)
+    check_attention(out[:1], lse[:1], q[:1], lambda _: (k[keep], v[keep]), 32 ** -0.5)
+    assert torch.all(out[1] == 0) and torch.all(lse[1] == -math.inf)
+
+
+def test_attention_offsets_beyond_32_bits(cuda):
+    """Blocks whose element offset passes 2^31 (and byte offset 2^32)."""
+    block, n_kv, hd = 256, 8, 128
+    nb = (1 << 31) // (block * n_kv * hd) + 6
+    pages = torch.zeros(nb, block, n_kv, hd, dtype=BF, device=cuda)
+    lens = [700, 300]
+    c = Cache(lens, n_kv, hd, block, BF, cuda)
+    moved = c.tables.clone()
+    for i, (b, j) in enumerate([(0, 0), (0, 1), (0, 2), (1, 0), (1, 1)]):
+        moved[b, j] = nb - 1 - i
+        pages[nb - 1 - i] = c.k[c.tables[b, j].long()]
+    vp = pages.clone()
+    for i, (b, j) in enumerate([(0, 0), (0, 1), (0, 2), (1, 0), (1, 1)]):
+        vp[nb - 1 - i] = c.v[c.tables[b, j].long()]
+    q = torch.randn(2, 32, hd, device=cuda).to(BF)
+    want = dkv.paged_decode_attention(q, c.k, c.v, c.seqs())
+    seqs = dkv.SeqBatchTensors(cu_seqlens=c.cu, block_tables=moved, max_seq_len=700)
+    assert torch.equal(dkv.paged_decode_attention(q, pages, vp, seqs, check=True), want)
+    check_attention(want, None, q, c.tokens, hd ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_bad_blocks_are_left_out(cuda, dtype):
+    c = Cache([100, 50], 2, 64, 16, dtype, cuda)
+    q = torch.randn(2, 4, 64, device=cuda).to(dtype)
+    c.tables[0, 2] = c.k.shape[0]  # one past the cache
+    c.tables[1, 0] = -1
+    with pytest.raises(dkv.DkvError, match="block id outside"):
+        dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), check=True)
+    out, lse = dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), return_lse=True)
+    ops.status_word(cuda).t.zero_()
+
+    def good(b):
+        ids = c.tables[b].long()
+        ids = ids[(ids >= 0) & (ids < c.k.shape[0])]
+        n = c.lens[b] - 16
+        return tuple(t[ids].reshape(-1, 2, 64)[:n] for t in (c.k, c.v))
+
+    check_attention(out, lse, q, good, 64 ** -0.5)
+
+
+def test_attention_short_table(cuda):
+    c = Cache([100, 50], 2, 64, 16, BF, cuda)
+    q = torch.randn(2, 4, 64, device=cuda).to(BF)
+    seqs = c.seqs(table_lens=torch.tensor([3, 4], dtype=torch.int32, device=cuda))
+    with pytest.raises(dkv.DkvError, match="block_table shorter"):
+        dkv.paged_decode_attention(q, c.k, c.v, seqs, check=True)
+    out = dkv.paged_decode_attention(q, c.k, c.v, seqs)
+    ops.status_word(cuda).t.zero_()
+    check_attention(out, None, q, lambda b: tuple(t[: (48, 50)[b]] for t in c.tokens(b)), 64 ** -0.5)
+    # a table without columns: no token has a block
+    seqs = dkv.SeqBatchTensors(cu_seqlens=c.cu, block_tables=c.tables[:, :0], max_seq_len=100)
+    assert torch.all(dkv.paged_decode_attention(q, c.k, c.v, seqs) == 0)
+    ops.status_word(cuda).t.zero_()
+
+
+def test_attention_empty_batch_and_understated_bound(cuda):
+    c = Cache([900, 20], 2, 64, 16, BF, cuda)
+    q = torch.randn(2, 4, 64, device=cuda).to(BF)
+    none = dkv.SeqBatchTensors(cu_seqlens=c.cu[:1], block_tables=c.tables[:0], max_seq_len=0)
+    assert dkv.paged_decode_attention(q[:0], c.k, c.v, none).shape == (0, 4, 64)
+    for bound in (0, 7, 1 << 20):  # a wrong bound costs speed, not the answer
+        seqs = dkv.SeqBatchTensors(cu_seqlens=c.cu, block_tables=c.tables, max_seq_len=bound)
+        check_attention(dkv.paged_decode_attention(q, c.k, c.v, seqs, check=True), None, q, c.tokens, 64 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_parts_join_by_lse(cuda, dtype):
+    c = Cache([600], 2, 64, 16, dtype, cuda)
+    q, _, lse = run_attention(c, 8, 64, dtype, cuda)
+    got = []
+    for lo, hi in ((0, 25), (25, 38)):  # blocks
+        n = min(600, hi * 16) - lo * 16
+        seqs = dkv.SeqBatchTensors(cu_seqlens=torch.tensor([0, n], dtype=torch.int32, device=cuda),
+                                   block_tables=c.tables[:, lo:hi].contiguous(), max_seq_len=n)
+        got.append(dkv.paged_decode_attention(q, c.k, c.v, seqs, return_lse=True))
+    joined = torch.logaddexp(got[0][1].double(), got[1][1].double())
+    assert float((joined - lse.double()).abs().max()) < 1e-5
+
+
+def test_attention_is_deterministic_and_reads_the_right_stream(cuda):
+    c = Cache([5000, 300, 0, 17], 2, 128, 16, BF, cuda)
+    q = torch.randn(4, 8, 128, device=cuda).to(BF)
+    want = dkv.paged_decode_attention(q, c.k, c.v, c.seqs())
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        late = torch.zeros_like(q)
+        torch.cuda._sleep(20_000_000)
+        late.copy_(q)  # only ordered before the call on this stream
+        got = dkv.paged_decode_attention(late, c.k, c.v, c.seqs())
+    other = dkv.paged_decode_attention(q, c.k, c.v, c.seqs())  # at the same time on another
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(other, want)
+
+
+# ---------------------------------------------------------------------------------------
+# plan
+# ---------------------------------------------------------------------------------------
+def plan_oracle(lens, new, held, tables, free, block, rows):
+    """The definition, one sequence at a time, on Python lists."""
+    tables = [list(t) for t in tables]
+    width = len(tables[0]) if tables else 0
+    cu, cu_new, out_lens, pos, slot, used = [0], [0], [], [], [], 0
+    for b, n in enumerate(lens):
+        n = max(n, 0)
+        k = min(max(new[b], 0), n)
+        h = min(max(held[b], 0), width)
+        extra = max(min(-(-n // block), width) - h, 0)
+        got = max(min(extra, len(free) - used), 0)
+        for j in range(got):
+            tables[b][h + j] = free[used + j]
+        used += extra
+        cu.append(cu[-1] + n)
+        cu_new.append(cu_new[-1] + k)
+        out_lens.append(h + got)
+        for i in range(n - k, n):
+            pos.append(i)
+            ok = i // block < h + got and tables[b][i // block] >= 0
+            slot.append(tables[b][i // block] * block + i % block if ok else -1)
+    pos, slot, cu_new = pos[:rows], slot[:rows], [min(x, rows) for x in cu_new]
+    return cu, cu_new, out_lens, pos + [0] * (rows - len(pos)), slot + [-1] * (rows - len(slot)), min(used, len(free)), tables
+
+
+def run_plan(dev, lens, new, held, tables, free, block, rows, check=True, view=False):
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    n, width = len(lens), len(tables[0]) if tables else 0
+    t = ints(tables).view(n, width)
+    if view:  # a column slice of a wider table
+        wide = torch.full((n, width + 5), -9, dtype=torch.int32, device=dev)
+        wide[:, 2:2 + width] = t
+        t = wide[:, 2:2 + width]
+    step = dkv.plan_paged_step(ints(lens), t, block, rows=rows, max_seq_len=max(lens, default=0),
+                               new_lengths=None if new is None else ints(new),
+                               table_lens=None if held is None else ints(held),
+                               free_blocks=None if free is None else ints(free), check=check)
+    want = plan_oracle(lens, lens if new is None else new, [width] * n if held is None else held, tables, free or [],
+                       block, rows)
+    got = (step.seqs.cu_seqlens, step.cu_new, step.seqs.table_lens, step.positions, step.slots, step.blocks_used, t)
+    names = ("cu_seqlens", "cu_new", "table_lens", "positions", "slots", "used", "tables")
+    for name, g, w in zip(names, got, want):
+        assert g.reshape(-1).tolist() == torch.tensor(w).reshape(-1).tolist(), name
+    assert step.seqs.block_tables.data_ptr() == t.data_ptr()
+    if view:
+        assert torch.all(wide[:, :2] == -9) and torch.all(wide[:, 2 + width:] == -9)
+    return step
+
+
+def random_plan(rng, n, longest, most_new, block):
+    lens = [rng.choice([0, 1, rng.randrange(longest + 1)]) for _ in range(n)]
+    new = [rng.randint(0, min(x, most_new)) for x in lens]
+    held = [-(-(x - k) // block) for x, k in zip(lens, new)]
+    width = max(-(-x // block) for x in lens) + 1
+    ids = rng.sample(range(10 * n * width), n * width)
+    tables = [[ids.pop() if j < held[b] else 0 for j in range(width)] for b in range(n)]
+    free = [rng.randrange(10 ** 6) for _ in range(sum(-(-x // block) - h for x, h in zip(lens, held)) + 3)]
+    return lens, new, held, tables, free
+
+
+@pytest.mark.parametrize("n,longest,most_new,block,view", [(1, 5, 5, 16, False), (7, 100, 1, 16, True),
+                                                           (40, 300, 300, 5, False), (513, 200, 3, 8, True),
+                                                           (1100, 60, 60, 1, False), (100, 2000, 700, 64, False)])
+def test_plan_random(cuda, n, longest, most_new, block, view):
+    rng = random.Random(n)
+    lens, new, held, tables, free = random_plan(rng, n, longest, most_new, block)
+    total = sum(new)
+    for rows in (total, total + 333):
+        run_plan(cuda, lens, new, held, tables, free, block, rows, view=view)
+
+
+def test_plan_forms_and_edges(cuda):
+    run_plan(cuda, [], [], [], [], [], 16, 0)
+    run_plan(cuda, [], [], [], [], [], 16, 5)                                  # only padding rows
+    run_plan(cuda, [0, 0], None, None, [[4], [5]], None, 16, 0)
+    run_plan(cuda, [3, 20], None, None, [[4, 1], [5, 2]], None, 16, 23)        # full tables, all tokens new
+    run_plan(cuda, [3, 20], [1, 1], [1, 2], [[4, 1], [5, 2]], None, 16, 2)     # blocks held beyond the need
+    run_plan(cuda, [33], None, [0], [[0, 0, 0]], [7, 8, 9], 16, 33)            # a fresh prefill
+    run_plan(cuda, [0, 0], [0, 0], [0, 0], [[], []], [], 16, 0)                # a table without columns
+
+
+def test_plan_largest_batch(cuda):
+    n = 16384
+    lens = [1 + (i * 7) % 40 for i in range(n)]
+    held = [-(-(x - 1) // 16) for x in lens]
+    tables = [[3 * i + j for j in range(3)] for i in range(n)]
+    free = list(range(10 ** 6, 10 ** 6 + n))
+    run_plan(cuda, lens, [1] * n, held, tables, free, 16, n)
+    with pytest.raises(dkv.DkvError, match="unsupported"):
+        z = torch.zeros(n + 1, dtype=torch.int32, device=cuda)
+        dkv.plan_paged_step(z, z[:, None].clone(), 16, rows=0, max_seq_len=0)
+
+
+@pytest.mark.parametrize("text,lens,new,held,tables,free,rows", [
+    ("free block list", [40, 40], [40, 40], [0, 0], [[0] * 3, [0] * 3], [5, 6, 7, 8], 80),
+    ("block_table shorter", [40, 20], [2, 1], [2, 2], [[4, 5], [6, 7]], [9], 3),
+    ("invalid argument", [-3, 20], [1, 1], [1, 2], [[4, 5], [6, 7]], [], 2),
+    ("invalid argument", [3, 20], [5, -1], [1, 2], [[4, 5], [6, 7]], [], 3),
+    ("invalid argument", [3, 20], [1, 1], [-1, 9], [[4, 5], [6, 7]], [8], 2),
+    ("invalid argument", [3, 20], [3, 4], [1, 2], [[4, 5], [6, 7]], [], 5),
+])
+def test_plan_records_what_does_not_fit(cuda, text, lens, new, held, tables, free, rows):
+    with pytest.raises(dkv.DkvError, match=text):
+        run_plan(cuda, lens, new, held, tables, free, 16, rows)
+    run_plan(cuda, lens, new, held, tables, free, 16, rows, check=False)  # the rest is as documented
+    ops.status_word(cuda).t.zero_()
+
+
+# ---------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------
+def rope_tables(hd, n, dev):
+    rope = dkv.RotaryEmbedding(hd, n)
+    return rope, rope.cos_cached[:, : hd // 2].to(dev), rope.sin_cached[:, : hd // 2].to(dev)
+
+
+def check_append(dev, c, dtype, heads, n_kv, hd, rows, seed=0, rope=True, with_q=True, fused=False, in_place=False):
+    g = torch.Generator().manual_seed(seed)
+    n_slots = c.k.shape[0] * c.block
+    slots = torch.randperm(n_slots, generator=g)[:rows]
+    slots[torch.rand(rows, generator=g) < 0.1] = -1
+    pos = torch.randint(0, 500, (rows,), generator=g, dtype=torch.int32)
+    qkv = torch.randn(rows, heads + 2 * n_kv, hd, generator=g).to(dtype).to(dev)
+    q, k, v = qkv.split([heads, n_kv, n_kv], 1)
+    if not fused:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    table, cos, sin = rope_tables(hd, 500, dev) if rope else (None, None, None)
+    want_k, want_v, q_in = c.k.clone(), c.v.clone(), q.clone()
+
+    def turn(x):
+        """In fp64, rounded once: off by the two fp32 products and their sum at most."""
+        if not rope:
+            return x.double()
+        cs, sn = cos[pos.to(dev).long()].double()[:, None], sin[pos.to(dev).long()].double()[:, None]
+        lo, hi = x.double().chunk(2, -1)
+        return torch.cat([lo * cs - hi * sn, hi * cs + lo * sn], -1)
+
+    got = dkv.append_into_paged(k, v, c.k, c.v, slots.to(dev), q=q if with_q else None,
+                                positions=pos.to(dev) if rope else None, rope=table,
+                                q_out=q if in_place else None, check=True)
+    at = slots >= 0
+    where = (slots[at].to(dev) // c.block, slots[at].to(dev) % c.block)
+
+    def close(a, ref, big):
+        eps = torch.finfo(a.dtype).eps / 2
+        tol = eps * ref.abs() + 2.0 ** -22 * big + torch.finfo(a.dtype).smallest_normal * torch.finfo(a.dtype).eps
+        assert torch.all((a.double() - ref).abs() <= tol)
+
+    biggest = lambda x: x.double().abs().amax(-1, keepdim=True)  # noqa: E731
+    close(c.k[where], turn(k if not in_place else k)[at.to(dev)], biggest(k)[at.to(dev)])
+    close(c.v[where], v.double()[at.to(dev)], biggest(v)[at.to(dev)])
+    if dtype == c.v.dtype:
+        assert torch.equal(c.v[where], v[at.to(dev)])
+    want_k[where], want_v[where] = c.k[where], c.v[where]
+    assert torch.equal(want_k, c.k) and torch.equal(want_v, c.v)  # nothing else was touched
+    if with_q:
+        close(got, turn(q_in), biggest(q_in))
+        assert (got.data_ptr() == q.data_ptr()) == in_place
+    else:
+        assert got is None
+
+
+@pytest.mark.parametrize("dtype,pages", [(BF, BF), (F16, F16), (F32, F32), (F32, BF), (F32, F16)])
+@pytest.mark.parametrize("heads,n_kv,hd,rows", [(32, 8, 128, 64), (9, 3, 64, 111), (1, 1, 2, 5), (4, 4, 80, 33),
+                                                (6, 2, 36, 17), (16, 1, 256, 3), (8, 8, 16, 1), (5, 5, 32, 500)])
+def test_append_shapes(cuda, dtype, pages, heads, n_kv, hd, rows):
+    c = Cache([600], n_kv, hd, 16, pages, cuda)
+    check_append(cuda, c, dtype, heads, n_kv, hd, rows)
+    check_append(cuda, c, dtype, heads, n_kv, hd, rows, seed=1, fused=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["block_first", "odd", "heads_first"])
+def test_append_layouts(cuda, dtype, layout):
+    c = Cache([600], 3, 64, 24, dtype, cuda, layout=layout)
+    check_append(cuda, c, dtype, 9, 3, 64, 100, in_place=True)
+    check_append(cuda, c, dtype, 9, 3, 64, 100, fused=True, in_place=True)
+    check_append(cuda, c, dtype, 9, 3, 64, 100, with_q=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [1, 7, 64, 100])
+def test_append_without_rope(cuda, dtype, hd):
+    check_append(cuda, Cache([300], 2, hd, 16, dtype, cuda), dtype, 2, 2, hd, 90, rope=False, with_q=False)
+
+
+def test_append_ranges(cuda):
+    """A slot beyond the pages and a position beyond the tables: recorded, nothing written."""
+    c = Cache([100], 2, 64, 16, BF, cuda)
+    rope, _, _ = rope_tables(64, 50, cuda)
+    k = torch.randn(4, 2, 64, device=cuda).to(BF)
+    q, out = torch.randn(4, 4, 64, device=cuda).to(BF), torch.full((4, 4, 64), 3.0, dtype=BF, device=cuda)
+    before = c.k.clone(), c.v.clone()
+    n_slots = c.k.shape[0] * 16
+    slots = torch.tensor([n_slots, 1 << 40, 5, 6], device=cuda)
+    pos = torch.tensor([1, 2, 50, -1], dtype=torch.int32, device=cuda)
+    with pytest.raises(dkv.DkvError):
+        dkv.append_into_paged(k, k, c.k, c.v, slots, q=q, positions=pos, rope=rope, q_out=out, check=True)
+    assert torch.equal(c.k, before[0]) and torch.equal(c.v, before[1])
+    assert torch.all(out[2:] == 3.0) and not torch.any(torch.all(out[:2] == 3.0, -1))
+    assert dkv.append_into_paged(k[:0], k[:0], c.k, c.v, slots[:0]) is None
+    with pytest.raises(ValueError, match="do not cover head_dim"):
+        dkv.append_into_paged(k, k, c.k, c.v, slots, positions=pos, rope=rope_tables(32, 50, cuda)[0])
+
+
+# ---------------------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------------------
+class Server:
+    """A small serving loop on the three operators; keeps every token's K and V beside the pages."""
+
+    def __init__(self, dev, dtype, n_req=5, heads=8, n_kv=2, hd=64, block=16, width=20, rows=64, layout="kv_first"):
+        self.dev, self.dtype, self.heads, self.n_kv, self.hd, self.block = dev, dtype, heads, n_kv, hd, block
+        nb = n_req * width
+        cache = torch.full((2, nb, block, n_kv, hd), math.nan, dtype=dtype, device=dev)
+        self.k, self.v = ops.page_view(cache, 0), ops.page_view(cache, 1)
+        ints = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)  # noqa: E731
+        self.tables, self.held, self.lens, self.new = ints(n_req, width), ints(n_req), ints(n_req), ints(n_req)
+        self.free = torch.randperm(nb, generator=torch.Generator().manual_seed(9)).to(torch.int32).to(dev)
+        self.rope, self.cos, self.sin = rope_tables(hd, width * block, dev)
+        self.qkv = torch.zeros(rows, heads + 2 * n_kv, hd, dtype=dtype, device=dev)
+        self.rows = rows
+        self.n_req = n_req
+        self.max_len = width * block
+        self.stored = [[] for _ in range(n_req)]
+        self.q_of = None
+
+    def launch(self):
+        """The calls of one step, free of any host round trip."""
+        step = dkv.plan_paged_step(self.lens, self.tables, self.block, rows=self.rows, max_seq_len=self.max_len,
+                                   new_lengths=self.new, table_lens=self.held, free_blocks=self.free)
+        q, k, v = self.qkv.split([self.heads, self.n_kv, self.n_kv], 1)
+        q = dkv.append_into_paged(k, v, self.k, self.v, step.slots, q=q, positions=step.positions, rope=self.rope)
+        last = (step.cu_new[1:].long() - 1).clamp(min=0)
+        out = dkv.paged_decode_attention(q[last], self.k, self.v, step.seqs)
+        return step, out
+
+    def feed(self, new, seed):
+        """This step's inputs, in the buffers a captured step reads."""
+        g = torch.Generator().manual_seed(seed)
+        assert sum(new) <= self.rows
+        self.new.copy_(torch.tensor(new, dtype=torch.int32))
+        self.lens += self.new
+        self.qkv.copy_(torch.randn(self.qkv.shape, generator=g).to(self.dtype))
+
+    def verify(self, new, step, out):
+        cu = step.cu_new.tolist()
+        pos = step.positions[: cu[-1]].long()
+        cs, sn = self.cos[pos].double()[:, None], self.sin[pos].double()[:, None]
+
+        def turn(x):
+            lo, hi = x[: cu[-1]].double().chunk(2, -1)
+            return torch.cat([lo * cs - hi * sn, hi * cs + lo * sn], -1).to(self.dtype)
+
+        q, k, v = self.qkv.split([self.heads, self.n_kv, self.n_kv], 1)
+        q, k = turn(q), turn(k)
+        for b in range(self.n_req):
+            self.stored[b] += [(k[r], v[r].clone()) for r in range(cu[b], cu[b + 1])]
+        rows = [cu[b + 1] - 1 for b in range(self.n_req)]
+
+        def tokens(b):
+            if not self.stored[b]:
+                return (torch.zeros(0, self.n_kv, self.hd, device=self.dev),) * 2
+            return tuple(torch.stack([t[i] for t in self.stored[b]]) for i in (0, 1))
+
+        # a rotation in fp32 may round to the neighbour of the fp64 one: compare through what is stored
+        for b in range(self.n_req):
+            k_ref, v_ref = tokens(b)
+            n = k_ref.shape[0]
+            ids = step.seqs.block_tables[b, : -(-n // self.block)].long()
+            kk, vv = (t[ids].reshape(-1, self.n_kv, self.hd)[:n] for t in (self.k, self.v))
+            assert torch.equal(vv, v_ref)
+            assert torch.all((kk.double() - k_ref.double()).abs() <= 2.0 ** -20 * 8 + torch.finfo(self.dtype).eps * k_ref.double().abs())
+        have = [b for b in range(self.n_req) if new[b]]
+        for b in have:
+            n = len(self.stored[b])
+            ids = step.seqs.block_tables[b, : -(-n // self.block)].long()
+            pages = tuple(t[ids].reshape(-1, self.n_kv, self.hd)[:n] for t in (self.k, self.v))
+            qd = q[rows[b]].double()
+            s = torch.einsum("ugd,nud->ugn", qd.view(self.n_kv, -1, self.hd), pages[0].double()) * self.hd ** -0.5
+            ref = torch.einsum("ugn,nud->ugd", torch.softmax(s, -1), pages[1].double()).reshape(self.heads, self.hd)
+            # q's rotation may round to its neighbour (eps of q): the scores move by eps sum |q k| scale at most
+            ds = torch.finfo(self.dtype).eps * float((torch.einsum(
+                "ugd,nud->ugn", qd.abs().view(self.n_kv, -1, self.hd), pages[0].double().abs()) * self.hd ** -0.5).max())
+            spread = float(pages[1].double().abs().max())
+            assert float((out[b].double() - ref).abs().max()) <= (torch.finfo(self.dtype).eps + 2 * ds) * spread
+        self.held.copy_(step.seqs.table_lens)
+        used = int(step.blocks_used)
+        self.free.copy_(torch.cat([self.free[used:], self.free[:used]]))  # taken entries to the end
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_steps_of_a_serving_loop(cuda, dtype):
+    """A ragged prefill, then decode steps that cross block borders, one request idle for a while."""
+    s = Server(cuda, dtype)
+    for i, new in enumerate([[13, 0, 30, 5, 16], [1, 1, 1, 1, 1], [1, 20, 1, 0, 1], [1, 1, 1, 1, 1], [1, 0, 1, 1, 17]]):
+        s.feed(new, i)
+        step, out = s.launch()
+        s.verify(new, step, out)
+    ops.status_word(cuda).raise_if_set("steps")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_captured_steps(cuda, dtype):
+    """The whole step in one graph, replayed with other lengths; a second captured step shares the allocator."""
+    a, b = Server(cuda, dtype), Server(cuda, dtype, n_req=3, heads=6, n_kv=3, hd=32, block=8, rows=40)
+    for i, (s, new) in enumerate([(a, [13, 2, 30, 5, 3]), (b, [9, 1, 20])]):
+        s.feed(new, i)
+        s.verify(new, *s.launch())  # eager first: everything is loaded
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(side):
+        for s in (a, b):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                made = s.launch()
+            graphs.append((graph, made))
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for i in range(4):
+        news = ([1, 1, 3, 0, 1], [1, 7, 1])
+        a.feed(news[0], 10 + i)
+        b.feed(news[1], 20 + i)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):  # both at once
+            graphs[0][0].replay()
+        graphs[1][0].replay()
+        torch.cuda.synchronize()
+        a.verify(news[0], *graphs[0][1])
+        b.verify(news[1], *graphs[1][1])
+    ops.status_word(cuda).raise_if_set("captured steps")
+
+
+def test_step_beside_a_patch(cuda):
+    """The pages the step writes are the ones the patch operators change: attend, patch, attend."""
+    s = Server(cuda, BF)
+    new = [13, 4, 26, 5, 16]
+    s.feed(new, 0)
+    step, out = s.launch()
+    s.verify(new, step, out)
+    g = torch.Generator().manual_seed(4)
+    total = sum(new)
+    delta = (0.5 * torch.randn(total, 2, 64, generator=g)).to(cuda)
+    q = torch.randn(5, 8, 64, generator=g).to(BF).to(cuda)
+    dkv.scatter_into_paged_batched(delta, s.v, step.seqs, check=True)
+    got = dkv.paged_decode_attention(q, s.k, s.v, step.seqs)
+
+    def tokens(b):
+        ids = step.seqs.block_tables[b, : -(-new[b] // 16)].long()
+        return tuple(t[ids].reshape(-1, 2, 64)[: new[b]] for t in (s.k, s.v))
+
+    check_attention(got, None, q, tokens, 64 ** -0.5)
+    lo = sum(new[:2])
+    patched = torch.stack([v for _, v in s.stored[2]]).float() + delta[lo:lo + 26]
+    assert torch.equal(tokens(2)[1], patched.to(BF))
