@@ -36,6 +36,7 @@ struct Params {
   int64_t num_blocks;
   float *part_o, *part_ml;  // [range][unit][2][kGroup][head_dim], [...][kGroup][2]
   int32_t *status;
+  float bias;        // l and O of the parts carry 2^bias
   float scale_log2;  // scale * log2(e): scores are kept in base 2
   int n_seqs, n_kv, heads, group, chunks, units, ranges;
   int hd, block_size, vec;
@@ -88,7 +89,7 @@ enum { kFirst = 1, kLast = 2, kFromStart = 4, kToEnd = 8 };
 struct Walk {
   int64_t x0, x1;  // the range
   int64_t at;      // line_pos of sequence b
-  int b, next;     // sequence, its first token's index in cu terms of b + 1
+  int b;           // sequence
   int i, end;      // tile start and end of the piece within the sequence
   uint32_t flags;
   bool live;
@@ -133,59 +134,123 @@ __device__ __forceinline__ void walk_next(const Params &p, Walk &w, int h0, int 
   walk_seq<T>(p, w, h0, n_h, lane);
 }
 
-// byte address of this lane's row (lanes 0-15: K of token i + lane, 16-31: V of token i + lane - 16), 0 if none
-__device__ __forceinline__ uint64_t row_address(const Params &p, const Walk &w, int u, int lane) {
-  const int i = w.i + (lane & 15);
-  if (i >= w.end) return 0;
-  const int blk = i / p.block_size, slot = i - blk * p.block_size;
-  const int64_t tlen = p.table_lens ? p.table_lens[w.b] : p.table_stride;
-  if (blk >= tlen) {
-    record_error(p.status, DKV_ERR_BLOCK_TABLE_SHORT);
-    return 0;
-  }
-  const int64_t id = p.tables[w.b * p.table_stride + blk];
-  if (id < 0 || id >= p.num_blocks) {
-    record_error(p.status, DKV_ERR_PAGE_RANGE);
-    return 0;
-  }
-  const char *a = lane < 16 ? p.k + id * p.k_block + slot * p.k_slot + u * p.k_head
-                            : p.v + id * p.v_block + slot * p.v_slot + u * p.v_head;
-  return reinterpret_cast<uint64_t>(a);
+// the walk of range r
+__device__ __forceinline__ Walk range_walk(const Params &p, const Line &ln, int r, int lane) {
+  Walk w;
+  w.x0 = range_start(ln, r), w.x1 = range_start(ln, r + 1);
+  w.b = seq_at(p, w.x0, lane);
+  w.at = line_pos(p, w.b);
+  return w;
 }
 
-// four consecutive elements of a shared-memory row as floats
-__device__ __forceinline__ float4 row4(const float *r) { return *reinterpret_cast<const float4 *>(r); }
-__device__ __forceinline__ float4 row4(const __half *r) {
-  const uint2 w = *reinterpret_cast<const uint2 *>(r);
-  return make_float4(f16lo(w.x), f16hi(w.x), f16lo(w.y), f16hi(w.y));
-}
-__device__ __forceinline__ float4 row4(const __nv_bfloat16 *r) {
-  const uint2 w = *reinterpret_cast<const uint2 *>(r);
-  return make_float4(bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y));
-}
+// One warp's stream of tiles into its ring of kStages shared-memory stages.  A stage holds 16
+// rows of K, then 16 rows of V, kRow bytes apart (16 more than a row: consecutive rows start 4
+// banks apart, so neither the fragment loads nor 16-byte reads of 8 rows conflict); lanes 0-15
+// look up the K rows, 16-31 the V rows.  The block ids of a tile are loaded one tile ahead and
+// first used when its copies are issued, so their latency passes behind a tile's arithmetic.
+template <typename T, int HD, int kStages>
+struct Stream {
+  static constexpr int kRow = HD * static_cast<int>(sizeof(T)) + 16;
+  static constexpr int kStage = 2 * kTile * kRow;
+  static constexpr int kBytes = kStages * (kStage + 16);
+  static constexpr int64_t kNoRow = -1, kShort = -(static_cast<int64_t>(1) << 40);  // no token; beyond the table row
+
+  const Params &p;
+  Walk w;
+  char *ring;
+  uint4 *meta;  // per stage: sequence, flags, bit per token that takes part, end of the stream
+  int u, h0, n_h, lane;
+  int64_t id;  // block of this lane's row of the next tile, or one of the above
+  int slot;
+
+  __device__ __forceinline__ Stream(const Params &p_, char *mine, int u_, int h0_, int n_h_, int lane_)
+      : p(p_), ring(mine), meta(reinterpret_cast<uint4 *>(mine + kStages * kStage)), u(u_), h0(h0_), n_h(n_h_),
+        lane(lane_), id(kNoRow), slot(0) {
+    if (p.hd < HD) {  // columns past head_dim stay zero in every stage: nothing writes them again
+      for (int i = lane; i < kStages * kStage / 16; i += 32)
+        reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+    }
+  }
+  __device__ __forceinline__ void look_up() {
+    id = kNoRow;
+    const int i = w.i + (lane & 15);
+    if (!w.live || i >= w.end) return;
+    const int blk = i / p.block_size;
+    slot = i - blk * p.block_size;
+    const int64_t tlen = p.table_lens ? p.table_lens[w.b] : p.table_stride;
+    id = blk < tlen ? p.tables[w.b * p.table_stride + blk] : kShort;
+  }
+  // the address of this lane's row, 0 if it takes no part
+  __device__ __forceinline__ uint64_t row_address() const {
+    const int i = w.i + (lane & 15);
+    if (i >= w.end) return 0;
+    if (id < 0 || id >= p.num_blocks) {
+      record_error(p.status, id == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
+      return 0;
+    }
+    const char *a = lane < 16 ? p.k + id * p.k_block + slot * p.k_slot + u * p.k_head
+                              : p.v + id * p.v_block + slot * p.v_slot + u * p.v_head;
+    return reinterpret_cast<uint64_t>(a);
+  }
+  __device__ __forceinline__ void start(const Walk &from) {
+    w = from;
+    walk_seq<T>(p, w, h0, n_h, lane);
+    look_up();
+  }
+  // issues the next tile's copies into stage s (one cp.async group, empty past the end)
+  __device__ __forceinline__ void fill(int s) {
+    if (w.live) {
+      const uint64_t addr = row_address();
+      const uint32_t there = __ballot_sync(0xffffffffu, addr != 0);
+      char *stage = ring + s * kStage;
+      if (p.vec) {
+        constexpr int kPieces = HD * static_cast<int>(sizeof(T)) / 16;  // 16-byte pieces of a row
+#pragma unroll
+        for (int c = lane; c < 32 * kPieces; c += 32) {
+          const int row = c / kPieces, piece = c % kPieces;
+          const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
+          if (piece * 16 < p.hd * static_cast<int>(sizeof(T)))
+            cp_async16(stage + row * kRow + piece * 16,
+                       a ? reinterpret_cast<const char *>(a) + piece * 16 : p.k, a ? 16 : 0);
+        }
+      } else {
+        for (int row = 0; row < 32; ++row) {
+          const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
+          T *dst = reinterpret_cast<T *>(stage + row * kRow);
+          for (int d = lane; d < p.hd; d += 32) dst[d] = a ? reinterpret_cast<const T *>(a)[d] : T(0.f);
+        }
+      }
+      const bool last = w.i + kTile >= w.end;
+      if (lane == 0) meta[s] = make_uint4(w.b, w.flags | (last ? kLast : 0), there & 0xffffu, 0);
+      walk_next<T>(p, w, h0, n_h, lane);
+      look_up();
+    } else if (lane == 0) {
+      meta[s] = make_uint4(0, 0, 0, 1);  // the end
+    }
+    cp_async_commit();
+  }
+};
 
 // ---------------------------------------------------------------------------------------
 // the walk with fp32 arithmetic on the ordinary pipes
 // ---------------------------------------------------------------------------------------
-// HD: head_dim rounded up (columns past head_dim are zero), G: query heads of the unit (rounded
-// up), W: warps per CTA.  Scores: lane = (token, half of the head); output: lane = 4 columns,
-// the tokens dealt to 128 / HD groups of lanes where the head is shorter than 128.
-template <int DT, int HD, int G, int W>
+// fp32 pages (the tensor cores round fp32 operands).  HD: head_dim rounded up (columns past
+// head_dim are zero), G: query heads of the unit (rounded up), W: warps per CTA.  Scores: lane =
+// (token, half of the head); output: lane = 4 columns, the tokens dealt to 128 / HD groups of
+// lanes where the head is shorter than 128.
+template <int HD, int G, int W>
 struct Simt {
-  using T = typename Elem<DT>::T;
-  static constexpr int kRow = HD * static_cast<int>(sizeof(T)) + 16;  // 16 B of padding: no bank conflicts
-  static constexpr int kStage = 2 * kTile * kRow;
-  static constexpr int kQRow = (HD + 8) * 4;  // two halves, 16 B apart in banks
-  static constexpr int kExtra = G * kQRow + kTile * G * 4;
   static constexpr int kStages = 3;
-  static constexpr int kWarpBytes = kStages * kStage + kStages * 16 + kExtra;
+  using S = Stream<float, HD, kStages>;
+  static constexpr int kQRow = (HD + 8) * 4;  // two halves, 16 B apart in banks
+  static constexpr int kWarpBytes = S::kBytes + G * kQRow + kTile * G * 4;
   static constexpr int kSmem = W * kWarpBytes;
 };
 
-template <int DT, int HD, int G, int W>
-__global__ void __launch_bounds__(W * 32) simt_kernel(Params p) {
-  using C = Simt<DT, HD, G, W>;
-  using T = typename C::T;
+template <int HD, int G, int W>
+__global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Params p) {
+  using C = Simt<HD, G, W>;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -197,50 +262,10 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(Params p) {
   const int n_h = min(G, p.group - chunk * G), h0 = u * p.group + chunk * G;
 
   char *mine = smem + warp * C::kWarpBytes;
-  uint4 *meta = reinterpret_cast<uint4 *>(mine + C::kStages * C::kStage);
-  float *qs = reinterpret_cast<float *>(mine + C::kStages * C::kStage + C::kStages * 16);
+  float *qs = reinterpret_cast<float *>(mine + C::S::kBytes);
   float *ps = qs + C::kQRow / 4 * G;
-  // columns past head_dim stay zero in every stage: nothing writes them again
-  for (int i = lane; i < C::kStages * C::kStage / 16; i += 32)
-    reinterpret_cast<uint4 *>(mine)[i] = make_uint4(0, 0, 0, 0);
-  __syncwarp();
-
-  Walk w;
-  w.x0 = range_start(ln, r), w.x1 = range_start(ln, r + 1);
-  w.b = seq_at(p, w.x0, lane);
-  w.at = line_pos(p, w.b);
-  walk_seq<T>(p, w, h0, n_h, lane);
-
-  constexpr int kChunks = HD * static_cast<int>(sizeof(T)) / 16;  // 16-byte pieces of a row
-  auto fill = [&](int s) {
-    if (w.live) {
-      const uint64_t addr = row_address(p, w, u, lane);
-      const uint32_t there = __ballot_sync(0xffffffffu, addr != 0);
-      char *stage = mine + s * C::kStage;
-      if (p.vec) {
-#pragma unroll 4
-        for (int c = lane; c < 32 * kChunks; c += 32) {
-          const int row = c / kChunks, piece = c % kChunks;
-          const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
-          if (piece * 16 < p.hd * static_cast<int>(sizeof(T)))
-            cp_async16(stage + row * C::kRow + piece * 16,
-                       a ? reinterpret_cast<const char *>(a) + piece * 16 : p.k, a ? 16 : 0);
-        }
-      } else {
-        for (int row = 0; row < 32; ++row) {
-          const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
-          T *dst = reinterpret_cast<T *>(stage + row * C::kRow);
-          for (int d = lane; d < p.hd; d += 32) dst[d] = a ? reinterpret_cast<const T *>(a)[d] : T(0.f);
-        }
-      }
-      const bool last = w.i + kTile >= w.end;
-      if (lane == 0) meta[s] = make_uint4(w.b, w.flags | (last ? kLast : 0), there & 0xffffu, 0);
-      walk_next<T>(p, w, h0, n_h, lane);
-    } else if (lane == 0) {
-      meta[s] = make_uint4(0, 0, 0, 1);  // the end
-    }
-    cp_async_commit();
-  };
+  typename C::S stream(p, mine, u, h0, n_h, lane);
+  stream.start(range_walk(p, ln, r, lane));
 
   constexpr int kVec = HD >= 128 ? HD / 128 : 1;         // float4 columns per lane
   constexpr int kLanes = HD >= 128 ? 32 : HD / 4;        // lanes per token in the output product
@@ -249,11 +274,11 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(Params p) {
   const int key = lane & 15, half = lane >> 4;
   const int oc = lane % kLanes, ok = lane / kLanes;
 
-  for (int s = 0; s < C::kStages; ++s) fill(s);
+  for (int s = 0; s < C::kStages; ++s) stream.fill(s);
   for (int s = 0;; s = s + 1 == C::kStages ? 0 : s + 1) {
     cp_async_wait<C::kStages - 1>();
     __syncwarp();
-    const uint4 mt = meta[s];
+    const uint4 mt = stream.meta[s];
     if (mt.w) break;
     const int b = mt.x;
     if (mt.y & kFirst) {
@@ -261,7 +286,7 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(Params p) {
         const int g = i / HD, d = i % HD;
         float x = 0.f;
         if (g < n_h && d < p.hd)
-          x = Elem<DT>::to_f(reinterpret_cast<const T *>(p.q + b * p.q_seq + (h0 + g) * p.q_head)[d]);
+          x = reinterpret_cast<const float *>(p.q + b * p.q_seq + (h0 + g) * p.q_head)[d];
         qs[g * (C::kQRow / 4) + d + (d >= HD / 2 ? 4 : 0)] = x;
       }
 #pragma unroll
@@ -274,13 +299,13 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(Params p) {
       }
       __syncwarp();
     }
-    const T *kr = reinterpret_cast<const T *>(mine + s * C::kStage + key * C::kRow) + half * (HD / 2);
+    const float *kr = reinterpret_cast<const float *>(mine + s * C::S::kStage + key * C::S::kRow) + half * (HD / 2);
     float acc[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[g] = 0.f;
 #pragma unroll 4
     for (int d = 0; d < HD / 2; d += 4) {
-      const float4 x = row4(kr + d);
+      const float4 x = *reinterpret_cast<const float4 *>(kr + d);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const float4 y = *reinterpret_cast<const float4 *>(qs + g * (C::kQRow / 4) + half * (HD / 2 + 4) + d);
@@ -310,13 +335,13 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(Params p) {
     __syncwarp();
 #pragma unroll 4
     for (int t = ok; t < kTile; t += kSplit) {
-      const T *vr = reinterpret_cast<const T *>(mine + s * C::kStage + (kTile + t) * C::kRow);
+      const float *vr = reinterpret_cast<const float *>(mine + s * C::S::kStage + (kTile + t) * C::S::kRow);
       float e[G];
 #pragma unroll
       for (int g = 0; g < G; ++g) e[g] = ps[t * G + g];
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        const float4 x = row4(vr + j * 128 + oc * 4);
+        const float4 x = *reinterpret_cast<const float4 *>(vr + j * 128 + oc * 4);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           o[g][j][0] = fmaf(e[g], x.x, o[g][j][0]);
@@ -344,12 +369,12 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(Params p) {
           const int h = h0 + g;
           if (whole) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + h * p.out_head);
+            float *dst = reinterpret_cast<float *>(p.out + b * p.out_seq + h * p.out_head);
 #pragma unroll
             for (int j = 0; j < kVec; ++j)
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                if (j * 128 + oc * 4 + i < p.hd) dst[j * 128 + oc * 4 + i] = Elem<DT>::from_f(o[g][j][i] * inv);
+                if (j * 128 + oc * 4 + i < p.hd) dst[j * 128 + oc * 4 + i] = o[g][j][i] * inv;
             if (p.lse && lane == 0)
               p.lse[static_cast<int64_t>(b) * p.heads + h] = (m[g] + log2f(sum)) * 0.6931471805599453f;
           } else {
@@ -368,7 +393,225 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(Params p) {
       }
     }
     __syncwarp();
-    fill(s);
+    stream.fill(s);
+  }
+  cp_async_wait<0>();
+}
+
+// ---------------------------------------------------------------------------------------
+// the walk with 16-bit pages on the tensor cores
+// ---------------------------------------------------------------------------------------
+// Transposed products, so that the query heads (few) are the narrow side n = 8 of
+// mma.m16n8k16 and nothing is wasted on padding a group of 1..8 heads to 16:
+//   S^T [16 tokens x 8 heads] = K [16 x 16 per step] . Q^T,  K fragments by ldmatrix,
+//   O^T [16 columns x 8 heads] += V^T . P^T [16 tokens x 8 heads], V^T by ldmatrix.trans.
+// P^T needs the tokens along the operand's k side where S^T has them along m: movmatrix
+// transposes each 8 x 8 block in registers.  A K or V element meets 8 multiply-adds a head
+// block: at the HBM rate of 12 elements a clock and SM that is 100 of the ~1000 a clock that
+// mma.sync can do, so the tensor cores are far from the bound and tcgen05's 128-row tiles
+// (16 times the padding, operands through tensor memory) would buy nothing.
+// Weights enter the product as two 16-bit terms (value and rest: 2^-17 relative for bf16) -
+// one term would add an error as large as the output's own rounding.  In f16 they are scaled by
+// 2^14, which l shares, so that weights down to 2^-28 of the largest keep all their bits.
+template <int DT>
+struct Half;
+template <>
+struct Half<DKV_BF16> {
+  static constexpr float kBias = 0.f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+  static __device__ __forceinline__ float lo(uint32_t w) { return bf16lo(w); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return bf16hi(w); }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma16816_bf16(c, a[0], a[1], a[2], a[3], b0, b1);
+  }
+};
+template <>
+struct Half<DKV_F16> {
+  static constexpr float kBias = 14.f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_f16x2(a, b); }
+  static __device__ __forceinline__ float lo(uint32_t w) { return f16lo(w); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return f16hi(w); }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma16816(c, a[0], a[1], a[2], a[3], b0, b1);
+  }
+};
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// N: blocks of 8 query heads of the unit
+template <int DT, int HD, int N, int W, int kStages_>
+struct Mma {
+  static constexpr int kStages = kStages_;
+  using T = typename Elem<DT>::T;
+  using S = Stream<T, HD, kStages>;
+  static constexpr int kSmem = W * S::kBytes;
+};
+
+template <int DT, int HD, int N, int W, int kStages>
+__global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ Params p) {
+  using C = Mma<DT, HD, N, W, kStages>;
+  using T = typename C::T;
+  using E = Half<DT>;
+  constexpr int kSteps = HD / 16;
+  const float kNegInf = __int_as_float(0xff800000);
+  extern __shared__ __align__(16) char smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int gw = blockIdx.x * W + warp;
+  const int r = gw / p.units, unit = gw - r * p.units;
+  const Line ln = line_of(p);
+  if (r >= ln.ranges) return;
+  const int u = unit / p.chunks, chunk = unit - u * p.chunks;
+  const int n_h = min(8 * N, p.group - chunk * 8 * N), h0 = u * p.group + chunk * 8 * N;
+
+  char *mine = smem + warp * C::S::kBytes;
+  typename C::S stream(p, mine, u, h0, n_h, lane);
+  stream.start(range_walk(p, ln, r, lane));
+
+  const int g = lane >> 2, t = lane & 3;
+  // ldmatrix rows: K as (token, k half), V as (token half, column half) of a 16 x 16 block
+  const uint32_t k_at = smem_u32(mine) + (lane & 15) * C::S::kRow + (lane >> 4) * 16;
+  const uint32_t v_at =
+      smem_u32(mine) + (kTile + (lane & 7) + (lane >> 4) * 8) * C::S::kRow + ((lane >> 3) & 1) * 16;
+  uint32_t qf[N][kSteps][2];
+  float o[N][kSteps][4], m[N][2], l[N][2];
+
+  for (int s = 0; s < kStages; ++s) stream.fill(s);
+  for (int s = 0;; s = s + 1 == kStages ? 0 : s + 1) {
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+    const uint4 mt = stream.meta[s];
+    if (mt.w) break;
+    const int b = mt.x;
+    if (mt.y & kFirst) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int h = n * 8 + g;
+        const unsigned short *qr =
+            reinterpret_cast<const unsigned short *>(p.q + b * p.q_seq + (h0 + min(h, n_h - 1)) * p.q_head);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int d = k * 16 + e * 8 + t * 2;
+            uint32_t w = d < p.hd ? qr[d] : 0;
+            w |= (d + 1 < p.hd ? static_cast<uint32_t>(qr[d + 1]) : 0u) << 16;
+            qf[n][k][e] = h < n_h ? w : 0;
+          }
+        m[n][0] = m[n][1] = kNegInf;
+        l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][k][e] = 0.f;
+      }
+    }
+    float sc[N][2][4];  // two chains over the head: even and odd steps
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[n][0][e] = sc[n][1][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      uint32_t a[4];
+      ldmatrix_x4(a[0], a[1], a[2], a[3], k_at + s * C::S::kStage + k * 32);
+#pragma unroll
+      for (int n = 0; n < N; ++n) E::mma(sc[n][k & 1], a, qf[n][k][0], qf[n][k][1]);
+    }
+    const bool in0 = (mt.z >> g) & 1, in1 = (mt.z >> (g + 8)) & 1;
+    uint32_t ph[N][2], pl[N][2];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      // sc: {token g, token g + 8} x {head 2t, head 2t + 1}
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[e] = (e < 2 ? in0 : in1) ? (sc[n][0][e] + sc[n][1][e]) * p.scale_log2 : kNegInf;
+      float keep[2];
+      bool moved = false;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float top = fmaxf(x[c], x[c + 2]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        top = fmaxf(top, m[n][c]);
+        moved |= top > m[n][c];
+        const float base = top == kNegInf ? 0.f : top;  // nothing seen yet: any finite base
+        keep[c] = exp2f(m[n][c] - base);
+        x[c] = exp2f(x[c] - base + E::kBias);
+        x[c + 2] = exp2f(x[c + 2] - base + E::kBias);
+        m[n][c] = top;
+        l[n][c] = fmaf(l[n][c], keep[c], x[c] + x[c + 2]);
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          o[n][k][0] *= keep[0], o[n][k][1] *= keep[1];
+          o[n][k][2] *= keep[0], o[n][k][3] *= keep[1];
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t w = E::pack(x[2 * c], x[2 * c + 1]);
+        ph[n][c] = transpose8x8(w);
+        pl[n][c] = transpose8x8(E::pack(x[2 * c] - E::lo(w), x[2 * c + 1] - E::hi(w)));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      uint32_t a[4];
+      ldmatrix_x4_trans(a[0], a[1], a[2], a[3], v_at + s * C::S::kStage + k * 32);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        E::mma(o[n][k], a, ph[n][0], ph[n][1]);
+        E::mma(o[n][k], a, pl[n][0], pl[n][1]);
+      }
+    }
+    if (mt.y & kLast) {
+      const bool whole = (mt.y & kFromStart) && (mt.y & kToEnd);
+      const int64_t part = (static_cast<int64_t>(r) * p.units + unit) * 2 + (mt.y & kFromStart ? 1 : 0);
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float sum = l[n][c];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int in = n * 8 + t * 2 + c, h = h0 + in;
+          if (in >= n_h) continue;
+          if (whole) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + h * p.out_head);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (k * 16 + e * 8 + g < p.hd)
+                  dst[k * 16 + e * 8 + g] = Elem<DT>::from_f(o[n][k][e * 2 + c] * inv);
+            if (p.lse && g == 0)
+              p.lse[static_cast<int64_t>(b) * p.heads + h] =
+                  (m[n][c] + (log2f(sum) - E::kBias)) * 0.6931471805599453f;
+          } else {
+            float *dst = p.part_o + (part * 8 * N + in) * p.hd;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (k * 16 + e * 8 + g < p.hd) dst[k * 16 + e * 8 + g] = o[n][k][e * 2 + c];
+            if (g == 0) {
+              p.part_ml[(part * 8 * N + in) * 2] = m[n][c];
+              p.part_ml[(part * 8 * N + in) * 2 + 1] = sum;
+            }
+          }
+        }
+    }
+    __syncwarp();
+    stream.fill(s);
   }
   cp_async_wait<0>();
 }
@@ -472,7 +715,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(Params p, int g_u
     dst[d] = Elem<DT>::from_f(x * inv);
   }
   if (p.lse && threadIdx.x == 0)
-    p.lse[static_cast<int64_t>(b) * p.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
+    p.lse[static_cast<int64_t>(b) * p.heads + h] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -523,8 +766,13 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   if (rc != DKV_OK) return rc;
   const int hd = a->k_pages.head_dim, group = a->n_q_heads / a->k_pages.n_heads;
   s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-  s->g = group <= 4 ? 4 : 8;
-  s->warps = s->hd_pad == 256 ? 2 : 4;
+  if (a->k_pages.dtype == DKV_F32) {
+    s->g = group <= 4 ? 4 : 8;
+    s->warps = s->hd_pad == 256 ? 2 : 4;
+  } else {
+    s->g = group <= 8 ? 8 : 16;
+    s->warps = s->hd_pad == 256 ? 4 : 8;
+  }
   s->chunks = (group + s->g - 1) / s->g;
   s->units = a->k_pages.n_heads * s->chunks;
   const int64_t most = static_cast<int64_t>(sms) * s->warps / s->units;
@@ -537,32 +785,56 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   return DKV_OK;
 }
 
-template <int DT, int HD, int G, int W>
+template <int HD, int G, int W>
 int launch_simt(const Params &p, int grid, cudaStream_t st) {
-  using C = Simt<DT, HD, G, W>;
+  using C = Simt<HD, G, W>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
-  DKV_CUDA_CHECK(cudaFuncSetAttribute(simt_kernel<DT, HD, G, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  simt_kernel<DT, HD, G, W><<<grid, W * 32, C::kSmem, st>>>(p);
+  DKV_CUDA_CHECK(cudaFuncSetAttribute(simt_kernel<HD, G, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  simt_kernel<HD, G, W><<<grid, W * 32, C::kSmem, st>>>(p);
+  DKV_CUDA_CHECK(cudaGetLastError());
+  return DKV_OK;
+}
+
+template <int DT, int HD, int N, int W, int kStages>
+int launch_mma(const Params &p, int grid, cudaStream_t st) {
+  using C = Mma<DT, HD, N, W, kStages>;
+  static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
+  DKV_CUDA_CHECK(cudaFuncSetAttribute(mma_kernel<DT, HD, N, W, kStages>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      C::kSmem));
+  mma_kernel<DT, HD, N, W, kStages><<<grid, W * 32, C::kSmem, st>>>(p);
   DKV_CUDA_CHECK(cudaGetLastError());
   return DKV_OK;
 }
 
 template <int DT>
+int launch_walk(const Params &p, const Shape &s, int grid, cudaStream_t st) {
+#define DKV_MMA_CASE(HD, W, S)                                                    \
+  if (s.hd_pad == HD && s.g == 8) return launch_mma<DT, HD, 1, W, S>(p, grid, st); \
+  if (s.hd_pad == HD && s.g == 16) return launch_mma<DT, HD, 2, W, S>(p, grid, st);
+  DKV_MMA_CASE(32, 8, 8)
+  DKV_MMA_CASE(64, 8, 6)
+  DKV_MMA_CASE(128, 8, 3)
+  DKV_MMA_CASE(256, 4, 3)
+#undef DKV_MMA_CASE
+  return DKV_ERR_UNSUPPORTED;
+}
+template <>
+int launch_walk<DKV_F32>(const Params &p, const Shape &s, int grid, cudaStream_t st) {
+#define DKV_SIMT_CASE(HD, W)                                                 \
+  if (s.hd_pad == HD && s.g == 4) return launch_simt<HD, 4, W>(p, grid, st); \
+  if (s.hd_pad == HD && s.g == 8) return launch_simt<HD, 8, W>(p, grid, st);
+  DKV_SIMT_CASE(32, 4)
+  DKV_SIMT_CASE(64, 4)
+  DKV_SIMT_CASE(128, 4)
+  DKV_SIMT_CASE(256, 2)
+#undef DKV_SIMT_CASE
+  return DKV_ERR_UNSUPPORTED;
+}
+
+template <int DT>
 int launch(const Params &p, const Shape &s, cudaStream_t st) {
   const int64_t warps = static_cast<int64_t>(s.ranges) * s.units;
-  const int grid = static_cast<int>((warps + s.warps - 1) / s.warps);
-  int rc = DKV_ERR_UNSUPPORTED;
-#define DKV_SIMT_CASE(HD, G, W) \
-  if (s.hd_pad == HD && s.g == G && s.warps == W) rc = launch_simt<DT, HD, G, W>(p, grid, st);
-  DKV_SIMT_CASE(32, 4, 4)
-  DKV_SIMT_CASE(32, 8, 4)
-  DKV_SIMT_CASE(64, 4, 4)
-  DKV_SIMT_CASE(64, 8, 4)
-  DKV_SIMT_CASE(128, 4, 4)
-  DKV_SIMT_CASE(128, 8, 4)
-  DKV_SIMT_CASE(256, 4, 2)
-  DKV_SIMT_CASE(256, 8, 2)
-#undef DKV_SIMT_CASE
+  const int rc = launch_walk<DT>(p, s, static_cast<int>((warps + s.warps - 1) / s.warps), st);
   if (rc != DKV_OK || s.ranges == 1) return rc;
   // the join starts as soon as every CTA of the walk is under way and waits in the kernel for its end
   cudaLaunchConfig_t cfg = {};
@@ -624,6 +896,7 @@ extern "C" int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv
   p.part_o = static_cast<float *>(a.workspace);
   p.part_ml = s.parts ? p.part_o + s.o_bytes / 4 : nullptr;
   p.status = a.status;
+  p.bias = k.dtype == DKV_F16 ? pattn::Half<DKV_F16>::kBias : 0.f;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.n_seqs = a.seqs.n_seqs, p.n_kv = k.n_heads, p.heads = a.n_q_heads, p.group = a.n_q_heads / k.n_heads;
   p.chunks = s.chunks, p.units = s.units, p.ranges = s.ranges;
