@@ -43,43 +43,65 @@ struct Params {
 };
 
 // ---------------------------------------------------------------------------------------
-// the line of tokens and its ranges
+// the line of tokens and its ranges (at most 2^31 tokens and 2^16 sequences: 32 bits hold it)
 // ---------------------------------------------------------------------------------------
 struct Line {
-  int64_t total;  // virtual tokens
-  int ranges;     // in use
+  uint32_t total;  // virtual tokens
+  uint32_t ranges; // in use
+  uint32_t each, more;  // range r has each tokens, the first `more` ranges one more
+  __device__ __forceinline__ uint32_t start(uint32_t r) const { return r * each + min(r, more); }
+  __device__ __forceinline__ uint32_t owner(uint32_t x) const {  // the range of token x < total
+    const uint32_t big = more * (each + 1);
+    return x < big ? x / (each + 1) : more + (x - big) / each;
+  }
 };
-__device__ __forceinline__ int64_t line_pos(const Params &p, int b) {
-  return static_cast<int64_t>(p.cu[b]) + static_cast<int64_t>(kSeqCost) * b;
-}
-__device__ __forceinline__ Line line_of(const Params &p) {
+__device__ __forceinline__ Line line_of(uint32_t tokens, int n_seqs, int most) {
   Line ln;
-  ln.total = line_pos(p, p.n_seqs);
-  const int64_t most = ln.total / kMinRange;
-  ln.ranges = most < 1 ? 1 : (most < p.ranges ? static_cast<int>(most) : p.ranges);
+  ln.total = tokens + static_cast<uint32_t>(kSeqCost) * n_seqs;
+  ln.ranges = min(max(ln.total / kMinRange, 1u), static_cast<uint32_t>(most));
+  ln.each = ln.total / ln.ranges;
+  ln.more = ln.total - ln.each * ln.ranges;
   return ln;
 }
-__device__ __forceinline__ int64_t range_start(const Line &ln, int r) { return r * ln.total / ln.ranges; }
 // the token of sequence [at, at + len) that a range border at x falls on: a multiple of the tile
-__device__ __forceinline__ int border(int64_t x, int64_t at, int len) {
+__device__ __forceinline__ int border(uint32_t x, uint32_t at, int len) {
   if (x <= at) return 0;
-  if (x >= at + len + kSeqCost) return len;
-  const int i = static_cast<int>(x - at) & ~(kTile - 1);
-  return i < len ? i : len;
+  if (x - at >= static_cast<uint32_t>(len) + kSeqCost) return len;
+  return min(static_cast<int>(x - at) & ~(kTile - 1), len);
 }
-// largest b with line_pos(b) <= x, 32 candidates a step (whole warp)
-__device__ __forceinline__ int seq_at(const Params &p, int64_t x, int lane) {
-  int lo = 0, hi = p.n_seqs;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32;
-    const int b = lo + lane * step;
-    const bool in = b < hi && line_pos(p, b) <= x;
-    const int k = __popc(__ballot_sync(0xffffffffu, in));
-    if (k > 1) lo += (k - 1) * step;
-    hi = min(hi, lo + step);
+
+// cu_seqlens and table lengths of 32 consecutive sequences in a warp's registers, so that
+// walking from one sequence to the next waits for memory once in 31 sequences
+struct Window {
+  int base;  // lane i holds cu[base + i] and the table length of sequence base + i
+  int cu, tlen;
+  __device__ __forceinline__ void load(const Params &p, int b, int lane) {
+    base = b;
+    const int at = b + lane;
+    cu = p.cu[min(at, p.n_seqs)];
+    tlen = p.table_lens ? p.table_lens[min(at, p.n_seqs - 1)] : 0;
   }
-  return lo;
-}
+  __device__ __forceinline__ void need(const Params &p, int b, int lane) {
+    if (b - base > 30) load(p, b, lane);
+  }
+  __device__ __forceinline__ int at(int b) const { return __shfl_sync(0xffffffffu, cu, b - base); }
+  __device__ __forceinline__ int table_len(int b) const { return __shfl_sync(0xffffffffu, tlen, b - base); }
+  // the largest b with cu[b] + kSeqCost b <= x, and a window that starts at or before it
+  __device__ __forceinline__ int find(const Params &p, uint32_t x, int lane) {
+    int lo = 0, hi = p.n_seqs;
+    while (hi - lo > 31) {
+      const int step = (hi - lo + 31) / 32;
+      const int b = lo + lane * step;
+      const bool in = b < hi && static_cast<uint32_t>(p.cu[b]) + static_cast<uint32_t>(kSeqCost) * b <= x;
+      const int k = __popc(__ballot_sync(0xffffffffu, in));
+      if (k > 1) lo += (k - 1) * step;
+      hi = min(hi, lo + step);
+    }
+    load(p, lo, lane);
+    const bool in = lo + lane < hi && static_cast<uint32_t>(cu) + static_cast<uint32_t>(kSeqCost) * (lo + lane) <= x;
+    return lo + max(__popc(__ballot_sync(0xffffffffu, in)) - 1, 0);
+  }
+};
 
 // ---------------------------------------------------------------------------------------
 // a warp's walk over its range: one kTile-token tile after the other
@@ -87,10 +109,11 @@ __device__ __forceinline__ int seq_at(const Params &p, int64_t x, int lane) {
 enum { kFirst = 1, kLast = 2, kFromStart = 4, kToEnd = 8 };
 
 struct Walk {
-  int64_t x0, x1;  // the range
-  int64_t at;      // line_pos of sequence b
-  int b;           // sequence
-  int i, end;      // tile start and end of the piece within the sequence
+  Window win;
+  uint32_t x0, x1;  // the range
+  int b;            // sequence
+  int i, end;       // tile start and end of the piece within the sequence
+  int64_t tlen;     // valid entries of its table row
   uint32_t flags;
   bool live;
 };
@@ -109,19 +132,21 @@ __device__ __forceinline__ void write_empty(const Params &p, int b, int h0, int 
 template <typename T>
 __device__ __forceinline__ void walk_seq(const Params &p, Walk &w, int h0, int n_h, int lane) {
   w.live = false;
-  while (w.b < p.n_seqs && w.at < w.x1) {
-    const int start = p.cu[w.b];
-    const int len = max(p.cu[w.b + 1] - start, 0);
-    const int i0 = border(w.x0, w.at, len), i1 = border(w.x1, w.at, len);
+  for (; w.b < p.n_seqs; ++w.b) {
+    w.win.need(p, w.b, lane);
+    const int first = w.win.at(w.b);
+    const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * w.b;
+    if (at >= w.x1) return;
+    const int len = max(w.win.at(w.b + 1) - first, 0);
+    const int i0 = border(w.x0, at, len), i1 = border(w.x1, at, len);
     if (i1 > i0) {
       w.i = i0, w.end = i1;
       w.flags = kFirst | (i0 == 0 ? kFromStart : 0) | (i1 == len ? kToEnd : 0);
+      w.tlen = p.table_lens ? w.win.table_len(w.b) : p.table_stride;
       w.live = true;
       return;
     }
-    if (len == 0 && w.at >= w.x0) write_empty<T>(p, w.b, h0, n_h, lane);
-    ++w.b;
-    w.at += len + kSeqCost;
+    if (len == 0 && at >= w.x0) write_empty<T>(p, w.b, h0, n_h, lane);
   }
 }
 template <typename T>
@@ -129,17 +154,14 @@ __device__ __forceinline__ void walk_next(const Params &p, Walk &w, int h0, int 
   w.i += kTile;
   w.flags &= ~kFirst;
   if (w.i < w.end) return;
-  w.at = line_pos(p, w.b + 1);
   ++w.b;
   walk_seq<T>(p, w, h0, n_h, lane);
 }
-
 // the walk of range r
-__device__ __forceinline__ Walk range_walk(const Params &p, const Line &ln, int r, int lane) {
+__device__ __forceinline__ Walk range_walk(const Params &p, const Line &ln, uint32_t r, int lane) {
   Walk w;
-  w.x0 = range_start(ln, r), w.x1 = range_start(ln, r + 1);
-  w.b = seq_at(p, w.x0, lane);
-  w.at = line_pos(p, w.b);
+  w.x0 = ln.start(r), w.x1 = ln.start(r + 1);
+  w.b = w.win.find(p, w.x0, lane);
   return w;
 }
 
@@ -178,8 +200,7 @@ struct Stream {
     if (!w.live || i >= w.end) return;
     const int blk = i / p.block_size;
     slot = i - blk * p.block_size;
-    const int64_t tlen = p.table_lens ? p.table_lens[w.b] : p.table_stride;
-    id = blk < tlen ? p.tables[w.b * p.table_stride + blk] : kShort;
+    id = blk < w.tlen ? p.tables[w.b * p.table_stride + blk] : kShort;
   }
   // the address of this lane's row, 0 if it takes no part
   __device__ __forceinline__ uint64_t row_address() const {
@@ -256,8 +277,8 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
   asm volatile("griddepcontrol.launch_dependents;");
   const int gw = blockIdx.x * W + warp;
   const int r = gw / p.units, unit = gw - r * p.units;
-  const Line ln = line_of(p);
-  if (r >= ln.ranges) return;
+  const Line ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
+  if (r >= static_cast<int>(ln.ranges)) return;
   const int u = unit / p.chunks, chunk = unit - u * p.chunks;
   const int n_h = min(G, p.group - chunk * G), h0 = u * p.group + chunk * G;
 
@@ -462,8 +483,8 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
   asm volatile("griddepcontrol.launch_dependents;");
   const int gw = blockIdx.x * W + warp;
   const int r = gw / p.units, unit = gw - r * p.units;
-  const Line ln = line_of(p);
-  if (r >= ln.ranges) return;
+  const Line ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
+  if (r >= static_cast<int>(ln.ranges)) return;
   const int u = unit / p.chunks, chunk = unit - u * p.chunks;
   const int n_h = min(8 * N, p.group - chunk * 8 * N), h0 = u * p.group + chunk * 8 * N;
 
@@ -619,102 +640,113 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
 // ---------------------------------------------------------------------------------------
 // join of the parts
 // ---------------------------------------------------------------------------------------
-constexpr int kJoinWarps = 8;
+constexpr int kJoinThreads = 256;
+constexpr int kMaxRanges = 2048;
 
 // One CTA per (cut sequence, query head).  blockIdx.x is a sequence where by_seq, else a range
-// border (at most ranges - 1 sequences are cut); warps take every kJoinWarps-th part.
-template <int DT>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(Params p, int g_unit, int by_seq) {
+// border (at most ranges - 1 sequences are cut).  Which parts there are follows from the lengths
+// alone and is worked out before the walk's end is waited for; then a thread per part forms its
+// weight, and VW columns a thread are summed over the parts, kJoinThreads / (head_dim / VW) parts
+// at a time, with the loads of several parts in flight (one at a time cost 1.5 us each: 38 us
+// for the 148 parts of one long sequence).
+template <int DT, int VW>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int g_unit, int by_seq) {
   using T = typename Elem<DT>::T;
-  __shared__ float red[kJoinWarps][256];
-  __shared__ float red_l[kJoinWarps], red_m[kJoinWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Line ln = line_of(p);
+  __shared__ int part[kMaxRanges];
+  __shared__ float weight[kMaxRanges];
+  __shared__ float red[kJoinThreads * VW];
+  __shared__ float red_m[kJoinThreads / 32], red_l[kJoinThreads / 32];
+  const float kNegInf = __int_as_float(0xff800000);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Line ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
   const int h = blockIdx.y;
-  int b, r0;
+  int b = blockIdx.x, first, next;
   if (by_seq) {
-    b = blockIdx.x;
-    const int64_t at = line_pos(p, b);
-    r0 = static_cast<int>(at * ln.ranges / ln.total);
-    while (r0 > 0 && range_start(ln, r0) > at) --r0;
-    while (r0 + 1 < ln.ranges && range_start(ln, r0 + 1) <= at) ++r0;
+    first = p.cu[b], next = p.cu[b + 1];
   } else {
-    const int rb = blockIdx.x + 1;
+    const uint32_t rb = blockIdx.x + 1;
     if (rb >= ln.ranges) return;
-    const int64_t x = range_start(ln, rb);
-    b = seq_at(p, x, lane);
-    const int64_t at = line_pos(p, b);
-    r0 = rb - 1;
-    if (r0 > 0 && range_start(ln, r0) >= at) return;  // an earlier border has this sequence
+    Window win;
+    b = win.find(p, ln.start(rb), lane);
+    win.need(p, b, lane);
+    first = win.at(b), next = win.at(b + 1);
+    const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
+    if (rb > 1 && ln.start(rb - 1) >= at) return;  // an earlier border has this sequence
   }
-  const int64_t at = line_pos(p, b);
-  const int len = max(p.cu[b + 1] - p.cu[b], 0);
+  const int len = max(next - first, 0);
+  const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
   if (len == 0) return;
-  int r1 = r0;  // last range with a part of the sequence
-  {
-    const int64_t tail = at + len + kSeqCost - 1;
-    r1 = static_cast<int>(tail * ln.ranges / ln.total);
-    r1 = min(r1, ln.ranges - 1);
-    while (r1 > 0 && range_start(ln, r1) > tail) --r1;
-    while (r1 + 1 < ln.ranges && range_start(ln, r1 + 1) <= tail) ++r1;
-  }
+  const uint32_t r0 = ln.owner(at), r1 = ln.owner(at + len + kSeqCost - 1);
   if (r1 == r0) return;  // not cut
+  const int n = r1 - r0 + 1;
   const int u = h / p.group, in = h - u * p.group;
   const int unit = u * p.chunks + in / g_unit, g = in % g_unit;
-  auto part_of = [&](int r, bool &some, bool &all) {
-    const int i0 = border(range_start(ln, r), at, len), i1 = border(range_start(ln, r + 1), at, len);
-    some = i1 > i0;
-    all = i0 == 0 && i1 == len;
-    return ((static_cast<int64_t>(r) * p.units + unit) * 2 + (i0 == 0 ? 1 : 0)) * g_unit + g;
-  };
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  float top = __int_as_float(0xff800000);
-  int done = 0;
-  for (int r = r0 + threadIdx.x; r <= r1; r += kJoinWarps * 32) {
-    bool some, all;
-    const int64_t i = part_of(r, some, all);
-    done |= all;
-    if (some && !all) top = fmaxf(top, p.part_ml[i * 2]);
+  bool done = false;
+  for (int i = tid; i < n; i += kJoinThreads) {
+    const uint32_t r = r0 + i;
+    const int i0 = border(ln.start(r), at, len), i1 = border(ln.start(r + 1), at, len);
+    done |= i0 == 0 && i1 == len;
+    part[i] = i1 > i0 ? ((static_cast<int>(r) * p.units + unit) * 2 + (i0 == 0 ? 1 : 0)) * g_unit + g : -1;
   }
   if (__syncthreads_or(done)) return;  // all its tokens fell into one range: already written
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float top = kNegInf;
+  for (int i = tid; i < n; i += kJoinThreads) {
+    const float m = part[i] >= 0 ? p.part_ml[2 * static_cast<int64_t>(part[i])] : kNegInf;
+    weight[i] = m;
+    top = fmaxf(top, m);
+  }
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
   if (lane == 0) red_m[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, red_m[i]);
-  const float base = top == __int_as_float(0xff800000) ? 0.f : top;
-  float acc[8], sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-  for (int r = r0 + warp; r <= r1; r += kJoinWarps) {
-    bool some, all;
-    const int64_t i = part_of(r, some, all);
-    if (!some) continue;
-    const float e = exp2f(p.part_ml[i * 2] - base);
-    sum = fmaf(p.part_ml[i * 2 + 1], e, sum);
-    const float *src = p.part_o + i * p.hd;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j * 32 + lane < p.hd) acc[j] = fmaf(src[j * 32 + lane], e, acc[j]);
+  for (int i = 0; i < kJoinThreads / 32; ++i) top = fmaxf(top, red_m[i]);
+  const float base = top == kNegInf ? 0.f : top;
+  float sum = 0.f;
+  for (int i = tid; i < n; i += kJoinThreads) {
+    const float e = exp2f(weight[i] - base);
+    weight[i] = e;
+    if (part[i] >= 0) sum = fmaf(p.part_ml[2 * static_cast<int64_t>(part[i]) + 1], e, sum);
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j * 32 + lane < p.hd) red[warp][j * 32 + lane] = acc[j];
+  for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
   if (lane == 0) red_l[warp] = sum;
+  __syncthreads();
+  const int cols = p.hd / VW, groups = kJoinThreads / cols;
+  const int c = tid % cols, pg = tid / cols;
+  float acc[VW];
+#pragma unroll
+  for (int e = 0; e < VW; ++e) acc[e] = 0.f;
+  if (pg < groups) {
+#pragma unroll 8
+    for (int i = pg; i < n; i += groups) {
+      if (part[i] < 0) continue;
+      const float *src = p.part_o + static_cast<int64_t>(part[i]) * p.hd + c * VW;
+      const float w = weight[i];
+      if constexpr (VW == 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(src);
+        acc[0] = fmaf(x.x, w, acc[0]), acc[1] = fmaf(x.y, w, acc[1]);
+        acc[2] = fmaf(x.z, w, acc[2]), acc[3] = fmaf(x.w, w, acc[3]);
+      } else {
+        acc[0] = fmaf(src[0], w, acc[0]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < VW; ++e) red[(pg * cols + c) * VW + e] = acc[e];
+  }
   __syncthreads();
   float total = 0.f;
 #pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) total += red_l[i];
+  for (int i = 0; i < kJoinThreads / 32; ++i) total += red_l[i];
   const float inv = total == 0.f ? 0.f : 1.f / total;
   T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + h * p.out_head);
-  for (int d = threadIdx.x; d < p.hd; d += kJoinWarps * 32) {
+  if (tid < p.hd) {
     float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < kJoinWarps; ++i) x += red[i][d];
-    dst[d] = Elem<DT>::from_f(x * inv);
+    for (int i = 0; i < groups; ++i) x += red[i * p.hd + tid];
+    dst[tid] = Elem<DT>::from_f(x * inv);
   }
-  if (p.lse && threadIdx.x == 0)
+  if (p.lse && tid == 0)
     p.lse[static_cast<int64_t>(b) * p.heads + h] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
 }
 
@@ -779,9 +811,23 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   const int64_t line = static_cast<int64_t>(a->seqs.n_seqs) * (static_cast<int64_t>(a->seqs.max_seq_len) + kSeqCost);
   const int64_t want = line / kMinRange;
   s->ranges = static_cast<int>(most < 1 || want < 1 ? 1 : (want < most ? want : most));
+  if (s->ranges > kMaxRanges) s->ranges = kMaxRanges;
   s->parts = s->ranges > 1 ? static_cast<int64_t>(s->ranges) * s->units * 2 * s->g : 0;
   s->o_bytes = (s->parts * hd * 4 + 15) / 16 * 16;
   s->bytes = s->o_bytes + s->parts * 8;
+  return DKV_OK;
+}
+
+// raises a kernel's shared-memory limit once per device
+template <auto kKernel>
+int allow_smem(int bytes) {
+  static unsigned long long done = 0;  // a bit per device; a race only sets the same value twice
+  int dev = 0;
+  DKV_CUDA_CHECK(cudaGetDevice(&dev));
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (__atomic_load_n(&done, __ATOMIC_RELAXED) & bit)) return DKV_OK;
+  DKV_CUDA_CHECK(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
   return DKV_OK;
 }
 
@@ -789,7 +835,8 @@ template <int HD, int G, int W>
 int launch_simt(const Params &p, int grid, cudaStream_t st) {
   using C = Simt<HD, G, W>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
-  DKV_CUDA_CHECK(cudaFuncSetAttribute(simt_kernel<HD, G, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  const int rc = allow_smem<simt_kernel<HD, G, W>>(C::kSmem);
+  if (rc != DKV_OK) return rc;
   simt_kernel<HD, G, W><<<grid, W * 32, C::kSmem, st>>>(p);
   DKV_CUDA_CHECK(cudaGetLastError());
   return DKV_OK;
@@ -799,8 +846,8 @@ template <int DT, int HD, int N, int W, int kStages>
 int launch_mma(const Params &p, int grid, cudaStream_t st) {
   using C = Mma<DT, HD, N, W, kStages>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
-  DKV_CUDA_CHECK(cudaFuncSetAttribute(mma_kernel<DT, HD, N, W, kStages>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      C::kSmem));
+  const int rc = allow_smem<mma_kernel<DT, HD, N, W, kStages>>(C::kSmem);
+  if (rc != DKV_OK) return rc;
   mma_kernel<DT, HD, N, W, kStages><<<grid, W * 32, C::kSmem, st>>>(p);
   DKV_CUDA_CHECK(cudaGetLastError());
   return DKV_OK;
@@ -843,11 +890,14 @@ int launch(const Params &p, const Shape &s, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   const int by_seq = p.n_seqs <= s.ranges - 1;
   cfg.gridDim = dim3(by_seq ? p.n_seqs : s.ranges - 1, p.heads);
-  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  DKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<DT>, p, s.g, by_seq));
+  if (p.hd % 4 == 0)
+    DKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<DT, 4>, p, s.g, by_seq));
+  else
+    DKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<DT, 1>, p, s.g, by_seq));
   return DKV_OK;
 }
 

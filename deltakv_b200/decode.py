@@ -31,7 +31,8 @@ from deltakv_b200.rope import half_tables
 
 def _same_device(where: str, first: Tensor, *rest: Tensor | None) -> torch.device:
     dev = first.device
-    ops._require_cuda(first)
+    if not first.is_cuda:
+        ops._require_cuda(first)
     for t in rest:
         if t is not None and t.device != dev:
             if not t.is_cuda:
@@ -42,11 +43,13 @@ def _same_device(where: str, first: Tensor, *rest: Tensor | None) -> torch.devic
 
 def _call(fn, args, dev: torch.device, where: str) -> None:
     """Launch on the current stream of ``dev``, which need not be the current device."""
+    # the raw handle: current_stream() builds a Stream object, 3 us of a 15 us call
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
     if dev.index == torch.cuda.current_device():
-        rc = fn(C.byref(args), torch.cuda.current_stream().cuda_stream)
+        rc = fn(C.byref(args), stream)
     else:
         with torch.cuda.device(dev):
-            rc = fn(C.byref(args), torch.cuda.current_stream().cuda_stream)
+            rc = fn(C.byref(args), stream)
     if rc != L.DKV_OK:
         raise L.DkvError(rc, where)
 
@@ -104,7 +107,7 @@ def plan_paged_step(lengths: Tensor, block_tables: Tensor, block_size: int, *, r
         raise ValueError("block_size must be positive, rows and max_seq_len not negative")
     dev = _same_device("plan_paged_step", lengths, block_tables, new_lengths, table_lens, free_blocks)
     out = torch.empty(3 * n + 3 + rows, dtype=torch.int32, device=dev)
-    cu, cu_new, lens, used, positions = out.split((n + 1, n + 1, n, 1, rows))
+    cu, cu_new, lens, used, positions = torch.unsafe_split_with_sizes(out, (n + 1, n + 1, n, 1, rows))
     slots = torch.empty(rows, dtype=torch.int64, device=dev)
     st = ops.status_word(dev)
     base = out.data_ptr()
