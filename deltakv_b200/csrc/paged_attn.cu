@@ -20,7 +20,10 @@ namespace dkv {
 namespace pattn {
 
 constexpr int kTile = 16;      // tokens per pipeline stage of a warp
-constexpr int kSeqCost = 16;   // virtual tokens per sequence: the cost of starting one
+// Virtual tokens per sequence: what starting and finishing one costs a warp.  Walk of 256 sequences
+// of 1..600 tokens at 16 / 32 / 48 / 64 / 96: 38 / 34 / 31 / 34 / 39 us; of 64 of 1..8192:
+// 73 / 61 / 59 / 60 / 61 us; long sequences do not notice.
+constexpr int kSeqCost = 48;
 constexpr int kMinRange = 32;  // tokens below which a range is not cut further
 
 struct Params {
@@ -39,7 +42,9 @@ struct Params {
   float bias;        // l and O of the parts carry 2^bias
   float scale_log2;  // scale * log2(e): scores are kept in base 2
   int n_seqs, n_kv, heads, group, chunks, units, ranges;
-  int hd, block_size, vec;
+  int hd, block_size;
+  int vec;    // rows of K and V in whole 16-byte pieces
+  int pairs;  // rows of q and out in whole pairs of 16-bit elements
 };
 
 // ---------------------------------------------------------------------------------------
@@ -518,8 +523,13 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int d = k * 16 + e * 8 + t * 2;
-            uint32_t w = d < p.hd ? qr[d] : 0;
-            w |= (d + 1 < p.hd ? static_cast<uint32_t>(qr[d + 1]) : 0u) << 16;
+            uint32_t w = 0;
+            if (p.pairs) {
+              if (d < p.hd) w = *reinterpret_cast<const uint32_t *>(qr + d);
+            } else {
+              if (d < p.hd) w = qr[d];
+              if (d + 1 < p.hd) w |= static_cast<uint32_t>(qr[d + 1]) << 16;
+            }
             qf[n][k][e] = h < n_h ? w : 0;
           }
         m[n][0] = m[n][1] = kNegInf;
@@ -596,28 +606,46 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
       const bool whole = (mt.y & kFromStart) && (mt.y & kToEnd);
       const int64_t part = (static_cast<int64_t>(r) * p.units + unit) * 2 + (mt.y & kFromStart ? 1 : 0);
 #pragma unroll
-      for (int n = 0; n < N; ++n)
+      for (int n = 0; n < N; ++n) {
+        float sum[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float sum = l[n][c];
-          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-          const int in = n * 8 + t * 2 + c, h = h0 + in;
-          if (in >= n_h) continue;
-          if (whole) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + h * p.out_head);
+          sum[c] = l[n][c];
+          sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], 4);
+          sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], 8);
+          sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], 16);
+        }
+        if (whole) {
+          // heads to rows, so that a lane stores two neighbouring columns of one head
+          const float inv0 = sum[0] == 0.f ? 0.f : 1.f / sum[0], inv1 = sum[1] == 0.f ? 0.f : 1.f / sum[1];
+          const int in = n * 8 + g;
+          T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + (h0 + in) * p.out_head);
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k)
+          for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (k * 16 + e * 8 + g < p.hd)
-                  dst[k * 16 + e * 8 + g] = Elem<DT>::from_f(o[n][k][e * 2 + c] * inv);
-            if (p.lse && g == 0)
-              p.lse[static_cast<int64_t>(b) * p.heads + h] =
-                  (m[n][c] + (log2f(sum) - E::kBias)) * 0.6931471805599453f;
-          } else {
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t w = transpose8x8(E::pack(o[n][k][e * 2] * inv0, o[n][k][e * 2 + 1] * inv1));
+              const int d = k * 16 + e * 8 + t * 2;
+              if (in < n_h) {
+                if (p.pairs) {
+                  if (d < p.hd) *reinterpret_cast<uint32_t *>(dst + d) = w;
+                } else {
+                  unsigned short *two = reinterpret_cast<unsigned short *>(dst + d);
+                  if (d < p.hd) two[0] = static_cast<unsigned short>(w);
+                  if (d + 1 < p.hd) two[1] = static_cast<unsigned short>(w >> 16);
+                }
+              }
+            }
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            if (p.lse && g == 0 && n * 8 + t * 2 + c < n_h)
+              p.lse[static_cast<int64_t>(b) * p.heads + h0 + n * 8 + t * 2 + c] =
+                  (m[n][c] + (log2f(sum[c]) - E::kBias)) * 0.6931471805599453f;
+        } else {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int in = n * 8 + t * 2 + c;
+            if (in >= n_h) continue;
             float *dst = p.part_o + (part * 8 * N + in) * p.hd;
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
@@ -626,10 +654,11 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
                 if (k * 16 + e * 8 + g < p.hd) dst[k * 16 + e * 8 + g] = o[n][k][e * 2 + c];
             if (g == 0) {
               p.part_ml[(part * 8 * N + in) * 2] = m[n][c];
-              p.part_ml[(part * 8 * N + in) * 2 + 1] = sum;
+              p.part_ml[(part * 8 * N + in) * 2 + 1] = sum[c];
             }
           }
         }
+      }
     }
     __syncwarp();
     stream.fill(s);
@@ -640,26 +669,41 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
 // ---------------------------------------------------------------------------------------
 // join of the parts
 // ---------------------------------------------------------------------------------------
-constexpr int kJoinThreads = 256;
 constexpr int kMaxRanges = 2048;
 
-// One CTA per (cut sequence, query head).  blockIdx.x is a sequence where by_seq, else a range
-// border (at most ranges - 1 sequences are cut).  Which parts there are follows from the lengths
-// alone and is worked out before the walk's end is waited for; then a thread per part forms its
-// weight, and VW columns a thread are summed over the parts, kJoinThreads / (head_dim / VW) parts
-// at a time, with the loads of several parts in flight (one at a time cost 1.5 us each: 38 us
-// for the 148 parts of one long sequence).
+// A CTA has `hpc` query heads (1 or a warp each) of a cut sequence.  blockIdx.x is a sequence
+// where by_seq, else a range border (at most ranges - 1 sequences are cut).  Which parts there are
+// follows from the lengths alone and is worked out before the walk's end is waited for.  Up to 32
+// parts a warp joins alone, a lane per part's weight; more are joined by the CTA: a thread per
+// part's weight, then VW columns a thread, kJoinThreads / (head_dim / VW) parts at a time.  Either
+// way several parts' loads are in flight (one at a time cost 1.5 us each: 38 us for the 148 parts
+// of one long sequence, 6 us so).  128 threads fit beside the walk's CTA (registers), so most
+// CTAs are in place before the walk ends.
+constexpr int kJoinThreads = 128;
+
+template <int VW>
+__device__ __forceinline__ void add_part(float (&acc)[VW], const float *src, float w) {
+  if constexpr (VW == 4) {
+    const float4 x = *reinterpret_cast<const float4 *>(src);
+    acc[0] = fmaf(x.x, w, acc[0]), acc[1] = fmaf(x.y, w, acc[1]);
+    acc[2] = fmaf(x.z, w, acc[2]), acc[3] = fmaf(x.w, w, acc[3]);
+  } else {
+    acc[0] = fmaf(src[0], w, acc[0]);
+  }
+}
+
 template <int DT, int VW>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int g_unit, int by_seq) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int g_unit, int by_seq,
+                                                           int hpc) {
   using T = typename Elem<DT>::T;
-  __shared__ int part[kMaxRanges];
-  __shared__ float weight[kMaxRanges];
+  extern __shared__ __align__(16) char smem[];
+  int *part = reinterpret_cast<int *>(smem);
+  float *weight = reinterpret_cast<float *>(part + p.ranges);
   __shared__ float red[kJoinThreads * VW];
   __shared__ float red_m[kJoinThreads / 32], red_l[kJoinThreads / 32];
   const float kNegInf = __int_as_float(0xff800000);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Line ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
-  const int h = blockIdx.y;
   int b = blockIdx.x, first, next;
   if (by_seq) {
     first = p.cu[b], next = p.cu[b + 1];
@@ -679,75 +723,123 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const uint32_t r0 = ln.owner(at), r1 = ln.owner(at + len + kSeqCost - 1);
   if (r1 == r0) return;  // not cut
   const int n = r1 - r0 + 1;
-  const int u = h / p.group, in = h - u * p.group;
-  const int unit = u * p.chunks + in / g_unit, g = in % g_unit;
-  bool done = false;
-  for (int i = tid; i < n; i += kJoinThreads) {
+  // the part slots of range r0 + i, for head 0 of the unit; -1: no part; all: the range has it whole
+  auto slot_of = [&](int i, bool &all) {
     const uint32_t r = r0 + i;
     const int i0 = border(ln.start(r), at, len), i1 = border(ln.start(r + 1), at, len);
-    done |= i0 == 0 && i1 == len;
-    part[i] = i1 > i0 ? ((static_cast<int>(r) * p.units + unit) * 2 + (i0 == 0 ? 1 : 0)) * g_unit + g : -1;
-  }
-  if (__syncthreads_or(done)) return;  // all its tokens fell into one range: already written
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  float top = kNegInf;
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const float m = part[i] >= 0 ? p.part_ml[2 * static_cast<int64_t>(part[i])] : kNegInf;
-    weight[i] = m;
-    top = fmaxf(top, m);
-  }
+    all |= i0 == 0 && i1 == len;
+    return i1 > i0 ? (static_cast<int>(r) * p.units * 2 + (i0 == 0 ? 1 : 0)) * g_unit : -1;
+  };
+  auto head_of = [&](int h) {  // what head h adds to a part slot
+    const int u = h / p.group, in = h - u * p.group;
+    return (u * p.chunks + in / g_unit) * 2 * g_unit + in % g_unit;
+  };
+  auto store = [&](int h, int c, const float (&x)[VW], float inv) {
+    T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + h * p.out_head) + c * VW;
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-  if (lane == 0) red_m[warp] = top;
-  __syncthreads();
+    for (int e = 0; e < VW; ++e) dst[e] = Elem<DT>::from_f(x[e] * inv);
+  };
+  const int cols = p.hd / VW;
+  const int h0 = blockIdx.y * hpc, h1 = min(h0 + hpc, p.heads);
+
+  if (n <= 32) {
+    bool all = false;
+    int mine = lane < n ? slot_of(lane, all) : -1;
+    if (__any_sync(0xffffffffu, all)) return;  // all its tokens fell into one range: already written
+    const int h = h0 + warp;
+    if (h >= h1) return;
+    if (mine >= 0) mine += head_of(h);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    float m = kNegInf, l = 0.f;
+    if (mine >= 0) {
+      const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * static_cast<int64_t>(mine));
+      m = ml.x, l = ml.y;
+    }
+    float top = m;
 #pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) top = fmaxf(top, red_m[i]);
-  const float base = top == kNegInf ? 0.f : top;
-  float sum = 0.f;
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const float e = exp2f(weight[i] - base);
-    weight[i] = e;
-    if (part[i] >= 0) sum = fmaf(p.part_ml[2 * static_cast<int64_t>(part[i]) + 1], e, sum);
-  }
+    for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    const float w = exp2f(m - (top == kNegInf ? 0.f : top));
+    float total = l * w;
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-  if (lane == 0) red_l[warp] = sum;
-  __syncthreads();
-  const int cols = p.hd / VW, groups = kJoinThreads / cols;
-  const int c = tid % cols, pg = tid / cols;
-  float acc[VW];
+    for (int k = 16; k > 0; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    for (int c0 = 0; c0 < cols; c0 += 32) {
+      const int c = c0 + lane;
+      float acc[VW];
 #pragma unroll
-  for (int e = 0; e < VW; ++e) acc[e] = 0.f;
-  if (pg < groups) {
-#pragma unroll 8
-    for (int i = pg; i < n; i += groups) {
-      if (part[i] < 0) continue;
-      const float *src = p.part_o + static_cast<int64_t>(part[i]) * p.hd + c * VW;
-      const float w = weight[i];
-      if constexpr (VW == 4) {
-        const float4 x = *reinterpret_cast<const float4 *>(src);
-        acc[0] = fmaf(x.x, w, acc[0]), acc[1] = fmaf(x.y, w, acc[1]);
-        acc[2] = fmaf(x.z, w, acc[2]), acc[3] = fmaf(x.w, w, acc[3]);
-      } else {
-        acc[0] = fmaf(src[0], w, acc[0]);
+      for (int e = 0; e < VW; ++e) acc[e] = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const int at_i = __shfl_sync(0xffffffffu, mine, i);
+        const float w_i = __shfl_sync(0xffffffffu, w, i);
+        if (at_i >= 0 && c < cols) add_part<VW>(acc, p.part_o + static_cast<int64_t>(at_i) * p.hd + c * VW, w_i);
       }
+      if (c < cols) store(h, c, acc, inv);
+    }
+    if (p.lse && lane == 0)
+      p.lse[static_cast<int64_t>(b) * p.heads + h] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
+    return;
+  }
+
+  bool all = false;
+  for (int i = tid; i < n; i += kJoinThreads) part[i] = slot_of(i, all);
+  if (__syncthreads_or(all)) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int h = h0; h < h1; ++h) {
+    const int add = head_of(h);
+    float top = kNegInf;
+    for (int i = tid; i < n; i += kJoinThreads) {
+      const float m = part[i] >= 0 ? p.part_ml[2 * static_cast<int64_t>(part[i] + add)] : kNegInf;
+      weight[i] = m;
+      top = fmaxf(top, m);
     }
 #pragma unroll
-    for (int e = 0; e < VW; ++e) red[(pg * cols + c) * VW + e] = acc[e];
-  }
-  __syncthreads();
-  float total = 0.f;
+    for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    if (lane == 0) red_m[warp] = top;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) total += red_l[i];
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + h * p.out_head);
-  if (tid < p.hd) {
-    float x = 0.f;
-    for (int i = 0; i < groups; ++i) x += red[i * p.hd + tid];
-    dst[tid] = Elem<DT>::from_f(x * inv);
+    for (int i = 0; i < kJoinThreads / 32; ++i) top = fmaxf(top, red_m[i]);
+    const float base = top == kNegInf ? 0.f : top;
+    float sum = 0.f;
+    for (int i = tid; i < n; i += kJoinThreads) {
+      const float e = exp2f(weight[i] - base);
+      weight[i] = e;
+      if (part[i] >= 0) sum = fmaf(p.part_ml[2 * static_cast<int64_t>(part[i] + add) + 1], e, sum);
+    }
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    if (lane == 0) red_l[warp] = sum;
+    __syncthreads();
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) total += red_l[i];
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const int wide = min(cols, kJoinThreads), groups = kJoinThreads / wide;
+    for (int c0 = 0; c0 < cols; c0 += wide) {  // one pass unless head_dim is odd and above 128
+      const int c = c0 + tid % wide, pg = tid / wide;
+      float acc[VW];
+#pragma unroll
+      for (int e = 0; e < VW; ++e) acc[e] = 0.f;
+      if (pg < groups && c < cols) {
+#pragma unroll 8
+        for (int i = pg; i < n; i += groups)
+          if (part[i] >= 0)
+            add_part<VW>(acc, p.part_o + static_cast<int64_t>(part[i] + add) * p.hd + c * VW, weight[i]);
+      }
+#pragma unroll
+      for (int e = 0; e < VW; ++e) red[tid * VW + e] = acc[e];
+      __syncthreads();
+      if (pg == 0 && c < cols) {
+        for (int i = 1; i < groups; ++i)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) acc[e] += red[(i * wide + tid) * VW + e];
+        store(h, c, acc, inv);
+      }
+      __syncthreads();
+    }
+    if (p.lse && tid == 0)
+      p.lse[static_cast<int64_t>(b) * p.heads + h] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
   }
-  if (p.lse && tid == 0)
-    p.lse[static_cast<int64_t>(b) * p.heads + h] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -800,7 +892,7 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
   if (a->k_pages.dtype == DKV_F32) {
     s->g = group <= 4 ? 4 : 8;
-    s->warps = s->hd_pad == 256 ? 2 : 4;
+    s->warps = s->hd_pad == 256 ? 2 : s->hd_pad == 128 ? 4 : 8;
   } else {
     s->g = group <= 8 ? 8 : 16;
     s->warps = s->hd_pad == 256 ? 4 : 8;
@@ -870,8 +962,8 @@ int launch_walk<DKV_F32>(const Params &p, const Shape &s, int grid, cudaStream_t
 #define DKV_SIMT_CASE(HD, W)                                                 \
   if (s.hd_pad == HD && s.g == 4) return launch_simt<HD, 4, W>(p, grid, st); \
   if (s.hd_pad == HD && s.g == 8) return launch_simt<HD, 8, W>(p, grid, st);
-  DKV_SIMT_CASE(32, 4)
-  DKV_SIMT_CASE(64, 4)
+  DKV_SIMT_CASE(32, 8)
+  DKV_SIMT_CASE(64, 8)
   DKV_SIMT_CASE(128, 4)
   DKV_SIMT_CASE(256, 2)
 #undef DKV_SIMT_CASE
@@ -889,15 +981,19 @@ int launch(const Params &p, const Shape &s, cudaStream_t st) {
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   const int by_seq = p.n_seqs <= s.ranges - 1;
-  cfg.gridDim = dim3(by_seq ? p.n_seqs : s.ranges - 1, p.heads);
+  const int cut = by_seq ? p.n_seqs : s.ranges - 1;
+  // few cut sequences: a CTA for each head (they may have many parts); else a warp each
+  const int hpc = static_cast<int64_t>(cut) * p.heads <= 148 * 8 ? 1 : kJoinThreads / 32;
+  cfg.gridDim = dim3(cut, (p.heads + hpc - 1) / hpc);
   cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = s.ranges * 8;
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   if (p.hd % 4 == 0)
-    DKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<DT, 4>, p, s.g, by_seq));
+    DKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<DT, 4>, p, s.g, by_seq, hpc));
   else
-    DKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<DT, 1>, p, s.g, by_seq));
+    DKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<DT, 1>, p, s.g, by_seq, hpc));
   return DKV_OK;
 }
 
@@ -955,6 +1051,9 @@ extern "C" int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv
   const int64_t all = p.k_block | p.k_slot | p.k_head | p.v_block | p.v_slot | p.v_head | (p.hd * sz) |
                       static_cast<int64_t>(reinterpret_cast<uintptr_t>(k.base) | reinterpret_cast<uintptr_t>(v.base));
   p.vec = all % 16 == 0;
+  const int64_t two = p.q_seq | p.q_head | p.out_seq | p.out_head | (p.hd * sz) |
+                      static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out));
+  p.pairs = two % 4 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (k.dtype) {
     case DKV_F32: return pattn::launch<DKV_F32>(p, s, st);
