@@ -739,7 +739,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 #pragma unroll
     for (int e = 0; e < VW; ++e) dst[e] = Elem<DT>::from_f(x[e] * inv);
   };
-  const int cols = p.hd / VW;
+  // gridDim.z CTAs share a head's columns
+  const int share = (p.hd / VW + gridDim.z - 1) / gridDim.z, col0 = blockIdx.z * share;
+  const int cols = min(p.hd / VW, col0 + share);
   const int h0 = blockIdx.y * hpc, h1 = min(h0 + hpc, p.heads);
 
   if (n <= 32) {
@@ -763,7 +765,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    for (int c0 = 0; c0 < cols; c0 += 32) {
+    for (int c0 = col0; c0 < cols; c0 += 32) {
       const int c = c0 + lane;
       float acc[VW];
 #pragma unroll
@@ -776,7 +778,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       }
       if (c < cols) store(h, c, acc, inv);
     }
-    if (p.lse && lane == 0)
+    if (p.lse && lane == 0 && blockIdx.z == 0)
       p.lse[static_cast<int64_t>(b) * p.heads + h] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
     return;
   }
@@ -814,8 +816,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 #pragma unroll
     for (int i = 0; i < kJoinThreads / 32; ++i) total += red_l[i];
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    const int wide = min(cols, kJoinThreads), groups = kJoinThreads / wide;
-    for (int c0 = 0; c0 < cols; c0 += wide) {  // one pass unless head_dim is odd and above 128
+    const int wide = min(share, kJoinThreads), groups = kJoinThreads / wide;
+    for (int c0 = col0; c0 < cols; c0 += wide) {  // one pass unless head_dim is odd and above 128
       const int c = c0 + tid % wide, pg = tid / wide;
       float acc[VW];
 #pragma unroll
@@ -837,7 +839,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       }
       __syncthreads();
     }
-    if (p.lse && tid == 0)
+    if (p.lse && tid == 0 && blockIdx.z == 0)
       p.lse[static_cast<int64_t>(b) * p.heads + h] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
   }
 }
@@ -984,7 +986,9 @@ int launch(const Params &p, const Shape &s, cudaStream_t st) {
   const int cut = by_seq ? p.n_seqs : s.ranges - 1;
   // few cut sequences: a CTA for each head (they may have many parts); else a warp each
   const int hpc = static_cast<int64_t>(cut) * p.heads <= 148 * 8 ? 1 : kJoinThreads / 32;
-  cfg.gridDim = dim3(cut, (p.heads + hpc - 1) / hpc);
+  // very few: several CTAs for each head
+  const int split = static_cast<int64_t>(cut) * p.heads <= 148 && p.hd >= 64 ? 4 : 1;
+  cfg.gridDim = dim3(cut, (p.heads + hpc - 1) / hpc, split);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = s.ranges * 8;
   cfg.stream = st;

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(dkv_step_plan_args a
 // ---------------------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------------------
-constexpr int kAppThreads = 256;
+constexpr int kAppThreads = 128;
 
 struct Append {
   const void *src[3];  // q, k, v
@@ -163,63 +163,127 @@ struct Append {
   int32_t *status;
   int heads[3];
   int hd, half, block_size, rope_max_pos;
+  int wide;  // more than 2^32 threads
 };
 
-// One element pair (x[i], x[i + half]) at a time: the simplest form.
-template <int SDT, int PDT>
-__global__ void __launch_bounds__(kAppThreads) append_kernel(Append a) {
+// VEC consecutive elements of a type as they lie in memory, in 16-byte pieces (one: as it is)
+template <int DT, int VEC>
+struct Raw {
+  static constexpr int kPieces = VEC * static_cast<int>(sizeof(typename Elem<DT>::T)) / 16;
+  uint4 v[kPieces];
+  __device__ __forceinline__ void load(const typename Elem<DT>::T *src) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) v[i] = reinterpret_cast<const uint4 *>(src)[i];
+  }
+  __device__ __forceinline__ void store(typename Elem<DT>::T *dst) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4 *>(dst)[i] = v[i];
+  }
+  __device__ __forceinline__ float get(int i) const {
+    const int per = VEC / kPieces;
+    const uint4 u = v[i / per];
+    const int e = i % per;
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if (DT == DKV_F32) return __uint_as_float(w[e & 3]);
+    const uint32_t x = w[(e / 2) & 3];
+    return DT == DKV_BF16 ? (e & 1 ? bf16hi(x) : bf16lo(x)) : (e & 1 ? f16hi(x) : f16lo(x));
+  }
+  __device__ __forceinline__ void set(const float (&x)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const float *y = x + i * (VEC / kPieces);
+      if constexpr (DT == DKV_F32)
+        v[i] = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+      else if constexpr (DT == DKV_BF16)
+        v[i] = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                          pack_bf16x2(y[6], y[7]));
+      else
+        v[i] = make_uint4(pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]), pack_f16x2(y[4], y[5]),
+                          pack_f16x2(y[6], y[7]));
+    }
+  }
+};
+template <int DT>
+struct Raw<DT, 1> {
+  typename Elem<DT>::T v;
+  __device__ __forceinline__ void load(const typename Elem<DT>::T *src) { v = src[0]; }
+  __device__ __forceinline__ void store(typename Elem<DT>::T *dst) const { dst[0] = v; }
+  __device__ __forceinline__ float get(int) const { return Elem<DT>::to_f(v); }
+  __device__ __forceinline__ void set(const float (&x)[1]) { v = Elem<DT>::from_f(x[0]); }
+};
+
+// A thread has VEC columns i and their partners i + half of up to kHeads heads of a row, so that
+// the row's slot, position and cos / sin are read once for all of them and 2 kHeads 16-byte loads
+// are in flight.  Bound by memory: every q, k and v element is read once and written once.
+constexpr int kHeads = 4;
+
+template <int SDT, int PDT, int VEC>
+__global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_constant__ Append a) {
   using ST = typename Elem<SDT>::T;
   using PT = typename Elem<PDT>::T;
   const int all = a.heads[0] + a.heads[1] + a.heads[2];
-  const int64_t total = a.n_rows * all * a.half;
-  for (int64_t e = static_cast<int64_t>(blockIdx.x) * kAppThreads + threadIdx.x; e < total;
-       e += static_cast<int64_t>(gridDim.x) * kAppThreads) {
-    const int j = static_cast<int>(e % a.half);
-    const int64_t rh = e / a.half;
-    int h = static_cast<int>(rh % all);
-    const int64_t row = rh / all;
-    int w = 0;
-    if (h >= a.heads[0]) h -= a.heads[0], w = 1;
-    if (w == 1 && h >= a.heads[1]) h -= a.heads[1], w = 2;
-    int64_t off = row * a.dst_row[0];
-    if (w) {
-      const int64_t slot = a.slots[row];
-      if (slot < 0) continue;
-      if (slot >= a.n_slots) {
-        record_error(a.status, DKV_ERR_PAGE_RANGE);
-        continue;
+  const int cols = a.half / VEC, per_row = cols * ((all + kHeads - 1) / kHeads);
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * kAppThreads + threadIdx.x;
+  const int64_t row = a.wide ? e / per_row : static_cast<uint32_t>(e) / static_cast<uint32_t>(per_row);
+  if (row >= a.n_rows) return;
+  const int in = static_cast<int>(e - row * per_row);
+  const int hg = in / cols, j = (in - hg * cols) * VEC;
+  const bool pair = j + a.half < a.hd;  // false only for the middle of an odd head without RoPE
+
+  const int64_t slot = a.slots[row];
+  const int pos = a.cos_t ? a.positions[row] : 0;
+  Raw<SDT, VEC> x[kHeads][2];
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    int h = hg * kHeads + k;
+    if (h >= all) break;
+    const int w = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
+    h -= w == 0 ? 0 : w == 1 ? a.heads[0] : a.heads[0] + a.heads[1];
+    const ST *src = static_cast<const ST *>(a.src[w]) + row * a.src_row[w] + h * a.src_head[w] + j;
+    x[k][0].load(src);
+    if (pair) x[k][1].load(src + a.half);
+  }
+  if (a.cos_t && (pos < 0 || pos >= a.rope_max_pos)) {
+    record_error(a.status, DKV_ERR_ROPE_RANGE);
+    return;
+  }
+  if (slot >= a.n_slots) record_error(a.status, DKV_ERR_PAGE_RANGE);
+  const bool kept = slot >= 0 && slot < a.n_slots;
+  Raw<DKV_F32, VEC> c, s;
+  if (a.cos_t) {
+    c.load(a.cos_t + static_cast<int64_t>(pos) * a.half + j);
+    s.load(a.sin_t + static_cast<int64_t>(pos) * a.half + j);
+  }
+  const int64_t block = kept ? slot / a.block_size : 0;
+  const int64_t off = kept ? slot - block * a.block_size : 0;
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    int h = hg * kHeads + k;
+    if (h >= all) break;
+    const int w = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
+    h -= w == 0 ? 0 : w == 1 ? a.heads[0] : a.heads[0] + a.heads[1];
+    if (w && !kept) continue;
+    float lo[VEC], hi[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) lo[i] = x[k][0].get(i), hi[i] = pair ? x[k][1].get(i) : 0.f;
+    if (a.cos_t && w < 2) {  // products and sum each rounded, as the reference's tensor operations do
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float u = lo[i], v = hi[i];
+        lo[i] = __fsub_rn(__fmul_rn(u, c.get(i)), __fmul_rn(v, s.get(i)));
+        hi[i] = __fadd_rn(__fmul_rn(v, c.get(i)), __fmul_rn(u, s.get(i)));
       }
-      off = slot / a.block_size * a.dst_block[w] + slot % a.block_size * a.dst_row[w];
-    }
-    off += h * a.dst_head[w] + j;
-    float c = 1.f, s = 0.f;
-    if (a.cos_t) {
-      const int pos = a.positions[row];
-      if (pos < 0 || pos >= a.rope_max_pos) {
-        record_error(a.status, DKV_ERR_ROPE_RANGE);
-        continue;
-      }
-      if (w < 2) {
-        c = a.cos_t[static_cast<int64_t>(pos) * a.half + j];
-        s = a.sin_t[static_cast<int64_t>(pos) * a.half + j];
-      }
-    }
-    const ST *x = static_cast<const ST *>(a.src[w]) + row * a.src_row[w] + h * a.src_head[w] + j;
-    const bool pair = j + a.half < a.hd;
-    const float lo = Elem<SDT>::to_f(x[0]), hi = pair ? Elem<SDT>::to_f(x[a.half]) : 0.f;
-    float ylo = lo, yhi = hi;
-    if (a.cos_t && w < 2) {
-      ylo = __fsub_rn(__fmul_rn(lo, c), __fmul_rn(hi, s));
-      yhi = __fadd_rn(__fmul_rn(hi, c), __fmul_rn(lo, s));
     }
     if (w == 0) {
-      ST *y = static_cast<ST *>(a.dst[0]) + off;
-      y[0] = Elem<SDT>::from_f(ylo);
-      if (pair) y[a.half] = Elem<SDT>::from_f(yhi);
+      ST *dst = static_cast<ST *>(a.dst[0]) + row * a.dst_row[0] + h * a.dst_head[0] + j;
+      Raw<SDT, VEC> y;
+      y.set(lo), y.store(dst);
+      if (pair) y.set(hi), y.store(dst + a.half);
     } else {
-      PT *y = static_cast<PT *>(a.dst[w]) + off;
-      y[0] = Elem<PDT>::from_f(ylo);
-      if (pair) y[a.half] = Elem<PDT>::from_f(yhi);
+      PT *dst = static_cast<PT *>(a.dst[w]) + block * a.dst_block[w] + off * a.dst_row[w] + h * a.dst_head[w] + j;
+      Raw<PDT, VEC> y;
+      y.set(lo), y.store(dst);
+      if (pair) y.set(hi), y.store(dst + a.half);
     }
   }
 }
@@ -288,15 +352,34 @@ extern "C" int dkv_append_paged(const dkv_append_args *args, dkv_stream_t stream
   a.status = g.status;
   a.heads[0] = g.q != nullptr ? g.n_q_heads : 0, a.heads[1] = a.heads[2] = kp.n_heads;
   a.hd = kp.head_dim, a.half = (kp.head_dim + 1) / 2, a.block_size = kp.block_size, a.rope_max_pos = g.rope_max_pos;
-  const int64_t total = a.n_rows * (a.heads[0] + a.heads[1] + a.heads[2]) * a.half;
+  // 16-byte accesses where every half row of a head starts on 16 bytes 
+  const int64_t ssz = g.in_dtype == DKV_F32 ? 4 : 2, psz = kp.dtype == DKV_F32 ? 4 : 2;
+  const int vec = static_cast<int>(16 / psz);
+  int64_t in_bits = 0, page_bits = 0;
+  for (int w = g.q != nullptr ? 0 : 1; w < 3; ++w) {
+    in_bits |= reinterpret_cast<intptr_t>(a.src[w]) | a.src_row[w] * ssz | a.src_head[w] * ssz;
+    if (w == 0)
+      in_bits |= reinterpret_cast<intptr_t>(a.dst[0]) | a.dst_row[0] * ssz | a.dst_head[0] * ssz;
+    else
+      page_bits |= reinterpret_cast<intptr_t>(a.dst[w]) | a.dst_row[w] * psz | a.dst_head[w] * psz | a.dst_block[w] * psz;
+  }
+  in_bits |= reinterpret_cast<intptr_t>(a.cos_t) | reinterpret_cast<intptr_t>(a.sin_t);
+  const bool wide = kp.head_dim % (2 * vec) == 0 && (in_bits | page_bits) % 16 == 0;
+  const int all = a.heads[0] + a.heads[1] + a.heads[2];
+  const int64_t total = a.n_rows * ((all + step::kHeads - 1) / step::kHeads) * (a.half / (wide ? vec : 1));
+  a.wide = total > UINT32_MAX;
   const int64_t ctas = (total + step::kAppThreads - 1) / step::kAppThreads;
-  const unsigned grid = static_cast<unsigned>(ctas < 148 * 64 ? ctas : 148 * 64);
+  if (ctas > INT32_MAX) return DKV_ERR_UNSUPPORTED;
+  const unsigned grid = static_cast<unsigned>(ctas);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-#define DKV_APPEND_CASE(S, P)                                               \
-  if (g.in_dtype == S && kp.dtype == P) {                                   \
-    step::append_kernel<S, P><<<grid, step::kAppThreads, 0, st>>>(a);       \
-    DKV_CUDA_CHECK(cudaGetLastError());                                     \
-    return DKV_OK;                                                          \
+#define DKV_APPEND_CASE(S, P)                                                                     \
+  if (g.in_dtype == S && kp.dtype == P) {                                                         \
+    if (wide)                                                                                     \
+      step::append_kernel<S, P, P == DKV_F32 ? 4 : 8><<<grid, step::kAppThreads, 0, st>>>(a);     \
+    else                                                                                          \
+      step::append_kernel<S, P, 1><<<grid, step::kAppThreads, 0, st>>>(a);                        \
+    DKV_CUDA_CHECK(cudaGetLastError());                                                           \
+    return DKV_OK;                                                                                \
   }
   DKV_APPEND_CASE(DKV_BF16, DKV_BF16)
   DKV_APPEND_CASE(DKV_F16, DKV_F16)
