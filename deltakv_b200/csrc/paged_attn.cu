@@ -24,6 +24,10 @@ constexpr int kTile = 16;      // tokens per pipeline stage of a warp
 // of 1..600 tokens at 16 / 32 / 48 / 64 / 96: 38 / 34 / 31 / 34 / 39 us; of 64 of 1..8192:
 // 73 / 61 / 59 / 60 / 61 us; long sequences do not notice.
 constexpr int kSeqCost = 48;
+#ifndef LOCAL_TOKENS
+#define LOCAL_TOKENS 512
+#endif
+constexpr int kLocalTokens = LOCAL_TOKENS;
 constexpr int kMinRange = 32;  // tokens below which a range is not cut further
 
 struct Params {
@@ -43,6 +47,7 @@ struct Params {
   float scale_log2;  // scale * log2(e): scores are kept in base 2
   int n_seqs, n_kv, heads, group, chunks, units, ranges;
   int hd, block_size;
+  int local;  // a CTA per (sequence, unit): no ranges, no parts
   int vec;    // rows of K and V in whole 16-byte pieces
   int pairs;  // rows of q and out in whole pairs of 16-bit elements
 };
@@ -118,6 +123,7 @@ struct Walk {
   uint32_t x0, x1;  // the range
   int b;            // sequence
   int i, end;       // tile start and end of the piece within the sequence
+  int step;         // tokens from one tile to the next (more than a tile: the other warps' tiles between)
   int64_t tlen;     // valid entries of its table row
   uint32_t flags;
   bool live;
@@ -156,9 +162,13 @@ __device__ __forceinline__ void walk_seq(const Params &p, Walk &w, int h0, int n
 }
 template <typename T>
 __device__ __forceinline__ void walk_next(const Params &p, Walk &w, int h0, int n_h, int lane) {
-  w.i += kTile;
+  w.i += w.step;
   w.flags &= ~kFirst;
   if (w.i < w.end) return;
+  if (p.local) {
+    w.live = false;
+    return;
+  }
   ++w.b;
   walk_seq<T>(p, w, h0, n_h, lane);
 }
@@ -167,6 +177,18 @@ __device__ __forceinline__ Walk range_walk(const Params &p, const Line &ln, uint
   Walk w;
   w.x0 = ln.start(r), w.x1 = ln.start(r + 1);
   w.b = w.win.find(p, w.x0, lane);
+  w.step = kTile;
+  return w;
+}
+// every n_warps-th tile of sequence b
+__device__ __forceinline__ Walk local_walk(const Params &p, int b, int warp, int n_warps) {
+  Walk w;
+  w.b = b;
+  w.i = warp * kTile, w.step = n_warps * kTile;
+  w.end = max(p.cu[b + 1] - p.cu[b], 0);
+  w.tlen = p.table_lens ? p.table_lens[b] : p.table_stride;
+  w.flags = kFirst;
+  w.live = w.i < w.end;
   return w;
 }
 
@@ -221,7 +243,7 @@ struct Stream {
   }
   __device__ __forceinline__ void start(const Walk &from) {
     w = from;
-    walk_seq<T>(p, w, h0, n_h, lane);
+    if (!p.local) walk_seq<T>(p, w, h0, n_h, lane);
     look_up();
   }
   // issues the next tile's copies into stage s (one cp.async group, empty past the end)
@@ -247,7 +269,7 @@ struct Stream {
           for (int d = lane; d < p.hd; d += 32) dst[d] = a ? reinterpret_cast<const T *>(a)[d] : T(0.f);
         }
       }
-      const bool last = w.i + kTile >= w.end;
+      const bool last = !p.local && w.i + kTile >= w.end;
       if (lane == 0) meta[s] = make_uint4(w.b, w.flags | (last ? kLast : 0), there & 0xffffu, 0);
       walk_next<T>(p, w, h0, n_h, lane);
       look_up();
@@ -257,6 +279,40 @@ struct Stream {
     cp_async_commit();
   }
 };
+
+// The join within a CTA: each warp's (m, l) and O (rows of HD + 4: no bank conflicts) lie at the
+// front of its ring.
+template <int HD, int kRows>
+struct LocalState {
+  float o[kRows][HD + 4];
+  float m[kRows], l[kRows];
+};
+template <int DT, int HD, int kRows>
+__device__ __forceinline__ void local_join(const Params &p, const char *smem, int warp_bytes, int n_warps, int b, int h0,
+                                           int n_h) {
+  using T = typename Elem<DT>::T;
+  using State = LocalState<HD, kRows>;
+  const float kNegInf = __int_as_float(0xff800000);
+  __syncthreads();
+  for (int i = threadIdx.x; i < n_h * p.hd; i += n_warps * 32) {
+    const int g = i / p.hd, d = i - g * p.hd;
+    float top = kNegInf;
+    for (int w = 0; w < n_warps; ++w)
+      top = fmaxf(top, reinterpret_cast<const State *>(smem + w * warp_bytes)->m[g]);
+    const float base = top == kNegInf ? 0.f : top;
+    float x = 0.f, total = 0.f;
+    for (int w = 0; w < n_warps; ++w) {
+      const State *s = reinterpret_cast<const State *>(smem + w * warp_bytes);
+      const float e = exp2f(s->m[g] - base);
+      total = fmaf(s->l[g], e, total);
+      x = fmaf(s->o[g][d], e, x);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    reinterpret_cast<T *>(p.out + b * p.out_seq + (h0 + g) * p.out_head)[d] = Elem<DT>::from_f(x * inv);
+    if (p.lse && d == 0)
+      p.lse[static_cast<int64_t>(b) * p.heads + h0 + g] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
+  }
+}
 
 // ---------------------------------------------------------------------------------------
 // the walk with fp32 arithmetic on the ordinary pipes
@@ -280,10 +336,13 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.launch_dependents;");
-  const int gw = blockIdx.x * W + warp;
-  const int r = gw / p.units, unit = gw - r * p.units;
-  const Line ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
-  if (r >= static_cast<int>(ln.ranges)) return;
+  const int gw = p.local ? blockIdx.x : blockIdx.x * W + warp;
+  const int r = gw / p.units, unit = gw - r * p.units;  // r: the range, or the sequence where local
+  Line ln;
+  if (!p.local) {
+    ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
+    if (r >= static_cast<int>(ln.ranges)) return;
+  }
   const int u = unit / p.chunks, chunk = unit - u * p.chunks;
   const int n_h = min(G, p.group - chunk * G), h0 = u * p.group + chunk * G;
 
@@ -291,7 +350,7 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
   float *qs = reinterpret_cast<float *>(mine + C::S::kBytes);
   float *ps = qs + C::kQRow / 4 * G;
   typename C::S stream(p, mine, u, h0, n_h, lane);
-  stream.start(range_walk(p, ln, r, lane));
+  stream.start(p.local ? local_walk(p, r, warp, W) : range_walk(p, ln, r, lane));
 
   constexpr int kVec = HD >= 128 ? HD / 128 : 1;         // float4 columns per lane
   constexpr int kLanes = HD >= 128 ? 32 : HD / 4;        // lanes per token in the output product
@@ -299,6 +358,28 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
   float m[G], l[G], o[G][kVec][4];
   const int key = lane & 15, half = lane >> 4;
   const int oc = lane % kLanes, ok = lane / kLanes;
+  auto clear = [&]() {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      m[g] = __int_as_float(0xff800000), l[g] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[g][j][e] = 0.f;
+    }
+  };
+  // sums over the lanes that share a head (l) or a column (o)
+  auto reduce = [&](int g) {
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], k);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = kLanes; k < 32; k <<= 1) o[g][j][i] += __shfl_xor_sync(0xffffffffu, o[g][j][i], k);
+  };
+  clear();
 
   for (int s = 0; s < C::kStages; ++s) stream.fill(s);
   for (int s = 0;; s = s + 1 == C::kStages ? 0 : s + 1) {
@@ -315,14 +396,7 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
           x = reinterpret_cast<const float *>(p.q + b * p.q_seq + (h0 + g) * p.q_head)[d];
         qs[g * (C::kQRow / 4) + d + (d >= HD / 2 ? 4 : 0)] = x;
       }
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        m[g] = __int_as_float(0xff800000), l[g] = 0.f;
-#pragma unroll
-        for (int j = 0; j < kVec; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[g][j][e] = 0.f;
-      }
+      clear();
       __syncwarp();
     }
     const float *kr = reinterpret_cast<const float *>(mine + s * C::S::kStage + key * C::S::kRow) + half * (HD / 2);
@@ -382,15 +456,8 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
       const int64_t part = (static_cast<int64_t>(r) * p.units + unit) * 2 + (mt.y & kFromStart ? 1 : 0);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        float sum = l[g];
-#pragma unroll
-        for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-#pragma unroll
-        for (int j = 0; j < kVec; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int k = kLanes; k < 32; k <<= 1) o[g][j][i] += __shfl_xor_sync(0xffffffffu, o[g][j][i], k);
+        reduce(g);
+        const float sum = l[g];
         if (g < n_h && lane < kLanes) {
           const int h = h0 + g;
           if (whole) {
@@ -422,6 +489,23 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
     stream.fill(s);
   }
   cp_async_wait<0>();
+  if (p.local) {
+    __syncwarp();
+    LocalState<HD, G> *mine_out = reinterpret_cast<LocalState<HD, G> *>(mine);
+    static_assert(sizeof(LocalState<HD, G>) <= C::kStages * C::S::kStage, "the state fits the ring");
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      reduce(g);
+      if (lane < kLanes) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine_out->o[g][j * 128 + oc * 4 + e] = o[g][j][e];
+      }
+      if (lane == 0) mine_out->m[g] = m[g], mine_out->l[g] = l[g];
+    }
+    local_join<DKV_F32, HD, G>(p, smem, C::kWarpBytes, W, r, h0, n_h);
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -486,16 +570,19 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.launch_dependents;");
-  const int gw = blockIdx.x * W + warp;
-  const int r = gw / p.units, unit = gw - r * p.units;
-  const Line ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
-  if (r >= static_cast<int>(ln.ranges)) return;
+  const int gw = p.local ? blockIdx.x : blockIdx.x * W + warp;
+  const int r = gw / p.units, unit = gw - r * p.units;  // r: the range, or the sequence where local
+  Line ln;
+  if (!p.local) {
+    ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
+    if (r >= static_cast<int>(ln.ranges)) return;
+  }
   const int u = unit / p.chunks, chunk = unit - u * p.chunks;
   const int n_h = min(8 * N, p.group - chunk * 8 * N), h0 = u * p.group + chunk * 8 * N;
 
   char *mine = smem + warp * C::S::kBytes;
   typename C::S stream(p, mine, u, h0, n_h, lane);
-  stream.start(range_walk(p, ln, r, lane));
+  stream.start(p.local ? local_walk(p, r, warp, W) : range_walk(p, ln, r, lane));
 
   const int g = lane >> 2, t = lane & 3;
   // ldmatrix rows: K as (token, k half), V as (token half, column half) of a 16 x 16 block
@@ -504,6 +591,24 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
       smem_u32(mine) + (kTile + (lane & 7) + (lane >> 4) * 8) * C::S::kRow + ((lane >> 3) & 1) * 16;
   uint32_t qf[N][kSteps][2];
   float o[N][kSteps][4], m[N][2], l[N][2];
+  auto clear = [&]() {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      m[n][0] = m[n][1] = kNegInf;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][k][e] = 0.f;
+    }
+  };
+  auto sum_of = [&](int n, int c) {  // l over the lanes that share a head
+    float x = l[n][c];
+    x += __shfl_xor_sync(0xffffffffu, x, 4);
+    x += __shfl_xor_sync(0xffffffffu, x, 8);
+    return x + __shfl_xor_sync(0xffffffffu, x, 16);
+  };
+  clear();
 
   for (int s = 0; s < kStages; ++s) stream.fill(s);
   for (int s = 0;; s = s + 1 == kStages ? 0 : s + 1) {
@@ -532,13 +637,8 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
             }
             qf[n][k][e] = h < n_h ? w : 0;
           }
-        m[n][0] = m[n][1] = kNegInf;
-        l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][k][e] = 0.f;
       }
+      clear();
     }
     float sc[N][2][4];  // two chains over the head: even and odd steps
 #pragma unroll
@@ -607,14 +707,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
       const int64_t part = (static_cast<int64_t>(r) * p.units + unit) * 2 + (mt.y & kFromStart ? 1 : 0);
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        float sum[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          sum[c] = l[n][c];
-          sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], 4);
-          sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], 8);
-          sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], 16);
-        }
+        const float sum[2] = {sum_of(n, 0), sum_of(n, 1)};
         if (whole) {
           // heads to rows, so that a lane stores two neighbouring columns of one head
           const float inv0 = sum[0] == 0.f ? 0.f : 1.f / sum[0], inv1 = sum[1] == 0.f ? 0.f : 1.f / sum[1];
@@ -664,6 +757,25 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
     stream.fill(s);
   }
   cp_async_wait<0>();
+  if (p.local) {
+    __syncwarp();
+    LocalState<HD, 8 * N> *mine_out = reinterpret_cast<LocalState<HD, 8 * N> *>(mine);
+    static_assert(sizeof(LocalState<HD, 8 * N>) <= kStages * C::S::kStage, "the state fits the ring");
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float sum = sum_of(n, c);
+        const int in = n * 8 + t * 2 + c;
+        if (g == 0) mine_out->m[in] = m[n][c], mine_out->l[in] = sum;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          mine_out->o[in][k * 16 + g] = o[n][k][c];
+          mine_out->o[in][k * 16 + 8 + g] = o[n][k][2 + c];
+        }
+      }
+    local_join<DT, HD, 8 * N>(p, smem, C::S::kBytes, W, r, h0, n_h);
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -850,6 +962,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 struct Shape {
   int hd_pad, g, warps;  // kernel variant
   int chunks, units;     // chunks of a group, KV heads x chunks
+  int local;             // a CTA per (sequence, unit) instead of ranges
   int ranges;            // upper bound of the ranges in use
   int64_t parts;         // part slots
   int64_t o_bytes, bytes;
@@ -901,10 +1014,11 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   }
   s->chunks = (group + s->g - 1) / s->g;
   s->units = a->k_pages.n_heads * s->chunks;
+  s->local = a->seqs.max_seq_len <= kLocalTokens && static_cast<int64_t>(a->seqs.n_seqs) * s->units <= sms;
   const int64_t most = static_cast<int64_t>(sms) * s->warps / s->units;
   const int64_t line = static_cast<int64_t>(a->seqs.n_seqs) * (static_cast<int64_t>(a->seqs.max_seq_len) + kSeqCost);
   const int64_t want = line / kMinRange;
-  s->ranges = static_cast<int>(most < 1 || want < 1 ? 1 : (want < most ? want : most));
+  s->ranges = static_cast<int>(s->local || most < 1 || want < 1 ? 1 : (want < most ? want : most));
   if (s->ranges > kMaxRanges) s->ranges = kMaxRanges;
   s->parts = s->ranges > 1 ? static_cast<int64_t>(s->ranges) * s->units * 2 * s->g : 0;
   s->o_bytes = (s->parts * hd * 4 + 15) / 16 * 16;
@@ -975,7 +1089,8 @@ int launch_walk<DKV_F32>(const Params &p, const Shape &s, int grid, cudaStream_t
 template <int DT>
 int launch(const Params &p, const Shape &s, cudaStream_t st) {
   const int64_t warps = static_cast<int64_t>(s.ranges) * s.units;
-  const int rc = launch_walk<DT>(p, s, static_cast<int>((warps + s.warps - 1) / s.warps), st);
+  const int64_t ctas = s.local ? static_cast<int64_t>(p.n_seqs) * s.units : (warps + s.warps - 1) / s.warps;
+  const int rc = launch_walk<DT>(p, s, static_cast<int>(ctas), st);
   if (rc != DKV_OK || s.ranges == 1) return rc;
   // the join starts as soon as every CTA of the walk is under way and waits in the kernel for its end
   cudaLaunchConfig_t cfg = {};
@@ -1050,6 +1165,7 @@ extern "C" int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.n_seqs = a.seqs.n_seqs, p.n_kv = k.n_heads, p.heads = a.n_q_heads, p.group = a.n_q_heads / k.n_heads;
   p.chunks = s.chunks, p.units = s.units, p.ranges = s.ranges;
+  p.local = s.local;
   p.hd = k.head_dim, p.block_size = k.block_size;
   // 16-byte copies where every row of K and V starts on 16 bytes and is a multiple of 16 long
   const int64_t all = p.k_block | p.k_slot | p.k_head | p.v_block | p.v_slot | p.v_head | (p.hd * sz) |

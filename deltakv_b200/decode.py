@@ -29,38 +29,67 @@ from deltakv_b200 import ops
 from deltakv_b200.rope import half_tables
 
 
+_I32 = torch.int32
+_empty, _raw_stream = torch.empty, torch._C._cuda_getCurrentRawStream
+# A decode step calls these operators once a layer, with kernels of a few microseconds: the checks
+# read each attribute once and take strides as tuples, and the stream is taken as its raw handle
+# (current_stream() builds an object: 3 us).
+
+
 def _same_device(where: str, first: Tensor, *rest: Tensor | None) -> torch.device:
     dev = first.device
-    if not first.is_cuda:
+    if dev.type != "cuda":
         ops._require_cuda(first)
     for t in rest:
         if t is not None and t.device != dev:
-            if not t.is_cuda:
-                raise ValueError("deltakv_b200 kernels need CUDA tensors (there is no CPU path)")
+            ops._require_cuda(t)
             raise ValueError(f"{where}: tensors on {dev} and {t.device}")
     return dev
 
 
 def _call(fn, args, dev: torch.device, where: str) -> None:
     """Launch on the current stream of ``dev``, which need not be the current device."""
-    # the raw handle: current_stream() builds a Stream object, 3 us of a 15 us call
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(C.byref(args), stream)
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = fn(C.byref(args), _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(C.byref(args), stream)
-    if rc != L.DKV_OK:
+            rc = fn(C.byref(args), _raw_stream(index))
+    if rc:
         raise L.DkvError(rc, where)
 
 
-def _int32_vector(t: Tensor | None, name: str, n: int | None) -> None:
-    if t is None:
-        return
-    if t.dtype != torch.int32:
+def _int32_vector(t: Tensor, name: str, n: int | None) -> None:
+    if t.dtype is not _I32:
         raise TypeError(f"{name} must be int32")
-    if t.ndim != 1 or (t.numel() > 1 and t.stride(0) != 1) or (n is not None and t.numel() != n):
+    if t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
         raise ValueError(f"{name} must be a contiguous vector" + ("" if n is None else f" of {n}"))
+
+
+def _rows(t: Tensor, name: str, rows: int, heads: int | None, hd: int) -> tuple[int, ...]:
+    """The strides of a ``[rows, heads, hd]`` tensor."""
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != rows or shape[2] != hd or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} {tuple(shape)} must be [{rows}, {'heads' if heads is None else heads}, {hd}]")
+    strides = t.stride()
+    if strides[2] != 1 and hd > 1:
+        raise ValueError(f"{name} must have contiguous head_dim")
+    return strides
+
+
+def _page_pair(k_pages: Tensor, v_pages: Tensor) -> tuple[L.PagedCache, L.PagedCache]:
+    shape, v_shape, dtype = k_pages.shape, v_pages.shape, k_pages.dtype
+    if len(shape) != 4 or len(v_shape) != 4:
+        raise ValueError(f"unsupported paged KV layout {tuple(shape)}, {tuple(v_shape)}")
+    nb, bs, h, d = shape
+    if dtype is not v_pages.dtype or bs != v_shape[1] or h != v_shape[2] or d != v_shape[3]:
+        raise ValueError("k_pages and v_pages must share dtype, block size, heads and head_dim")
+    code = ops.dkv_dtype(dtype)
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if (ks[3] != 1 or vs[3] != 1) and d > 1:
+        raise ValueError("paged cache head_dim must be contiguous")
+    return (L.PagedCache(k_pages.data_ptr(), code, bs, h, d, nb, ks[0], ks[1], ks[2]),
+            L.PagedCache(v_pages.data_ptr(), code, bs, h, d, v_shape[0], vs[0], vs[1], vs[2]))
 
 
 @dataclass
@@ -93,49 +122,39 @@ def plan_paged_step(lengths: Tensor, block_tables: Tensor, block_size: int, *, r
     """
     n = lengths.numel()
     _int32_vector(lengths, "lengths", n)
-    _int32_vector(new_lengths, "new_lengths", n)
-    _int32_vector(table_lens, "table_lens", n)
-    _int32_vector(free_blocks, "free_blocks", None)
-    if block_tables.dtype != torch.int32:
+    if new_lengths is not None:
+        _int32_vector(new_lengths, "new_lengths", n)
+    if table_lens is not None:
+        _int32_vector(table_lens, "table_lens", n)
+    n_free = 0
+    if free_blocks is not None:
+        _int32_vector(free_blocks, "free_blocks", None)
+        n_free = free_blocks.numel()
+    if block_tables.dtype is not _I32:
         raise TypeError("block_tables must be int32")
-    if block_tables.ndim != 2 or block_tables.shape[0] != n or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+    shape, strides = block_tables.shape, block_tables.stride()
+    if len(shape) != 2 or shape[0] != n or (strides[1] != 1 and shape[1] > 1):
         raise ValueError("block_tables must be a row-major [n_seqs, max_blocks] int32 tensor")
-    width = block_tables.shape[1]
-    if n > 1 and block_tables.stride(0) < width:
+    width = shape[1]
+    if n > 1 and strides[0] < width:
         raise ValueError("block_tables rows overlap: the plan writes them")
     if block_size <= 0 or rows < 0 or max_seq_len < 0:
         raise ValueError("block_size must be positive, rows and max_seq_len not negative")
     dev = _same_device("plan_paged_step", lengths, block_tables, new_lengths, table_lens, free_blocks)
-    out = torch.empty(3 * n + 3 + rows, dtype=torch.int32, device=dev)
+    out = _empty(3 * n + 3 + rows, dtype=_I32, device=dev)
     cu, cu_new, lens, used, positions = torch.unsafe_split_with_sizes(out, (n + 1, n + 1, n, 1, rows))
-    slots = torch.empty(rows, dtype=torch.int64, device=dev)
+    slots = _empty(rows, dtype=torch.int64, device=dev)
     st = ops.status_word(dev)
     base = out.data_ptr()
     args = L.StepPlanArgs(
-        lengths.data_ptr(), ops.ptr(new_lengths), ops.ptr(table_lens), ops.ptr(free_blocks),
-        0 if free_blocks is None else free_blocks.numel(), block_tables.data_ptr(), block_tables.stride(0), width, n,
-        block_size, rows, base, base + 4 * (n + 1), base + 8 * (n + 1), base + 4 * (3 * n + 2),
-        base + 4 * (3 * n + 3), slots.data_ptr(), st.ptr)
+        lengths.data_ptr(), ops.ptr(new_lengths), ops.ptr(table_lens), ops.ptr(free_blocks), n_free,
+        block_tables.data_ptr(), strides[0], width, n, block_size, rows, base, base + 4 * (n + 1), base + 8 * (n + 1),
+        base + 4 * (3 * n + 2), base + 4 * (3 * n + 3), slots.data_ptr(), st.ptr)
     _call(L.lib().dkv_plan_paged_step, args, dev, "dkv_plan_paged_step")
     if check:
         st.raise_if_set("plan_paged_step")
     seqs = ops.SeqBatchTensors(cu_seqlens=cu, block_tables=block_tables, max_seq_len=max_seq_len, table_lens=lens)
     return PagedStep(seqs, cu_new, positions, slots, used)
-
-
-def _rows(t: Tensor, name: str, rows: int, heads: int | None, hd: int) -> None:
-    if t.ndim != 3 or t.shape[0] != rows or t.shape[2] != hd or (heads is not None and t.shape[1] != heads):
-        want = f"[{rows}, {'heads' if heads is None else heads}, {hd}]"
-        raise ValueError(f"{name} {tuple(t.shape)} must be {want}")
-    if t.stride(2) != 1 and hd > 1:
-        raise ValueError(f"{name} must have contiguous head_dim")
-
-
-def _page_pair(k_pages: Tensor, v_pages: Tensor) -> None:
-    if k_pages.ndim != 4 or v_pages.ndim != 4:
-        raise ValueError(f"unsupported paged KV layout {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
-    if k_pages.dtype != v_pages.dtype or k_pages.shape[1:] != v_pages.shape[1:]:
-        raise ValueError("k_pages and v_pages must share dtype, block size, heads and head_dim")
 
 
 def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slots: Tensor, *,
@@ -154,49 +173,50 @@ def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, sl
     distinct.  ``check=True`` raises recorded range errors (a slot beyond the pages, a position
     beyond the tables: those rows store nothing).
     """
-    _page_pair(k_pages, v_pages)
-    rows, n_kv, hd = slots.numel(), k_pages.shape[2], k_pages.shape[3]
-    if slots.dtype != torch.int64:
+    kd, vd = _page_pair(k_pages, v_pages)
+    rows, n_kv, hd, dtype = slots.numel(), kd.n_heads, kd.head_dim, k.dtype
+    if slots.dtype is not torch.int64:
         raise TypeError("slots must be int64")
-    if slots.ndim != 1 or (rows > 1 and slots.stride(0) != 1):
+    if slots.dim() != 1 or not slots.is_contiguous():
         raise ValueError("slots must be a contiguous vector")
-    _rows(k, "k", rows, n_kv, hd)
-    _rows(v, "v", rows, n_kv, hd)
-    if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
+    ks, vs = _rows(k, "k", rows, n_kv, hd), _rows(v, "v", rows, n_kv, hd)
+    if v.dtype is not dtype or (q is not None and q.dtype is not dtype):
         raise TypeError("q, k and v must share a dtype")
-    if k.dtype != k_pages.dtype and k.dtype != torch.float32:
-        raise TypeError(f"{k.dtype} rows do not go into {k_pages.dtype} pages (pass the pages' dtype or fp32)")
+    if dtype is not k_pages.dtype and dtype is not torch.float32:
+        raise TypeError(f"{dtype} rows do not go into {k_pages.dtype} pages (pass the pages' dtype or fp32)")
     if rope is not None:
         if positions is None:
             raise ValueError("rope needs positions")
         _int32_vector(positions, "positions", rows)
+    n_q, qs, os = 0, (0, 0), (0, 0)
     if q is None:
         if q_out is not None:
             raise ValueError("q_out without q")
     else:
         if rope is None:
             raise ValueError("q is only rotated: pass rope and positions with it")
-        _rows(q, "q", rows, None, hd)
+        qs, n_q = _rows(q, "q", rows, None, hd), q.shape[1]
         if q_out is not None:
-            _rows(q_out, "q_out", rows, q.shape[1], hd)
-            if q_out.dtype != q.dtype:
+            os = _rows(q_out, "q_out", rows, n_q, hd)
+            if q_out.dtype is not dtype:
                 raise TypeError("q_out must have q's dtype")
     dev = _same_device("append_into_paged", k, v, k_pages, v_pages, slots, q, positions, q_out)
     cos = sin = None
+    max_pos = 0
     if rope is not None:
         cos, sin = half_tables(rope, dev)
-        if cos.ndim != 2 or cos.shape != sin.shape or 2 * cos.shape[1] != hd:
-            raise ValueError(f"rope tables {tuple(cos.shape)} do not cover head_dim {hd}")
-    kd, vd = ops.paged_desc(k_pages), ops.paged_desc(v_pages)
+        shape = cos.shape
+        if len(shape) != 2 or shape != sin.shape or 2 * shape[1] != hd:
+            raise ValueError(f"rope tables {tuple(shape)} do not cover head_dim {hd}")
+        max_pos = shape[0]
     if q is not None and q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        q_out = _empty((rows, n_q, hd), dtype=dtype, device=dev)
+        os = (n_q * hd, hd)
     st = ops.status_word(dev)
     args = L.AppendArgs(
-        k.data_ptr(), v.data_ptr(), ops.ptr(q), ops.dkv_dtype(k.dtype), 0 if q is None else q.shape[1], rows,
-        k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0 if q is None else q.stride(0),
-        0 if q is None else q.stride(1), ops.ptr(q_out), 0 if q is None else q_out.stride(0),
-        0 if q is None else q_out.stride(1), slots.data_ptr(), None if rope is None else positions.data_ptr(),
-        ops.ptr(cos), ops.ptr(sin), 0 if cos is None else cos.shape[0], kd, vd, st.ptr)
+        k.data_ptr(), v.data_ptr(), ops.ptr(q), ops.dkv_dtype(dtype), n_q, rows, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1],
+        ops.ptr(q_out), os[0], os[1], slots.data_ptr(), ops.ptr(positions) if max_pos else None, ops.ptr(cos),
+        ops.ptr(sin), max_pos, kd, vd, st.ptr)
     _call(L.lib().dkv_append_paged, args, dev, "dkv_append_paged")
     if check:
         st.raise_if_set("append_into_paged")
@@ -224,33 +244,36 @@ def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: op
     in blocks outside the cache or beyond the table are left out and recorded (``check=True``
     raises).
     """
-    _page_pair(k_pages, v_pages)
-    n_kv, hd = k_pages.shape[2], k_pages.shape[3]
-    n = seqs.cu_seqlens.numel() - 1
-    _rows(q, "q", n, None, hd)
+    kd, vd = _page_pair(k_pages, v_pages)
+    n_kv, hd, dtype = kd.n_heads, kd.head_dim, q.dtype
+    cu, tables, lens = seqs.cu_seqlens, seqs.block_tables, seqs.table_lens
+    n = cu.numel() - 1
+    qs = _rows(q, "q", n, None, hd)
     heads = q.shape[1]
-    if q.dtype != k_pages.dtype:
-        raise TypeError(f"q is {q.dtype}, the pages are {k_pages.dtype}")
+    if dtype is not k_pages.dtype:
+        raise TypeError(f"q is {dtype}, the pages are {k_pages.dtype}")
     if hd > 256:
         raise ValueError(f"head_dim {hd} is above 256")
     if heads == 0 or n_kv == 0 or heads % n_kv:
         raise ValueError(f"{heads} query heads do not share {n_kv} KV heads evenly")
-    if seqs.block_tables.shape[0] < n:
-        raise ValueError(f"block_tables has {seqs.block_tables.shape[0]} rows for {n} sequences")
+    if tables.dim() == 2 and tables.shape[0] < n:
+        raise ValueError(f"block_tables has {tables.shape[0]} rows for {n} sequences")
+    if lens is not None and (lens.numel() < n or not lens.is_contiguous()):
+        raise ValueError(f"table_lens must be a contiguous vector of {n}")
+    os = (heads * hd, hd)
     if out is not None:
-        _rows(out, "out", n, heads, hd)
-        if out.dtype != q.dtype:
+        os = _rows(out, "out", n, heads, hd)
+        if out.dtype is not dtype:
             raise TypeError("out must have q's dtype")
-    dev = _same_device("paged_decode_attention", q, k_pages, v_pages, seqs.cu_seqlens, seqs.block_tables,
-                       seqs.table_lens, out)
-    sb, kd, vd = seqs.struct(), ops.paged_desc(k_pages), ops.paged_desc(v_pages)
+    dev = _same_device("paged_decode_attention", q, k_pages, v_pages, cu, tables, lens, out)
+    sb = seqs.struct()
     if out is None:
-        out = torch.empty(n, heads, hd, dtype=q.dtype, device=dev)
-    lse = torch.empty(n, heads, dtype=torch.float32, device=dev) if return_lse else None
+        out = _empty((n, heads, hd), dtype=dtype, device=dev)
+    lse = _empty((n, heads), dtype=torch.float32, device=dev) if return_lse else None
     st = ops.status_word(dev)
     args = L.PagedDecodeArgs(
-        q.data_ptr(), q.stride(0), q.stride(1), heads, hd ** -0.5 if scale is None else scale, sb, kd, vd,
-        out.data_ptr(), out.stride(0), out.stride(1), ops.ptr(lse), None, 0, st.ptr)
+        q.data_ptr(), qs[0], qs[1], heads, hd ** -0.5 if scale is None else scale, sb, kd, vd,
+        out.data_ptr(), os[0], os[1], ops.ptr(lse), None, 0, st.ptr)
     key = (dev.index, heads, n_kv, hd, kd.dtype, n, sb.max_seq_len)
     nbytes = _workspace_bytes.get(key)
     if nbytes is None:
@@ -262,7 +285,7 @@ def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: op
             _workspace_bytes.clear()
         nbytes = _workspace_bytes[key] = got.value
     if nbytes:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = _empty(nbytes, dtype=torch.uint8, device=dev)
         args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
     _call(L.lib().dkv_paged_decode_attention, args, dev, "dkv_paged_decode_attention")
     if check:

@@ -50,6 +50,9 @@ def half_tables(rope, device: torch.device) -> tuple[Tensor, Tensor]:
     """
     if isinstance(rope, tuple):
         c, s = rope
+        if (c.dtype is torch.float32 and s.dtype is torch.float32 and c.device == device and s.device == device
+                and c.is_contiguous() and s.is_contiguous()):
+            return c, s
         return c.to(device=device, dtype=torch.float32).contiguous(), s.to(device=device, dtype=torch.float32).contiguous()
     cos_full, sin_full = rope.cos_cached, rope.sin_cached
     try:

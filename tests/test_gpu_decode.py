@@ -116,8 +116,10 @@ def check_attention(got, lse, q, tokens_of, scale):
 def run_attention(c, heads, hd, dtype, dev, seed=1, scale=None, amp=1.5):
     g = torch.Generator().manual_seed(seed)
     q = (amp * torch.randn(len(c.lens), heads, hd, generator=g)).to(dtype).to(dev)
-    out, lse = dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), scale=scale, return_lse=True, check=True)
-    check_attention(out, lse, q, c.tokens, hd ** -0.5 if scale is None else scale)
+    for bound in (max(c.lens), 5000):  # short batches are joined within a CTA unless the bound is long
+        seqs = dkv.SeqBatchTensors(cu_seqlens=c.cu, block_tables=c.tables, max_seq_len=bound)
+        out, lse = dkv.paged_decode_attention(q, c.k, c.v, seqs, scale=scale, return_lse=True, check=True)
+        check_attention(out, lse, q, c.tokens, hd ** -0.5 if scale is None else scale)
     return q, out, lse
 
 
@@ -155,6 +157,7 @@ def test_attention_layouts_and_strides(cuda, dtype, layout):
     wide = torch.zeros(4, 11, 70, dtype=dtype, device=cuda)
     qs = wide[:, 1:10, 3:67]
     qs.copy_(q)
+    out = dkv.paged_decode_attention(q, c.k, c.v, c.seqs())
     into = torch.full((4, 10, 65), 7.0, dtype=dtype, device=cuda)
     got = dkv.paged_decode_attention(qs, c.k, c.v, c.seqs(), out=into[:, 1:, 1:])
     assert got.data_ptr() == into[:, 1:, 1:].data_ptr() and torch.equal(got, out)
