@@ -40,15 +40,16 @@ struct Params {
   int64_t table_stride;
   const char *k, *v;
   int64_t k_block, k_slot, k_head, v_block, v_slot, v_head;  // bytes
-  int64_t num_blocks;
+  int num_blocks;
   float *part_o, *part_ml;  // [range][unit][2][kGroup][head_dim], [...][kGroup][2]
   int32_t *status;
   float bias;        // l and O of the parts carry 2^bias
   float scale_log2;  // scale * log2(e): scores are kept in base 2
   int n_seqs, n_kv, heads, group, chunks, units, ranges;
   int hd, block_size;
+  uint32_t div_mul, div_shift;  // i / block_size = i div_mul >> div_shift
   int local;  // a CTA per (sequence, unit): no ranges, no parts
-  int vec;    // rows of K and V in whole 16-byte pieces
+  int copy;   // kPlain, kRows or kPages
   int pairs;  // rows of q and out in whole pairs of 16-bit elements
 };
 
@@ -194,27 +195,46 @@ __device__ __forceinline__ Walk local_walk(const Params &p, int b, int warp, int
 
 // One warp's stream of tiles into its ring of kStages shared-memory stages.  A stage holds 16
 // rows of K, then 16 rows of V, kRow bytes apart (16 more than a row: consecutive rows start 4
-// banks apart, so neither the fragment loads nor 16-byte reads of 8 rows conflict); lanes 0-15
-// look up the K rows, 16-31 the V rows.  The block ids of a tile are loaded one tile ahead and
-// first used when its copies are issued, so their latency passes behind a tile's arithmetic.
+// banks apart, so neither the fragment loads nor 16-byte reads of 8 rows conflict).  The block ids
+// of a tile are loaded one tile ahead and first used when its copies are issued, so their latency
+// passes behind a tile's arithmetic.  Three ways to copy:
+//   kPages  block_size a multiple of the tile: a tile lies in one block, its rows a fixed stride
+//           apart, and a lane's addresses are one base and an immediate or a running sum;
+//   kRows   any block_size: lanes 0-15 look up the K rows, 16-31 the V rows, and pass them on;
+//   kPlain  rows that are not whole 16-byte pieces: element by element.
+// A bulk copy per row (one instruction instead of 8 to 32) is slower for rows of 128 and 256 bytes:
+// such copies start at about one in 14 clocks on an SM, 18 B/clock (681 us against 545 for the
+// 3.5 GB of 32 long sequences).
+enum { kPlain = 0, kRows = 1, kPages = 2 };
+
 template <typename T, int HD, int kStages>
 struct Stream {
-  static constexpr int kRow = HD * static_cast<int>(sizeof(T)) + 16;
+  static constexpr int kSize = static_cast<int>(sizeof(T));
+  static constexpr int kRow = HD * kSize + 16;
   static constexpr int kStage = 2 * kTile * kRow;
-  static constexpr int kBytes = kStages * (kStage + 16);
-  static constexpr int64_t kNoRow = -1, kShort = -(static_cast<int64_t>(1) << 40);  // no token; beyond the table row
+  static constexpr int kBytes = kStages * (kStage + 16);  // the stages' descriptions behind them
+  static constexpr int kPieces = HD * kSize / 16;         // 16-byte pieces of a row
+  static constexpr int kRowLanes = kPieces < 32 ? kPieces : 32;
+  static constexpr int kAtOnce = 32 / kRowLanes;          // rows a copy instruction covers
 
   const Params &p;
   Walk w;
   char *ring;
   uint4 *meta;  // per stage: sequence, flags, bit per token that takes part, end of the stream
-  int u, h0, n_h, lane;
-  int64_t id;  // block of this lane's row of the next tile, or one of the above
-  int slot;
+  const char *k, *v;  // kPages: this lane's first piece of slot 0 of block 0; else its side's base
+  int h0, n_h, lane;
+  int id, slot;  // block and slot of the next tile (kPages) or of this lane's row of it
+  static constexpr int kNoRow = -1, kShort = INT32_MIN;  // negative ids in a table read as kNoRow
 
-  __device__ __forceinline__ Stream(const Params &p_, char *mine, int u_, int h0_, int n_h_, int lane_)
-      : p(p_), ring(mine), meta(reinterpret_cast<uint4 *>(mine + kStages * kStage)), u(u_), h0(h0_), n_h(n_h_),
-        lane(lane_), id(kNoRow), slot(0) {
+  __device__ __forceinline__ Stream(const Params &p_, char *mine, int u, int h0_, int n_h_, int lane_)
+      : p(p_), ring(mine), meta(reinterpret_cast<uint4 *>(mine + kStages * kStage)), h0(h0_), n_h(n_h_), lane(lane_),
+        id(kNoRow), slot(0) {
+    const int row = lane / kRowLanes, piece = lane % kRowLanes;
+    k = p.k + u * p.k_head, v = p.v + u * p.v_head;
+    if (p.copy == kPages) {
+      k += row * p.k_slot + piece * 16;
+      v += row * p.v_slot + piece * 16;
+    }
     if (p.hd < HD) {  // columns past head_dim stay zero in every stage: nothing writes them again
       for (int i = lane; i < kStages * kStage / 16; i += 32)
         reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0, 0, 0, 0);
@@ -223,54 +243,93 @@ struct Stream {
   }
   __device__ __forceinline__ void look_up() {
     id = kNoRow;
-    const int i = w.i + (lane & 15);
+    const int i = w.i + (p.copy == kPages ? 0 : lane & 15);
     if (!w.live || i >= w.end) return;
-    const int blk = i / p.block_size;
+    // i / block_size for any i < 2^31 (multiply by the rounded-up reciprocal)
+    const int blk = static_cast<int>((static_cast<uint64_t>(i) * p.div_mul) >> p.div_shift);
     slot = i - blk * p.block_size;
-    id = blk < w.tlen ? p.tables[w.b * p.table_stride + blk] : kShort;
-  }
-  // the address of this lane's row, 0 if it takes no part
-  __device__ __forceinline__ uint64_t row_address() const {
-    const int i = w.i + (lane & 15);
-    if (i >= w.end) return 0;
-    if (id < 0 || id >= p.num_blocks) {
-      record_error(p.status, id == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
-      return 0;
-    }
-    const char *a = lane < 16 ? p.k + id * p.k_block + slot * p.k_slot + u * p.k_head
-                              : p.v + id * p.v_block + slot * p.v_slot + u * p.v_head;
-    return reinterpret_cast<uint64_t>(a);
+    id = kShort;
+    if (blk < w.tlen) id = max(__ldg(p.tables + w.b * p.table_stride + blk), kNoRow);
   }
   __device__ __forceinline__ void start(const Walk &from) {
     w = from;
     if (!p.local) walk_seq<T>(p, w, h0, n_h, lane);
     look_up();
   }
+  // the rows of one side of a tile in one block, `rows` of them (the others zero)
+  __device__ __forceinline__ void copy_side(uint32_t dst, const char *src, int64_t slot_bytes, int rows) {
+    const int64_t step = slot_bytes * kAtOnce;
+#pragma unroll
+    for (int r = 0; r < kTile; r += kAtOnce) {
+#pragma unroll
+      for (int c = 0; c < kPieces; c += 32) {
+        if ((c + lane % kRowLanes) * 16 < p.hd * kSize)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * kRow + c * 16), "l"(src + c * 16),
+                       "r"(r + lane / kRowLanes < rows ? 16 : 0)
+                       : "memory");
+      }
+      src += step;
+    }
+  }
+  __device__ __forceinline__ void copy_side(uint32_t dst, const char *src, int64_t slot_bytes) {  // all of them
+    const int64_t step = slot_bytes * kAtOnce;
+#pragma unroll
+    for (int r = 0; r < kTile; r += kAtOnce) {
+#pragma unroll
+      for (int c = 0; c < kPieces; c += 32)
+        if ((c + lane % kRowLanes) * 16 < p.hd * kSize) cp_async_16(dst + r * kRow + c * 16, src + c * 16);
+      src += step;
+    }
+  }
   // issues the next tile's copies into stage s (one cp.async group, empty past the end)
   __device__ __forceinline__ void fill(int s) {
     if (w.live) {
-      const uint64_t addr = row_address();
-      const uint32_t there = __ballot_sync(0xffffffffu, addr != 0);
       char *stage = ring + s * kStage;
-      if (p.vec) {
-        constexpr int kPieces = HD * static_cast<int>(sizeof(T)) / 16;  // 16-byte pieces of a row
-#pragma unroll
-        for (int c = lane; c < 32 * kPieces; c += 32) {
-          const int row = c / kPieces, piece = c % kPieces;
-          const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
-          if (piece * 16 < p.hd * static_cast<int>(sizeof(T)))
-            cp_async16(stage + row * kRow + piece * 16,
-                       a ? reinterpret_cast<const char *>(a) + piece * 16 : p.k, a ? 16 : 0);
+      uint32_t there;
+      if (p.copy == kPages) {
+        int rows = min(w.end - w.i, kTile);
+        const bool good = id >= 0 && id < p.num_blocks;
+        if (!good) {
+          if (lane == 0) record_error(p.status, id == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
+          rows = 0;
+        }
+        there = (1u << rows) - 1;
+        const uint32_t dst = smem_u32(stage) + lane / kRowLanes * kRow + lane % kRowLanes * 16;
+        const int64_t at = rows ? id : 0;
+        const char *ks = k + at * p.k_block + slot * p.k_slot, *vs = v + at * p.v_block + slot * p.v_slot;
+        if (rows == kTile) {
+          copy_side(dst, ks, p.k_slot);
+          copy_side(dst + kTile * kRow, vs, p.v_slot);
+        } else {
+          copy_side(dst, ks, p.k_slot, rows);
+          copy_side(dst + kTile * kRow, vs, p.v_slot, rows);
         }
       } else {
-        for (int row = 0; row < 32; ++row) {
-          const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
-          T *dst = reinterpret_cast<T *>(stage + row * kRow);
-          for (int d = lane; d < p.hd; d += 32) dst[d] = a ? reinterpret_cast<const T *>(a)[d] : T(0.f);
+        const bool wanted = w.i + (lane & 15) < w.end;
+        const bool good = wanted && id >= 0 && id < p.num_blocks;
+        if (wanted && !good) record_error(p.status, id == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
+        there = __ballot_sync(0xffffffffu, good) & 0xffffu;
+        const char *src = lane < 16 ? k + id * p.k_block + slot * p.k_slot : v + id * p.v_block + slot * p.v_slot;
+        const uint64_t addr = good ? reinterpret_cast<uint64_t>(src) : 0;
+        if (p.copy == kRows) {
+#pragma unroll
+          for (int c = lane; c < 32 * kPieces; c += 32) {
+            const int row = c / kPieces, piece = c % kPieces;
+            const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
+            if (piece * 16 < p.hd * kSize)
+              cp_async16(stage + row * kRow + piece * 16, a ? reinterpret_cast<const char *>(a) + piece * 16 : p.k,
+                         a ? 16 : 0);
+          }
+        } else {
+          for (int row = 0; row < 32; ++row) {
+            const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
+            T *dst = reinterpret_cast<T *>(stage + row * kRow);
+            for (int d = lane; d < p.hd; d += 32) dst[d] = a ? reinterpret_cast<const T *>(a)[d] : T(0.f);
+          }
         }
       }
       const bool last = !p.local && w.i + kTile >= w.end;
-      if (lane == 0) meta[s] = make_uint4(w.b, w.flags | (last ? kLast : 0), there & 0xffffu, 0);
+      if (lane == 0) meta[s] = make_uint4(w.b, w.flags | (last ? kLast : 0), there, 0);
       walk_next<T>(p, w, h0, n_h, lane);
       look_up();
     } else if (lane == 0) {
@@ -279,6 +338,12 @@ struct Stream {
     cp_async_commit();
   }
 };
+
+__device__ __forceinline__ float ex2(float x) {  // 2^x to 2 ulp, subnormal results 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
 // The join within a CTA: each warp's (m, l) and O (rows of HD + 4: no bank conflicts) lie at the
 // front of its ring.
@@ -422,8 +487,8 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
       for (int k = 8; k > 0; k >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, k));
       const float top = fmaxf(m[g], t);
       const float base = top == __int_as_float(0xff800000) ? 0.f : top;  // nothing seen yet: any finite base
-      const float keep = exp2f(m[g] - base);
-      const float e = exp2f(x - base);
+      const float keep = ex2(m[g] - base);
+      const float e = ex2(x - base);
       m[g] = top;
       l[g] = l[g] * keep + (half == 0 ? e : 0.f);
       if (half == 0) ps[key * G + g] = e;
@@ -652,38 +717,42 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
 #pragma unroll
       for (int n = 0; n < N; ++n) E::mma(sc[n][k & 1], a, qf[n][k][0], qf[n][k][1]);
     }
-    const bool in0 = (mt.z >> g) & 1, in1 = (mt.z >> (g + 8)) & 1;
     uint32_t ph[N][2], pl[N][2];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      // sc: {token g, token g + 8} x {head 2t, head 2t + 1}
+      // x: {token g, token g + 8} x {head 2t, head 2t + 1}
       float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        x[e] = (e < 2 ? in0 : in1) ? (sc[n][0][e] + sc[n][1][e]) * p.scale_log2 : kNegInf;
-      float keep[2];
-      bool moved = false;
+      for (int e = 0; e < 4; ++e) x[e] = (sc[n][0][e] + sc[n][1][e]) * p.scale_log2;
+      if (mt.z != 0xffffu) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!((mt.z >> (g + (e & 2) * 4)) & 1)) x[e] = kNegInf;
+      }
+      // m is any value not far below the scores so far: it moves (and O with it) only when a
+      // score passes it, which after the first tiles is rare
+      const float top0 = fmaxf(x[0], x[2]), top1 = fmaxf(x[1], x[3]);
+      if (__any_sync(0xffffffffu, top0 > m[n][0] || top1 > m[n][1])) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float top = c ? top1 : top0;
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          top = fmaxf(top, m[n][c]);
+          const float keep = ex2(m[n][c] - (top == kNegInf ? 0.f : top));
+          m[n][c] = top;
+          l[n][c] *= keep;
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) o[n][k][c] *= keep, o[n][k][2 + c] *= keep;
+        }
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float top = fmaxf(x[c], x[c + 2]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        top = fmaxf(top, m[n][c]);
-        moved |= top > m[n][c];
-        const float base = top == kNegInf ? 0.f : top;  // nothing seen yet: any finite base
-        keep[c] = exp2f(m[n][c] - base);
-        x[c] = exp2f(x[c] - base + E::kBias);
-        x[c + 2] = exp2f(x[c + 2] - base + E::kBias);
-        m[n][c] = top;
-        l[n][c] = fmaf(l[n][c], keep[c], x[c] + x[c + 2]);
-      }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          o[n][k][0] *= keep[0], o[n][k][1] *= keep[1];
-          o[n][k][2] *= keep[0], o[n][k][3] *= keep[1];
-        }
+        const float base = (m[n][c] == kNegInf ? 0.f : m[n][c]) - E::kBias;  // nothing seen yet: any finite base
+        x[c] = ex2(x[c] - base);
+        x[c + 2] = ex2(x[c + 2] - base);
+        l[n][c] += x[c] + x[c + 2];
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -1157,7 +1226,8 @@ extern "C" int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv
   p.k = static_cast<const char *>(k.base), p.v = static_cast<const char *>(v.base);
   p.k_block = k.stride_block * sz, p.k_slot = k.stride_slot * sz, p.k_head = k.stride_head * sz;
   p.v_block = v.stride_block * sz, p.v_slot = v.stride_slot * sz, p.v_head = v.stride_head * sz;
-  p.num_blocks = k.num_blocks < v.num_blocks ? k.num_blocks : v.num_blocks;
+  const int64_t blocks = k.num_blocks < v.num_blocks ? k.num_blocks : v.num_blocks;
+  p.num_blocks = static_cast<int>(blocks < INT32_MAX ? blocks : INT32_MAX);  // ids are 32-bit
   p.part_o = static_cast<float *>(a.workspace);
   p.part_ml = s.parts ? p.part_o + s.o_bytes / 4 : nullptr;
   p.status = a.status;
@@ -1167,10 +1237,15 @@ extern "C" int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv
   p.chunks = s.chunks, p.units = s.units, p.ranges = s.ranges;
   p.local = s.local;
   p.hd = k.head_dim, p.block_size = k.block_size;
+  // for i < 2^31 and 2^(s - 1) < block_size <= 2^s: mul = floor(2^(31 + s) / block_size) + 1 is off by at
+  // most one part in 2^31 and fits 32 bits (division by invariant integers, Granlund and Montgomery)
+  p.div_shift = 31;
+  while ((1u << (p.div_shift - 31)) < static_cast<uint32_t>(k.block_size)) ++p.div_shift;
+  p.div_mul = static_cast<uint32_t>((1ull << p.div_shift) / static_cast<uint32_t>(k.block_size) + 1);
   // 16-byte copies where every row of K and V starts on 16 bytes and is a multiple of 16 long
   const int64_t all = p.k_block | p.k_slot | p.k_head | p.v_block | p.v_slot | p.v_head | (p.hd * sz) |
                       static_cast<int64_t>(reinterpret_cast<uintptr_t>(k.base) | reinterpret_cast<uintptr_t>(v.base));
-  p.vec = all % 16 == 0;
+  p.copy = all % 16 ? pattn::kPlain : k.block_size % pattn::kTile ? pattn::kRows : pattn::kPages;
   const int64_t two = p.q_seq | p.q_head | p.out_seq | p.out_head | (p.hd * sz) |
                       static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out));
   p.pairs = two % 4 == 0;
