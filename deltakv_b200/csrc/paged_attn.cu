@@ -195,12 +195,14 @@ __device__ __forceinline__ Walk local_walk(const Params &p, int b, int warp, int
 
 // One warp's stream of tiles into its ring of kStages shared-memory stages.  A stage holds 16
 // rows of K, then 16 rows of V, kRow bytes apart (16 more than a row: consecutive rows start 4
-// banks apart, so neither the fragment loads nor 16-byte reads of 8 rows conflict).  The block ids
-// of a tile are loaded one tile ahead and first used when its copies are issued, so their latency
-// passes behind a tile's arithmetic.  Three ways to copy:
+// banks apart, so neither the fragment loads nor 16-byte reads of 8 rows conflict).  Three ways to
+// copy:
 //   kPages  block_size a multiple of the tile: a tile lies in one block, its rows a fixed stride
-//           apart, and a lane's addresses are one base and an immediate or a running sum;
-//   kRows   any block_size: lanes 0-15 look up the K rows, 16-31 the V rows, and pass them on;
+//           apart, and a lane's addresses are one base and an immediate or a running sum.  Each
+//           lane holds the block id of another tile to come, so the table is waited for once in
+//           32 tiles;
+//   kRows   any block_size: lanes 0-15 look up the K rows, 16-31 the V rows, a tile ahead, and
+//           pass them on;
 //   kPlain  rows that are not whole 16-byte pieces: element by element.
 // A bulk copy per row (one instruction instead of 8 to 32) is slower for rows of 128 and 256 bytes:
 // such copies start at about one in 14 clocks on an SM, 18 B/clock (681 us against 545 for the
@@ -223,12 +225,13 @@ struct Stream {
   uint4 *meta;  // per stage: sequence, flags, bit per token that takes part, end of the stream
   const char *k, *v;  // kPages: this lane's first piece of slot 0 of block 0; else its side's base
   int h0, n_h, lane;
-  int id, slot;  // block and slot of the next tile (kPages) or of this lane's row of it
+  int id, slot;  // block and slot of this lane's row of the next tile; kPages: block of the tile
+  int tile;      // kPages: of the 32 tiles that the lanes hold ids of, the next
   static constexpr int kNoRow = -1, kShort = INT32_MIN;  // negative ids in a table read as kNoRow
 
   __device__ __forceinline__ Stream(const Params &p_, char *mine, int u, int h0_, int n_h_, int lane_)
       : p(p_), ring(mine), meta(reinterpret_cast<uint4 *>(mine + kStages * kStage)), h0(h0_), n_h(n_h_), lane(lane_),
-        id(kNoRow), slot(0) {
+        id(kNoRow), slot(0), tile(0) {
     const int row = lane / kRowLanes, piece = lane % kRowLanes;
     k = p.k + u * p.k_head, v = p.v + u * p.v_head;
     if (p.copy == kPages) {
@@ -241,15 +244,27 @@ struct Stream {
       __syncwarp();
     }
   }
+  __device__ __forceinline__ int block_of(int i) const {  // i / block_size for any i < 2^31
+    return static_cast<int>((static_cast<uint64_t>(i) * p.div_mul) >> p.div_shift);
+  }
+  __device__ __forceinline__ int id_at(int blk) const {
+    return blk < w.tlen ? max(__ldg(p.tables + w.b * p.table_stride + blk), kNoRow) : kShort;
+  }
   __device__ __forceinline__ void look_up() {
-    id = kNoRow;
-    const int i = w.i + (p.copy == kPages ? 0 : lane & 15);
-    if (!w.live || i >= w.end) return;
-    // i / block_size for any i < 2^31 (multiply by the rounded-up reciprocal)
-    const int blk = static_cast<int>((static_cast<uint64_t>(i) * p.div_mul) >> p.div_shift);
-    slot = i - blk * p.block_size;
-    id = kShort;
-    if (blk < w.tlen) id = max(__ldg(p.tables + w.b * p.table_stride + blk), kNoRow);
+    if (!w.live) return;
+    if (p.copy == kPages) {
+      if (++tile < 32 && !(w.flags & kFirst)) return;
+      tile = 0;
+      const int i = w.i + lane * w.step;
+      id = i >= 0 && i < w.end ? id_at(block_of(i)) : kNoRow;
+    } else {
+      const int i = w.i + (lane & 15);
+      id = kNoRow;
+      if (i >= w.end) return;
+      const int blk = block_of(i);
+      slot = i - blk * p.block_size;
+      id = id_at(blk);
+    }
   }
   __device__ __forceinline__ void start(const Walk &from) {
     w = from;
@@ -288,15 +303,15 @@ struct Stream {
       uint32_t there;
       if (p.copy == kPages) {
         int rows = min(w.end - w.i, kTile);
-        const bool good = id >= 0 && id < p.num_blocks;
-        if (!good) {
-          if (lane == 0) record_error(p.status, id == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
+        const int block = __shfl_sync(0xffffffffu, id, tile);
+        if (block < 0 || block >= p.num_blocks) {
+          if (lane == 0) record_error(p.status, block == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
           rows = 0;
         }
         there = (1u << rows) - 1;
         const uint32_t dst = smem_u32(stage) + lane / kRowLanes * kRow + lane % kRowLanes * 16;
-        const int64_t at = rows ? id : 0;
-        const char *ks = k + at * p.k_block + slot * p.k_slot, *vs = v + at * p.v_block + slot * p.v_slot;
+        const int64_t at = rows ? block : 0, in = w.i - block_of(w.i) * p.block_size;
+        const char *ks = k + at * p.k_block + in * p.k_slot, *vs = v + at * p.v_block + in * p.v_slot;
         if (rows == kTile) {
           copy_side(dst, ks, p.k_slot);
           copy_side(dst + kTile * kRow, vs, p.v_slot);

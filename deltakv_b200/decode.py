@@ -30,7 +30,7 @@ from deltakv_b200.rope import half_tables
 
 
 _I32 = torch.int32
-_empty, _raw_stream = torch.empty, torch._C._cuda_getCurrentRawStream
+_empty, _empty_like, _raw_stream = torch.empty, torch.empty_like, torch._C._cuda_getCurrentRawStream
 # A decode step calls these operators once a layer, with kernels of a few microseconds: the checks
 # read each attribute once and take strides as tuples, and the stream is taken as its raw handle
 # (current_stream() builds an object: 3 us).
@@ -210,8 +210,8 @@ def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, sl
             raise ValueError(f"rope tables {tuple(shape)} do not cover head_dim {hd}")
         max_pos = shape[0]
     if q is not None and q_out is None:
-        q_out = _empty((rows, n_q, hd), dtype=dtype, device=dev)
-        os = (n_q * hd, hd)
+        q_out = _empty_like(q)
+        os = q_out.stride()
     st = ops.status_word(dev)
     args = L.AppendArgs(
         k.data_ptr(), v.data_ptr(), ops.ptr(q), ops.dkv_dtype(dtype), n_q, rows, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1],
@@ -260,7 +260,6 @@ def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: op
         raise ValueError(f"block_tables has {tables.shape[0]} rows for {n} sequences")
     if lens is not None and (lens.numel() < n or not lens.is_contiguous()):
         raise ValueError(f"table_lens must be a contiguous vector of {n}")
-    os = (heads * hd, hd)
     if out is not None:
         os = _rows(out, "out", n, heads, hd)
         if out.dtype is not dtype:
@@ -268,7 +267,8 @@ def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: op
     dev = _same_device("paged_decode_attention", q, k_pages, v_pages, cu, tables, lens, out)
     sb = seqs.struct()
     if out is None:
-        out = _empty((n, heads, hd), dtype=dtype, device=dev)
+        out = _empty_like(q)
+        os = out.stride()
     lse = _empty((n, heads), dtype=torch.float32, device=dev) if return_lse else None
     st = ops.status_word(dev)
     args = L.PagedDecodeArgs(
