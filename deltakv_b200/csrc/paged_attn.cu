@@ -401,18 +401,18 @@ __device__ __forceinline__ void local_join(const Params &p, const char *smem, in
 // head_dim are zero), G: query heads of the unit (rounded up), W: warps per CTA.  Scores: lane =
 // (token, half of the head); output: lane = 4 columns, the tokens dealt to 128 / HD groups of
 // lanes where the head is shorter than 128.
-template <int HD, int G, int W>
+template <int HD, int G, int W, int kStages_>
 struct Simt {
-  static constexpr int kStages = 3;
+  static constexpr int kStages = kStages_;
   using S = Stream<float, HD, kStages>;
   static constexpr int kQRow = (HD + 8) * 4;  // two halves, 16 B apart in banks
-  static constexpr int kWarpBytes = S::kBytes + G * kQRow + kTile * G * 4;
+  static constexpr int kWarpBytes = S::kBytes + G * kQRow + kTile * G * 8;
   static constexpr int kSmem = W * kWarpBytes;
 };
 
-template <int HD, int G, int W>
-__global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Params p) {
-  using C = Simt<HD, G, W>;
+template <int HD, int G, int W, int kStages>
+__global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__ Params p) {
+  using C = Simt<HD, G, W, kStages>;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -428,14 +428,15 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
 
   char *mine = smem + warp * C::kWarpBytes;
   float *qs = reinterpret_cast<float *>(mine + C::S::kBytes);
-  float *ps = qs + C::kQRow / 4 * G;
+  uint64_t *ps = reinterpret_cast<uint64_t *>(qs + C::kQRow / 4 * G);  // [token][head]: the weight, twice
   typename C::S stream(p, mine, u, h0, n_h, lane);
   stream.start(p.local ? local_walk(p, r, warp, W) : range_walk(p, ln, r, lane));
 
   constexpr int kVec = HD >= 128 ? HD / 128 : 1;         // float4 columns per lane
   constexpr int kLanes = HD >= 128 ? 32 : HD / 4;        // lanes per token in the output product
   constexpr int kSplit = 32 / kLanes;                    // tokens handled at once there
-  float m[G], l[G], o[G][kVec][4];
+  float m[G], l[G];
+  uint64_t o[G][kVec][2];  // pairs of columns, for the packed fma
   const int key = lane & 15, half = lane >> 4;
   const int oc = lane % kLanes, ok = lane / kLanes;
   auto clear = [&]() {
@@ -445,7 +446,7 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
 #pragma unroll
       for (int j = 0; j < kVec; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[g][j][e] = 0.f;
+        for (int e = 0; e < 2; ++e) o[g][j][e] = 0;
     }
   };
   // sums over the lanes that share a head (l) or a column (o)
@@ -455,9 +456,14 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
 #pragma unroll
     for (int j = 0; j < kVec; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int k = kLanes; k < 32; k <<= 1) o[g][j][i] += __shfl_xor_sync(0xffffffffu, o[g][j][i], k);
+        for (int k = kLanes; k < 32; k <<= 1) o[g][j][i] = add2(o[g][j][i], __shfl_xor_sync(0xffffffffu, o[g][j][i], k));
+  };
+  auto column = [&](int g, int j, int e) {
+    float x, y;
+    f2unpack(o[g][j][e / 2], x, y);
+    return e & 1 ? y : x;
   };
   clear();
 
@@ -480,54 +486,71 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
       __syncwarp();
     }
     const float *kr = reinterpret_cast<const float *>(mine + s * C::S::kStage + key * C::S::kRow) + half * (HD / 2);
-    float acc[G];
+    uint64_t acc[G];
 #pragma unroll
-    for (int g = 0; g < G; ++g) acc[g] = 0.f;
+    for (int g = 0; g < G; ++g) acc[g] = 0;
 #pragma unroll 4
     for (int d = 0; d < HD / 2; d += 4) {
-      const float4 x = *reinterpret_cast<const float4 *>(kr + d);
+      const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(kr + d);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const float4 y = *reinterpret_cast<const float4 *>(qs + g * (C::kQRow / 4) + half * (HD / 2 + 4) + d);
-        acc[g] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, acc[g]))));
+        const ulonglong2 y =
+            *reinterpret_cast<const ulonglong2 *>(qs + g * (C::kQRow / 4) + half * (HD / 2 + 4) + d);
+        acc[g] = fma2(x.y, y.y, fma2(x.x, y.x, acc[g]));
       }
     }
     const bool there = (mt.z >> key) & 1;
+    float x[G];
+    bool past = false;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      float x = acc[g] + __shfl_xor_sync(0xffffffffu, acc[g], 16);
-      x = there ? x * p.scale_log2 : __int_as_float(0xff800000);
-      float t = x;
+      float lo, hi;
+      f2unpack(acc[g], lo, hi);
+      lo += hi;
+      lo += __shfl_xor_sync(0xffffffffu, lo, 16);
+      x[g] = there ? lo * p.scale_log2 : __int_as_float(0xff800000);
+      past |= x[g] > m[g];
+    }
+    if (__any_sync(0xffffffffu, past)) {  // as in the tensor-core walk: m moves only when it must
 #pragma unroll
-      for (int k = 8; k > 0; k >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, k));
-      const float top = fmaxf(m[g], t);
-      const float base = top == __int_as_float(0xff800000) ? 0.f : top;  // nothing seen yet: any finite base
-      const float keep = ex2(m[g] - base);
-      const float e = ex2(x - base);
-      m[g] = top;
-      l[g] = l[g] * keep + (half == 0 ? e : 0.f);
-      if (half == 0) ps[key * G + g] = e;
+      for (int g = 0; g < G; ++g) {
+        float top = x[g];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j)
+        for (int k = 8; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        top = fmaxf(m[g], top);
+        const float keep = ex2(m[g] - (top == __int_as_float(0xff800000) ? 0.f : top));
+        m[g] = top;
+        l[g] *= keep;
+        const uint64_t two = f2pack(keep, keep);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[g][j][i] *= keep;
+        for (int j = 0; j < kVec; ++j) o[g][j][0] = mul2(o[g][j][0], two), o[g][j][1] = mul2(o[g][j][1], two);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float e = ex2(x[g] - (m[g] == __int_as_float(0xff800000) ? 0.f : m[g]));
+      if (half == 0) {
+        l[g] += e;
+        ps[key * G + g] = f2pack(e, e);
+      }
     }
     __syncwarp();
 #pragma unroll 4
     for (int t = ok; t < kTile; t += kSplit) {
       const float *vr = reinterpret_cast<const float *>(mine + s * C::S::kStage + (kTile + t) * C::S::kRow);
-      float e[G];
+      uint64_t e[G];
 #pragma unroll
-      for (int g = 0; g < G; ++g) e[g] = ps[t * G + g];
+      for (int g = 0; g < G; g += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(ps + t * G + g);
+        e[g] = two.x, e[g + 1] = two.y;
+      }
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        const float4 x = *reinterpret_cast<const float4 *>(vr + j * 128 + oc * 4);
+        const ulonglong2 y = *reinterpret_cast<const ulonglong2 *>(vr + j * 128 + oc * 4);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          o[g][j][0] = fmaf(e[g], x.x, o[g][j][0]);
-          o[g][j][1] = fmaf(e[g], x.y, o[g][j][1]);
-          o[g][j][2] = fmaf(e[g], x.z, o[g][j][2]);
-          o[g][j][3] = fmaf(e[g], x.w, o[g][j][3]);
+          o[g][j][0] = fma2(e[g], y.x, o[g][j][0]);
+          o[g][j][1] = fma2(e[g], y.y, o[g][j][1]);
         }
       }
     }
@@ -547,7 +570,7 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
             for (int j = 0; j < kVec; ++j)
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                if (j * 128 + oc * 4 + i < p.hd) dst[j * 128 + oc * 4 + i] = o[g][j][i] * inv;
+                if (j * 128 + oc * 4 + i < p.hd) dst[j * 128 + oc * 4 + i] = column(g, j, i) * inv;
             if (p.lse && lane == 0)
               p.lse[static_cast<int64_t>(b) * p.heads + h] = (m[g] + log2f(sum)) * 0.6931471805599453f;
           } else {
@@ -556,7 +579,7 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
             for (int j = 0; j < kVec; ++j)
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                if (j * 128 + oc * 4 + i < p.hd) dst[j * 128 + oc * 4 + i] = o[g][j][i];
+                if (j * 128 + oc * 4 + i < p.hd) dst[j * 128 + oc * 4 + i] = column(g, j, i);
             if (lane == 0) {
               p.part_ml[(part * G + g) * 2] = m[g];
               p.part_ml[(part * G + g) * 2 + 1] = sum;
@@ -580,7 +603,7 @@ __global__ void __launch_bounds__(W * 32) simt_kernel(const __grid_constant__ Pa
 #pragma unroll
         for (int j = 0; j < kVec; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mine_out->o[g][j * 128 + oc * 4 + e] = o[g][j][e];
+          for (int e = 0; e < 4; ++e) mine_out->o[g][j * 128 + oc * 4 + e] = column(g, j, e);
       }
       if (lane == 0) mine_out->m[g] = m[g], mine_out->l[g] = l[g];
     }
@@ -1052,6 +1075,23 @@ struct Shape {
   int64_t o_bytes, bytes;
 };
 
+// Warps of a CTA (one CTA an SM) and stages of a warp's ring: as many warps as registers and 220 KB
+// allow.  More warps hide each other's latency better than more stages: at head_dim 128 and 16 bits,
+// 4 x 6 / 6 x 4 / 8 x 3 / 12 x 2 (warps x stages) walk 32 long sequences in 653 / 596 / 564 / 549 us.
+// Two blocks of heads need more than the 168 registers that 12 warps leave.
+struct Variant {
+  int warps, stages;
+};
+constexpr Variant variant(bool f32, int hd, int g) {
+  if (f32 && hd == 256) return {3, 2};
+  if (f32 && hd == 128) return g == 4 ? Variant{6, 2} : Variant{5, 2};
+  if (f32) return hd == 64 ? (g == 4 ? Variant{12, 2} : Variant{10, 2}) : Variant{12, 3};
+  if (hd == 256) return {6, 2};
+  if (hd == 128) return g == 8 ? Variant{12, 2} : Variant{8, 3};
+  if (hd == 64) return g == 8 ? Variant{12, 4} : Variant{8, 6};
+  return g == 8 ? Variant{16, 4} : Variant{12, 6};
+}
+
 int sm_count(int *out) {
   static int cached[64];
   int dev = 0;
@@ -1089,13 +1129,9 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   if (rc != DKV_OK) return rc;
   const int hd = a->k_pages.head_dim, group = a->n_q_heads / a->k_pages.n_heads;
   s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-  if (a->k_pages.dtype == DKV_F32) {
-    s->g = group <= 4 ? 4 : 8;
-    s->warps = s->hd_pad == 256 ? 2 : s->hd_pad == 128 ? 4 : 8;
-  } else {
-    s->g = group <= 8 ? 8 : 16;
-    s->warps = s->hd_pad == 256 ? 4 : 8;
-  }
+  const bool f32 = a->k_pages.dtype == DKV_F32;
+  s->g = f32 ? (group <= 4 ? 4 : 8) : (group <= 8 ? 8 : 16);
+  s->warps = variant(f32, s->hd_pad, s->g).warps;
   s->chunks = (group + s->g - 1) / s->g;
   s->units = a->k_pages.n_heads * s->chunks;
   s->local = a->seqs.max_seq_len <= kLocalTokens && static_cast<int64_t>(a->seqs.n_seqs) * s->units <= sms;
@@ -1123,13 +1159,13 @@ int allow_smem(int bytes) {
   return DKV_OK;
 }
 
-template <int HD, int G, int W>
+template <int HD, int G, int W, int kStages>
 int launch_simt(const Params &p, int grid, cudaStream_t st) {
-  using C = Simt<HD, G, W>;
+  using C = Simt<HD, G, W, kStages>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
-  const int rc = allow_smem<simt_kernel<HD, G, W>>(C::kSmem);
+  const int rc = allow_smem<simt_kernel<HD, G, W, kStages>>(C::kSmem);
   if (rc != DKV_OK) return rc;
-  simt_kernel<HD, G, W><<<grid, W * 32, C::kSmem, st>>>(p);
+  simt_kernel<HD, G, W, kStages><<<grid, W * 32, C::kSmem, st>>>(p);
   DKV_CUDA_CHECK(cudaGetLastError());
   return DKV_OK;
 }
@@ -1145,28 +1181,38 @@ int launch_mma(const Params &p, int grid, cudaStream_t st) {
   return DKV_OK;
 }
 
+#define DKV_WALK_CASE(HD, G)        \
+  if (s.hd_pad == HD && s.g == G) { \
+    constexpr Variant v = variant(kF32, HD, G); \
+    DKV_WALK_LAUNCH(HD, G, v)       \
+  }
 template <int DT>
 int launch_walk(const Params &p, const Shape &s, int grid, cudaStream_t st) {
-#define DKV_MMA_CASE(HD, W, S)                                                    \
-  if (s.hd_pad == HD && s.g == 8) return launch_mma<DT, HD, 1, W, S>(p, grid, st); \
-  if (s.hd_pad == HD && s.g == 16) return launch_mma<DT, HD, 2, W, S>(p, grid, st);
-  DKV_MMA_CASE(32, 8, 8)
-  DKV_MMA_CASE(64, 8, 6)
-  DKV_MMA_CASE(128, 8, 3)
-  DKV_MMA_CASE(256, 4, 3)
-#undef DKV_MMA_CASE
-  return DKV_ERR_UNSUPPORTED;
-}
-template <>
-int launch_walk<DKV_F32>(const Params &p, const Shape &s, int grid, cudaStream_t st) {
-#define DKV_SIMT_CASE(HD, W)                                                 \
-  if (s.hd_pad == HD && s.g == 4) return launch_simt<HD, 4, W>(p, grid, st); \
-  if (s.hd_pad == HD && s.g == 8) return launch_simt<HD, 8, W>(p, grid, st);
-  DKV_SIMT_CASE(32, 8)
-  DKV_SIMT_CASE(64, 8)
-  DKV_SIMT_CASE(128, 4)
-  DKV_SIMT_CASE(256, 2)
-#undef DKV_SIMT_CASE
+  constexpr bool kF32 = DT == DKV_F32;
+  if constexpr (kF32) {
+#define DKV_WALK_LAUNCH(HD, G, v) return launch_simt<HD, G, v.warps, v.stages>(p, grid, st);
+    DKV_WALK_CASE(32, 4)
+    DKV_WALK_CASE(32, 8)
+    DKV_WALK_CASE(64, 4)
+    DKV_WALK_CASE(64, 8)
+    DKV_WALK_CASE(128, 4)
+    DKV_WALK_CASE(128, 8)
+    DKV_WALK_CASE(256, 4)
+    DKV_WALK_CASE(256, 8)
+#undef DKV_WALK_LAUNCH
+  } else {
+#define DKV_WALK_LAUNCH(HD, G, v) return launch_mma<DT, HD, G / 8, v.warps, v.stages>(p, grid, st);
+    DKV_WALK_CASE(32, 8)
+    DKV_WALK_CASE(32, 16)
+    DKV_WALK_CASE(64, 8)
+    DKV_WALK_CASE(64, 16)
+    DKV_WALK_CASE(128, 8)
+    DKV_WALK_CASE(128, 16)
+    DKV_WALK_CASE(256, 8)
+    DKV_WALK_CASE(256, 16)
+#undef DKV_WALK_LAUNCH
+  }
+#undef DKV_WALK_CASE
   return DKV_ERR_UNSUPPORTED;
 }
 
