@@ -97,18 +97,26 @@ struct Window {
   }
   __device__ __forceinline__ int at(int b) const { return __shfl_sync(0xffffffffu, cu, b - base); }
   __device__ __forceinline__ int table_len(int b) const { return __shfl_sync(0xffffffffu, tlen, b - base); }
+  // the first look of find, which does not depend on x: issued while the line's length is loaded
+  __device__ __forceinline__ void look(const Params &p, int lane) {
+    if (p.n_seqs > 31)
+      cu = p.cu[min(lane * ((p.n_seqs + 31) / 32), p.n_seqs)];
+    else
+      load(p, 0, lane);
+  }
   // the largest b with cu[b] + kSeqCost b <= x, and a window that starts at or before it
   __device__ __forceinline__ int find(const Params &p, uint32_t x, int lane) {
     int lo = 0, hi = p.n_seqs;
     while (hi - lo > 31) {
       const int step = (hi - lo + 31) / 32;
       const int b = lo + lane * step;
-      const bool in = b < hi && static_cast<uint32_t>(p.cu[b]) + static_cast<uint32_t>(kSeqCost) * b <= x;
+      if (lo > 0 || hi < p.n_seqs) cu = p.cu[min(b, p.n_seqs)];
+      const bool in = b < hi && static_cast<uint32_t>(cu) + static_cast<uint32_t>(kSeqCost) * b <= x;
       const int k = __popc(__ballot_sync(0xffffffffu, in));
       if (k > 1) lo += (k - 1) * step;
       hi = min(hi, lo + step);
     }
-    load(p, lo, lane);
+    if (p.n_seqs > 31) load(p, lo, lane);
     const bool in = lo + lane < hi && static_cast<uint32_t>(cu) + static_cast<uint32_t>(kSeqCost) * (lo + lane) <= x;
     return lo + max(__popc(__ballot_sync(0xffffffffu, in)) - 1, 0);
   }
@@ -174,8 +182,9 @@ __device__ __forceinline__ void walk_next(const Params &p, Walk &w, int h0, int 
   walk_seq<T>(p, w, h0, n_h, lane);
 }
 // the walk of range r
-__device__ __forceinline__ Walk range_walk(const Params &p, const Line &ln, uint32_t r, int lane) {
+__device__ __forceinline__ Walk range_walk(const Params &p, const Window &win, const Line &ln, uint32_t r, int lane) {
   Walk w;
+  w.win = win;
   w.x0 = ln.start(r), w.x1 = ln.start(r + 1);
   w.b = w.win.find(p, w.x0, lane);
   w.step = kTile;
@@ -419,7 +428,9 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
   const int gw = p.local ? blockIdx.x : blockIdx.x * W + warp;
   const int r = gw / p.units, unit = gw - r * p.units;  // r: the range, or the sequence where local
   Line ln;
+  Window win;
   if (!p.local) {
+    win.look(p, lane);
     ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
     if (r >= static_cast<int>(ln.ranges)) return;
   }
@@ -430,7 +441,7 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
   float *qs = reinterpret_cast<float *>(mine + C::S::kBytes);
   uint64_t *ps = reinterpret_cast<uint64_t *>(qs + C::kQRow / 4 * G);  // [token][head]: the weight, twice
   typename C::S stream(p, mine, u, h0, n_h, lane);
-  stream.start(p.local ? local_walk(p, r, warp, W) : range_walk(p, ln, r, lane));
+  stream.start(p.local ? local_walk(p, r, warp, W) : range_walk(p, win, ln, r, lane));
 
   constexpr int kVec = HD >= 128 ? HD / 128 : 1;         // float4 columns per lane
   constexpr int kLanes = HD >= 128 ? 32 : HD / 4;        // lanes per token in the output product
@@ -469,7 +480,6 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
 
   for (int s = 0; s < C::kStages; ++s) stream.fill(s);
   for (int s = 0;; s = s + 1 == C::kStages ? 0 : s + 1) {
-    cp_async_wait<C::kStages - 1>();
     __syncwarp();
     const uint4 mt = stream.meta[s];
     if (mt.w) break;
@@ -483,8 +493,9 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
         qs[g * (C::kQRow / 4) + d + (d >= HD / 2 ? 4 : 0)] = x;
       }
       clear();
-      __syncwarp();
     }
+    cp_async_wait<C::kStages - 1>();  // after a first tile's q is on its way
+    __syncwarp();
     const float *kr = reinterpret_cast<const float *>(mine + s * C::S::kStage + key * C::S::kRow) + half * (HD / 2);
     uint64_t acc[G];
 #pragma unroll
@@ -676,7 +687,9 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
   const int gw = p.local ? blockIdx.x : blockIdx.x * W + warp;
   const int r = gw / p.units, unit = gw - r * p.units;  // r: the range, or the sequence where local
   Line ln;
+  Window win;
   if (!p.local) {
+    win.look(p, lane);
     ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
     if (r >= static_cast<int>(ln.ranges)) return;
   }
@@ -685,7 +698,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
 
   char *mine = smem + warp * C::S::kBytes;
   typename C::S stream(p, mine, u, h0, n_h, lane);
-  stream.start(p.local ? local_walk(p, r, warp, W) : range_walk(p, ln, r, lane));
+  stream.start(p.local ? local_walk(p, r, warp, W) : range_walk(p, win, ln, r, lane));
 
   const int g = lane >> 2, t = lane & 3;
   // ldmatrix rows: K as (token, k half), V as (token half, column half) of a 16 x 16 block
@@ -715,7 +728,6 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
 
   for (int s = 0; s < kStages; ++s) stream.fill(s);
   for (int s = 0;; s = s + 1 == kStages ? 0 : s + 1) {
-    cp_async_wait<kStages - 1>();
     __syncwarp();
     const uint4 mt = stream.meta[s];
     if (mt.w) break;
@@ -743,6 +755,8 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
       }
       clear();
     }
+    cp_async_wait<kStages - 1>();  // after a first tile's q is on its way
+    __syncwarp();
     float sc[N][2][4];  // two chains over the head: even and odd steps
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -930,6 +944,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     const uint32_t rb = blockIdx.x + 1;
     if (rb >= ln.ranges) return;
     Window win;
+    win.look(p, lane);
     b = win.find(p, ln.start(rb), lane);
     win.need(p, b, lane);
     first = win.at(b), next = win.at(b + 1);
