@@ -13,7 +13,13 @@
 // raggedness keeps all warps equally busy and the host needs no lengths.  A sequence inside
 // one range is finished by its warp; a sequence cut by a range border leaves (m, l, O) of its
 // parts in the workspace, and a second launch joins them in the order of the ranges (the
-// result does not depend on scheduling).
+// result does not depend on scheduling).  A short small batch takes one launch instead: a CTA for each
+// sequence and KV head, its warps' parts joined in shared memory.
+//
+// Measured on a B200 (walk and join, device time; HBM floor at the measured 6535 GB/s): 32 sequences of
+// 20000..32768, 8 KV heads x 128, bf16: 549-560 us (floor 529); one of 131071: 98 us (82); 64 of
+// 1..8192: 61 us (46); 256 of 1..600, f16: 27 us (17).  About 8 us of each are the launch, the
+// dependent loads before the first copy and the last warps; the rest streams at 0.93-0.97 of the peak.
 #include "dkv_common.cuh"
 
 namespace dkv {
@@ -24,10 +30,11 @@ constexpr int kTile = 16;      // tokens per pipeline stage of a warp
 // of 1..600 tokens at 16 / 32 / 48 / 64 / 96: 38 / 34 / 31 / 34 / 39 us; of 64 of 1..8192:
 // 73 / 61 / 59 / 60 / 61 us; long sequences do not notice.
 constexpr int kSeqCost = 48;
-#ifndef LOCAL_TOKENS
-#define LOCAL_TOKENS 512
-#endif
-constexpr int kLocalTokens = LOCAL_TOKENS;
+// Up to so many tiles a warp, a batch of no more sequences x units than SMs runs as one launch, a CTA
+// for each sequence and unit: at 1 / 2 / 4 / 6 tiles 6.4 / 8.2 / 11.6 / 14.7 us against 10.5 / 10.6 /
+// 12.8 / 12.3 split and joined (one sequence, 8 KV heads x 128, 16 bits; 4.9 / 5.9 / 7.8 / 9.9 against
+// 8.2 / 8.3 / 10.3 / 9.8 at 3 x 64; fp32 6.6 / 9.0 / 13.6 / 17.7 against 11.5 / 11.6 / 13.9 / 13.4).
+constexpr int kLocalTiles = 4;
 constexpr int kMinRange = 32;  // tokens below which a range is not cut further
 
 struct Params {
@@ -41,7 +48,8 @@ struct Params {
   const char *k, *v;
   int64_t k_block, k_slot, k_head, v_block, v_slot, v_head;  // bytes
   int num_blocks;
-  float *part_o, *part_ml;  // [range][unit][2][kGroup][head_dim], [...][kGroup][2]
+  // parts: [range][unit][starts before / in the range][head of the unit][head_dim], and m, l of each
+  float *part_o, *part_ml;
   int32_t *status;
   float bias;        // l and O of the parts carry 2^bias
   float scale_log2;  // scale * log2(e): scores are kept in base 2
@@ -78,7 +86,7 @@ __device__ __forceinline__ Line line_of(uint32_t tokens, int n_seqs, int most) {
 __device__ __forceinline__ int border(uint32_t x, uint32_t at, int len) {
   if (x <= at) return 0;
   if (x - at >= static_cast<uint32_t>(len) + kSeqCost) return len;
-  return min(static_cast<int>(x - at) & ~(kTile - 1), len);
+  return static_cast<int>(min((x - at) & ~static_cast<uint32_t>(kTile - 1), static_cast<uint32_t>(len)));
 }
 
 // cu_seqlens and table lengths of 32 consecutive sequences in a warp's registers, so that
@@ -171,9 +179,11 @@ __device__ __forceinline__ void walk_seq(const Params &p, Walk &w, int h0, int n
 }
 template <typename T>
 __device__ __forceinline__ void walk_next(const Params &p, Walk &w, int h0, int n_h, int lane) {
-  w.i += w.step;
   w.flags &= ~kFirst;
-  if (w.i < w.end) return;
+  if (w.end - w.i > w.step) {
+    w.i += w.step;
+    return;
+  }
   if (p.local) {
     w.live = false;
     return;
@@ -264,13 +274,12 @@ struct Stream {
     if (p.copy == kPages) {
       if (++tile < 32 && !(w.flags & kFirst)) return;
       tile = 0;
-      const int i = w.i + lane * w.step;
-      id = i >= 0 && i < w.end ? id_at(block_of(i)) : kNoRow;
+      const int ahead = lane * w.step;
+      id = ahead < w.end - w.i ? id_at(block_of(w.i + ahead)) : kNoRow;
     } else {
-      const int i = w.i + (lane & 15);
       id = kNoRow;
-      if (i >= w.end) return;
-      const int blk = block_of(i);
+      if ((lane & 15) >= w.end - w.i) return;
+      const int i = w.i + (lane & 15), blk = block_of(i);
       slot = i - blk * p.block_size;
       id = id_at(blk);
     }
@@ -329,7 +338,7 @@ struct Stream {
           copy_side(dst + kTile * kRow, vs, p.v_slot, rows);
         }
       } else {
-        const bool wanted = w.i + (lane & 15) < w.end;
+        const bool wanted = (lane & 15) < w.end - w.i;
         const bool good = wanted && id >= 0 && id < p.num_blocks;
         if (wanted && !good) record_error(p.status, id == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
         there = __ballot_sync(0xffffffffu, good) & 0xffffu;
@@ -352,7 +361,7 @@ struct Stream {
           }
         }
       }
-      const bool last = !p.local && w.i + kTile >= w.end;
+      const bool last = !p.local && w.end - w.i <= kTile;
       if (lane == 0) meta[s] = make_uint4(w.b, w.flags | (last ? kLast : 0), there, 0);
       walk_next<T>(p, w, h0, n_h, lane);
       look_up();
@@ -936,6 +945,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   __shared__ float red_m[kJoinThreads / 32], red_l[kJoinThreads / 32];
   const float kNegInf = __int_as_float(0xff800000);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // The kernel after this one may start when this grid has ended, and many of its CTAs end early: one
+  // waits for the walk whatever it has to do, so that the grid cannot end before the walk.
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   const Line ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
   int b = blockIdx.x, first, next;
   if (by_seq) {
@@ -1149,7 +1161,7 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   s->warps = variant(f32, s->hd_pad, s->g).warps;
   s->chunks = (group + s->g - 1) / s->g;
   s->units = a->k_pages.n_heads * s->chunks;
-  s->local = a->seqs.max_seq_len <= kLocalTokens && static_cast<int64_t>(a->seqs.n_seqs) * s->units <= sms;
+  s->local = a->seqs.max_seq_len <= kLocalTiles * kTile * s->warps && static_cast<int64_t>(a->seqs.n_seqs) * s->units <= sms;
   const int64_t most = static_cast<int64_t>(sms) * s->warps / s->units;
   const int64_t line = static_cast<int64_t>(a->seqs.n_seqs) * (static_cast<int64_t>(a->seqs.max_seq_len) + kSeqCost);
   const int64_t want = line / kMinRange;
@@ -1321,7 +1333,8 @@ extern "C" int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv
   // 16-byte copies where every row of K and V starts on 16 bytes and is a multiple of 16 long
   const int64_t all = p.k_block | p.k_slot | p.k_head | p.v_block | p.v_slot | p.v_head | (p.hd * sz) |
                       static_cast<int64_t>(reinterpret_cast<uintptr_t>(k.base) | reinterpret_cast<uintptr_t>(v.base));
-  p.copy = all % 16 ? pattn::kPlain : k.block_size % pattn::kTile ? pattn::kRows : pattn::kPages;
+  // (without blocks there is no address to give to a copy of nothing)
+  p.copy = all % 16 || blocks == 0 ? pattn::kPlain : k.block_size % pattn::kTile ? pattn::kRows : pattn::kPages;
   const int64_t two = p.q_seq | p.q_head | p.out_seq | p.out_head | (p.hd * sz) |
                       static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out));
   p.pairs = two % 4 == 0;

@@ -309,6 +309,45 @@ def test_attention_is_deterministic_and_reads_the_right_stream(cuda):
     assert torch.equal(got, want) and torch.equal(other, want)
 
 
+def test_attention_is_done_when_the_stream_is(cuda):
+    """As many equal sequences as ranges: none is cut, the joining launch has nothing to do, and still a
+    copy queued behind the call reads the finished output."""
+    sms = torch.cuda.get_device_properties(cuda).multi_processor_count
+    n = sms * 12 // 8  # twelve warps an SM over eight KV heads
+    c = Cache([16] * n, 8, 128, 16, BF, cuda)
+    q = torch.randn(n, 32, 128, device=cuda).to(BF)
+    length = 1024
+    tables = torch.randint(0, n, (n, length // 16), dtype=torch.int32, device=cuda)
+    seqs = dkv.SeqBatchTensors(cu_seqlens=torch.arange(n + 1, dtype=torch.int32, device=cuda) * length,
+                               block_tables=tables, max_seq_len=length)
+    out = torch.zeros_like(q)
+    copies = []
+    for _ in range(5):
+        out.zero_()
+        dkv.paged_decode_attention(q, c.k, c.v, seqs, out=out)
+        copies.append(out.clone())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, out) for x in copies) and bool(out.abs().amax(-1).min() > 0)
+
+
+@pytest.mark.parametrize("lens", [[40, 0, 300], [6000, 3]])
+def test_attention_into_its_query(cuda, lens):
+    c = Cache(lens, 2, 64, 16, BF, cuda)
+    q = torch.randn(len(lens), 8, 64, device=cuda).to(BF)
+    want = dkv.paged_decode_attention(q, c.k, c.v, c.seqs())
+    assert dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), out=q) is q and torch.equal(q, want)
+
+
+def test_attention_without_blocks(cuda):
+    pages = torch.zeros(0, 16, 2, 64, dtype=BF, device=cuda)
+    q = torch.randn(2, 4, 64, device=cuda).to(BF)
+    seqs = dkv.SeqBatchTensors(cu_seqlens=torch.tensor([0, 0, 5], dtype=torch.int32, device=cuda),
+                               block_tables=torch.zeros(2, 1, dtype=torch.int32, device=cuda), max_seq_len=5)
+    assert torch.all(dkv.paged_decode_attention(q, pages, pages, seqs) == 0)
+    with pytest.raises(dkv.DkvError, match="block id outside"):
+        ops.status_word(cuda).raise_if_set("attention")
+
+
 # ---------------------------------------------------------------------------------------
 # plan
 # ---------------------------------------------------------------------------------------
