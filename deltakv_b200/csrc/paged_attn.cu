@@ -914,13 +914,13 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
 constexpr int kMaxRanges = 2048;
 
 // A CTA has `hpc` query heads (1 or a warp each) of a cut sequence.  blockIdx.x is a sequence
-// where by_seq, else a range border (at most ranges - 1 sequences are cut).  Which parts there are
-// follows from the lengths alone and is worked out before the walk's end is waited for.  Up to 32
-// parts a warp joins alone, a lane per part's weight; more are joined by the CTA: a thread per
-// part's weight, then VW columns a thread, kJoinThreads / (head_dim / VW) parts at a time.  Either
-// way several parts' loads are in flight (one at a time cost 1.5 us each: 38 us for the 148 parts
-// of one long sequence, 6 us so).  128 threads fit beside the walk's CTA (registers), so most
-// CTAs are in place before the walk ends.
+// where by_seq, else a range border (at most ranges - 1 sequences are cut); gridDim.z CTAs share a
+// head's columns.  Which parts there are follows from the lengths alone and is worked out before
+// the walk's end is waited for.  Up to 32 parts a warp joins alone, a lane per part's weight; more are
+// joined by the CTA: a thread per part's weight, then VW columns a thread, a group of threads for
+// every so many-th part.  The parts' addresses are an arithmetic sequence, so that several parts'
+// loads are in flight: with a test in front of each load, the 222 parts of one long sequence took
+// 12 us.  128 threads fit beside the walk's CTA, so most CTAs are in place before the walk ends.
 constexpr int kJoinThreads = 128;
 
 template <int VW>
@@ -939,8 +939,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
                                                            int hpc) {
   using T = typename Elem<DT>::T;
   extern __shared__ __align__(16) char smem[];
-  int *part = reinterpret_cast<int *>(smem);
-  float *weight = reinterpret_cast<float *>(part + p.ranges);
+  float *weight = reinterpret_cast<float *>(smem), *part_l = weight + p.ranges;
   __shared__ float red[kJoinThreads * VW];
   __shared__ float red_m[kJoinThreads / 32], red_l[kJoinThreads / 32];
   const float kNegInf = __int_as_float(0xff800000);
@@ -964,43 +963,38 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     if (rb > 1 && ln.start(rb - 1) >= at) return;  // an earlier border has this sequence
   }
   const int len = max(next - first, 0);
-  const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
   if (len == 0) return;
-  const uint32_t r0 = ln.owner(at), r1 = ln.owner(at + len + kSeqCost - 1);
-  if (r1 == r0) return;  // not cut
+  const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
+  // the ranges with a part: a range is at least two tiles wide, so only those at the ends of the
+  // sequence and of its virtual tokens can have none
+  uint32_t r0 = ln.owner(at), r1 = ln.owner(at + len + kSeqCost - 1);
+  while (r0 < r1 && border(ln.start(r0 + 1), at, len) == 0) ++r0;
+  while (r0 < r1 && border(ln.start(r1), at, len) == len) --r1;
+  if (r1 == r0) return;  // not cut: written by its warp
   const int n = r1 - r0 + 1;
-  // the part slots of range r0 + i, for head 0 of the unit; -1: no part; all: the range has it whole
-  auto slot_of = [&](int i, bool &all) {
-    const uint32_t r = r0 + i;
-    const int i0 = border(ln.start(r), at, len), i1 = border(ln.start(r + 1), at, len);
-    all |= i0 == 0 && i1 == len;
-    return i1 > i0 ? (static_cast<int>(r) * p.units * 2 + (i0 == 0 ? 1 : 0)) * g_unit : -1;
-  };
-  auto head_of = [&](int h) {  // what head h adds to a part slot
+  // part i of head h: slots as the walk numbers them, [range][unit][0, or 1 for the first part][head]
+  auto part_at = [&](int h) {
     const int u = h / p.group, in = h - u * p.group;
-    return (u * p.chunks + in / g_unit) * 2 * g_unit + in % g_unit;
+    return ((static_cast<int64_t>(r0) * p.units + u * p.chunks + in / g_unit) * 2) * g_unit + in % g_unit;
   };
+  const int64_t stride = static_cast<int64_t>(p.units) * 2 * g_unit;
   auto store = [&](int h, int c, const float (&x)[VW], float inv) {
     T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + h * p.out_head) + c * VW;
 #pragma unroll
     for (int e = 0; e < VW; ++e) dst[e] = Elem<DT>::from_f(x[e] * inv);
   };
-  // gridDim.z CTAs share a head's columns
   const int share = (p.hd / VW + gridDim.z - 1) / gridDim.z, col0 = blockIdx.z * share;
   const int cols = min(p.hd / VW, col0 + share);
   const int h0 = blockIdx.y * hpc, h1 = min(h0 + hpc, p.heads);
 
   if (n <= 32) {
-    bool all = false;
-    int mine = lane < n ? slot_of(lane, all) : -1;
-    if (__any_sync(0xffffffffu, all)) return;  // all its tokens fell into one range: already written
     const int h = h0 + warp;
     if (h >= h1) return;
-    if (mine >= 0) mine += head_of(h);
+    const int64_t part0 = part_at(h);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     float m = kNegInf, l = 0.f;
-    if (mine >= 0) {
-      const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * static_cast<int64_t>(mine));
+    if (lane < n) {
+      const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (part0 + lane * stride + (lane ? 0 : g_unit)));
       m = ml.x, l = ml.y;
     }
     float top = m;
@@ -1012,34 +1006,30 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     for (int k = 16; k > 0; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
     const float inv = total == 0.f ? 0.f : 1.f / total;
     for (int c0 = col0; c0 < cols; c0 += 32) {
-      const int c = c0 + lane;
+      const int c = min(c0 + lane, cols - 1);  // lanes past the end repeat the last column
       float acc[VW];
 #pragma unroll
       for (int e = 0; e < VW; ++e) acc[e] = 0.f;
+      add_part<VW>(acc, p.part_o + (part0 + g_unit) * p.hd + c * VW, __shfl_sync(0xffffffffu, w, 0));
+      const float *src = p.part_o + part0 * p.hd + c * VW;
 #pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const int at_i = __shfl_sync(0xffffffffu, mine, i);
-        const float w_i = __shfl_sync(0xffffffffu, w, i);
-        if (at_i >= 0 && c < cols) add_part<VW>(acc, p.part_o + static_cast<int64_t>(at_i) * p.hd + c * VW, w_i);
-      }
-      if (c < cols) store(h, c, acc, inv);
+      for (int i = 1; i < n; ++i)
+        add_part<VW>(acc, src + i * stride * p.hd, __shfl_sync(0xffffffffu, w, i));
+      if (c0 + lane < cols) store(h, c, acc, inv);
     }
     if (p.lse && lane == 0 && blockIdx.z == 0)
       p.lse[static_cast<int64_t>(b) * p.heads + h] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
     return;
   }
 
-  bool all = false;
-  for (int i = tid; i < n; i += kJoinThreads) part[i] = slot_of(i, all);
-  if (__syncthreads_or(all)) return;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int h = h0; h < h1; ++h) {
-    const int add = head_of(h);
+    const int64_t part0 = part_at(h);
     float top = kNegInf;
     for (int i = tid; i < n; i += kJoinThreads) {
-      const float m = part[i] >= 0 ? p.part_ml[2 * static_cast<int64_t>(part[i] + add)] : kNegInf;
-      weight[i] = m;
-      top = fmaxf(top, m);
+      const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (part0 + i * stride + (i ? 0 : g_unit)));
+      weight[i] = ml.x, part_l[i] = ml.y;
+      top = fmaxf(top, ml.x);
     }
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
@@ -1052,7 +1042,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     for (int i = tid; i < n; i += kJoinThreads) {
       const float e = exp2f(weight[i] - base);
       weight[i] = e;
-      if (part[i] >= 0) sum = fmaf(p.part_ml[2 * static_cast<int64_t>(part[i] + add) + 1], e, sum);
+      sum = fmaf(part_l[i], e, sum);
     }
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
@@ -1064,20 +1054,20 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     const float inv = total == 0.f ? 0.f : 1.f / total;
     const int wide = min(share, kJoinThreads), groups = kJoinThreads / wide;
     for (int c0 = col0; c0 < cols; c0 += wide) {  // one pass unless head_dim is odd and above 128
-      const int c = c0 + tid % wide, pg = tid / wide;
+      const int c = min(c0 + tid % wide, cols - 1), pg = tid / wide;
       float acc[VW];
 #pragma unroll
       for (int e = 0; e < VW; ++e) acc[e] = 0.f;
-      if (pg < groups && c < cols) {
+      if (pg < groups) {
+        const float *src = p.part_o + part0 * p.hd + c * VW;
+        if (pg == 0) add_part<VW>(acc, src + g_unit * p.hd, weight[0]);
 #pragma unroll 8
-        for (int i = pg; i < n; i += groups)
-          if (part[i] >= 0)
-            add_part<VW>(acc, p.part_o + static_cast<int64_t>(part[i] + add) * p.hd + c * VW, weight[i]);
+        for (int i = pg ? pg : groups; i < n; i += groups) add_part<VW>(acc, src + i * stride * p.hd, weight[i]);
       }
 #pragma unroll
       for (int e = 0; e < VW; ++e) red[tid * VW + e] = acc[e];
       __syncthreads();
-      if (pg == 0 && c < cols) {
+      if (pg == 0 && c0 + tid < cols) {
         for (int i = 1; i < groups; ++i)
 #pragma unroll
           for (int e = 0; e < VW; ++e) acc[e] += red[(i * wide + tid) * VW + e];
