@@ -923,14 +923,32 @@ constexpr int kMaxRanges = 2048;
 // 12 us.  128 threads fit beside the walk's CTA, so most CTAs are in place before the walk ends.
 constexpr int kJoinThreads = 128;
 
-template <int VW>
-__device__ __forceinline__ void add_part(float (&acc)[VW], const float *src, float w) {
-  if constexpr (VW == 4) {
-    const float4 x = *reinterpret_cast<const float4 *>(src);
-    acc[0] = fmaf(x.x, w, acc[0]), acc[1] = fmaf(x.y, w, acc[1]);
-    acc[2] = fmaf(x.z, w, acc[2]), acc[3] = fmaf(x.w, w, acc[3]);
-  } else {
-    acc[0] = fmaf(src[0], w, acc[0]);
+// acc += sum of w(i) part(i) over i = i0, i0 + by, ... < n, eight loads at a time (past the end the last
+// part is loaded again and left out: a loop for the remainder would wait for each)
+template <int VW, typename W>
+__device__ __forceinline__ void add_parts(float (&acc)[VW], const float *src, int64_t stride, int first, int i0, int by,
+                                          int n, W weight) {
+  for (int i = i0; i < n; i += 8 * by) {
+    float x[8][VW];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int j = min(i + k * by, n - 1);
+      const float *at = src + j * stride + (j ? 0 : first);
+      if constexpr (VW == 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(at);
+        x[k][0] = v.x, x[k][1] = v.y, x[k][2] = v.z, x[k][3] = v.w;
+      } else {
+        x[k][0] = *at;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float w = weight(min(i + k * by, n - 1));
+      if (i + k * by < n) {
+#pragma unroll
+        for (int e = 0; e < VW; ++e) acc[e] = fmaf(x[k][e], w, acc[e]);
+      }
+    }
   }
 }
 
@@ -1010,11 +1028,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       float acc[VW];
 #pragma unroll
       for (int e = 0; e < VW; ++e) acc[e] = 0.f;
-      add_part<VW>(acc, p.part_o + (part0 + g_unit) * p.hd + c * VW, __shfl_sync(0xffffffffu, w, 0));
-      const float *src = p.part_o + part0 * p.hd + c * VW;
-#pragma unroll 4
-      for (int i = 1; i < n; ++i)
-        add_part<VW>(acc, src + i * stride * p.hd, __shfl_sync(0xffffffffu, w, i));
+      add_parts<VW>(acc, p.part_o + part0 * p.hd + c * VW, stride * p.hd, g_unit * p.hd, 0, 1, n,
+                    [&](int i) { return __shfl_sync(0xffffffffu, w, i); });
       if (c0 + lane < cols) store(h, c, acc, inv);
     }
     if (p.lse && lane == 0 && blockIdx.z == 0)
@@ -1059,10 +1074,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 #pragma unroll
       for (int e = 0; e < VW; ++e) acc[e] = 0.f;
       if (pg < groups) {
-        const float *src = p.part_o + part0 * p.hd + c * VW;
-        if (pg == 0) add_part<VW>(acc, src + g_unit * p.hd, weight[0]);
-#pragma unroll 8
-        for (int i = pg ? pg : groups; i < n; i += groups) add_part<VW>(acc, src + i * stride * p.hd, weight[i]);
+        add_parts<VW>(acc, p.part_o + part0 * p.hd + c * VW, stride * p.hd, g_unit * p.hd, pg, groups, n,
+                      [&](int i) { return weight[i]; });
       }
 #pragma unroll
       for (int e = 0; e < VW; ++e) red[tid * VW + e] = acc[e];
