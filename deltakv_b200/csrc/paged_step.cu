@@ -46,6 +46,11 @@ __device__ __forceinline__ int owner(const int *cu, int n, int x) {
 
 __device__ __forceinline__ int saturate(int64_t v) { return v > INT32_MAX ? INT32_MAX : static_cast<int>(v); }
 
+// Latency: a plan reads and writes a few hundred bytes to a few hundred KB (0.04 us at the HBM
+// rate), so what counts is one launch and a short chain of dependent loads (lengths, table entry).
+// Measured on a B200: 8 sequences of one new token 3.9 us, 512 of one 5.4 us, 96 prefill chunks of
+// up to 2048 tokens 5.9 us of device time.
+//
 // Every CTA scans all sequences itself (their lengths are a few KB, resident in L2) and then
 // fills its share of the rows and of the new table entries, so the whole plan is one launch;
 // CTA 0 also writes the per-sequence outputs.  A new entry comes from the free list by index,
@@ -214,7 +219,10 @@ struct Raw<DT, 1> {
 
 // A thread has VEC columns i and their partners i + half of up to kHeads heads of a row, so that
 // the row's slot, position and cos / sin are read once for all of them and 2 kHeads 16-byte loads
-// are in flight.  Bound by memory: every q, k and v element is read once and written once.
+// are in flight; the heads of a thread are `groups` apart, so that neighbouring threads read
+// neighbouring heads.  Bound by memory: every q, k and v element is read once and written once.  Measured
+// on a B200: 16384 rows of 32 + 8 + 8 heads x 128, bf16 69.5 us = 5.92 TB/s, 0.91 of the measured HBM rate
+// (an element pair a thread: 312 us; two heads a thread 75 us; a thread's heads adjacent 71 us); 64 rows 3.0 us.
 constexpr int kHeads = 4;
 
 template <int SDT, int PDT, int VEC>
@@ -222,7 +230,7 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
   using ST = typename Elem<SDT>::T;
   using PT = typename Elem<PDT>::T;
   const int all = a.heads[0] + a.heads[1] + a.heads[2];
-  const int cols = a.half / VEC, per_row = cols * ((all + kHeads - 1) / kHeads);
+  const int cols = a.half / VEC, groups = (all + kHeads - 1) / kHeads, per_row = cols * groups;
   const int64_t e = static_cast<int64_t>(blockIdx.x) * kAppThreads + threadIdx.x;
   const int64_t row = a.wide ? e / per_row : static_cast<uint32_t>(e) / static_cast<uint32_t>(per_row);
   if (row >= a.n_rows) return;
@@ -235,7 +243,7 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
   Raw<SDT, VEC> x[kHeads][2];
 #pragma unroll
   for (int k = 0; k < kHeads; ++k) {
-    int h = hg * kHeads + k;
+    int h = hg + k * groups;
     if (h >= all) break;
     const int w = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
     h -= w == 0 ? 0 : w == 1 ? a.heads[0] : a.heads[0] + a.heads[1];
@@ -258,7 +266,7 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
   const int64_t off = kept ? slot - block * a.block_size : 0;
 #pragma unroll
   for (int k = 0; k < kHeads; ++k) {
-    int h = hg * kHeads + k;
+    int h = hg + k * groups;
     if (h >= all) break;
     const int w = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
     h -= w == 0 ? 0 : w == 1 ? a.heads[0] : a.heads[0] + a.heads[1];

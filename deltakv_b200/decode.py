@@ -10,7 +10,7 @@ and :class:`~deltakv_b200.ops.SeqBatchTensors`:
 
 None of them reads anything back to the host (``check=True`` does, to raise what the kernels
 recorded), so a step can be captured into a CUDA graph and replayed with other lengths.  They
-run on the current stream of the tensors' device.  The cache layouts are the ones of
+are forms for serving: their outputs carry no gradient.  They run on the current stream of the tensors' device.  The cache layouts are the ones of
 :func:`~deltakv_b200.paged.scatter_into_paged`; for its 5-D forms pass the K and V views
 (``ops.page_view(cache, 0)``, ``ops.page_view(cache, 1)``).  The rotation is the reference's
 (src/deltakv/rope.py:9-63), the page arithmetic that of src/deltakv/paged.py:39-43.
@@ -138,8 +138,8 @@ def plan_paged_step(lengths: Tensor, block_tables: Tensor, block_size: int, *, r
     width = shape[1]
     if n > 1 and strides[0] < width:
         raise ValueError("block_tables rows overlap: the plan writes them")
-    if block_size <= 0 or rows < 0 or max_seq_len < 0:
-        raise ValueError("block_size must be positive, rows and max_seq_len not negative")
+    if not 0 < block_size < 1 << 31 or not 0 <= rows < 1 << 31 or not 0 <= max_seq_len < 1 << 31:
+        raise ValueError("block_size must be positive, rows and max_seq_len not negative, all below 2**31")
     dev = _same_device("plan_paged_step", lengths, block_tables, new_lengths, table_lens, free_blocks)
     out = _empty(3 * n + 3 + rows, dtype=_I32, device=dev)
     cu, cu_new, lens, used, positions = torch.unsafe_split_with_sizes(out, (n + 1, n + 1, n, 1, rows))

@@ -100,22 +100,16 @@ class SeqBatchTensors:
             self.block_tables = torch.empty(bt.shape, dtype=bt.dtype, device=bt.device).copy_(bt)
 
     def struct(self) -> L.SeqBatch:
-        _require_cuda(self.cu_seqlens, self.block_tables, self.table_lens, self.positions)
-        for t in (self.cu_seqlens, self.block_tables, self.table_lens, self.positions):
-            if t is not None and t.dtype != torch.int32:
+        cu, bt, lens, pos = self.cu_seqlens, self.block_tables, self.table_lens, self.positions
+        for t in (cu, bt, lens, pos):
+            if t is not None and (t.dtype is not torch.int32 or not t.is_cuda):
+                _require_cuda(cu, bt, lens, pos)
                 raise TypeError("sequence metadata must be int32")
-        bt = self.block_tables
-        if bt.ndim != 2 or bt.stride(1) != 1:
+        strides = bt.stride()
+        if len(strides) != 2 or strides[1] != 1:
             raise ValueError("block_tables must be a row-major [n_seqs, max_blocks] int32 tensor")
-        return L.SeqBatch(
-            cu_seqlens=self.cu_seqlens.data_ptr(),
-            block_tables=bt.data_ptr(),
-            table_lens=ptr(self.table_lens),
-            positions=ptr(self.positions),
-            table_stride=bt.stride(0),
-            n_seqs=self.cu_seqlens.numel() - 1,
-            max_seq_len=int(self.max_seq_len),
-        )
+        return L.SeqBatch(cu.data_ptr(), bt.data_ptr(), ptr(lens), ptr(pos), strides[0], cu.numel() - 1,
+                          int(self.max_seq_len))
 
     @staticmethod
     def single(seq_len: int, block_table: Sequence[int], device: torch.device) -> "SeqBatchTensors":

@@ -34,6 +34,8 @@ def _plan(**change):
     (dict(block_tables=torch.zeros(1, 4, dtype=I32).expand(2, 4)), ValueError, "overlap"),
     (dict(block_size=0), ValueError, "positive"),
     (dict(rows=-1), ValueError, "negative"),
+    (dict(rows=1 << 31), ValueError, "below"),
+    (dict(max_seq_len=1 << 31), ValueError, "below"),
 ])
 def test_plan_refuses(change, error, text):
     with pytest.raises(error, match=text):
@@ -108,6 +110,11 @@ def _cache(**change):
              stride_slot=128, stride_head=64)
     a.update(change)
     return L.PagedCache(**a)
+
+
+def test_struct_sizes_match_the_header():
+    # under the x86-64 SysV layout of include/dkv_b200.h
+    assert (C.sizeof(L.StepPlanArgs), C.sizeof(L.AppendArgs), C.sizeof(L.PagedDecodeArgs)) == (128, 272, 248)
 
 
 def test_c_entries_check_before_touching_the_device():
