@@ -1,8 +1,9 @@
-"""Build libdkv_b200.so (sm_100a) in-tree with nvcc.
+"""Build libdkv_b200.so (sm_100a) in-tree with nvcc, and the extension module _step.so with g++.
 
 Each ``csrc/*.cu`` is compiled to an object under ``deltakv_b200/_build`` (skipped when
 it is newer than its source and every header), then linked into
-``deltakv_b200/libdkv_b200.so``.  ``python -m deltakv_b200.build`` rebuilds; ``--ptxas``
+``deltakv_b200/libdkv_b200.so``.  ``csrc/step_binding.cpp`` (host side of the paged step
+operators, against the installed torch and Python) becomes ``deltakv_b200/_step.so``.  ``python -m deltakv_b200.build`` rebuilds; ``--ptxas``
 prints register / spill / shared-memory usage per kernel.
 """
 
@@ -12,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -20,6 +22,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libdkv_b200.so"
+STEP_SRC, STEP = CSRC / "step_binding.cpp", PKG / "_step.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -62,11 +65,45 @@ def _compile(src: Path, ptxas: bool) -> tuple[Path, str]:
     return obj, res.stderr
 
 
+def _step_stamp() -> str:
+    import torch
+
+    return f"{sys.version} torch {torch.__version__}"
+
+
+def build_step() -> Path:
+    """The extension module; rebuilt when its source, the C header, Python or torch changed."""
+    import torch
+
+    stamp = BUILD / "step.stamp"
+    newest = max(STEP_SRC.stat().st_mtime, *(h.stat().st_mtime for h in (ROOT / "include").glob("*.h")))
+    if STEP.exists() and STEP.stat().st_mtime >= newest and stamp.exists() and stamp.read_text() == _step_stamp():
+        return STEP
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    tmp = STEP.with_suffix(".so.tmp")
+    # the system's g++, whose libstdc++ is the one that torch loads
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-I", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
+           "-isystem", str(root / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
+           str(STEP_SRC), "-o", str(tmp), "-L", str(root / "lib"),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {STEP_SRC.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, STEP)
+    stamp.write_text(_step_stamp())
+    return STEP
+
+
 def build(ptxas: bool = False, verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
-    with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        step = ex.submit(build_step)
         results = list(ex.map(lambda s: _compile(s, ptxas), srcs))
+        step.result()
     if ptxas or verbose:
         for _, log in results:
             if log:
