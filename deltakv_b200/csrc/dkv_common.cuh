@@ -399,6 +399,40 @@ namespace dkv {
 void note_cuda_error(cudaError_t err, const char *what);
 }  // namespace dkv
 
+// ---------------------------------------------------------------------------
+// overlapped launches
+// ---------------------------------------------------------------------------
+namespace dkv {
+// A kernel launched by launch_overlapped begins by waiting until every earlier kernel of the stream has
+// ended and its writes are visible, and only then lets the next one be put in place: so a kernel that is
+// running has all but the one before it behind it.  Every CTA passes here before it touches global memory
+// or ends; what a stream orders stays ordered.
+__device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void begin_overlapped() {
+  wait_for_earlier();
+  let_next_start();
+}
+
+// Launches a kernel that may be put in place while the kernel before it in the stream still runs (if
+// that one said let_next_start): about 2 us less between two short kernels.
+template <typename... Params, typename... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                              Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+}  // namespace dkv
+
 // host-side helper: map cudaError to DKV status, remembering the cause
 #define DKV_CUDA_CHECK(expr)                      \
   do {                                            \

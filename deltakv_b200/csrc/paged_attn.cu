@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
   using C = Simt<HD, G, W, kStages>;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  asm volatile("griddepcontrol.launch_dependents;");
+  begin_overlapped();
   const int gw = p.local ? blockIdx.x : blockIdx.x * W + warp;
   const int r = gw / p.units, unit = gw - r * p.units;  // r: the range, or the sequence where local
   Line ln;
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
   const float kNegInf = __int_as_float(0xff800000);
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  asm volatile("griddepcontrol.launch_dependents;");
+  begin_overlapped();
   const int gw = p.local ? blockIdx.x : blockIdx.x * W + warp;
   const int r = gw / p.units, unit = gw - r * p.units;  // r: the range, or the sequence where local
   Line ln;
@@ -962,9 +962,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   __shared__ float red_m[kJoinThreads / 32], red_l[kJoinThreads / 32];
   const float kNegInf = __int_as_float(0xff800000);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // The kernel after this one may start when this grid has ended, and many of its CTAs end early: one
-  // waits for the walk whatever it has to do, so that the grid cannot end before the walk.
-  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // This grid is put in place once every CTA of the walk has begun, that is after all that was before the
+  // walk: the lengths may be read, the parts not yet.  The kernel after this one may start when this
+  // grid has ended, and many of its CTAs end early: one waits for the walk whatever it has to do, so that
+  // the grid cannot end before the walk.
+  let_next_start();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) wait_for_earlier();
   const Line ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
   int b = blockIdx.x, first, next;
   if (by_seq) {
@@ -1009,7 +1012,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     const int h = h0 + warp;
     if (h >= h1) return;
     const int64_t part0 = part_at(h);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_earlier();
     float m = kNegInf, l = 0.f;
     if (lane < n) {
       const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (part0 + lane * stride + (lane ? 0 : g_unit)));
@@ -1037,7 +1040,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     return;
   }
 
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_earlier();
   for (int h = h0; h < h1; ++h) {
     const int64_t part0 = part_at(h);
     float top = kNegInf;
@@ -1195,8 +1198,7 @@ int launch_simt(const Params &p, int grid, cudaStream_t st) {
   static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
   const int rc = allow_smem<simt_kernel<HD, G, W, kStages>>(C::kSmem);
   if (rc != DKV_OK) return rc;
-  simt_kernel<HD, G, W, kStages><<<grid, W * 32, C::kSmem, st>>>(p);
-  DKV_CUDA_CHECK(cudaGetLastError());
+  DKV_CUDA_CHECK(launch_overlapped(simt_kernel<HD, G, W, kStages>, dim3(grid), W * 32, C::kSmem, st, p));
   return DKV_OK;
 }
 
@@ -1206,8 +1208,7 @@ int launch_mma(const Params &p, int grid, cudaStream_t st) {
   static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
   const int rc = allow_smem<mma_kernel<DT, HD, N, W, kStages>>(C::kSmem);
   if (rc != DKV_OK) return rc;
-  mma_kernel<DT, HD, N, W, kStages><<<grid, W * 32, C::kSmem, st>>>(p);
-  DKV_CUDA_CHECK(cudaGetLastError());
+  DKV_CUDA_CHECK(launch_overlapped(mma_kernel<DT, HD, N, W, kStages>, dim3(grid), W * 32, C::kSmem, st, p));
   return DKV_OK;
 }
 
@@ -1252,27 +1253,15 @@ int launch(const Params &p, const Shape &s, cudaStream_t st) {
   const int64_t ctas = s.local ? static_cast<int64_t>(p.n_seqs) * s.units : (warps + s.warps - 1) / s.warps;
   const int rc = launch_walk<DT>(p, s, static_cast<int>(ctas), st);
   if (rc != DKV_OK || s.ranges == 1) return rc;
-  // the join starts as soon as every CTA of the walk is under way and waits in the kernel for its end
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
   const int by_seq = p.n_seqs <= s.ranges - 1;
   const int cut = by_seq ? p.n_seqs : s.ranges - 1;
   // few cut sequences: a CTA for each head (they may have many parts); else a warp each
   const int hpc = static_cast<int64_t>(cut) * p.heads <= 148 * 8 ? 1 : kJoinThreads / 32;
   // very few: several CTAs for each head
   const int split = static_cast<int64_t>(cut) * p.heads <= 148 && p.hd >= 64 ? 4 : 1;
-  cfg.gridDim = dim3(cut, (p.heads + hpc - 1) / hpc, split);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.dynamicSmemBytes = s.ranges * 8;
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (p.hd % 4 == 0)
-    DKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<DT, 4>, p, s.g, by_seq, hpc));
-  else
-    DKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<DT, 1>, p, s.g, by_seq, hpc));
+  const dim3 grid(cut, (p.heads + hpc - 1) / hpc, split);
+  const auto kernel = p.hd % 4 == 0 ? join_kernel<DT, 4> : join_kernel<DT, 1>;
+  DKV_CUDA_CHECK(launch_overlapped(kernel, grid, kJoinThreads, s.ranges * 8, st, p, s.g, by_seq, hpc));
   return DKV_OK;
 }
 

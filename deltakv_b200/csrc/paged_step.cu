@@ -57,6 +57,7 @@ __device__ __forceinline__ int saturate(int64_t v) { return v > INT32_MAX ? INT3
 // never from the table another CTA may be writing.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(dkv_step_plan_args a) {
   extern __shared__ int sm[];
+  begin_overlapped();
   const int n = a.n_seqs;
   int *cu_new = sm, *cu_ext = sm + n + 1;
   __shared__ int64_t warp_sum[3][kPlanThreads / 32];
@@ -229,6 +230,7 @@ template <int SDT, int PDT, int VEC>
 __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_constant__ Append a) {
   using ST = typename Elem<SDT>::T;
   using PT = typename Elem<PDT>::T;
+  begin_overlapped();
   const int all = a.heads[0] + a.heads[1] + a.heads[2];
   const int cols = a.half / VEC, groups = (all + kHeads - 1) / kHeads, per_row = cols * groups;
   const int64_t e = static_cast<int64_t>(blockIdx.x) * kAppThreads + threadIdx.x;
@@ -323,8 +325,8 @@ extern "C" int dkv_plan_paged_step(const dkv_step_plan_args *args, dkv_stream_t 
                                         2 * (step::kMaxSeqs + 1) * static_cast<int>(sizeof(int))));
   const int64_t want = (static_cast<int64_t>(a.n_rows) + 2 * step::kPlanThreads - 1) / (2 * step::kPlanThreads);
   const int grid = static_cast<int>(want < 1 ? 1 : (want > 148 ? 148 : want));
-  step::plan_kernel<<<grid, step::kPlanThreads, smem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  DKV_CUDA_CHECK(cudaGetLastError());
+  DKV_CUDA_CHECK(launch_overlapped(step::plan_kernel, dim3(grid), step::kPlanThreads, smem,
+                                   reinterpret_cast<cudaStream_t>(stream), a));
   return DKV_OK;
 }
 
@@ -380,14 +382,11 @@ extern "C" int dkv_append_paged(const dkv_append_args *args, dkv_stream_t stream
   if (ctas > INT32_MAX) return DKV_ERR_UNSUPPORTED;
   const unsigned grid = static_cast<unsigned>(ctas);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-#define DKV_APPEND_CASE(S, P)                                                                     \
-  if (g.in_dtype == S && kp.dtype == P) {                                                         \
-    if (wide)                                                                                     \
-      step::append_kernel<S, P, P == DKV_F32 ? 4 : 8><<<grid, step::kAppThreads, 0, st>>>(a);     \
-    else                                                                                          \
-      step::append_kernel<S, P, 1><<<grid, step::kAppThreads, 0, st>>>(a);                        \
-    DKV_CUDA_CHECK(cudaGetLastError());                                                           \
-    return DKV_OK;                                                                                \
+#define DKV_APPEND_CASE(S, P)                                                                              \
+  if (g.in_dtype == S && kp.dtype == P) {                                                                  \
+    const auto kernel = wide ? step::append_kernel<S, P, P == DKV_F32 ? 4 : 8> : step::append_kernel<S, P, 1>; \
+    DKV_CUDA_CHECK(launch_overlapped(kernel, dim3(grid), step::kAppThreads, 0, st, a));                    \
+    return DKV_OK;                                                                                         \
   }
   DKV_APPEND_CASE(DKV_BF16, DKV_BF16)
   DKV_APPEND_CASE(DKV_F16, DKV_F16)

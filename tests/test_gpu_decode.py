@@ -685,6 +685,65 @@ def test_captured_steps(cuda, dtype):
     ops.status_word(cuda).raise_if_set("captured steps")
 
 
+@pytest.mark.parametrize("lens", [[300, 40], [9000, 40]])
+def test_calls_behind_one_another(cuda, lens):
+    """Each call reads what the one before it wrote; nothing waits in between."""
+    c = Cache(lens, 2, 64, 16, BF, cuda)
+    rope, _, _ = rope_tables(64, 50, cuda)
+    k = torch.randn(2, 2, 64, device=cuda).to(BF)
+    pos = torch.tensor([3, 4], dtype=torch.int32, device=cuda)
+    slots = torch.tensor([int(c.tables[b, 0]) * 16 for b in range(2)], device=cuda)  # the sequences' first tokens
+    first = torch.randn(2, 8, 64, device=cuda).to(BF)
+
+    def chain(wait):
+        c.k.copy_(keep[0]), c.v.copy_(keep[1])
+        x = first
+        for _ in range(12):
+            x = dkv.append_into_paged(x[:, :2], x[:, 2:4], c.k, c.v, slots, q=x, positions=pos, rope=rope)
+            wait()
+            x = dkv.paged_decode_attention(x, c.k, c.v, c.seqs())
+            wait()
+        return x
+
+    keep = c.k.clone(), c.v.clone()
+    want = chain(torch.cuda.synchronize)
+    for _ in range(5):
+        assert torch.equal(chain(lambda: None), want)
+
+
+def test_captured_between_copies_and_memsets(cuda):
+    """The operators in a graph whose other nodes are copies and memsets, on two branches."""
+    c = Cache([500, 40], 2, 64, 16, BF, cuda)
+    lens = torch.tensor([500, 40], dtype=torch.int32, device=cuda)
+    q = torch.randn(2, 8, 64, device=cuda).to(BF)
+    want = dkv.paged_decode_attention(q, c.k, c.v, c.seqs())
+    src, q_in, out = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q)
+    host = torch.zeros(2, 8, 64, dtype=BF).pin_memory()
+    free = torch.arange(c.k.shape[0], dtype=torch.int32, device=cuda)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        q_in.copy_(src)
+        out.zero_()
+        other.wait_stream(side)
+        with torch.cuda.stream(other):
+            held = torch.zeros(2, dtype=torch.int32, device=cuda)
+            tables = torch.zeros(2, 32, dtype=torch.int32, device=cuda)
+            step = dkv.plan_paged_step(lens, tables, 16, rows=540, max_seq_len=500, table_lens=held, free_blocks=free)
+        dkv.paged_decode_attention(q_in, c.k, c.v, c.seqs(), out=out)
+        side.wait_stream(other)
+        again = dkv.paged_decode_attention(out, c.k, c.v, step.seqs)
+        host.copy_(out, non_blocking=True)
+    for _ in range(3):
+        src.copy_(q)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(host.to(cuda), want)
+        assert int(step.blocks_used) == 35 and step.positions[:3].tolist() == [0, 1, 2]
+        assert torch.equal(again, dkv.paged_decode_attention(want, c.k, c.v, step.seqs))
+
+
 def test_step_beside_a_patch(cuda):
     """The pages the step writes are the ones the patch operators change: attend, patch, attend."""
     s = Server(cuda, BF)
