@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -140,6 +141,14 @@ void rows_of(const Tensor &t, const char *name, int64_t rows, int64_t heads, int
   if (t.stride(2) != 1 && hd > 1) value_error(std::string(name) + " must have contiguous head_dim");
 }
 
+// A tensor that is written: no element of it may lie over another one of its own, and it may be the input
+// but not lie across it (as far as the strides tell).
+void written(const Tensor &t, const char *name, const Tensor *input, const char *input_name) {
+  if (at::has_internal_overlap(t) == at::MemOverlap::Yes) value_error(std::string(name) + " has elements that share memory");
+  if (input != nullptr && at::get_overlap_status(t, *input) == at::MemOverlapStatus::Partial)
+    value_error(std::string(name) + " overlaps " + input_name + " without being it");
+}
+
 dkv_paged_cache describe(const Tensor &t, int code) {
   dkv_paged_cache c;
   c.base = t.data_ptr();
@@ -250,6 +259,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
     const int64_t rows = slots.numel();
     if (slots.scalar_type() != at::kLong) type_error("slots must be int64");
     if (slots.dim() != 1 || !slots.is_contiguous()) value_error("slots must be a contiguous vector");
+    written(pages.k, "k_pages", nullptr, ""), written(pages.v, "v_pages", nullptr, "");
     rows_of(k, "k", rows, pages.heads, pages.hd);
     rows_of(v, "v", rows, pages.heads, pages.hd);
     if (v.scalar_type() != k.scalar_type() || (q && q->scalar_type() != k.scalar_type()))
@@ -269,6 +279,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
       if (q_out) {
         rows_of(*q_out, "q_out", rows, q->size(1), pages.hd);
         if (q_out->scalar_type() != q->scalar_type()) type_error("q_out must have q's dtype");
+        written(*q_out, "q_out", q, "q");
       }
     }
     const Place at_("append_into_paged", k);
@@ -341,6 +352,7 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t count) {
     if (out) {
       rows_of(*out, "out", n, heads, hd);
       if (out->scalar_type() != q.scalar_type()) type_error("out must have q's dtype");
+      written(*out, "out", &q, "q");
     }
     const Place at_("paged_decode_attention", q);
     at_.also(&pages.k), at_.also(&pages.v), at_.also(&cu), at_.also(&tables), at_.also(lens), at_.also(out);

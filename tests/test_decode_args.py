@@ -50,6 +50,7 @@ def _append(**change):
     return dkv.append_into_paged(a.pop("k"), a.pop("v"), a.pop("k_pages"), a.pop("v_pages"), a.pop("slots"), **a)
 
 
+_ACROSS = torch.zeros(128, dtype=BF)
 _ROPE = dict(rope=(torch.zeros(9, 4), torch.zeros(9, 4)), positions=torch.zeros(3, dtype=I32))
 
 
@@ -72,6 +73,11 @@ _ROPE = dict(rope=(torch.zeros(9, 4), torch.zeros(9, 4)), positions=torch.zeros(
     (dict(q=torch.zeros(3, 4, 8), **_ROPE), TypeError, "share a dtype"),
     (dict(q=torch.zeros(3, 4, 8, dtype=BF), q_out=torch.zeros(3, 4, 8), **_ROPE), TypeError, "q_out"),
     (dict(q_out=torch.zeros(3, 4, 8, dtype=BF)), ValueError, "q_out without q"),
+    (dict(q=torch.zeros(3, 4, 8, dtype=BF), q_out=torch.zeros(1, 4, 8, dtype=BF).expand(3, 4, 8), **_ROPE), ValueError,
+     "share memory"),
+    (dict(q=_ACROSS[:96].view(3, 4, 8), q_out=_ACROSS[32:].view(3, 4, 8), **_ROPE), ValueError, "overlaps q"),
+    (dict(v_pages=torch.zeros(1, 4, 2, 8, dtype=BF).expand(4, 4, 2, 8)), ValueError, "v_pages has elements"),
+    (dict(k=None), TypeError, "k must be a tensor"),
 ])
 def test_append_refuses(change, error, text):
     with pytest.raises(error, match=text):
@@ -97,6 +103,10 @@ def _attend(**change):
     (dict(tables=torch.zeros(1, 1, dtype=I32)), ValueError, "block_tables has 1 rows"),
     (dict(out=torch.zeros(2, 4, 8)), TypeError, "out"),
     (dict(out=torch.zeros(2, 2, 8, dtype=BF)), ValueError, "out"),
+    (dict(out=torch.zeros(2, 1, 8, dtype=BF).expand(2, 4, 8)), ValueError, "share memory"),
+    (dict(q=_ACROSS[:64].view(2, 4, 8), out=_ACROSS[32:96].view(2, 4, 8)), ValueError, "overlaps q"),
+    (dict(q=[1.0]), TypeError, "q must be a tensor"),
+    (dict(scale="half"), TypeError, "real number"),
     (dict(q=torch.zeros(2, 4, 264, dtype=BF), k_pages=torch.zeros(4, 4, 2, 264, dtype=BF),
           v_pages=torch.zeros(4, 4, 2, 264, dtype=BF)), ValueError, "256"),
 ])

@@ -190,6 +190,44 @@ def test_attention_many_sequences(cuda, dtype):
     assert torch.all(out[empty] == 0) and torch.all(torch.isfinite(out))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_attention_largest_batch_and_dense_cache(cuda, dtype):
+    """65535 sequences, the most there can be; and a dense cache as one block of odd length."""
+    n = 65535
+    c = Cache([3], 1, 32, 16, dtype, cuda)
+    lens = torch.arange(n, device=cuda) % 4
+    cu = torch.cat([torch.zeros(1, device=cuda), lens.cumsum(0)]).to(torch.int32)
+    q = torch.randn(n, 1, 32, device=cuda).to(dtype)
+    seqs = dkv.SeqBatchTensors(cu_seqlens=cu, block_tables=c.tables.repeat(n, 1), max_seq_len=3)
+    out = dkv.paged_decode_attention(q, c.k, c.v, seqs, check=True)
+    k, v = c.tokens(0)
+    check_attention(out[-9:], None, q[-9:], lambda b: (k[: int(lens[n - 9 + b])], v[: int(lens[n - 9 + b])]), 32 ** -0.5)
+    check_attention(out[:9], None, q[:9], lambda b: (k[: int(lens[b])], v[: int(lens[b])]), 32 ** -0.5)
+    with pytest.raises(dkv.DkvError, match="unsupported"):
+        seqs = dkv.SeqBatchTensors(cu_seqlens=torch.zeros(n + 2, dtype=torch.int32, device=cuda),
+                                   block_tables=torch.zeros(n + 1, 1, dtype=torch.int32, device=cuda), max_seq_len=0)
+        dkv.paged_decode_attention(torch.zeros(n + 1, 1, 32, dtype=dtype, device=cuda), c.k, c.v, seqs)
+    length = 777
+    kd, vd = (torch.randn(length, 2, 64, device=cuda).to(dtype) for _ in range(2))
+    qd = torch.randn(1, 8, 64, device=cuda).to(dtype)
+    seqs = dkv.SeqBatchTensors(cu_seqlens=torch.tensor([0, length], dtype=torch.int32, device=cuda),
+                               block_tables=torch.zeros(1, 1, dtype=torch.int32, device=cuda), max_seq_len=length)
+    got = dkv.paged_decode_attention(qd, kd[None], vd[None], seqs, check=True)
+    check_attention(got, None, qd, lambda _: (kd, vd), 64 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_caches_of_unequal_size_and_a_slice_of_the_batch(cuda, dtype):
+    c = Cache([100, 50, 900, 30], 2, 64, 16, dtype, cuda)
+    q = torch.randn(4, 4, 64, device=cuda).to(dtype)
+    want = dkv.paged_decode_attention(q, c.k, c.v, c.seqs())
+    more = torch.cat([c.k, torch.full_like(c.k[:2], math.nan)])  # blocks that V does not have
+    assert torch.equal(dkv.paged_decode_attention(q, more, c.v, c.seqs(), check=True), want)
+    part = dkv.SeqBatchTensors(cu_seqlens=c.cu[1:4], block_tables=c.tables[1:3], max_seq_len=900)  # cu starts at 100
+    got = dkv.paged_decode_attention(q[1:3], c.k, c.v, part, check=True)
+    check_attention(got, None, q[1:3], lambda b: c.tokens(b + 1), 64 ** -0.5)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("amp,scale", [(1.5, 30.0), (60.0, None), (0.0, None), (1.5, -0.2)])
 def test_attention_extreme_scores(cuda, dtype, amp, scale):
