@@ -177,6 +177,16 @@ struct Pages {
   }
 };
 
+// n elements of a vector as a tensor of their own on its storage (integers: nothing for autograd to know),
+// without a dispatched call for each
+Tensor vector_in(const Tensor &whole, int64_t offset, int64_t n) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(whole.storage()),
+                                                      whole.key_set(), whole.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(whole.storage_offset() + offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(at::IntArrayRef(&n, 1));
+  return t;
+}
+
 // ---- operators --------------------------------------------------------------------------
 // plan(lengths, block_tables, block_size, rows, max_seq_len, new_lengths, table_lens, free_blocks)
 //   -> (cu_seqlens, cu_new, table_lens, blocks_used, positions, slots)
@@ -227,10 +237,10 @@ PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t count) {
     p.status = at_.status();
     check(g_plan(&p, at_.stream()), "dkv_plan_paged_step");
     const int64_t sizes[5] = {n + 1, n + 1, n, 1, rows};
-    const std::vector<Tensor> parts = at::unsafe_split_with_sizes(out, at::IntArrayRef(sizes, 5));
     PyObject *result = PyTuple_New(6);
     if (result == nullptr) throw Raised{nullptr, ""};
-    for (int i = 0; i < 5; ++i) PyTuple_SET_ITEM(result, i, THPVariable_Wrap(parts[i]));
+    for (int64_t i = 0, offset = 0; i < 5; offset += sizes[i++])
+      PyTuple_SET_ITEM(result, i, THPVariable_Wrap(vector_in(out, offset, sizes[i])));
     PyTuple_SET_ITEM(result, 5, THPVariable_Wrap(slots));
     return result;
   });
