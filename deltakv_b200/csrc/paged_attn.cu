@@ -58,6 +58,7 @@ struct Params {
   uint32_t div_mul, div_shift;  // i / block_size = i div_mul >> div_shift
   int local;  // a CTA per (sequence, unit): no ranges, no parts
   int copy;   // kPlain, kRows or kPages
+  int piece;  // kPlain: bytes of an asynchronous piece, 8 or 4, or 0 (element by element)
   int pairs;  // rows of q and out in whole pairs of 16-bit elements
 };
 
@@ -222,7 +223,8 @@ __device__ __forceinline__ Walk local_walk(const Params &p, int b, int warp, int
 //           32 tiles;
 //   kRows   any block_size: lanes 0-15 look up the K rows, 16-31 the V rows, a tile ahead, and
 //           pass them on;
-//   kPlain  rows that are not whole 16-byte pieces: element by element.
+//   kPlain  rows that do not start or end on 16 bytes: in asynchronous pieces of 8 or 4 bytes, or
+//           (16-bit rows that start on odd elements) element by element.
 // A bulk copy per row (one instruction instead of 8 to 32) is slower for rows of 128 and 256 bytes:
 // such copies start at about one in 14 clocks on an SM, 18 B/clock (681 us against 545 for the
 // 3.5 GB of 32 long sequences).
@@ -314,6 +316,36 @@ struct Stream {
       src += step;
     }
   }
+  // rows whose addresses the lanes hold (0: zeros), in pieces smaller than 16 bytes
+  __device__ __forceinline__ void copy_plain(char *stage, uint64_t addr) {
+    const int row_bytes = p.hd * kSize;
+    if (p.piece >= 4) {
+      for (int row = 0; row < 32; ++row) {
+        const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
+        const char *src = a ? reinterpret_cast<const char *>(a) : p.k;
+        for (int at = lane * p.piece; at < row_bytes; at += 32 * p.piece) {
+          if (p.piece == 8)
+            cp_async8(stage + row * kRow + at, src + at, a ? 8 : 0);
+          else
+            cp_async4(stage + row * kRow + at, src + at, a ? 4 : 0);
+        }
+      }
+      return;
+    }
+    for (int d = lane; d < (p.hd + 31) / 32 * 32; d += 32) {
+      for (int row = 0; row < 32; row += 8) {  // eight rows' loads in flight
+        T x[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const uint64_t a = __shfl_sync(0xffffffffu, addr, row + r);
+          x[r] = a && d < p.hd ? reinterpret_cast<const T *>(a)[d] : T(0.f);
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (d < p.hd) reinterpret_cast<T *>(stage + (row + r) * kRow)[d] = x[r];
+      }
+    }
+  }
   // issues the next tile's copies into stage s (one cp.async group, empty past the end)
   __device__ __forceinline__ void fill(int s) {
     if (w.live) {
@@ -354,11 +386,7 @@ struct Stream {
                          a ? 16 : 0);
           }
         } else {
-          for (int row = 0; row < 32; ++row) {
-            const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
-            T *dst = reinterpret_cast<T *>(stage + row * kRow);
-            for (int d = lane; d < p.hd; d += 32) dst[d] = a ? reinterpret_cast<const T *>(a)[d] : T(0.f);
-          }
+          copy_plain(stage, addr);
         }
       }
       const bool last = !p.local && w.end - w.i <= kTile;
@@ -1326,6 +1354,7 @@ extern "C" int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv
   const int64_t all = p.k_block | p.k_slot | p.k_head | p.v_block | p.v_slot | p.v_head | (p.hd * sz) |
                       static_cast<int64_t>(reinterpret_cast<uintptr_t>(k.base) | reinterpret_cast<uintptr_t>(v.base));
   // (without blocks there is no address to give to a copy of nothing)
+  p.piece = blocks == 0 ? 0 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 0;
   p.copy = all % 16 || blocks == 0 ? pattn::kPlain : k.block_size % pattn::kTile ? pattn::kRows : pattn::kPages;
   const int64_t two = p.q_seq | p.q_head | p.out_seq | p.out_head | (p.hd * sz) |
                       static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out));
