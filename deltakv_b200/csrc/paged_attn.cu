@@ -5,7 +5,7 @@
 // (m, l, O) of two disjoint parts of the tokens join exactly: with M = max(m1, m2) each part's l
 // and O are multiplied by exp(m - M) and added.  So the cache's length can be cut anywhere.
 //
-// Every K and V element is read once and used for the 1..16 query heads of its group: 2 to 16
+// Every K and V element is used for the query heads of its group, 2 to 16 of them mostly: 2 to 16
 // flops a byte, far below the ridge, so the kernel is built as a stream of the pages.  Work is
 // cut without regard to sequences: the tokens of all sequences are laid end to end (cu_seqlens
 // is that layout), with kSeqCost virtual tokens of overhead in front of each sequence, and the
@@ -673,7 +673,8 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
 // (16 times the padding, operands through tensor memory) would buy nothing.
 // Weights enter the product as two 16-bit terms (value and rest: 2^-17 relative for bf16) -
 // one term would add an error as large as the output's own rounding.  In f16 they are scaled by
-// 2^14, which l shares, so that weights down to 2^-28 of the largest keep all their bits.
+// 2^14, which l shares, so that weights down to 2^-28 of the largest keep all their bits.  (The rest
+// of a weight may be 0, so an infinite V value gives NaN where one term would give infinity.)
 template <int DT>
 struct Half;
 template <>
@@ -702,8 +703,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
-// N: blocks of 8 query heads of the unit
-template <int DT, int HD, int N, int W, int kStages_>
+template <int DT, int HD, int W, int kStages_>
 struct Mma {
   static constexpr int kStages = kStages_;
   using T = typename Elem<DT>::T;
@@ -711,9 +711,9 @@ struct Mma {
   static constexpr int kSmem = W * S::kBytes;
 };
 
-template <int DT, int HD, int N, int W, int kStages>
+template <int DT, int HD, int W, int kStages>
 __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ Params p) {
-  using C = Mma<DT, HD, N, W, kStages>;
+  using C = Mma<DT, HD, W, kStages>;
   using T = typename C::T;
   using E = Half<DT>;
   constexpr int kSteps = HD / 16;
@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
     if (r >= static_cast<int>(ln.ranges)) return;
   }
   const int u = unit / p.chunks, chunk = unit - u * p.chunks;
-  const int n_h = min(8 * N, p.group - chunk * 8 * N), h0 = u * p.group + chunk * 8 * N;
+  const int n_h = min(8, p.group - chunk * 8), h0 = u * p.group + chunk * 8;
 
   char *mine = smem + warp * C::S::kBytes;
   typename C::S stream(p, mine, u, h0, n_h, lane);
@@ -742,21 +742,18 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
   const uint32_t k_at = smem_u32(mine) + (lane & 15) * C::S::kRow + (lane >> 4) * 16;
   const uint32_t v_at =
       smem_u32(mine) + (kTile + (lane & 7) + (lane >> 4) * 8) * C::S::kRow + ((lane >> 3) & 1) * 16;
-  uint32_t qf[N][kSteps][2];
-  float o[N][kSteps][4], m[N][2], l[N][2];
+  uint32_t qf[kSteps][2];
+  float o[kSteps][4], m[2], l[2];
   auto clear = [&]() {
+    m[0] = m[1] = kNegInf;
+    l[0] = l[1] = 0.f;
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      m[n][0] = m[n][1] = kNegInf;
-      l[n][0] = l[n][1] = 0.f;
+    for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][k][e] = 0.f;
-    }
+      for (int e = 0; e < 4; ++e) o[k][e] = 0.f;
   };
-  auto sum_of = [&](int n, int c) {  // l over the lanes that share a head
-    float x = l[n][c];
+  auto sum_of = [&](int c) {  // l over the lanes that share a head
+    float x = l[c];
     x += __shfl_xor_sync(0xffffffffu, x, 4);
     x += __shfl_xor_sync(0xffffffffu, x, 8);
     return x + __shfl_xor_sync(0xffffffffu, x, 16);
@@ -770,143 +767,126 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
     if (mt.w) break;
     const int b = mt.x;
     if (mt.y & kFirst) {
+      const unsigned short *qr =
+          reinterpret_cast<const unsigned short *>(p.q + b * p.q_seq + (h0 + min(g, n_h - 1)) * p.q_head);
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int h = n * 8 + g;
-        const unsigned short *qr =
-            reinterpret_cast<const unsigned short *>(p.q + b * p.q_seq + (h0 + min(h, n_h - 1)) * p.q_head);
+      for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int d = k * 16 + e * 8 + t * 2;
-            uint32_t w = 0;
-            if (p.pairs) {
-              if (d < p.hd) w = *reinterpret_cast<const uint32_t *>(qr + d);
-            } else {
-              if (d < p.hd) w = qr[d];
-              if (d + 1 < p.hd) w |= static_cast<uint32_t>(qr[d + 1]) << 16;
-            }
-            qf[n][k][e] = h < n_h ? w : 0;
+        for (int e = 0; e < 2; ++e) {
+          const int d = k * 16 + e * 8 + t * 2;
+          uint32_t w = 0;
+          if (p.pairs) {
+            if (d < p.hd) w = *reinterpret_cast<const uint32_t *>(qr + d);
+          } else {
+            if (d < p.hd) w = qr[d];
+            if (d + 1 < p.hd) w |= static_cast<uint32_t>(qr[d + 1]) << 16;
           }
-      }
+          qf[k][e] = g < n_h ? w : 0;
+        }
       clear();
     }
     cp_async_wait<kStages - 1>();  // after a first tile's q is on its way
     __syncwarp();
-    float sc[N][2][4];  // two chains over the head: even and odd steps
+    float sc[2][4];  // two chains over the head: even and odd steps
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sc[n][0][e] = sc[n][1][e] = 0.f;
+    for (int e = 0; e < 4; ++e) sc[0][e] = sc[1][e] = 0.f;
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       uint32_t a[4];
       ldmatrix_x4(a[0], a[1], a[2], a[3], k_at + s * C::S::kStage + k * 32);
-#pragma unroll
-      for (int n = 0; n < N; ++n) E::mma(sc[n][k & 1], a, qf[n][k][0], qf[n][k][1]);
+      E::mma(sc[k & 1], a, qf[k][0], qf[k][1]);
     }
-    uint32_t ph[N][2], pl[N][2];
+    uint32_t ph[2], pl[2];
+    // x: {token g, token g + 8} x {head 2t, head 2t + 1}
+    float x[4];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      // x: {token g, token g + 8} x {head 2t, head 2t + 1}
-      float x[4];
+    for (int e = 0; e < 4; ++e) x[e] = (sc[0][e] + sc[1][e]) * p.scale_log2;
+    if (mt.z != 0xffffu) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = (sc[n][0][e] + sc[n][1][e]) * p.scale_log2;
-      if (mt.z != 0xffffu) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!((mt.z >> (g + (e & 2) * 4)) & 1)) x[e] = kNegInf;
-      }
-      // m is any value not far below the scores so far: it moves (and O with it) only when a
-      // score passes it, which after the first tiles is rare
-      const float top0 = fmaxf(x[0], x[2]), top1 = fmaxf(x[1], x[3]);
-      if (__any_sync(0xffffffffu, top0 > m[n][0] || top1 > m[n][1])) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float top = c ? top1 : top0;
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          top = fmaxf(top, m[n][c]);
-          const float keep = ex2(m[n][c] - (top == kNegInf ? 0.f : top));
-          m[n][c] = top;
-          l[n][c] *= keep;
-#pragma unroll
-          for (int k = 0; k < kSteps; ++k) o[n][k][c] *= keep, o[n][k][2 + c] *= keep;
-        }
-      }
+      for (int e = 0; e < 4; ++e)
+        if (!((mt.z >> (g + (e & 2) * 4)) & 1)) x[e] = kNegInf;
+    }
+    // m is any value not far below the scores so far: it moves (and O with it) only when a
+    // score passes it, which after the first tiles is rare
+    const float top0 = fmaxf(x[0], x[2]), top1 = fmaxf(x[1], x[3]);
+    if (__any_sync(0xffffffffu, top0 > m[0] || top1 > m[1])) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float base = (m[n][c] == kNegInf ? 0.f : m[n][c]) - E::kBias;  // nothing seen yet: any finite base
-        x[c] = ex2(x[c] - base);
-        x[c + 2] = ex2(x[c + 2] - base);
-        l[n][c] += x[c] + x[c + 2];
-      }
+        float top = c ? top1 : top0;
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        top = fmaxf(top, m[c]);
+        const float keep = ex2(m[c] - (top == kNegInf ? 0.f : top));
+        m[c] = top;
+        l[c] *= keep;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t w = E::pack(x[2 * c], x[2 * c + 1]);
-        ph[n][c] = transpose8x8(w);
-        pl[n][c] = transpose8x8(E::pack(x[2 * c] - E::lo(w), x[2 * c + 1] - E::hi(w)));
+        for (int k = 0; k < kSteps; ++k) o[k][c] *= keep, o[k][2 + c] *= keep;
       }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float base = (m[c] == kNegInf ? 0.f : m[c]) - E::kBias;  // nothing seen yet: any finite base
+      x[c] = ex2(x[c] - base);
+      x[c + 2] = ex2(x[c + 2] - base);
+      l[c] += x[c] + x[c + 2];
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const uint32_t w = E::pack(x[2 * c], x[2 * c + 1]);
+      ph[c] = transpose8x8(w);
+      pl[c] = transpose8x8(E::pack(x[2 * c] - E::lo(w), x[2 * c + 1] - E::hi(w)));
     }
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       uint32_t a[4];
       ldmatrix_x4_trans(a[0], a[1], a[2], a[3], v_at + s * C::S::kStage + k * 32);
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        E::mma(o[n][k], a, ph[n][0], ph[n][1]);
-        E::mma(o[n][k], a, pl[n][0], pl[n][1]);
-      }
+      E::mma(o[k], a, ph[0], ph[1]);
+      E::mma(o[k], a, pl[0], pl[1]);
     }
     if (mt.y & kLast) {
       const bool whole = (mt.y & kFromStart) && (mt.y & kToEnd);
       const int64_t part = (static_cast<int64_t>(r) * p.units + unit) * 2 + (mt.y & kFromStart ? 1 : 0);
+      const float sum[2] = {sum_of(0), sum_of(1)};
+      if (whole) {
+        // heads to rows, so that a lane stores two neighbouring columns of one head
+        const float inv0 = sum[0] == 0.f ? 0.f : 1.f / sum[0], inv1 = sum[1] == 0.f ? 0.f : 1.f / sum[1];
+        T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + (h0 + g) * p.out_head);
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const float sum[2] = {sum_of(n, 0), sum_of(n, 1)};
-        if (whole) {
-          // heads to rows, so that a lane stores two neighbouring columns of one head
-          const float inv0 = sum[0] == 0.f ? 0.f : 1.f / sum[0], inv1 = sum[1] == 0.f ? 0.f : 1.f / sum[1];
-          const int in = n * 8 + g;
-          T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + (h0 + in) * p.out_head);
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t w = transpose8x8(E::pack(o[k][e * 2] * inv0, o[k][e * 2 + 1] * inv1));
+            const int d = k * 16 + e * 8 + t * 2;
+            if (g < n_h) {
+              if (p.pairs) {
+                if (d < p.hd) *reinterpret_cast<uint32_t *>(dst + d) = w;
+              } else {
+                unsigned short *two = reinterpret_cast<unsigned short *>(dst + d);
+                if (d < p.hd) two[0] = static_cast<unsigned short>(w);
+                if (d + 1 < p.hd) two[1] = static_cast<unsigned short>(w >> 16);
+              }
+            }
+          }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (p.lse && g == 0 && t * 2 + c < n_h)
+            p.lse[static_cast<int64_t>(b) * p.heads + h0 + t * 2 + c] =
+                (m[c] + (log2f(sum[c]) - E::kBias)) * 0.6931471805599453f;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int in = t * 2 + c;
+          if (in >= n_h) continue;
+          float *dst = p.part_o + (part * 8 + in) * p.hd;
 #pragma unroll
           for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t w = transpose8x8(E::pack(o[n][k][e * 2] * inv0, o[n][k][e * 2 + 1] * inv1));
-              const int d = k * 16 + e * 8 + t * 2;
-              if (in < n_h) {
-                if (p.pairs) {
-                  if (d < p.hd) *reinterpret_cast<uint32_t *>(dst + d) = w;
-                } else {
-                  unsigned short *two = reinterpret_cast<unsigned short *>(dst + d);
-                  if (d < p.hd) two[0] = static_cast<unsigned short>(w);
-                  if (d + 1 < p.hd) two[1] = static_cast<unsigned short>(w >> 16);
-                }
-              }
-            }
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            if (p.lse && g == 0 && n * 8 + t * 2 + c < n_h)
-              p.lse[static_cast<int64_t>(b) * p.heads + h0 + n * 8 + t * 2 + c] =
-                  (m[n][c] + (log2f(sum[c]) - E::kBias)) * 0.6931471805599453f;
-        } else {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int in = n * 8 + t * 2 + c;
-            if (in >= n_h) continue;
-            float *dst = p.part_o + (part * 8 * N + in) * p.hd;
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (k * 16 + e * 8 + g < p.hd) dst[k * 16 + e * 8 + g] = o[n][k][e * 2 + c];
-            if (g == 0) {
-              p.part_ml[(part * 8 * N + in) * 2] = m[n][c];
-              p.part_ml[(part * 8 * N + in) * 2 + 1] = sum[c];
-            }
+            for (int e = 0; e < 2; ++e)
+              if (k * 16 + e * 8 + g < p.hd) dst[k * 16 + e * 8 + g] = o[k][e * 2 + c];
+          if (g == 0) {
+            p.part_ml[(part * 8 + in) * 2] = m[c];
+            p.part_ml[(part * 8 + in) * 2 + 1] = sum[c];
           }
         }
       }
@@ -917,22 +897,20 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
   cp_async_wait<0>();
   if (p.local) {
     __syncwarp();
-    LocalState<HD, 8 * N> *mine_out = reinterpret_cast<LocalState<HD, 8 * N> *>(mine);
-    static_assert(sizeof(LocalState<HD, 8 * N>) <= kStages * C::S::kStage, "the state fits the ring");
+    LocalState<HD, 8> *mine_out = reinterpret_cast<LocalState<HD, 8> *>(mine);
+    static_assert(sizeof(LocalState<HD, 8>) <= kStages * C::S::kStage, "the state fits the ring");
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+    for (int c = 0; c < 2; ++c) {
+      const float sum = sum_of(c);
+      const int in = t * 2 + c;
+      if (g == 0) mine_out->m[in] = m[c], mine_out->l[in] = sum;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float sum = sum_of(n, c);
-        const int in = n * 8 + t * 2 + c;
-        if (g == 0) mine_out->m[in] = m[n][c], mine_out->l[in] = sum;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          mine_out->o[in][k * 16 + g] = o[n][k][c];
-          mine_out->o[in][k * 16 + 8 + g] = o[n][k][2 + c];
-        }
+      for (int k = 0; k < kSteps; ++k) {
+        mine_out->o[in][k * 16 + g] = o[k][c];
+        mine_out->o[in][k * 16 + 8 + g] = o[k][2 + c];
       }
-    local_join<DT, HD, 8 * N>(p, smem, C::S::kBytes, W, r, h0, n_h);
+    }
+    local_join<DT, HD, 8>(p, smem, C::S::kBytes, W, r, h0, n_h);
   }
 }
 
@@ -1139,7 +1117,9 @@ struct Shape {
 // Warps of a CTA (one CTA an SM) and stages of a warp's ring: as many warps as registers and 220 KB
 // allow.  More warps hide each other's latency better than more stages: at head_dim 128 and 16 bits,
 // 4 x 6 / 6 x 4 / 8 x 3 / 12 x 2 (warps x stages) walk 32 long sequences in 653 / 596 / 564 / 549 us.
-// Two blocks of heads need more than the 168 registers that 12 warps leave.
+// Groups of more than 8 heads are several units, whose warps read the pages one after the other out of
+// L2: 16 heads a warp need more registers than 12 warps leave, and 8 warps of 16 heads were slower (16
+// heads a KV head: 78 against 73 us at head_dim 128, 37 / 31 at 64, 137 / 109 at 256; 36 / 41 at 32).
 struct Variant {
   int warps, stages;
 };
@@ -1148,9 +1128,7 @@ constexpr Variant variant(bool f32, int hd, int g) {
   if (f32 && hd == 128) return g == 4 ? Variant{6, 2} : Variant{5, 2};
   if (f32) return hd == 64 ? (g == 4 ? Variant{12, 2} : Variant{10, 2}) : Variant{12, 3};
   if (hd == 256) return {6, 2};
-  if (hd == 128) return g == 8 ? Variant{12, 2} : Variant{8, 3};
-  if (hd == 64) return g == 8 ? Variant{12, 4} : Variant{8, 6};
-  return g == 8 ? Variant{16, 4} : Variant{12, 6};
+  return hd == 128 ? Variant{12, 2} : hd == 64 ? Variant{12, 4} : Variant{16, 4};
 }
 
 int sm_count(int *out) {
@@ -1191,7 +1169,7 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   const int hd = a->k_pages.head_dim, group = a->n_q_heads / a->k_pages.n_heads;
   s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
   const bool f32 = a->k_pages.dtype == DKV_F32;
-  s->g = f32 ? (group <= 4 ? 4 : 8) : (group <= 8 ? 8 : 16);
+  s->g = f32 && group <= 4 ? 4 : 8;
   s->warps = variant(f32, s->hd_pad, s->g).warps;
   s->chunks = (group + s->g - 1) / s->g;
   s->units = a->k_pages.n_heads * s->chunks;
@@ -1230,13 +1208,13 @@ int launch_simt(const Params &p, int grid, cudaStream_t st) {
   return DKV_OK;
 }
 
-template <int DT, int HD, int N, int W, int kStages>
+template <int DT, int HD, int W, int kStages>
 int launch_mma(const Params &p, int grid, cudaStream_t st) {
-  using C = Mma<DT, HD, N, W, kStages>;
+  using C = Mma<DT, HD, W, kStages>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
-  const int rc = allow_smem<mma_kernel<DT, HD, N, W, kStages>>(C::kSmem);
+  const int rc = allow_smem<mma_kernel<DT, HD, W, kStages>>(C::kSmem);
   if (rc != DKV_OK) return rc;
-  DKV_CUDA_CHECK(launch_overlapped(mma_kernel<DT, HD, N, W, kStages>, dim3(grid), W * 32, C::kSmem, st, p));
+  DKV_CUDA_CHECK(launch_overlapped(mma_kernel<DT, HD, W, kStages>, dim3(grid), W * 32, C::kSmem, st, p));
   return DKV_OK;
 }
 
@@ -1260,15 +1238,11 @@ int launch_walk(const Params &p, const Shape &s, int grid, cudaStream_t st) {
     DKV_WALK_CASE(256, 8)
 #undef DKV_WALK_LAUNCH
   } else {
-#define DKV_WALK_LAUNCH(HD, G, v) return launch_mma<DT, HD, G / 8, v.warps, v.stages>(p, grid, st);
+#define DKV_WALK_LAUNCH(HD, G, v) return launch_mma<DT, HD, v.warps, v.stages>(p, grid, st);
     DKV_WALK_CASE(32, 8)
-    DKV_WALK_CASE(32, 16)
     DKV_WALK_CASE(64, 8)
-    DKV_WALK_CASE(64, 16)
     DKV_WALK_CASE(128, 8)
-    DKV_WALK_CASE(128, 16)
     DKV_WALK_CASE(256, 8)
-    DKV_WALK_CASE(256, 16)
 #undef DKV_WALK_LAUNCH
   }
 #undef DKV_WALK_CASE
