@@ -16,16 +16,17 @@
 // result does not depend on scheduling).  A short small batch takes one launch instead: a CTA for each
 // sequence and KV head, its warps' parts joined in shared memory.
 //
-// Measured on a B200 (walk and join, device time; HBM floor at the measured 6535 GB/s): 32 sequences of
-// 20000..32768, 8 KV heads x 128, bf16: 549-560 us (floor 529); one of 131071: 98 us (82); 64 of
-// 1..8192: 61 us (46); 256 of 1..600, f16: 27 us (17).  About 8 us of each are the launch, the
-// dependent loads before the first copy and the last warps; the rest streams at 0.93-0.97 of the peak.
+// Measured on a B200 (calls back to back; HBM floor at the measured 6535 GB/s): 32 sequences of
+// 20000..32768, 8 KV heads x 128, bf16: 569-591 us by the box's power (floor 529); one of 131071: 101-105 us
+// (82); 64 of 1..8192: 63-65 us (46); 256 of 1..600, f16: 29.6 us (17); fp32, 16 of 4096: 98 us (82).  About
+// 12 us of each are the launch, the dependent loads before the first copy, the last warps and the join; the
+// rest streams at 0.93-0.97 of the peak.
 #include "dkv_common.cuh"
 
 namespace dkv {
 namespace pattn {
 
-constexpr int kTile = 16;      // tokens per pipeline stage of a warp
+constexpr int kTile = 16;  // borders fall on multiples of it; a pipeline stage has 16 or 8 tokens
 // Virtual tokens per sequence: what starting and finishing one costs a warp.  Walk of 256 sequences
 // of 1..600 tokens at 16 / 32 / 48 / 64 / 96: 38 / 34 / 31 / 34 / 39 us; of 64 of 1..8192:
 // 73 / 61 / 59 / 60 / 61 us; long sequences do not notice.
@@ -132,7 +133,7 @@ struct Window {
 };
 
 // ---------------------------------------------------------------------------------------
-// a warp's walk over its range: one kTile-token tile after the other
+// a warp's walk over its range: one tile of tokens after the other
 // ---------------------------------------------------------------------------------------
 enum { kFirst = 1, kLast = 2, kFromStart = 4, kToEnd = 8 };
 
@@ -193,19 +194,20 @@ __device__ __forceinline__ void walk_next(const Params &p, Walk &w, int h0, int 
   walk_seq<T>(p, w, h0, n_h, lane);
 }
 // the walk of range r
-__device__ __forceinline__ Walk range_walk(const Params &p, const Window &win, const Line &ln, uint32_t r, int lane) {
+__device__ __forceinline__ Walk range_walk(const Params &p, const Window &win, const Line &ln, uint32_t r, int tokens,
+                                           int lane) {
   Walk w;
   w.win = win;
   w.x0 = ln.start(r), w.x1 = ln.start(r + 1);
   w.b = w.win.find(p, w.x0, lane);
-  w.step = kTile;
+  w.step = tokens;
   return w;
 }
 // every n_warps-th tile of sequence b
-__device__ __forceinline__ Walk local_walk(const Params &p, int b, int warp, int n_warps) {
+__device__ __forceinline__ Walk local_walk(const Params &p, int b, int tokens, int warp, int n_warps) {
   Walk w;
   w.b = b;
-  w.i = warp * kTile, w.step = n_warps * kTile;
+  w.i = warp * tokens, w.step = n_warps * tokens;
   w.end = max(p.cu[b + 1] - p.cu[b], 0);
   w.tlen = p.table_lens ? p.table_lens[b] : p.table_stride;
   w.flags = kFirst;
@@ -213,16 +215,16 @@ __device__ __forceinline__ Walk local_walk(const Params &p, int b, int warp, int
   return w;
 }
 
-// One warp's stream of tiles into its ring of kStages shared-memory stages.  A stage holds 16
-// rows of K, then 16 rows of V, kRow bytes apart (16 more than a row: consecutive rows start 4
+// One warp's stream of tiles into its ring of kStages shared-memory stages.  A stage holds kTok
+// rows of K, then as many of V, kRow bytes apart (16 more than a row: consecutive rows start 4
 // banks apart, so neither the fragment loads nor 16-byte reads of 8 rows conflict).  Three ways to
 // copy:
 //   kPages  block_size a multiple of the tile: a tile lies in one block, its rows a fixed stride
 //           apart, and a lane's addresses are one base and an immediate or a running sum.  Each
 //           lane holds the block id of another tile to come, so the table is waited for once in
 //           32 tiles;
-//   kRows   any block_size: lanes 0-15 look up the K rows, 16-31 the V rows, a tile ahead, and
-//           pass them on;
+//   kRows   any block_size: the first kTok lanes look up the K rows, the next the V rows, a tile
+//           ahead, and pass them on;
 //   kPlain  rows that do not start or end on 16 bytes: in asynchronous pieces of 8 or 4 bytes, or
 //           (16-bit rows that start on odd elements) element by element.
 // A bulk copy per row (one instruction instead of 8 to 32) is slower for rows of 128 and 256 bytes:
@@ -230,11 +232,11 @@ __device__ __forceinline__ Walk local_walk(const Params &p, int b, int warp, int
 // 3.5 GB of 32 long sequences).
 enum { kPlain = 0, kRows = 1, kPages = 2 };
 
-template <typename T, int HD, int kStages>
+template <typename T, int HD, int kStages, int kTok>
 struct Stream {
   static constexpr int kSize = static_cast<int>(sizeof(T));
   static constexpr int kRow = HD * kSize + 16;
-  static constexpr int kStage = 2 * kTile * kRow;
+  static constexpr int kStage = 2 * kTok * kRow;
   static constexpr int kBytes = kStages * (kStage + 16);  // the stages' descriptions behind them
   static constexpr int kPieces = HD * kSize / 16;         // 16-byte pieces of a row
   static constexpr int kRowLanes = kPieces < 32 ? kPieces : 32;
@@ -280,8 +282,8 @@ struct Stream {
       id = ahead < w.end - w.i ? id_at(block_of(w.i + ahead)) : kNoRow;
     } else {
       id = kNoRow;
-      if ((lane & 15) >= w.end - w.i) return;
-      const int i = w.i + (lane & 15), blk = block_of(i);
+      if (lane >= 2 * kTok || lane % kTok >= w.end - w.i) return;
+      const int i = w.i + lane % kTok, blk = block_of(i);
       slot = i - blk * p.block_size;
       id = id_at(blk);
     }
@@ -295,7 +297,7 @@ struct Stream {
   __device__ __forceinline__ void copy_side(uint32_t dst, const char *src, int64_t slot_bytes, int rows) {
     const int64_t step = slot_bytes * kAtOnce;
 #pragma unroll
-    for (int r = 0; r < kTile; r += kAtOnce) {
+    for (int r = 0; r < kTok; r += kAtOnce) {
 #pragma unroll
       for (int c = 0; c < kPieces; c += 32) {
         if ((c + lane % kRowLanes) * 16 < p.hd * kSize)
@@ -309,7 +311,7 @@ struct Stream {
   __device__ __forceinline__ void copy_side(uint32_t dst, const char *src, int64_t slot_bytes) {  // all of them
     const int64_t step = slot_bytes * kAtOnce;
 #pragma unroll
-    for (int r = 0; r < kTile; r += kAtOnce) {
+    for (int r = 0; r < kTok; r += kAtOnce) {
 #pragma unroll
       for (int c = 0; c < kPieces; c += 32)
         if ((c + lane % kRowLanes) * 16 < p.hd * kSize) cp_async_16(dst + r * kRow + c * 16, src + c * 16);
@@ -320,7 +322,7 @@ struct Stream {
   __device__ __forceinline__ void copy_plain(char *stage, uint64_t addr) {
     const int row_bytes = p.hd * kSize;
     if (p.piece >= 4) {
-      for (int row = 0; row < 32; ++row) {
+      for (int row = 0; row < 2 * kTok; ++row) {
         const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
         const char *src = a ? reinterpret_cast<const char *>(a) : p.k;
         for (int at = lane * p.piece; at < row_bytes; at += 32 * p.piece) {
@@ -333,7 +335,7 @@ struct Stream {
       return;
     }
     for (int d = lane; d < (p.hd + 31) / 32 * 32; d += 32) {
-      for (int row = 0; row < 32; row += 8) {  // eight rows' loads in flight
+      for (int row = 0; row < 2 * kTok; row += 8) {  // eight rows' loads in flight
         T x[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
@@ -352,7 +354,7 @@ struct Stream {
       char *stage = ring + s * kStage;
       uint32_t there;
       if (p.copy == kPages) {
-        int rows = min(w.end - w.i, kTile);
+        int rows = min(w.end - w.i, kTok);
         const int block = __shfl_sync(0xffffffffu, id, tile);
         if (block < 0 || block >= p.num_blocks) {
           if (lane == 0) record_error(p.status, block == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
@@ -362,23 +364,23 @@ struct Stream {
         const uint32_t dst = smem_u32(stage) + lane / kRowLanes * kRow + lane % kRowLanes * 16;
         const int64_t at = rows ? block : 0, in = w.i - block_of(w.i) * p.block_size;
         const char *ks = k + at * p.k_block + in * p.k_slot, *vs = v + at * p.v_block + in * p.v_slot;
-        if (rows == kTile) {
+        if (rows == kTok) {
           copy_side(dst, ks, p.k_slot);
-          copy_side(dst + kTile * kRow, vs, p.v_slot);
+          copy_side(dst + kTok * kRow, vs, p.v_slot);
         } else {
           copy_side(dst, ks, p.k_slot, rows);
-          copy_side(dst + kTile * kRow, vs, p.v_slot, rows);
+          copy_side(dst + kTok * kRow, vs, p.v_slot, rows);
         }
       } else {
-        const bool wanted = (lane & 15) < w.end - w.i;
+        const bool wanted = lane < 2 * kTok && lane % kTok < w.end - w.i;
         const bool good = wanted && id >= 0 && id < p.num_blocks;
         if (wanted && !good) record_error(p.status, id == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
-        there = __ballot_sync(0xffffffffu, good) & 0xffffu;
-        const char *src = lane < 16 ? k + id * p.k_block + slot * p.k_slot : v + id * p.v_block + slot * p.v_slot;
+        there = __ballot_sync(0xffffffffu, good) & ((1u << kTok) - 1);
+        const char *src = lane < kTok ? k + id * p.k_block + slot * p.k_slot : v + id * p.v_block + slot * p.v_slot;
         const uint64_t addr = good ? reinterpret_cast<uint64_t>(src) : 0;
         if (p.copy == kRows) {
 #pragma unroll
-          for (int c = lane; c < 32 * kPieces; c += 32) {
+          for (int c = lane; c < 2 * kTok * kPieces; c += 32) {
             const int row = c / kPieces, piece = c % kPieces;
             const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
             if (piece * 16 < p.hd * kSize)
@@ -389,7 +391,7 @@ struct Stream {
           copy_plain(stage, addr);
         }
       }
-      const bool last = !p.local && w.end - w.i <= kTile;
+      const bool last = !p.local && w.end - w.i <= kTok;
       if (lane == 0) meta[s] = make_uint4(w.b, w.flags | (last ? kLast : 0), there, 0);
       walk_next<T>(p, w, h0, n_h, lane);
       look_up();
@@ -445,20 +447,21 @@ __device__ __forceinline__ void local_join(const Params &p, const char *smem, in
 // ---------------------------------------------------------------------------------------
 // fp32 pages (the tensor cores round fp32 operands).  HD: head_dim rounded up (columns past
 // head_dim are zero), G: query heads of the unit (rounded up), W: warps per CTA.  Scores: lane =
-// (token, half of the head); output: lane = 4 columns, the tokens dealt to 128 / HD groups of
-// lanes where the head is shorter than 128.
-template <int HD, int G, int W, int kStages_>
+// (token, half or quarter of the head); output: lane = 4 columns, the tokens dealt to 128 / HD
+// groups of lanes where the head is shorter than 128.
+template <int HD, int G, int W, int kStages_, int kTok>
 struct Simt {
   static constexpr int kStages = kStages_;
-  using S = Stream<float, HD, kStages>;
-  static constexpr int kQRow = (HD + 8) * 4;  // two halves, 16 B apart in banks
-  static constexpr int kWarpBytes = S::kBytes + G * kQRow + kTile * G * 8;
+  using S = Stream<float, HD, kStages, kTok>;
+  static constexpr int kParts = 32 / kTok;              // lanes that share a token's score
+  static constexpr int kQRow = (HD + 4 * kParts) * 4;  // the parts of a head 16 B apart in banks
+  static constexpr int kWarpBytes = S::kBytes + G * kQRow + kTok * G * 8;
   static constexpr int kSmem = W * kWarpBytes;
 };
 
-template <int HD, int G, int W, int kStages>
+template <int HD, int G, int W, int kStages, int kTok>
 __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__ Params p) {
-  using C = Simt<HD, G, W, kStages>;
+  using C = Simt<HD, G, W, kStages, kTok>;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   begin_overlapped();
@@ -478,14 +481,14 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
   float *qs = reinterpret_cast<float *>(mine + C::S::kBytes);
   uint64_t *ps = reinterpret_cast<uint64_t *>(qs + C::kQRow / 4 * G);  // [token][head]: the weight, twice
   typename C::S stream(p, mine, u, h0, n_h, lane);
-  stream.start(p.local ? local_walk(p, r, warp, W) : range_walk(p, win, ln, r, lane));
+  stream.start(p.local ? local_walk(p, r, kTok, warp, W) : range_walk(p, win, ln, r, kTok, lane));
 
   constexpr int kVec = HD >= 128 ? HD / 128 : 1;         // float4 columns per lane
   constexpr int kLanes = HD >= 128 ? 32 : HD / 4;        // lanes per token in the output product
   constexpr int kSplit = 32 / kLanes;                    // tokens handled at once there
   float m[G], l[G];
   uint64_t o[G][kVec][2];  // pairs of columns, for the packed fma
-  const int key = lane & 15, half = lane >> 4;
+  const int key = lane % kTok, part = lane / kTok;
   const int oc = lane % kLanes, ok = lane / kLanes;
   auto clear = [&]() {
 #pragma unroll
@@ -527,23 +530,23 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
         float x = 0.f;
         if (g < n_h && d < p.hd)
           x = reinterpret_cast<const float *>(p.q + b * p.q_seq + (h0 + g) * p.q_head)[d];
-        qs[g * (C::kQRow / 4) + d + (d >= HD / 2 ? 4 : 0)] = x;
+        qs[g * (C::kQRow / 4) + d + d / (HD / C::kParts) * 4] = x;
       }
       clear();
     }
     cp_async_wait<C::kStages - 1>();  // after a first tile's q is on its way
     __syncwarp();
-    const float *kr = reinterpret_cast<const float *>(mine + s * C::S::kStage + key * C::S::kRow) + half * (HD / 2);
+    const float *kr = reinterpret_cast<const float *>(mine + s * C::S::kStage + key * C::S::kRow) + part * (HD / C::kParts);
     uint64_t acc[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[g] = 0;
 #pragma unroll 4
-    for (int d = 0; d < HD / 2; d += 4) {
+    for (int d = 0; d < HD / C::kParts; d += 4) {
       const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(kr + d);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const ulonglong2 y =
-            *reinterpret_cast<const ulonglong2 *>(qs + g * (C::kQRow / 4) + half * (HD / 2 + 4) + d);
+            *reinterpret_cast<const ulonglong2 *>(qs + g * (C::kQRow / 4) + part * (HD / C::kParts + 4) + d);
         acc[g] = fma2(x.y, y.y, fma2(x.x, y.x, acc[g]));
       }
     }
@@ -555,7 +558,8 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
       float lo, hi;
       f2unpack(acc[g], lo, hi);
       lo += hi;
-      lo += __shfl_xor_sync(0xffffffffu, lo, 16);
+#pragma unroll
+      for (int k = kTok; k < 32; k <<= 1) lo += __shfl_xor_sync(0xffffffffu, lo, k);
       x[g] = there ? lo * p.scale_log2 : __int_as_float(0xff800000);
       past |= x[g] > m[g];
     }
@@ -564,7 +568,7 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
       for (int g = 0; g < G; ++g) {
         float top = x[g];
 #pragma unroll
-        for (int k = 8; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        for (int k = kTok / 2; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
         top = fmaxf(m[g], top);
         const float keep = ex2(m[g] - (top == __int_as_float(0xff800000) ? 0.f : top));
         m[g] = top;
@@ -577,15 +581,15 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const float e = ex2(x[g] - (m[g] == __int_as_float(0xff800000) ? 0.f : m[g]));
-      if (half == 0) {
+      if (part == 0) {
         l[g] += e;
         ps[key * G + g] = f2pack(e, e);
       }
     }
     __syncwarp();
 #pragma unroll 4
-    for (int t = ok; t < kTile; t += kSplit) {
-      const float *vr = reinterpret_cast<const float *>(mine + s * C::S::kStage + (kTile + t) * C::S::kRow);
+    for (int t = ok; t < kTok; t += kSplit) {
+      const float *vr = reinterpret_cast<const float *>(mine + s * C::S::kStage + (kTok + t) * C::S::kRow);
       uint64_t e[G];
 #pragma unroll
       for (int g = 0; g < G; g += 2) {
@@ -604,7 +608,7 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
     }
     if (mt.y & kLast) {
       const bool whole = (mt.y & kFromStart) && (mt.y & kToEnd);
-      const int64_t part = (static_cast<int64_t>(r) * p.units + unit) * 2 + (mt.y & kFromStart ? 1 : 0);
+      const int64_t slot = (static_cast<int64_t>(r) * p.units + unit) * 2 + (mt.y & kFromStart ? 1 : 0);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         reduce(g);
@@ -622,15 +626,15 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
             if (p.lse && lane == 0)
               p.lse[static_cast<int64_t>(b) * p.heads + h] = (m[g] + log2f(sum)) * 0.6931471805599453f;
           } else {
-            float *dst = p.part_o + (part * G + g) * p.hd;
+            float *dst = p.part_o + (slot * G + g) * p.hd;
 #pragma unroll
             for (int j = 0; j < kVec; ++j)
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 if (j * 128 + oc * 4 + i < p.hd) dst[j * 128 + oc * 4 + i] = column(g, j, i);
             if (lane == 0) {
-              p.part_ml[(part * G + g) * 2] = m[g];
-              p.part_ml[(part * G + g) * 2 + 1] = sum;
+              p.part_ml[(slot * G + g) * 2] = m[g];
+              p.part_ml[(slot * G + g) * 2 + 1] = sum;
             }
           }
         }
@@ -707,7 +711,7 @@ template <int DT, int HD, int W, int kStages_>
 struct Mma {
   static constexpr int kStages = kStages_;
   using T = typename Elem<DT>::T;
-  using S = Stream<T, HD, kStages>;
+  using S = Stream<T, HD, kStages, kTile>;
   static constexpr int kSmem = W * S::kBytes;
 };
 
@@ -735,7 +739,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
 
   char *mine = smem + warp * C::S::kBytes;
   typename C::S stream(p, mine, u, h0, n_h, lane);
-  stream.start(p.local ? local_walk(p, r, warp, W) : range_walk(p, win, ln, r, lane));
+  stream.start(p.local ? local_walk(p, r, kTile, warp, W) : range_walk(p, win, ln, r, kTile, lane));
 
   const int g = lane >> 2, t = lane & 3;
   // ldmatrix rows: K as (token, k half), V as (token half, column half) of a 16 x 16 block
@@ -1106,7 +1110,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 // host side
 // ---------------------------------------------------------------------------------------
 struct Shape {
-  int hd_pad, g, warps;  // kernel variant
+  int hd_pad, g, warps, tokens;  // kernel variant
   int chunks, units;     // chunks of a group, KV heads x chunks
   int local;             // a CTA per (sequence, unit) instead of ranges
   int ranges;            // upper bound of the ranges in use
@@ -1117,18 +1121,22 @@ struct Shape {
 // Warps of a CTA (one CTA an SM) and stages of a warp's ring: as many warps as registers and 220 KB
 // allow.  More warps hide each other's latency better than more stages: at head_dim 128 and 16 bits,
 // 4 x 6 / 6 x 4 / 8 x 3 / 12 x 2 (warps x stages) walk 32 long sequences in 653 / 596 / 564 / 549 us.
+// fp32 walks, which do more arithmetic a byte, want whole sets of four warps (one a scheduler), and tiles
+// of 8 tokens to have them at 128 columns: at 8 KV heads x 128, 64 sequences of 1..8192, 4 / 8 heads a KV
+// head take 115 / 170 us with 6 / 5 warps of 16 tokens, 119 / 154 with 11 / 10 of 8, 110 / 145 with 8 of 8.
 // Groups of more than 8 heads are several units, whose warps read the pages one after the other out of
 // L2: 16 heads a warp need more registers than 12 warps leave, and 8 warps of 16 heads were slower (16
 // heads a KV head: 78 against 73 us at head_dim 128, 37 / 31 at 64, 137 / 109 at 256; 36 / 41 at 32).
 struct Variant {
-  int warps, stages;
+  int warps, stages, tokens;
 };
 constexpr Variant variant(bool f32, int hd, int g) {
-  if (f32 && hd == 256) return {3, 2};
-  if (f32 && hd == 128) return g == 4 ? Variant{6, 2} : Variant{5, 2};
-  if (f32) return hd == 64 ? (g == 4 ? Variant{12, 2} : Variant{10, 2}) : Variant{12, 3};
-  if (hd == 256) return {6, 2};
-  return hd == 128 ? Variant{12, 2} : hd == 64 ? Variant{12, 4} : Variant{16, 4};
+  if (f32 && hd == 256) return {4, 2, 8};
+  if (f32 && hd == 128) return {8, 2, 8};
+  if (f32 && hd == 64) return g == 4 ? Variant{8, 3, 16} : Variant{10, 2, 16};
+  if (f32) return {12, 3, 16};
+  if (hd == 256) return {6, 2, 16};
+  return hd == 128 ? Variant{12, 2, 16} : hd == 64 ? Variant{12, 4, 16} : Variant{16, 4, 16};
 }
 
 int sm_count(int *out) {
@@ -1170,10 +1178,11 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
   const bool f32 = a->k_pages.dtype == DKV_F32;
   s->g = f32 && group <= 4 ? 4 : 8;
-  s->warps = variant(f32, s->hd_pad, s->g).warps;
+  const Variant v = variant(f32, s->hd_pad, s->g);
+  s->warps = v.warps, s->tokens = v.tokens;
   s->chunks = (group + s->g - 1) / s->g;
   s->units = a->k_pages.n_heads * s->chunks;
-  s->local = a->seqs.max_seq_len <= kLocalTiles * kTile * s->warps && static_cast<int64_t>(a->seqs.n_seqs) * s->units <= sms;
+  s->local = a->seqs.max_seq_len <= kLocalTiles * s->tokens * s->warps && static_cast<int64_t>(a->seqs.n_seqs) * s->units <= sms;
   const int64_t most = static_cast<int64_t>(sms) * s->warps / s->units;
   const int64_t line = static_cast<int64_t>(a->seqs.n_seqs) * (static_cast<int64_t>(a->seqs.max_seq_len) + kSeqCost);
   const int64_t want = line / kMinRange;
@@ -1198,13 +1207,13 @@ int allow_smem(int bytes) {
   return DKV_OK;
 }
 
-template <int HD, int G, int W, int kStages>
+template <int HD, int G, int W, int kStages, int kTok>
 int launch_simt(const Params &p, int grid, cudaStream_t st) {
-  using C = Simt<HD, G, W, kStages>;
+  using C = Simt<HD, G, W, kStages, kTok>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
-  const int rc = allow_smem<simt_kernel<HD, G, W, kStages>>(C::kSmem);
+  const int rc = allow_smem<simt_kernel<HD, G, W, kStages, kTok>>(C::kSmem);
   if (rc != DKV_OK) return rc;
-  DKV_CUDA_CHECK(launch_overlapped(simt_kernel<HD, G, W, kStages>, dim3(grid), W * 32, C::kSmem, st, p));
+  DKV_CUDA_CHECK(launch_overlapped(simt_kernel<HD, G, W, kStages, kTok>, dim3(grid), W * 32, C::kSmem, st, p));
   return DKV_OK;
 }
 
@@ -1227,7 +1236,7 @@ template <int DT>
 int launch_walk(const Params &p, const Shape &s, int grid, cudaStream_t st) {
   constexpr bool kF32 = DT == DKV_F32;
   if constexpr (kF32) {
-#define DKV_WALK_LAUNCH(HD, G, v) return launch_simt<HD, G, v.warps, v.stages>(p, grid, st);
+#define DKV_WALK_LAUNCH(HD, G, v) return launch_simt<HD, G, v.warps, v.stages, v.tokens>(p, grid, st);
     DKV_WALK_CASE(32, 4)
     DKV_WALK_CASE(32, 8)
     DKV_WALK_CASE(64, 4)
@@ -1329,7 +1338,7 @@ extern "C" int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv
                       static_cast<int64_t>(reinterpret_cast<uintptr_t>(k.base) | reinterpret_cast<uintptr_t>(v.base));
   // (without blocks there is no address to give to a copy of nothing)
   p.piece = blocks == 0 ? 0 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 0;
-  p.copy = all % 16 || blocks == 0 ? pattn::kPlain : k.block_size % pattn::kTile ? pattn::kRows : pattn::kPages;
+  p.copy = all % 16 || blocks == 0 ? pattn::kPlain : k.block_size % s.tokens ? pattn::kRows : pattn::kPages;
   const int64_t two = p.q_seq | p.q_head | p.out_seq | p.out_head | (p.hd * sz) |
                       static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out));
   p.pairs = two % 4 == 0;
