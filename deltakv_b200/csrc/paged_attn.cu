@@ -31,11 +31,12 @@ constexpr int kTile = 16;  // borders fall on multiples of it; a pipeline stage 
 // of 1..600 tokens at 16 / 32 / 48 / 64 / 96: 38 / 34 / 31 / 34 / 39 us; of 64 of 1..8192:
 // 73 / 61 / 59 / 60 / 61 us; long sequences do not notice.
 constexpr int kSeqCost = 48;
-// Up to so many tiles a warp, a batch of no more sequences x units than SMs runs as one launch, a CTA
-// for each sequence and unit: at 1 / 2 / 4 / 6 tiles 6.4 / 8.2 / 11.6 / 14.7 us against 10.5 / 10.6 /
-// 12.8 / 12.3 split and joined (one sequence, 8 KV heads x 128, 16 bits; 4.9 / 5.9 / 7.8 / 9.9 against
-// 8.2 / 8.3 / 10.3 / 9.8 at 3 x 64; fp32 6.6 / 9.0 / 13.6 / 17.7 against 11.5 / 11.6 / 13.9 / 13.4).
-constexpr int kLocalTiles = 4;
+// Up to so many tiles a warp, a batch runs as one launch, a CTA for each sequence and unit, of as many warps
+// as let all CTAs run at once (an SM holds the warps of one CTA of the walk).  Split and joined / one launch, us,
+// bf16, 8 KV heads x 128: 4 sequences of 100 / 200 / 300 tokens (1 / 2 / 2 tiles) 9.7 / 5.0, 10.2 / 6.6, 10.6 / 7.0;
+// 60 of 100 / 200 / 300 (3 / 5 / 7 tiles of 3 warps) 11.8 / 8.7, 14.7 / 11.8, 16.8 / 14.7, and of 1..100 / 200 /
+// 300 10.4 / 6.6, 10.6 / 9.1, 11.1 / 11.7.  The border is at 5 to 7 tiles for other head sizes and fp32 as well.
+constexpr int kLocalTiles = 5;
 constexpr int kMinRange = 32;  // tokens below which a range is not cut further
 
 struct Params {
@@ -57,7 +58,7 @@ struct Params {
   int n_seqs, n_kv, heads, group, chunks, units, ranges;
   int hd, block_size;
   uint32_t div_mul, div_shift;  // i / block_size = i div_mul >> div_shift
-  int local;  // a CTA per (sequence, unit): no ranges, no parts
+  int local;  // not 0: a CTA of so many warps per (sequence, unit), no ranges, no parts
   int copy;   // kPlain, kRows or kPages
   int piece;  // kPlain: bytes of an asynchronous piece, 8 or 4, or 0 (element by element)
   int pairs;  // rows of q and out in whole pairs of 16-bit elements
@@ -409,36 +410,51 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x to 2 ulp, subnormal resu
 }
 
 // The join within a CTA: each warp's (m, l) and O (rows of HD + 4: no bank conflicts) lie at the
-// front of its ring.
+// front of its ring.  A thread per head turns every warp's m into that warp's weight, then the threads sum
+// the weighted O, four columns at a time.
 template <int HD, int kRows>
 struct LocalState {
   float o[kRows][HD + 4];
   float m[kRows], l[kRows];
 };
 template <int DT, int HD, int kRows>
-__device__ __forceinline__ void local_join(const Params &p, const char *smem, int warp_bytes, int n_warps, int b, int h0,
+__device__ __forceinline__ void local_join(const Params &p, char *smem, int warp_bytes, int n_warps, int b, int h0,
                                            int n_h) {
   using T = typename Elem<DT>::T;
   using State = LocalState<HD, kRows>;
   const float kNegInf = __int_as_float(0xff800000);
+  auto state = [&](int w) { return reinterpret_cast<State *>(smem + w * warp_bytes); };
   __syncthreads();
-  for (int i = threadIdx.x; i < n_h * p.hd; i += n_warps * 32) {
-    const int g = i / p.hd, d = i - g * p.hd;
-    float top = kNegInf;
-    for (int w = 0; w < n_warps; ++w)
-      top = fmaxf(top, reinterpret_cast<const State *>(smem + w * warp_bytes)->m[g]);
+  if (threadIdx.x < n_h) {
+    const int g = threadIdx.x;
+    float top = kNegInf, total = 0.f;
+    for (int w = 0; w < n_warps; ++w) top = fmaxf(top, state(w)->m[g]);
     const float base = top == kNegInf ? 0.f : top;
-    float x = 0.f, total = 0.f;
     for (int w = 0; w < n_warps; ++w) {
-      const State *s = reinterpret_cast<const State *>(smem + w * warp_bytes);
-      const float e = exp2f(s->m[g] - base);
-      total = fmaf(s->l[g], e, total);
-      x = fmaf(s->o[g][d], e, x);
+      const float e = exp2f(state(w)->m[g] - base);
+      total = fmaf(state(w)->l[g], e, total);
+      state(w)->m[g] = e;
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    reinterpret_cast<T *>(p.out + b * p.out_seq + (h0 + g) * p.out_head)[d] = Elem<DT>::from_f(x * inv);
-    if (p.lse && d == 0)
+    for (int w = 0; w < n_warps; ++w) state(w)->m[g] *= inv;
+    if (p.lse)
       p.lse[static_cast<int64_t>(b) * p.heads + h0 + g] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
+  }
+  __syncthreads();
+  constexpr int kCols = HD / 4;
+  for (int i = threadIdx.x; i < n_h * kCols; i += n_warps * 32) {
+    const int g = i / kCols, d = i % kCols * 4;
+    if (d >= p.hd) continue;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < n_warps; ++w) {
+      const float e = state(w)->m[g];
+      const float4 y = *reinterpret_cast<const float4 *>(&state(w)->o[g][d]);
+      x[0] = fmaf(y.x, e, x[0]), x[1] = fmaf(y.y, e, x[1]), x[2] = fmaf(y.z, e, x[2]), x[3] = fmaf(y.w, e, x[3]);
+    }
+    T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + (h0 + g) * p.out_head) + d;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (d + k < p.hd) dst[k] = Elem<DT>::from_f(x[k]);
   }
 }
 
@@ -456,7 +472,7 @@ struct Simt {
   static constexpr int kParts = 32 / kTok;              // lanes that share a token's score
   static constexpr int kQRow = (HD + 4 * kParts) * 4;  // the parts of a head 16 B apart in banks
   static constexpr int kWarpBytes = S::kBytes + G * kQRow + kTok * G * 8;
-  static constexpr int kSmem = W * kWarpBytes;
+  static constexpr int kWarp = kWarpBytes;
 };
 
 template <int HD, int G, int W, int kStages, int kTok>
@@ -481,7 +497,7 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
   float *qs = reinterpret_cast<float *>(mine + C::S::kBytes);
   uint64_t *ps = reinterpret_cast<uint64_t *>(qs + C::kQRow / 4 * G);  // [token][head]: the weight, twice
   typename C::S stream(p, mine, u, h0, n_h, lane);
-  stream.start(p.local ? local_walk(p, r, kTok, warp, W) : range_walk(p, win, ln, r, kTok, lane));
+  stream.start(p.local ? local_walk(p, r, kTok, warp, p.local) : range_walk(p, win, ln, r, kTok, lane));
 
   constexpr int kVec = HD >= 128 ? HD / 128 : 1;         // float4 columns per lane
   constexpr int kLanes = HD >= 128 ? 32 : HD / 4;        // lanes per token in the output product
@@ -659,7 +675,7 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
       }
       if (lane == 0) mine_out->m[g] = m[g], mine_out->l[g] = l[g];
     }
-    local_join<DKV_F32, HD, G>(p, smem, C::kWarpBytes, W, r, h0, n_h);
+    local_join<DKV_F32, HD, G>(p, smem, C::kWarpBytes, p.local, r, h0, n_h);
   }
 }
 
@@ -712,7 +728,7 @@ struct Mma {
   static constexpr int kStages = kStages_;
   using T = typename Elem<DT>::T;
   using S = Stream<T, HD, kStages, kTile>;
-  static constexpr int kSmem = W * S::kBytes;
+  static constexpr int kWarp = S::kBytes;
 };
 
 template <int DT, int HD, int W, int kStages>
@@ -739,7 +755,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
 
   char *mine = smem + warp * C::S::kBytes;
   typename C::S stream(p, mine, u, h0, n_h, lane);
-  stream.start(p.local ? local_walk(p, r, kTile, warp, W) : range_walk(p, win, ln, r, kTile, lane));
+  stream.start(p.local ? local_walk(p, r, kTile, warp, p.local) : range_walk(p, win, ln, r, kTile, lane));
 
   const int g = lane >> 2, t = lane & 3;
   // ldmatrix rows: K as (token, k half), V as (token half, column half) of a 16 x 16 block
@@ -914,7 +930,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
         mine_out->o[in][k * 16 + 8 + g] = o[k][2 + c];
       }
     }
-    local_join<DT, HD, 8>(p, smem, C::S::kBytes, W, r, h0, n_h);
+    local_join<DT, HD, 8>(p, smem, C::S::kBytes, p.local, r, h0, n_h);
   }
 }
 
@@ -1112,7 +1128,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 struct Shape {
   int hd_pad, g, warps, tokens;  // kernel variant
   int chunks, units;     // chunks of a group, KV heads x chunks
-  int local;             // a CTA per (sequence, unit) instead of ranges
+  int local;             // warps of a CTA per (sequence, unit), or 0: ranges
   int ranges;            // upper bound of the ranges in use
   int64_t parts;         // part slots
   int64_t o_bytes, bytes;
@@ -1182,7 +1198,10 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   s->warps = v.warps, s->tokens = v.tokens;
   s->chunks = (group + s->g - 1) / s->g;
   s->units = a->k_pages.n_heads * s->chunks;
-  s->local = a->seqs.max_seq_len <= kLocalTiles * s->tokens * s->warps && static_cast<int64_t>(a->seqs.n_seqs) * s->units <= sms;
+  const int64_t pairs = static_cast<int64_t>(a->seqs.n_seqs) * s->units;
+  s->local = s->warps;
+  while (s->local > 0 && pairs > static_cast<int64_t>(sms) * (s->warps / s->local)) --s->local;
+  if (a->seqs.max_seq_len > static_cast<int64_t>(kLocalTiles) * s->tokens * s->local) s->local = 0;
   const int64_t most = static_cast<int64_t>(sms) * s->warps / s->units;
   const int64_t line = static_cast<int64_t>(a->seqs.n_seqs) * (static_cast<int64_t>(a->seqs.max_seq_len) + kSeqCost);
   const int64_t want = line / kMinRange;
@@ -1210,20 +1229,22 @@ int allow_smem(int bytes) {
 template <int HD, int G, int W, int kStages, int kTok>
 int launch_simt(const Params &p, int grid, cudaStream_t st) {
   using C = Simt<HD, G, W, kStages, kTok>;
-  static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
-  const int rc = allow_smem<simt_kernel<HD, G, W, kStages, kTok>>(C::kSmem);
+  static_assert(W * C::kWarp <= 227 * 1024, "shared memory of the walk");
+  const int rc = allow_smem<simt_kernel<HD, G, W, kStages, kTok>>(W * C::kWarp);
   if (rc != DKV_OK) return rc;
-  DKV_CUDA_CHECK(launch_overlapped(simt_kernel<HD, G, W, kStages, kTok>, dim3(grid), W * 32, C::kSmem, st, p));
+  const int warps = p.local ? p.local : W;
+  DKV_CUDA_CHECK(launch_overlapped(simt_kernel<HD, G, W, kStages, kTok>, dim3(grid), warps * 32, warps * C::kWarp, st, p));
   return DKV_OK;
 }
 
 template <int DT, int HD, int W, int kStages>
 int launch_mma(const Params &p, int grid, cudaStream_t st) {
   using C = Mma<DT, HD, W, kStages>;
-  static_assert(C::kSmem <= 227 * 1024, "shared memory of the walk");
-  const int rc = allow_smem<mma_kernel<DT, HD, W, kStages>>(C::kSmem);
+  static_assert(W * C::kWarp <= 227 * 1024, "shared memory of the walk");
+  const int rc = allow_smem<mma_kernel<DT, HD, W, kStages>>(W * C::kWarp);
   if (rc != DKV_OK) return rc;
-  DKV_CUDA_CHECK(launch_overlapped(mma_kernel<DT, HD, W, kStages>, dim3(grid), W * 32, C::kSmem, st, p));
+  const int warps = p.local ? p.local : W;
+  DKV_CUDA_CHECK(launch_overlapped(mma_kernel<DT, HD, W, kStages>, dim3(grid), warps * 32, warps * C::kWarp, st, p));
   return DKV_OK;
 }
 

@@ -123,6 +123,23 @@ def run_attention(c, heads, hd, dtype, dev, seed=1, scale=None, amp=1.5):
     return q, out, lse
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_seq", [16, 40, 100, 220, 600, 900])
+def test_attention_one_launch_of_fewer_warps(cuda, dtype, n_seq):
+    """More pairs of sequence and KV head than SMs: CTAs of 6, 4, 3, 2 or 1 warps, up to one a CTA."""
+    rng = random.Random(n_seq)
+    c = Cache([rng.choice([0, 1, 16, rng.randrange(70)]) for _ in range(n_seq)], 4, 64, 16, dtype, cuda)
+    g = torch.Generator().manual_seed(7)
+    q = torch.randn(n_seq, 12, 64, generator=g).to(dtype).to(cuda)
+    out, lse = dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), return_lse=True, check=True)
+    for b in rng.sample(range(n_seq), 16):
+        check_attention(out[b:b + 1], lse[b:b + 1], q[b:b + 1], lambda _, b=b: c.tokens(b), 64 ** -0.5)
+    split = dkv.SeqBatchTensors(cu_seqlens=c.cu, block_tables=c.tables, max_seq_len=9000)
+    other = dkv.paged_decode_attention(q, c.k, c.v, split)
+    # both are within the derived tolerance of the exact result, here taken at its largest
+    assert float((out.double() - other.double()).abs().max()) <= 2 * (torch.finfo(dtype).eps + 2.0 ** -15) * float(c.v.double().abs().max())
+
+
 LENS = [0, 1, 2, 15, 16, 17, 33, 100, 0, 333, 64]
 
 
