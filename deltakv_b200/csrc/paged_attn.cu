@@ -410,8 +410,8 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x to 2 ulp, subnormal resu
 }
 
 // The join within a CTA: each warp's (m, l) and O (rows of HD + 4: no bank conflicts) lie at the
-// front of its ring.  A thread per head turns every warp's m into that warp's weight, then the threads sum
-// the weighted O, four columns at a time.
+// front of its ring.  Sixteen lanes a head (there are at most 16 warps) turn every warp's m into that warp's
+// weight, then the threads sum the weighted O, four columns at a time.
 template <int HD, int kRows>
 struct LocalState {
   float o[kRows][HD + 4];
@@ -425,19 +425,20 @@ __device__ __forceinline__ void local_join(const Params &p, char *smem, int warp
   const float kNegInf = __int_as_float(0xff800000);
   auto state = [&](int w) { return reinterpret_cast<State *>(smem + w * warp_bytes); };
   __syncthreads();
-  if (threadIdx.x < n_h) {
-    const int g = threadIdx.x;
-    float top = kNegInf, total = 0.f;
-    for (int w = 0; w < n_warps; ++w) top = fmaxf(top, state(w)->m[g]);
-    const float base = top == kNegInf ? 0.f : top;
-    for (int w = 0; w < n_warps; ++w) {
-      const float e = exp2f(state(w)->m[g] - base);
-      total = fmaf(state(w)->l[g], e, total);
-      state(w)->m[g] = e;
-    }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    for (int w = 0; w < n_warps; ++w) state(w)->m[g] *= inv;
-    if (p.lse)
+  const int lane = threadIdx.x & 31;
+  for (int i0 = threadIdx.x - lane; i0 < n_h * 16; i0 += n_warps * 32) {  // 16 lanes a head, one a warp's part
+    const int g = min((i0 + lane) / 16, n_h - 1), w = lane & 15;
+    const bool mine = w < n_warps && i0 + lane < n_h * 16;
+    const float m = w < n_warps ? state(w)->m[g] : kNegInf;
+    float top = m;
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    const float e = ex2(m - (top == kNegInf ? 0.f : top));
+    float total = w < n_warps ? state(w)->l[g] * e : 0.f;
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
+    if (mine) state(w)->m[g] = total == 0.f ? 0.f : e / total;
+    if (mine && w == 0 && p.lse)
       p.lse[static_cast<int64_t>(b) * p.heads + h0 + g] = (top + (log2f(total) - p.bias)) * 0.6931471805599453f;
   }
   __syncthreads();
