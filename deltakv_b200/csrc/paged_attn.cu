@@ -37,7 +37,10 @@ constexpr int kSeqCost = 48;
 // 60 of 100 / 200 / 300 (3 / 5 / 7 tiles of 3 warps) 11.8 / 8.7, 14.7 / 11.8, 16.8 / 14.7, and of 1..100 / 200 /
 // 300 10.4 / 6.6, 10.6 / 9.1, 11.1 / 11.7.  The border is at 5 to 7 tiles for other head sizes and fp32 as well.
 constexpr int kLocalTiles = 5;
-constexpr int kMinRange = 32;  // tokens below which a range is not cut further
+// Tokens below which a range is not cut further (at least two tiles: the join counts on it).  Sixteen mixed
+// shapes at 32 / 64 / 96: geometric mean 14.2 / 14.9 / 15.6 us.
+constexpr int kMinRange = 32;
+static_assert(kMinRange >= 2 * kTile, "a range inside a sequence has at least one tile");
 
 struct Params {
   const char *q;

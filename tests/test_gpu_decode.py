@@ -393,6 +393,34 @@ def test_attention_into_its_query(cuda, lens):
     assert dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), out=q) is q and torch.equal(q, want)
 
 
+def test_attention_workspace_of_the_c_entry(cuda):
+    """A missing, short or misaligned workspace is refused before anything is launched."""
+    import ctypes as C
+
+    from deltakv_b200 import _lib as L
+
+    c = Cache([9000], 2, 64, 16, BF, cuda)
+    q = torch.randn(1, 8, 64, device=cuda).to(BF)
+    out = torch.full_like(q, 7.0)
+    a = L.PagedDecodeArgs(q.data_ptr(), 512, 64, 8, 0.125, c.seqs().struct(), ops.paged_desc(c.k), ops.paged_desc(c.v),
+                          out.data_ptr(), 512, 64, None, None, 0, None)
+    need = C.c_int64()
+    lib = L.lib()
+    assert lib.dkv_paged_decode_workspace_bytes(C.byref(a), C.byref(need)) == L.DKV_OK and need.value > 0
+    stream = torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(need.value + 16, dtype=torch.uint8, device=cuda)
+    assert lib.dkv_paged_decode_attention(C.byref(a), stream) == L.DKV_ERR_WORKSPACE
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need.value - 1
+    assert lib.dkv_paged_decode_attention(C.byref(a), stream) == L.DKV_ERR_WORKSPACE
+    a.workspace, a.workspace_bytes = ws.data_ptr() + 4, need.value
+    assert lib.dkv_paged_decode_attention(C.byref(a), stream) == L.DKV_ERR_ALIGNMENT
+    torch.cuda.synchronize()
+    assert torch.all(out == 7.0)
+    a.workspace = ws.data_ptr()
+    assert lib.dkv_paged_decode_attention(C.byref(a), stream) == L.DKV_OK
+    assert torch.equal(out, dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), scale=0.125))
+
+
 def test_attention_without_blocks(cuda):
     pages = torch.zeros(0, 16, 2, 64, dtype=BF, device=cuda)
     q = torch.randn(2, 4, 64, device=cuda).to(BF)
