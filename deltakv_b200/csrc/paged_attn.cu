@@ -950,8 +950,10 @@ constexpr int kMaxRanges = 2048;
 // joined by the CTA: a thread per part's weight, then VW columns a thread, a group of threads for
 // every so many-th part.  The parts' addresses are an arithmetic sequence, so that several parts'
 // loads are in flight: with a test in front of each load, the 222 parts of one long sequence took
-// 12 us.  128 threads fit beside the walk's CTA, so most CTAs are in place before the walk ends.
+// 12 us.  (At head_dim 128 and 16 bits the walk's CTA leaves no registers, so a CTA starts where one of the
+// walk has ended.)
 constexpr int kJoinThreads = 128;
+constexpr int kJoinWide = 256;
 
 // acc += sum of w(i) part(i) over i = i0, i0 + by, ... < n, eight loads at a time (past the end the last
 // part is loaded again and left out: a loop for the remainder would wait for each)
@@ -982,14 +984,14 @@ __device__ __forceinline__ void add_parts(float (&acc)[VW], const float *src, in
   }
 }
 
-template <int DT, int VW>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int g_unit, int by_seq,
+template <int DT, int VW, int kThreads>
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p, int g_unit, int by_seq,
                                                            int hpc) {
   using T = typename Elem<DT>::T;
   extern __shared__ __align__(16) char smem[];
   float *weight = reinterpret_cast<float *>(smem), *part_l = weight + p.ranges;
-  __shared__ float red[kJoinThreads * VW];
-  __shared__ float red_m[kJoinThreads / 32], red_l[kJoinThreads / 32];
+  __shared__ float red[kThreads * VW];
+  __shared__ float red_m[kThreads / 32], red_l[kThreads / 32];
   const float kNegInf = __int_as_float(0xff800000);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // This grid is put in place once every CTA of the walk has begun, that is after all that was before the
@@ -1074,7 +1076,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   for (int h = h0; h < h1; ++h) {
     const int64_t part0 = part_at(h);
     float top = kNegInf;
-    for (int i = tid; i < n; i += kJoinThreads) {
+    for (int i = tid; i < n; i += kThreads) {
       const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (part0 + i * stride + (i ? 0 : g_unit)));
       weight[i] = ml.x, part_l[i] = ml.y;
       top = fmaxf(top, ml.x);
@@ -1084,10 +1086,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     if (lane == 0) red_m[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kJoinThreads / 32; ++i) top = fmaxf(top, red_m[i]);
+    for (int i = 0; i < kThreads / 32; ++i) top = fmaxf(top, red_m[i]);
     const float base = top == kNegInf ? 0.f : top;
     float sum = 0.f;
-    for (int i = tid; i < n; i += kJoinThreads) {
+    for (int i = tid; i < n; i += kThreads) {
       const float e = exp2f(weight[i] - base);
       weight[i] = e;
       sum = fmaf(part_l[i], e, sum);
@@ -1098,9 +1100,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     __syncthreads();
     float total = 0.f;
 #pragma unroll
-    for (int i = 0; i < kJoinThreads / 32; ++i) total += red_l[i];
+    for (int i = 0; i < kThreads / 32; ++i) total += red_l[i];
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    const int wide = min(share, kJoinThreads), groups = kJoinThreads / wide;
+    const int wide = min(share, kThreads), groups = kThreads / wide;
     for (int c0 = col0; c0 < cols; c0 += wide) {  // one pass unless head_dim is odd and above 128
       const int c = min(c0 + tid % wide, cols - 1), pg = tid / wide;
       float acc[VW];
@@ -1113,8 +1115,20 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 #pragma unroll
       for (int e = 0; e < VW; ++e) red[tid * VW + e] = acc[e];
       __syncthreads();
+      // the groups' sums: every eighth of them, then the eight
+      if (pg < min(groups, 8))
+        for (int i = pg + 8; i < groups; i += 8)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) acc[e] += red[(i * wide + tid % wide) * VW + e];
+      if (groups > 8) {
+        __syncthreads();
+        if (pg < 8)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) red[tid * VW + e] = acc[e];
+        __syncthreads();
+      }
       if (pg == 0 && c0 + tid < cols) {
-        for (int i = 1; i < groups; ++i)
+        for (int i = 1; i < min(groups, 8); ++i)
 #pragma unroll
           for (int e = 0; e < VW; ++e) acc[e] += red[(i * wide + tid) * VW + e];
         store(h, c, acc, inv);
@@ -1296,8 +1310,13 @@ int launch(const Params &p, const Shape &s, cudaStream_t st) {
   // very few: several CTAs for each head
   const int split = static_cast<int64_t>(cut) * p.heads <= 148 && p.hd >= 64 ? 4 : 1;
   const dim3 grid(cut, (p.heads + hpc - 1) / hpc, split);
-  const auto kernel = p.hd % 4 == 0 ? join_kernel<DT, 4> : join_kernel<DT, 1>;
-  DKV_CUDA_CHECK(launch_overlapped(kernel, grid, kJoinThreads, s.ranges * 8, st, p, s.g, by_seq, hpc));
+  // heads of which some may have more parts than a CTA has threads: more threads (one sequence of 131071, 8 KV heads:
+  // 99.5 -> 97.5 us; three of up to 13687, 2 KV heads: 17.4 -> 14.8), which cost time where there are fewer parts (one
+  // of 47238, 16 KV heads of 7 query heads each, 111 ranges: 72.9 -> 75.5)
+  const bool wide = split > 1 && s.ranges > kJoinThreads;
+  const auto kernel = wide ? (p.hd % 4 == 0 ? join_kernel<DT, 4, kJoinWide> : join_kernel<DT, 1, kJoinWide>)
+                           : (p.hd % 4 == 0 ? join_kernel<DT, 4, kJoinThreads> : join_kernel<DT, 1, kJoinThreads>);
+  DKV_CUDA_CHECK(launch_overlapped(kernel, grid, wide ? kJoinWide : kJoinThreads, s.ranges * 8, st, p, s.g, by_seq, hpc));
   return DKV_OK;
 }
 
