@@ -1311,9 +1311,10 @@ int launch(const Params &p, const Shape &s, cudaStream_t st) {
   const int split = static_cast<int64_t>(cut) * p.heads <= 148 && p.hd >= 64 ? 4 : 1;
   const dim3 grid(cut, (p.heads + hpc - 1) / hpc, split);
   // heads of which some may have more parts than a CTA has threads: more threads (one sequence of 131071, 8 KV heads:
-  // 99.5 -> 97.5 us; three of up to 13687, 2 KV heads: 17.4 -> 14.8), which cost time where there are fewer parts (one
-  // of 47238, 16 KV heads of 7 query heads each, 111 ranges: 72.9 -> 75.5)
-  const bool wide = split > 1 && s.ranges > kJoinThreads;
+  // 99.5 -> 97.5 us; three of up to 13687, 2 KV heads: 17.4 -> 14.8; 5 of 15930, 40 heads: 54 -> 52), which cost time
+  // where there are fewer parts (one of 47238, 16 KV heads of 7 query heads each, 111 ranges: 72.9 -> 75.5) and
+  // where not all CTAs run at once (62 of 6119, 6 heads: 72.8 -> 74.3; 84 of 1..3200, 12 heads: 11.6 -> 15.5)
+  const bool wide = static_cast<int64_t>(cut) * p.heads <= 148 * 2 && s.ranges > kJoinThreads;
   const auto kernel = wide ? (p.hd % 4 == 0 ? join_kernel<DT, 4, kJoinWide> : join_kernel<DT, 1, kJoinWide>)
                            : (p.hd % 4 == 0 ? join_kernel<DT, 4, kJoinThreads> : join_kernel<DT, 1, kJoinThreads>);
   DKV_CUDA_CHECK(launch_overlapped(kernel, grid, wide ? kJoinWide : kJoinThreads, s.ranges * 8, st, p, s.g, by_seq, hpc));
