@@ -88,7 +88,7 @@ def build_step() -> Path:
            "-I", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
            "-isystem", str(root / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
            str(STEP_SRC), "-o", str(tmp), "-L", str(root / "lib"),
-           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for {STEP_SRC.name}:\n{res.stdout}\n{res.stderr}")

@@ -13,6 +13,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -89,6 +90,13 @@ std::string shape_text(const Tensor &t) {
   std::string s = "(";
   for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
   return s + (t.dim() == 1 ? ",)" : ")");
+}
+// a new tensor straight from the device's allocator (the dispatcher's way to it costs as much again)
+Tensor fresh_tensor(at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
+  return Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
+}
+Tensor fresh_like(const Tensor &t) {
+  return t.is_contiguous() ? fresh_tensor(t.sizes(), t.scalar_type(), t.device()) : at::empty_like(t);
 }
 void *ptr(const Tensor *t) { return t == nullptr ? nullptr : t->data_ptr(); }
 
@@ -213,8 +221,8 @@ PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t count) {
     const Place at_("plan_paged_step", lengths);
     at_.also(&tables), at_.also(fresh), at_.also(held), at_.also(free_blocks);
     const c10::DeviceGuard guard(at_.device);
-    Tensor out = at::empty({3 * n + 3 + rows}, lengths.options().dtype(at::kInt));
-    Tensor slots = at::empty({rows}, lengths.options().dtype(at::kLong));
+    Tensor out = fresh_tensor({3 * n + 3 + rows}, at::kInt, at_.device);
+    Tensor slots = fresh_tensor({rows}, at::kLong, at_.device);
     dkv_step_plan_args p;
     p.lengths = lengths.data_ptr<int32_t>();
     p.new_lengths = static_cast<int32_t *>(ptr(fresh));
@@ -302,7 +310,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
     }
     const c10::DeviceGuard guard(at_.device);
     Tensor made;
-    if (q && !q_out) made = at::empty_like(*q), q_out = &made;
+    if (q && !q_out) made = fresh_like(*q), q_out = &made;
     dkv_append_args p;
     p.k = k.data_ptr(), p.v = v.data_ptr(), p.q = ptr(q);
     p.in_dtype = dtype_code(k.scalar_type());
@@ -372,8 +380,8 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t count) {
       value_error("block_tables must be a row-major [n_seqs, max_blocks] int32 tensor");
     const c10::DeviceGuard guard(at_.device);
     Tensor made, lse, workspace;
-    if (!out) made = at::empty_like(q), out = &made;
-    if (return_lse) lse = at::empty({n, heads}, q.options().dtype(at::kFloat));
+    if (!out) made = fresh_like(q), out = &made;
+    if (return_lse) lse = fresh_tensor({n, heads}, at::kFloat, at_.device);
     dkv_paged_decode_args p;
     p.q = q.data_ptr();
     p.q_stride_seq = q.stride(0), p.q_stride_head = q.stride(1);
@@ -395,7 +403,7 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t count) {
     int64_t bytes = 0;
     check(g_workspace(&p, &bytes), "dkv_paged_decode_workspace_bytes");
     if (bytes > 0) {  // in stream order the allocator may give it away once the launches are queued
-      workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+      workspace = fresh_tensor({bytes}, at::kByte, at_.device);
       p.workspace = workspace.data_ptr(), p.workspace_bytes = bytes;
     }
     check(g_attend(&p, at_.stream()), "dkv_paged_decode_attention");
