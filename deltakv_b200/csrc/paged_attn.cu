@@ -791,22 +791,27 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
     if (mt.w) break;
     const int b = mt.x;
     if (mt.y & kFirst) {
+      // (lanes past the unit's heads repeat the last one; their results are not stored)
       const unsigned short *qr =
-          reinterpret_cast<const unsigned short *>(p.q + b * p.q_seq + (h0 + min(g, n_h - 1)) * p.q_head);
+          reinterpret_cast<const unsigned short *>(p.q + b * p.q_seq + (h0 + min(g, n_h - 1)) * p.q_head) + t * 2;
+      if (p.pairs) {  // outside the loop: a branch between the loads would have each waited for
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k)
+        for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = k * 16 + e * 8 + t * 2;
-          uint32_t w = 0;
-          if (p.pairs) {
-            if (d < p.hd) w = *reinterpret_cast<const uint32_t *>(qr + d);
-          } else {
-            if (d < p.hd) w = qr[d];
-            if (d + 1 < p.hd) w |= static_cast<uint32_t>(qr[d + 1]) << 16;
+          for (int e = 0; e < 2; ++e) {
+            const int d = k * 16 + e * 8;
+            qf[k][e] = d + t * 2 < p.hd ? *reinterpret_cast<const uint32_t *>(qr + d) : 0;
           }
-          qf[k][e] = g < n_h ? w : 0;
-        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int d = k * 16 + e * 8;
+            const uint32_t lo = d + t * 2 < p.hd ? qr[d] : 0, hi = d + t * 2 + 1 < p.hd ? qr[d + 1] : 0;
+            qf[k][e] = lo | hi << 16;
+          }
+      }
       clear();
     }
     cp_async_wait<kStages - 1>();  // after a first tile's q is on its way
