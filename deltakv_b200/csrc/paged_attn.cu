@@ -545,12 +545,21 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
     if (mt.w) break;
     const int b = mt.x;
     if (mt.y & kFirst) {
-      for (int i = lane; i < G * HD; i += 32) {
-        const int g = i / HD, d = i % HD;
-        float x = 0.f;
-        if (g < n_h && d < p.hd)
-          x = reinterpret_cast<const float *>(p.q + b * p.q_seq + (h0 + g) * p.q_head)[d];
-        qs[g * (C::kQRow / 4) + d + d / (HD / C::kParts) * 4] = x;
+      // loads in flight together (8 heads x 32 with more of them spill)
+      constexpr int kLoads = G * HD / 32, kAtOnce = HD == 32 ? 4 : kLoads < 16 ? kLoads : 16;
+#pragma unroll 1
+      for (int k0 = 0; k0 < kLoads; k0 += kAtOnce) {
+        float x[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          const int g = (k0 + k) * 32 / HD, d = (k0 + k) * 32 % HD + lane;
+          x[k] = g < n_h && d < p.hd ? reinterpret_cast<const float *>(p.q + b * p.q_seq + (h0 + g) * p.q_head)[d] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          const int g = (k0 + k) * 32 / HD, d = (k0 + k) * 32 % HD + lane;
+          qs[g * (C::kQRow / 4) + d + d / (HD / C::kParts) * 4] = x[k];
+        }
       }
       clear();
     }
