@@ -17,8 +17,8 @@
 // each sequence and KV head, its warps' parts joined in shared memory.
 //
 // Measured on a B200 (calls back to back; HBM floor at the measured 6535 GB/s): 32 sequences of
-// 20000..32768, 8 KV heads x 128, bf16: 569-591 us by the box's power (floor 529); one of 131071: 101-105 us
-// (82); 64 of 1..8192: 63-65 us (46); 256 of 1..600, f16: 29.6 us (17); fp32, 16 of 4096: 98 us (82).  About
+// 20000..32768, 8 KV heads x 128, bf16: 559-591 us by the box's power (floor 529); one of 131071: 97-102 us
+// (82); 64 of 1..8192: 62-65 us (46); 256 of 1..600, f16: 28.6 us (17); fp32, 16 of 4096: 97 us (82).  About
 // 12 us of each are the launch, the dependent loads before the first copy, the last warps and the join; the
 // rest streams at 0.93-0.97 of the peak.
 #include "dkv_common.cuh"

@@ -222,7 +222,7 @@ struct Raw<DT, 1> {
 // the row's slot, position and cos / sin are read once for all of them and 2 kHeads 16-byte loads
 // are in flight; the heads of a thread are `groups` apart, so that neighbouring threads read
 // neighbouring heads.  Bound by memory: every q, k and v element is read once and written once.  Measured
-// on a B200: 16384 rows of 32 + 8 + 8 heads x 128, bf16 69.5 us = 5.92 TB/s, 0.91 of the measured HBM rate
+// on a B200: 16384 rows of 32 + 8 + 8 heads x 128, bf16 68-70 us = 5.9-6.0 TB/s, 0.90-0.92 of the measured HBM rate
 // (an element pair a thread: 312 us; two heads a thread 75 us; a thread's heads adjacent 71 us); 64 rows 3.0 us.
 constexpr int kHeads = 4;
 
