@@ -157,6 +157,13 @@ void written(const Tensor &t, const char *name, const Tensor *input, const char 
     value_error(std::string(name) + " overlaps " + input_name + " without being it");
 }
 
+// a tensor that is written and another that must not lie over it (as far as the strides tell)
+void apart(const Tensor &t, const char *name, const Tensor &other, const char *other_name) {
+  const at::MemOverlapStatus s = at::get_overlap_status(t, other);
+  if (s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial)
+    value_error(std::string(name) + " and " + other_name + " share memory");
+}
+
 dkv_paged_cache describe(const Tensor &t, int code) {
   dkv_paged_cache c;
   c.base = t.data_ptr();
@@ -278,6 +285,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
     if (slots.scalar_type() != at::kLong) type_error("slots must be int64");
     if (slots.dim() != 1 || !slots.is_contiguous()) value_error("slots must be a contiguous vector");
     written(pages.k, "k_pages", nullptr, ""), written(pages.v, "v_pages", nullptr, "");
+    apart(pages.k, "k_pages", pages.v, "v_pages");
     rows_of(k, "k", rows, pages.heads, pages.hd);
     rows_of(v, "v", rows, pages.heads, pages.hd);
     if (v.scalar_type() != k.scalar_type() || (q && q->scalar_type() != k.scalar_type()))
@@ -298,6 +306,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
         rows_of(*q_out, "q_out", rows, q->size(1), pages.hd);
         if (q_out->scalar_type() != q->scalar_type()) type_error("q_out must have q's dtype");
         written(*q_out, "q_out", q, "q");
+        apart(*q_out, "q_out", k, "k"), apart(*q_out, "q_out", v, "v");
       }
     }
     const Place at_("append_into_paged", k);

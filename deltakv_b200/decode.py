@@ -111,7 +111,8 @@ def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, sl
     is the pages' or fp32, rounded once on the way into the pages.
 
     The stored values replace what the slots held (``scatter_into_paged`` adds).  Slots must be
-    distinct.  ``check=True`` raises recorded range errors (a slot beyond the pages, a position
+    distinct, and the K pages, the V pages, ``q_out`` and the inputs other than ``q`` apart in memory.
+    ``check=True`` raises recorded range errors (a slot beyond the pages, a position
     beyond the tables: those rows store nothing).
     """
     native = _native_module or _native()

@@ -84,6 +84,19 @@ def test_append_refuses(change, error, text):
         _append(**change)
 
 
+@pytest.mark.parametrize("change,text", [
+    (lambda p, x: dict(k_pages=p, v_pages=p), "k_pages and v_pages share memory"),
+    (lambda p, x: dict(k_pages=p[:4], v_pages=p[2:6]), "k_pages and v_pages share memory"),
+    (lambda p, x: dict(q=torch.zeros(3, 2, 8, dtype=BF), k=x[:3], q_out=x[:3], **_ROPE), "q_out and k share memory"),
+    (lambda p, x: dict(q=torch.zeros(3, 2, 8, dtype=BF), v=x[:3], q_out=x[1:4], **_ROPE), "q_out and v share memory"),
+    (lambda p, x: dict(k_pages=p[:4], v_pages=p[4:]), "CUDA"),  # side by side: on to the next check
+])
+def test_append_refuses_shared_memory(change, text):
+    pages, rows = torch.zeros(8, 4, 2, 8, dtype=BF), torch.zeros(4, 2, 8, dtype=BF)
+    with pytest.raises(ValueError, match=text):
+        _append(**change(pages, rows))
+
+
 def _attend(**change):
     a = dict(q=torch.zeros(2, 4, 8, dtype=BF), k_pages=torch.zeros(4, 4, 2, 8, dtype=BF),
              v_pages=torch.zeros(4, 4, 2, 8, dtype=BF))

@@ -194,6 +194,16 @@ def test_attention_long_and_ragged(cuda, dtype, lens):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,n_kv,heads,hd", [
+    ([30001], 1, 2, 128), ([30001], 1, 2, 50), ([7000, 9000, 4], 1, 3, 32),  # hundreds of parts of few heads
+    ([5000] * 8, 2, 24, 80), ([3001] * 9, 1, 20, 33), ([20000, 30], 1, 140, 64),  # of more heads, each CTA with one
+    ([2500] * 12, 2, 64, 96), ([4000] * 30, 4, 40, 64), ([900] * 3, 3, 3, 256),  # parts of many heads; few parts
+])
+def test_attention_joins_of_every_kind(cuda, dtype, lens, n_kv, heads, hd):
+    run_attention(Cache(lens, n_kv, hd, 16, dtype, cuda), heads, hd, dtype, cuda)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_attention_many_sequences(cuda, dtype):
     rng = random.Random(5)
     lens = [rng.choice([0, 1, 5, rng.randrange(60)]) for _ in range(3000)]
@@ -766,6 +776,31 @@ def test_captured_steps(cuda, dtype):
         a.verify(news[0], *graphs[0][1])
         b.verify(news[1], *graphs[1][1])
     ops.status_word(cuda).raise_if_set("captured steps")
+
+
+def test_steps_without_autograd_or_with_it(cuda):
+    """Inference mode, no_grad and inputs that require gradients: the same values, and no graph behind them."""
+    c = Cache([40, 5], 2, 64, 16, BF, cuda)
+    rope, _, _ = rope_tables(64, 50, cuda)
+    lens = torch.tensor([40, 5], dtype=torch.int32, device=cuda)
+    qkv = torch.randn(2, 12, 64, device=cuda).to(BF)
+    ones = torch.ones(2, dtype=torch.int32, device=cuda)
+
+    def step(x):
+        plan = dkv.plan_paged_step(lens, c.tables, 16, rows=2, max_seq_len=40, new_lengths=ones)
+        q = dkv.append_into_paged(x[:, 8:10], x[:, 10:], c.k, c.v, plan.slots, q=x[:, :8], positions=plan.positions,
+                                  rope=rope)
+        return plan.slots, q, *dkv.paged_decode_attention(q, c.k, c.v, plan.seqs, return_lse=True)
+
+    want = step(qkv)
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(step(qkv), want))
+    with torch.inference_mode():
+        got = step(qkv)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(a.is_inference() for a in got)
+    got = step(qkv.clone().requires_grad_())
+    assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, want))
+    got[1].zero_(), got[2].mul_(2)  # ordinary tensors
 
 
 @pytest.mark.parametrize("lens", [[300, 40], [9000, 40]])
