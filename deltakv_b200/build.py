@@ -71,10 +71,15 @@ def _step_stamp() -> str:
     return f"{sys.version} torch {torch.__version__}"
 
 
-def build_step() -> Path:
-    """The extension module; rebuilt when its source, the C header, Python or torch changed."""
+def build_step() -> Path | None:
+    """The extension module; rebuilt when its source, the C header, Python or torch changed.
+
+    Against a torch without CUDA there is nothing to build it with (and no GPU tensor to call it on): None."""
     import torch
 
+    if torch.version.cuda is None:
+        print(f"{STEP.name} not built: torch {torch.__version__} has no CUDA", file=sys.stderr)
+        return None
     stamp = BUILD / "step.stamp"
     newest = max(STEP_SRC.stat().st_mtime, *(h.stat().st_mtime for h in (ROOT / "include").glob("*.h")))
     if STEP.exists() and STEP.stat().st_mtime >= newest and stamp.exists() and stamp.read_text() == _step_stamp():
@@ -98,12 +103,18 @@ def build_step() -> Path:
 
 
 def build(ptxas: bool = False, verbose: bool = False) -> Path:
+    """Both; the library does not depend on torch, so it is linked even where the module's build raises."""
     BUILD.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
     with ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
         step = ex.submit(build_step)
         results = list(ex.map(lambda s: _compile(s, ptxas), srcs))
+        out = _link(results, ptxas, verbose)
         step.result()
+    return out
+
+
+def _link(results: list[tuple[Path, str]], ptxas: bool, verbose: bool) -> Path:
     if ptxas or verbose:
         for _, log in results:
             if log:
