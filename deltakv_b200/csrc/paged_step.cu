@@ -320,7 +320,9 @@ extern "C" int dkv_plan_paged_step(const dkv_step_plan_args *args, dkv_stream_t 
   if (a.n_seqs > 0 && (a.table_lens_out == a.table_lens || a.table_lens_out == a.lengths))
     return DKV_ERR_INVALID_ARGUMENT;
   const int smem = 2 * (a.n_seqs + 1) * static_cast<int>(sizeof(int));
-  if (smem > 48 * 1024)  // always to the same limit: two threads' calls cannot lower each other's
+  // A launch without the opt-in has 48 KB, the kernel's own static arrays included (384 bytes now): opted in well
+  // before that.  Always to the same limit: two threads' calls cannot lower each other's.
+  if (smem > 40 * 1024)
     DKV_CUDA_CHECK(cudaFuncSetAttribute(step::plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         2 * (step::kMaxSeqs + 1) * static_cast<int>(sizeof(int))));
   const int64_t want = (static_cast<int64_t>(a.n_rows) + 2 * step::kPlanThreads - 1) / (2 * step::kPlanThreads);

@@ -13,6 +13,9 @@ from __future__ import annotations
 
 import math
 import random
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -535,6 +538,26 @@ def test_plan_largest_batch(cuda):
     with pytest.raises(dkv.DkvError, match="unsupported"):
         z = torch.zeros(n + 1, dtype=torch.int32, device=cuda)
         dkv.plan_paged_step(z, z[:, None].clone(), 16, rows=0, max_seq_len=0)
+
+
+_BATCHES_ALONE = """
+import torch, deltakv_b200 as dkv
+for n in (5119, 5120, 6095, 6096, 6100, 6143, 6144):
+    lens = torch.arange(1, n + 1, dtype=torch.int32, device="cuda") % 32 + 1
+    tables = torch.arange(2 * n, dtype=torch.int32, device="cuda").view(n, 2)
+    step = dkv.plan_paged_step(lens, tables, 16, rows=n, max_seq_len=32, new_lengths=torch.ones_like(lens), check=True)
+    pos = lens.long() - 1
+    assert torch.equal(step.slots, tables.gather(1, (pos // 16)[:, None])[:, 0].long() * 16 + pos % 16), n
+    assert torch.equal(step.positions.long(), pos) and int(step.seqs.cu_seqlens[-1]) == int(lens.sum()), n
+print("planned")
+"""
+
+
+def test_plan_batches_at_the_default_shared_memory_limit(cuda):
+    """Around 48 KB of shared memory, in a process that has planned no larger batch before."""
+    root = Path(__file__).resolve().parent.parent
+    got = subprocess.run([sys.executable, "-c", _BATCHES_ALONE], cwd=root, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and got.stdout.split()[-1] == "planned", got.stderr[-2000:]
 
 
 @pytest.mark.parametrize("text,lens,new,held,tables,free,rows", [
