@@ -353,7 +353,9 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t count) {
     const Tensor &cu = tensor(a[3], "cu_seqlens"), &tables = tensor(a[4], "block_tables");
     const Tensor *lens = maybe(a[5], "table_lens"), *out = maybe(a[8], "out");
     const int64_t max_seq_len = integer(a[6]);
-    const bool return_lse = PyObject_IsTrue(a[9]) == 1;
+    const int wanted = PyObject_IsTrue(a[9]);
+    if (wanted < 0) throw Raised{nullptr, ""};
+    const bool return_lse = wanted == 1;
     const int64_t n = cu.numel() - 1, hd = pages.hd;
     double scale = 1.0 / std::sqrt(static_cast<double>(hd > 0 ? hd : 1));
     if (a[7] != Py_None) {

@@ -128,6 +128,11 @@ def test_attention_refuses(change, error, text):
         _attend(**change)
 
 
+def test_attention_passes_on_a_truth_that_raises():
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        _attend(return_lse=torch.zeros(2))  # used to go on, with the error pending
+
+
 def _cache(**change):
     a = dict(base=P, dtype=L.DKV_BF16, block_size=16, n_heads=2, head_dim=64, num_blocks=4, stride_block=2048,
              stride_slot=128, stride_head=64)
