@@ -295,6 +295,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
                  dtype_name(pages.k.scalar_type()) + " pages (pass the pages' dtype or fp32)");
     if (cos) {
       if (!positions) value_error("rope needs positions");
+      if (cos->dim() == 2 && cos->size(0) == 0) value_error("rope tables without positions");
       int32_vector(*positions, "positions", rows);
     }
     if (!q && q_out) value_error("q_out without q");

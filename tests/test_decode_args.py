@@ -128,6 +128,13 @@ def test_attention_refuses(change, error, text):
         _attend(**change)
 
 
+def test_append_refuses_rope_tables_without_positions():
+    """No address stands for them: the C entry would take them for no rotation at all."""
+    for tables in ((torch.zeros(0, 4), torch.zeros(0, 4)), dkv.RotaryEmbedding(8, 0)):
+        with pytest.raises(ValueError, match="without positions"):
+            _append(rope=tables, positions=_ROPE["positions"])
+
+
 def test_attention_passes_on_a_truth_that_raises():
     with pytest.raises(RuntimeError, match="ambiguous"):
         _attend(return_lse=torch.zeros(2))  # used to go on, with the error pending
