@@ -51,6 +51,12 @@ PyObject *guarded(F f) {
     return f();
   } catch (const Raised &r) {
     if (r.type != nullptr) PyErr_SetString(r.type, r.text.c_str());
+  } catch (const c10::OutOfMemoryError &e) {  // what torch itself raises for it
+    PyObject *torch = PyImport_ImportModule("torch");
+    PyObject *type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    if (type != nullptr) PyErr_SetString(type, e.what_without_backtrace());
+    Py_XDECREF(type);
+    Py_XDECREF(torch);
   } catch (const c10::Error &e) {
     PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception &e) {

@@ -540,6 +540,20 @@ def test_plan_largest_batch(cuda):
         dkv.plan_paged_step(z, z[:, None].clone(), 16, rows=0, max_seq_len=0)
 
 
+def test_plan_without_memory_for_its_outputs(cuda):
+    """torch's own error, which a serving loop catches; the limit is this process's, nothing is filled up."""
+    z = torch.ones(1, dtype=torch.int32, device=cuda)
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(cuda).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved(cuda) + (64 << 20)) / total, cuda)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            dkv.plan_paged_step(z, z[:, None].clone(), 16, rows=1 << 28, max_seq_len=1)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0, cuda)
+    dkv.plan_paged_step(z, z[:, None].clone(), 16, rows=1, max_seq_len=1, check=True)
+
+
 _BATCHES_ALONE = """
 import torch, deltakv_b200 as dkv
 for n in (5119, 5120, 6095, 6096, 6100, 6143, 6144):
