@@ -101,8 +101,14 @@ std::string shape_text(const Tensor &t) {
 Tensor fresh_tensor(at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
   return Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }
+// [rows, heads, head_dim] like t, in t's order of rows and heads; head_dim stays contiguous, which empty_like
+// does not promise where t's rows or heads lie over each other (broadcast, sliding windows)
 Tensor fresh_like(const Tensor &t) {
-  return t.is_contiguous() ? fresh_tensor(t.sizes(), t.scalar_type(), t.device()) : at::empty_like(t);
+  if (!t.is_contiguous()) {
+    Tensor like = at::empty_like(t);
+    if (like.stride(2) == 1 || like.size(2) == 1) return like;
+  }
+  return fresh_tensor(t.sizes(), t.scalar_type(), t.device());
 }
 void *ptr(const Tensor *t) { return t == nullptr ? nullptr : t->data_ptr(); }
 

@@ -185,6 +185,25 @@ def test_attention_layouts_and_strides(cuda, dtype, layout):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("strides", [(1, 0, 1), (0, 0, 1), (7, 1, 1), (64, 2, 1), (0, 64, 1)])
+def test_queries_that_lie_over_each_other(cuda, dtype, strides):
+    """Broadcast and sliding-window q: the new output is an ordinary tensor."""
+    c = Cache([40, 3], 2, 64, 16, dtype, cuda)
+    rope, _, _ = rope_tables(64, 50, cuda)
+    slots = torch.tensor([3, 4], device=cuda)
+    pos = torch.tensor([7, 30], dtype=torch.int32, device=cuda)
+    k = torch.randn(2, 2, 64, device=cuda).to(dtype)
+    for n in (1, 2):
+        q = torch.randn(500, device=cuda).to(dtype).as_strided((n, 4, 64), strides)
+        seqs = dkv.SeqBatchTensors(cu_seqlens=c.cu[:n + 1], block_tables=c.tables[:n], max_seq_len=40)
+        got = dkv.paged_decode_attention(q, c.k, c.v, seqs, check=True)
+        assert torch.equal(got, dkv.paged_decode_attention(q.contiguous(), c.k, c.v, seqs)) and got.stride(2) == 1
+        turned = [dkv.append_into_paged(k[:n], k[:n], c.k, c.v, slots[:n], q=x, positions=pos[:n], rope=rope, check=True)
+                  for x in (q, q.contiguous())]
+        assert torch.equal(*turned) and turned[0].stride(2) == 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("fill", [math.nan, math.inf, -math.inf])
 def test_attention_never_reads_what_no_token_owns(cuda, dtype, fill):
     run_attention(Cache([1, 17, 0, 300, 15], 2, 64, 32, dtype, cuda, fill=fill), 8, 64, dtype, cuda)
