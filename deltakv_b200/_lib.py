@@ -33,6 +33,7 @@ DKV_MAX_LAYERS = 128
 
 EXPORTED = (
     "dkv_status_string",
+    "dkv_status_word",
     "dkv_abi_version",
     "dkv_last_cuda_error",
     "dkv_scatter_paged",
@@ -350,6 +351,8 @@ def _declare(lib: C.CDLL) -> None:
     P, I32, I64 = C.c_void_p, C.c_int32, C.c_int64
     lib.dkv_status_string.restype = C.c_char_p
     lib.dkv_status_string.argtypes = [C.c_int]
+    lib.dkv_status_word.restype = C.c_int
+    lib.dkv_status_word.argtypes = [C.POINTER(C.c_void_p)]
     lib.dkv_abi_version.restype = C.c_int
     lib.dkv_abi_version.argtypes = []
     lib.dkv_last_cuda_error.restype = C.c_char_p

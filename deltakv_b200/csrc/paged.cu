@@ -284,6 +284,16 @@ extern "C" int dkv_paged_compare_sums(const dkv_paged_cache *pages, int32_t n_la
                             fresh_head_stride, seqs, sums, status, stream);
 }
 
+namespace dkv {
+__device__ int32_t status_word;
+}
+
+extern "C" int dkv_status_word(int32_t **word) {
+  if (word == nullptr) return DKV_ERR_INVALID_ARGUMENT;
+  DKV_CUDA_CHECK(cudaGetSymbolAddress(reinterpret_cast<void **>(word), dkv::status_word));
+  return DKV_OK;
+}
+
 extern "C" const char *dkv_status_string(int status) {
   switch (status) {
     case DKV_OK: return "ok";

@@ -141,13 +141,40 @@ class StatusWord:
             raise L.DkvError(code, where)
 
 
+class _LibraryStatusWord(StatusWord):
+    """The library's own word of a device.
+
+    One made here on first use would, if that use is inside a graph capture, lie in the graph's
+    pool, unwritten until a replay and cleared by every one."""
+
+    def __init__(self, device: torch.device):
+        word = C.c_void_p()
+        with torch.cuda.device(device):
+            L.check(L.lib().dkv_status_word(C.byref(word)), "dkv_status_word")
+        self._ptr, self._device, self._t = int(word.value), device, None
+
+    @property
+    def ptr(self) -> int:
+        return self._ptr
+
+    @property
+    def __cuda_array_interface__(self) -> dict:
+        return {"shape": (1,), "typestr": "<i4", "data": (self._ptr, False), "strides": None, "version": 3}
+
+    @property
+    def t(self) -> torch.Tensor:
+        if self._t is None:
+            self._t = torch.as_tensor(self, device=self._device)
+        return self._t
+
+
 _status_words: dict[int, StatusWord] = {}
 
 
 def status_word(device: torch.device) -> StatusWord:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     if idx not in _status_words:
-        _status_words[idx] = StatusWord(torch.device("cuda", idx))
+        _status_words[idx] = _LibraryStatusWord(torch.device("cuda", idx))
     return _status_words[idx]
 
 

@@ -67,6 +67,11 @@ typedef struct CUstream_st *dkv_stream_t;
 
 /* Human-readable text of a status code (static storage). */
 const char *dkv_status_string(int status);
+
+/* *word: the device address of an int32 of the library on the current device, zero from the start, for
+ * the `status` arguments below.  It needs no allocation and no stream, so that a caller's first launch
+ * may be inside a graph capture; it is one word a device, shared by all who use it. */
+int dkv_status_word(int32_t **word);
 /* ABI version: bumped when a struct below changes.  2: dkv_exact_patch_args ends with x_sumsq and
    x_sumsq_layer_stride (a caller built against version 1 passes a shorter struct). */
 int dkv_abi_version(void);

@@ -918,6 +918,50 @@ def test_captured_between_copies_and_memsets(cuda):
         assert torch.equal(again, dkv.paged_decode_attention(want, c.k, c.v, step.seqs))
 
 
+_CAPTURE_FIRST = """
+import torch, deltakv_b200 as dkv
+from deltakv_b200 import ops
+dev = torch.device("cuda", 0)
+q = torch.ones(1, 4, 64, device=dev, dtype=torch.bfloat16)
+k = torch.ones(4, 16, 2, 64, device=dev, dtype=torch.bfloat16)
+v = torch.ones_like(k)
+ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+seqs = dkv.SeqBatchTensors(cu_seqlens=ints([0, 20]), block_tables=ints([[1, 9]]), max_seq_len=20)  # no block 9
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    out = dkv.paged_decode_attention(q, k, v, seqs)
+word = ops.status_word(dev)
+word.raise_if_set("nothing has run")
+good = dkv.SeqBatchTensors(cu_seqlens=ints([0, 20]), block_tables=ints([[1, 3]]), max_seq_len=20)
+assert torch.equal(dkv.paged_decode_attention(q, k, v, good, check=True), torch.ones_like(q))
+graph.replay()
+try:
+    word.raise_if_set("replay")
+except dkv.DkvError as e:
+    assert "block id outside" in str(e)
+else:
+    raise AssertionError("the replay recorded nothing")
+assert torch.equal(out, torch.ones_like(q))
+dkv.paged_decode_attention(q, k, v, seqs)  # recorded by an eager call
+seqs.block_tables.copy_(ints([[1, 3]]))
+graph.replay()                             # a good replay leaves it
+assert int(word.t) != 0
+del graph, out
+torch.cuda.empty_cache()
+word.t.zero_()
+dkv.paged_decode_attention(q, k, v, good, check=True)
+print("captured first")
+"""
+
+
+def test_first_use_inside_a_capture(cuda):
+    """The status word of a process whose first call is captured: eager calls and replays share one that is valid."""
+    root = Path(__file__).resolve().parent.parent
+    got = subprocess.run([sys.executable, "-c", _CAPTURE_FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and got.stdout.strip() == "captured first", got.stderr[-2000:]
+
+
 def test_step_beside_a_patch(cuda):
     """The pages the step writes are the ones the patch operators change: attend, patch, attend."""
     s = Server(cuda, BF)
