@@ -20,16 +20,17 @@ class RotaryEmbedding:
     def __init__(self, head_dim: int, max_seq: int = 8192, base: float = 10000.0):
         if head_dim % 2 != 0:
             raise ValueError("RoPE head_dim must be even")
-        inv_freq = 1.0 / (base ** (torch.arange(0, head_dim, 2, dtype=torch.float32) / head_dim))
-        t = torch.arange(max_seq, dtype=torch.float32)
-        freqs = torch.outer(t, inv_freq)
-        emb = torch.cat((freqs, freqs), dim=-1)
         self.head_dim = head_dim
         self.max_seq = max_seq
         self.base = base
-        self.inv_freq = inv_freq
-        self.cos_cached = emb.cos()
-        self.sin_cached = emb.sin()
+        with torch.inference_mode(False):  # ordinary tensors, whose changes half_tables can see
+            inv_freq = 1.0 / (base ** (torch.arange(0, head_dim, 2, dtype=torch.float32) / head_dim))
+            t = torch.arange(max_seq, dtype=torch.float32)
+            freqs = torch.outer(t, inv_freq)
+            emb = torch.cat((freqs, freqs), dim=-1)
+            self.inv_freq = inv_freq
+            self.cos_cached = emb.cos()
+            self.sin_cached = emb.sin()
 
 
 # per rope object (while it lives) and device: the tensors the tables were made from, their
@@ -38,15 +39,13 @@ class RotaryEmbedding:
 _table_cache: WeakKeyDictionary = WeakKeyDictionary()
 
 
-def _version(t: Tensor) -> int:
-    return 0 if t.is_inference() else t._version
-
-
 def half_tables(rope, device: torch.device) -> tuple[Tensor, Tensor]:
     """``(cos, sin)`` as contiguous fp32 ``[max_seq, head_dim/2]`` on ``device``.
 
     ``rope`` is a reference ``RotaryEmbedding`` module, one of this package, or a
-    ``(cos, sin)`` pair that is already half-width.
+    ``(cos, sin)`` pair that is already half-width.  A rope's tables are made once and again when
+    its tensors change; tensors made in inference mode do not tell, so theirs are made anew
+    each call (pass the pair to have none made).
     """
     if isinstance(rope, tuple):
         c, s = rope
@@ -55,19 +54,23 @@ def half_tables(rope, device: torch.device) -> tuple[Tensor, Tensor]:
             return c, s
         return c.to(device=device, dtype=torch.float32).contiguous(), s.to(device=device, dtype=torch.float32).contiguous()
     cos_full, sin_full = rope.cos_cached, rope.sin_cached
+    hd = cos_full.shape[-1]
+
+    def make() -> tuple[Tensor, Tensor]:
+        return (cos_full[:, : hd // 2].to(device=device, dtype=torch.float32).contiguous(),
+                sin_full[:, : hd // 2].to(device=device, dtype=torch.float32).contiguous())
+
+    if cos_full.is_inference() or sin_full.is_inference():
+        return make()
     try:
         made = _table_cache.setdefault(rope, {})
     except TypeError:  # an object without hash or weak references: made anew each call
         made = {}
-    source = (cos_full, sin_full, _version(cos_full), _version(sin_full))
+    source = (cos_full, sin_full, cos_full._version, sin_full._version)
     hit = made.get(str(device))
     if hit is not None and all(x is y for x, y in zip(hit[0][:2], source[:2])) and hit[0][2:] == source[2:]:
         return hit[1]
-    hd = cos_full.shape[-1]
-    out = (
-        cos_full[:, : hd // 2].to(device=device, dtype=torch.float32).contiguous(),
-        sin_full[:, : hd // 2].to(device=device, dtype=torch.float32).contiguous(),
-    )
+    out = make()
     made[str(device)] = (source, out)
     return out
 

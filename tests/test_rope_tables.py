@@ -43,3 +43,18 @@ def test_tables_from_a_module_and_inference_mode():
         rope = Rope()
         assert half_tables(rope, CPU)[0].shape == (9, 8)
     assert half_tables(rope, CPU)[1].shape == (9, 8)
+
+
+def test_tables_follow_a_rope_changed_in_inference_mode():
+    """Tensors of inference mode have no version; ordinary ones count changes made in it."""
+    with torch.inference_mode():
+        rope = RotaryEmbedding(64, 50)
+        bare = RotaryEmbedding(64, 50)
+        bare.cos_cached, bare.sin_cached = bare.cos_cached.clone(), bare.sin_cached.clone()
+        assert bare.cos_cached.is_inference() and not rope.cos_cached.is_inference()
+        for r in (rope, bare):
+            half_tables(r, CPU)
+            r.cos_cached.mul_(0.5)
+            assert torch.equal(half_tables(r, CPU)[0], r.cos_cached[:, :32])
+    assert half_tables(rope, CPU)[0] is half_tables(rope, CPU)[0]
+    assert torch.equal(half_tables(bare, CPU)[0], bare.cos_cached[:, :32])
