@@ -33,10 +33,39 @@ class RotaryEmbedding:
             self.sin_cached = emb.sin()
 
 
-# per rope object (while it lives) and device: the tensors the tables were made from, their
-# versions, and the tables.  Holding the source tensors keeps "is" meaningful: neither an object
-# nor a tensor whose address was reused can match.
-_table_cache: WeakKeyDictionary = WeakKeyDictionary()
+class _Kept:
+    """Half-width tables, and the tensors (with their versions) they were made from: holding those keeps
+    "is" meaningful, neither an object nor a tensor whose address was reused can match."""
+
+    __slots__ = ("cos_full", "sin_full", "versions", "tables", "captured")
+
+    def __init__(self, cos_full: Tensor, sin_full: Tensor, versions: tuple[int, int], tables: tuple[Tensor, Tensor]):
+        self.cos_full, self.sin_full, self.versions, self.tables = cos_full, sin_full, versions, tables
+        self.captured = False
+
+    def match(self, cos_full: Tensor, sin_full: Tensor) -> bool:
+        return (self.cos_full is cos_full and self.sin_full is sin_full
+                and self.versions == (cos_full._version, sin_full._version))
+
+
+_table_cache: WeakKeyDictionary = WeakKeyDictionary()  # per rope object, while it lives: {device: _Kept}
+_captured_tables: list[tuple[Tensor, Tensor]] = []     # what captured launches read: replays have only addresses
+
+
+def _capturing(device: torch.device) -> bool:
+    if device.type != "cuda":
+        return False
+    if device.index is None or device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _on_device(cos: Tensor, sin: Tensor, device: torch.device, capturing: bool) -> tuple[Tensor, Tensor]:
+    if capturing and (cos.device != device or sin.device != device):
+        raise RuntimeError(f"RoPE tables on {cos.device} cannot be copied to {device} inside a graph capture: "
+                           "call the operator (or half_tables) with this rope once before it")
+    return cos.to(device=device, dtype=torch.float32).contiguous(), sin.to(device=device, dtype=torch.float32).contiguous()
 
 
 def half_tables(rope, device: torch.device) -> tuple[Tensor, Tensor]:
@@ -46,33 +75,38 @@ def half_tables(rope, device: torch.device) -> tuple[Tensor, Tensor]:
     ``(cos, sin)`` pair that is already half-width.  A rope's tables are made once and again when
     its tensors change; tensors made in inference mode do not tell, so theirs are made anew
     each call (pass the pair to have none made).
+
+    Inside a graph capture, kept tables are used as they are and stay for the life of the process
+    (a replay knows their address alone, and goes on with the tables of its capture).  What is
+    not there yet is made by the graph itself, at every replay, and not kept; for that the rope's
+    tensors have to be on ``device``.
     """
     if isinstance(rope, tuple):
         c, s = rope
         if (c.dtype is torch.float32 and s.dtype is torch.float32 and c.device == device and s.device == device
                 and c.is_contiguous() and s.is_contiguous()):
             return c, s
-        return c.to(device=device, dtype=torch.float32).contiguous(), s.to(device=device, dtype=torch.float32).contiguous()
+        return _on_device(c, s, device, _capturing(device))
     cos_full, sin_full = rope.cos_cached, rope.sin_cached
-    hd = cos_full.shape[-1]
-
-    def make() -> tuple[Tensor, Tensor]:
-        return (cos_full[:, : hd // 2].to(device=device, dtype=torch.float32).contiguous(),
-                sin_full[:, : hd // 2].to(device=device, dtype=torch.float32).contiguous())
-
+    half = cos_full.shape[-1] // 2
+    capturing = _capturing(device)
     if cos_full.is_inference() or sin_full.is_inference():
-        return make()
+        return _on_device(cos_full[:, :half], sin_full[:, :half], device, capturing)
     try:
-        made = _table_cache.setdefault(rope, {})
+        kept = _table_cache.setdefault(rope, {})
     except TypeError:  # an object without hash or weak references: made anew each call
-        made = {}
-    source = (cos_full, sin_full, cos_full._version, sin_full._version)
-    hit = made.get(str(device))
-    if hit is not None and all(x is y for x, y in zip(hit[0][:2], source[:2])) and hit[0][2:] == source[2:]:
-        return hit[1]
-    out = make()
-    made[str(device)] = (source, out)
-    return out
+        kept = {}
+    hit = kept.get(str(device))
+    if hit is None or not hit.match(cos_full, sin_full):
+        versions = (cos_full._version, sin_full._version)
+        tables = _on_device(cos_full[:, :half], sin_full[:, :half], device, capturing)
+        if capturing:
+            return tables
+        hit = kept[str(device)] = _Kept(cos_full, sin_full, versions, tables)
+    if capturing and not hit.captured:
+        hit.captured = True
+        _captured_tables.append(hit.tables)
+    return hit.tables
 
 
 def max_positions(rope) -> int:

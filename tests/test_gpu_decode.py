@@ -918,6 +918,91 @@ def test_captured_between_copies_and_memsets(cuda):
         assert torch.equal(again, dkv.paged_decode_attention(want, c.k, c.v, step.seqs))
 
 
+class DeviceRope:
+    """A rope whose tables live on the GPU, as a module's buffers do; angles of the rows differ by `by`."""
+
+    def __init__(self, dev, hd=64, n=4096, by=1.0):
+        rope = dkv.RotaryEmbedding(hd, n, base=10000.0 * by)
+        self.cos_cached, self.sin_cached = rope.cos_cached.to(dev), rope.sin_cached.to(dev)
+
+    def turn(self, x, pos):
+        """fp32 in fp64, to be compared within two roundings."""
+        c, s = (t[pos.long(), : x.shape[2] // 2].double()[:, None] for t in (self.cos_cached, self.sin_cached))
+        lo, hi = x.double().chunk(2, -1)
+        return torch.cat([lo * c - hi * s, hi * c + lo * s], -1)
+
+
+class Turner:
+    """append_into_paged on fp32 rows of its own, for the q it returns."""
+
+    def __init__(self, dev, rows=3):
+        self.c = Cache([100], 2, 64, 16, F32, dev)
+        self.q, self.k = torch.randn(rows, 4, 64, device=dev), torch.randn(rows, 2, 64, device=dev)
+        self.pos = torch.arange(rows, dtype=torch.int32, device=dev) * 17 + 5
+        self.slots = torch.arange(rows, device=dev)
+
+    def __call__(self, rope):
+        return dkv.append_into_paged(self.k, self.k, self.c.k, self.c.v, self.slots, q=self.q, positions=self.pos, rope=rope)
+
+    def check(self, got, rope):
+        big = self.q.double().abs().amax(-1, keepdim=True)
+        assert torch.all((got.double() - rope.turn(self.q, self.pos)).abs() <= 2.0 ** -22 * big)
+
+
+def test_rope_first_used_inside_a_capture(cuda):
+    """The graph makes its tables itself; eager calls, also before any replay, have their own."""
+    turner, rope = Turner(cuda), DeviceRope(cuda)
+    turner(DeviceRope(cuda))  # the kernels are loaded
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = turner(rope)
+    turner.check(turner(rope), rope)
+    graph.replay()
+    turner.check(captured, rope)
+    rope.cos_cached.mul_(0.5)
+    graph.replay()  # reads the rope's tensors
+    turner.check(captured, rope)
+    turner.check(turner(rope), rope)
+
+
+def test_rope_changed_and_dropped_after_a_capture(cuda):
+    """A replay goes on with the tables of its capture, whatever took their rope's place."""
+    turner, rope = Turner(cuda), DeviceRope(cuda)
+    turner(rope)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = turner(rope)
+    graph.replay()
+    want = captured.clone()
+    turner.check(want, rope)
+    rope.sin_cached.mul_(3.0)
+    turner.check(turner(rope), rope)
+    del rope
+    junk = [torch.full((4096, 32), math.nan, device=cuda) for _ in range(20)]
+    captured.zero_()
+    graph.replay()
+    assert torch.equal(captured, want)
+    del junk
+
+
+def test_rope_on_the_host_cannot_be_copied_inside_a_capture(cuda):
+    turner, rope = Turner(cuda), dkv.RotaryEmbedding(64, 200)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="once before it"):
+        with torch.cuda.graph(graph):
+            turner.q.mul_(1.0)
+            turner(rope)
+    turner(rope)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = turner(rope)
+    graph.replay()
+    assert torch.equal(captured, turner(rope))
+
+
 _CAPTURE_FIRST = """
 import torch, deltakv_b200 as dkv
 from deltakv_b200 import ops
