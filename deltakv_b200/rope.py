@@ -35,28 +35,52 @@ class RotaryEmbedding:
 
 class _Kept:
     """Half-width tables, and the tensors (with their versions) they were made from: holding those keeps
-    "is" meaningful, neither an object nor a tensor whose address was reused can match."""
+    "is" meaningful, neither an object nor a tensor whose address was reused can match.
 
-    __slots__ = ("cos_full", "sin_full", "versions", "tables", "captured")
+    They are read on any stream.  So they are finished when they are kept, and each stream that reads
+    them is told to the allocator, which then does not hand out their memory before its work is done."""
+
+    __slots__ = ("cos_full", "sin_full", "versions", "tables", "captured", "streams")
 
     def __init__(self, cos_full: Tensor, sin_full: Tensor, versions: tuple[int, int], tables: tuple[Tensor, Tensor]):
         self.cos_full, self.sin_full, self.versions, self.tables = cos_full, sin_full, versions, tables
         self.captured = False
+        device = tables[0].device
+        if device.type == "cuda":
+            torch.cuda.current_stream(device).synchronize()
+            self.streams = {_raw_stream(device.index)}
 
     def match(self, cos_full: Tensor, sin_full: Tensor) -> bool:
         return (self.cos_full is cos_full and self.sin_full is sin_full
                 and self.versions == (cos_full._version, sin_full._version))
+
+    def read(self, capturing: bool) -> tuple[Tensor, Tensor]:
+        """The tables, for a launch on the current stream of their device."""
+        tables = self.tables
+        if capturing:
+            if not self.captured:
+                self.captured = True
+                _captured_tables.append(tables)
+        elif tables[0].is_cuda and (raw := _raw_stream(tables[0].device.index)) not in self.streams:
+            self.streams.add(raw)
+            stream = torch.cuda.current_stream(tables[0].device)
+            tables[0].record_stream(stream), tables[1].record_stream(stream)
+        return tables
 
 
 _table_cache: WeakKeyDictionary = WeakKeyDictionary()  # per rope object, while it lives: {device: _Kept}
 _captured_tables: list[tuple[Tensor, Tensor]] = []     # what captured launches read: replays have only addresses
 
 
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _capturing(device: torch.device) -> bool:
     if device.type != "cuda":
         return False
-    if device.index is None or device.index == torch.cuda.current_device():
-        return torch.cuda.is_current_stream_capturing()
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return torch._C._cuda_isCurrentStreamCapturing()
     with torch.cuda.device(device):
         return torch.cuda.is_current_stream_capturing()
 
@@ -95,18 +119,15 @@ def half_tables(rope, device: torch.device) -> tuple[Tensor, Tensor]:
     try:
         kept = _table_cache.setdefault(rope, {})
     except TypeError:  # an object without hash or weak references: made anew each call
-        kept = {}
-    hit = kept.get(str(device))
+        return _on_device(cos_full[:, :half], sin_full[:, :half], device, capturing)
+    hit = kept.get(device)
     if hit is None or not hit.match(cos_full, sin_full):
         versions = (cos_full._version, sin_full._version)
         tables = _on_device(cos_full[:, :half], sin_full[:, :half], device, capturing)
         if capturing:
             return tables
-        hit = kept[str(device)] = _Kept(cos_full, sin_full, versions, tables)
-    if capturing and not hit.captured:
-        hit.captured = True
-        _captured_tables.append(hit.tables)
-    return hit.tables
+        hit = kept[device] = _Kept(cos_full, sin_full, versions, tables)
+    return hit.read(capturing)
 
 
 def max_positions(rope) -> int:

@@ -1003,6 +1003,43 @@ def test_rope_on_the_host_cannot_be_copied_inside_a_capture(cuda):
     assert torch.equal(captured, turner(rope))
 
 
+def test_rope_tables_made_on_another_stream(cuda):
+    """The first use is behind other work of its stream; the second, elsewhere, does not wait for that stream."""
+    turner, side = Turner(cuda), torch.cuda.Stream()
+    turner(DeviceRope(cuda))
+    for _ in range(3):
+        rope = DeviceRope(cuda)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            first = turner(rope)
+        turner.check(turner(rope), rope)
+        torch.cuda.synchronize()
+        turner.check(first, rope)
+
+
+@pytest.mark.parametrize("how", ["dropped", "changed"])
+def test_rope_tables_outlive_the_streams_that_read_them(cuda, how):
+    turner, side = Turner(cuda), torch.cuda.Stream()
+    want = turner(DeviceRope(cuda))
+    for _ in range(3):
+        rope = DeviceRope(cuda)
+        turner(rope)  # the tables are made on this stream
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            got = turner(rope)
+        if how == "changed":
+            rope.cos_cached.zero_(), rope.sin_cached.zero_()
+            turner(rope)
+        else:
+            del rope
+        junk = [torch.full((4096, 32), math.nan, device=cuda) for _ in range(8)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del junk
+
+
 _CAPTURE_FIRST = """
 import torch, deltakv_b200 as dkv
 from deltakv_b200 import ops

@@ -58,3 +58,15 @@ def test_tables_follow_a_rope_changed_in_inference_mode():
             assert torch.equal(half_tables(r, CPU)[0], r.cos_cached[:, :32])
     assert half_tables(rope, CPU)[0] is half_tables(rope, CPU)[0]
     assert torch.equal(half_tables(bare, CPU)[0], bare.cos_cached[:, :32])
+
+
+def test_tables_of_a_rope_that_cannot_be_kept():
+    class Bare:
+        __slots__ = ("cos_cached", "sin_cached")  # no weak references
+
+    rope, source = Bare(), RotaryEmbedding(64, 50)
+    rope.cos_cached, rope.sin_cached = source.cos_cached, source.sin_cached
+    for _ in range(2):
+        cos, sin = half_tables(rope, CPU)
+        assert torch.equal(cos, source.cos_cached[:, :32]) and torch.equal(sin, source.sin_cached[:, :32])
+        rope.cos_cached.mul_(0.5)
