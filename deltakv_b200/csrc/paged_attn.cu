@@ -274,8 +274,10 @@ struct Stream {
   __device__ __forceinline__ int block_of(int i) const {  // i / block_size for any i < 2^31
     return static_cast<int>((static_cast<uint64_t>(i) * p.div_mul) >> p.div_shift);
   }
+  // (not through the read-only path: the plan before this launch may have written the table while this grid
+  // was already in place)
   __device__ __forceinline__ int id_at(int blk) const {
-    return blk < w.tlen ? max(__ldg(p.tables + w.b * p.table_stride + blk), kNoRow) : kShort;
+    return blk < w.tlen ? max(p.tables[w.b * p.table_stride + blk], kNoRow) : kShort;
   }
   __device__ __forceinline__ void look_up() {
     if (!w.live) return;

@@ -859,6 +859,34 @@ def test_steps_without_autograd_or_with_it(cuda):
     got[1].zero_(), got[2].mul_(2)  # ordinary tensors
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("width,bound", [(3, 48), (3, 5000), (40, 640)])
+def test_attention_right_behind_its_plan(cuda, dtype, width, bound):
+    """The plan fills the tables that the next launch reads: new blocks every time, and nothing in between."""
+    n = 6
+    c = Cache([16 * n * width], 2, 64, 16, dtype, cuda)  # pages of normal values, all owned
+    lens = torch.tensor([16 * width - b for b in range(n)], dtype=torch.int32, device=cuda)
+    q = torch.randn(n, 4, 64, device=cuda).to(dtype)
+    held = torch.zeros(n, dtype=torch.int32, device=cuda)
+    tables = torch.zeros(n, width, dtype=torch.int32, device=cuda)
+    free = [torch.randperm(n * width, device=cuda).to(torch.int32) for _ in range(12)]
+
+    def run(wait):
+        outs = []
+        for f in free:
+            step = dkv.plan_paged_step(lens, tables, 16, rows=0, max_seq_len=bound, table_lens=held, free_blocks=f,
+                                       new_lengths=held)
+            wait()
+            outs.append(dkv.paged_decode_attention(q, c.k, c.v, step.seqs))
+            wait()
+        return torch.stack(outs)
+
+    want = run(torch.cuda.synchronize)
+    assert float((want[0] - want[1]).abs().max()) > 0.01  # the tables do differ
+    for _ in range(10):
+        assert torch.equal(run(lambda: None), want)
+
+
 @pytest.mark.parametrize("lens", [[300, 40], [9000, 40]])
 def test_calls_behind_one_another(cuda, lens):
     """Each call reads what the one before it wrote; nothing waits in between."""
