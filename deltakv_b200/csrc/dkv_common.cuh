@@ -406,7 +406,9 @@ namespace dkv {
 // A kernel launched by launch_overlapped begins by waiting until every earlier kernel of the stream has
 // ended and its writes are visible, and only then lets the next one be put in place: so a kernel that is
 // running has all but the one before it behind it.  Every CTA passes here before it touches global memory
-// or ends; what a stream orders stays ordered.
+// or ends; what a stream orders stays ordered.  The exception is join_kernel of the paged attention, which lets the
+// next one be put in place first, reads some memory early and has CTAs that end without a wait; it says there
+// why that is in order.  (A kernel behind it still waits for its last CTA, and that one for the walk.)
 __device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void begin_overlapped() {

@@ -97,14 +97,23 @@ __device__ __forceinline__ int border(uint32_t x, uint32_t at, int len) {
 
 // cu_seqlens and table lengths of 32 consecutive sequences in a warp's registers, so that
 // walking from one sequence to the next waits for memory once in 31 sequences
-struct Window {
+//
+// kEarly: for a kernel that has not waited for the one before it yet, see join_kernel; lengths only.
+template <bool kEarly>
+struct WindowOf {
   int base;  // lane i holds cu[base + i] and the table length of sequence base + i
   int cu, tlen;
+  static __device__ __forceinline__ int cu_at(const Params &p, int b) {
+    if (!kEarly) return p.cu[b];
+    int v;
+    asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.cu + b) : "memory");
+    return v;
+  }
   __device__ __forceinline__ void load(const Params &p, int b, int lane) {
     base = b;
     const int at = b + lane;
-    cu = p.cu[min(at, p.n_seqs)];
-    tlen = p.table_lens ? p.table_lens[min(at, p.n_seqs - 1)] : 0;
+    cu = cu_at(p, min(at, p.n_seqs));
+    tlen = !kEarly && p.table_lens ? p.table_lens[min(at, p.n_seqs - 1)] : 0;
   }
   __device__ __forceinline__ void need(const Params &p, int b, int lane) {
     if (b - base > 30) load(p, b, lane);
@@ -114,7 +123,7 @@ struct Window {
   // the first look of find, which does not depend on x: issued while the line's length is loaded
   __device__ __forceinline__ void look(const Params &p, int lane) {
     if (p.n_seqs > 31)
-      cu = p.cu[min(lane * ((p.n_seqs + 31) / 32), p.n_seqs)];
+      cu = cu_at(p, min(lane * ((p.n_seqs + 31) / 32), p.n_seqs));
     else
       load(p, 0, lane);
   }
@@ -124,7 +133,7 @@ struct Window {
     while (hi - lo > 31) {
       const int step = (hi - lo + 31) / 32;
       const int b = lo + lane * step;
-      if (lo > 0 || hi < p.n_seqs) cu = p.cu[min(b, p.n_seqs)];
+      if (lo > 0 || hi < p.n_seqs) cu = cu_at(p, min(b, p.n_seqs));
       const bool in = b < hi && static_cast<uint32_t>(cu) + static_cast<uint32_t>(kSeqCost) * b <= x;
       const int k = __popc(__ballot_sync(0xffffffffu, in));
       if (k > 1) lo += (k - 1) * step;
@@ -135,6 +144,7 @@ struct Window {
     return lo + max(__popc(__ballot_sync(0xffffffffu, in)) - 1, 0);
   }
 };
+using Window = WindowOf<false>;
 
 // ---------------------------------------------------------------------------------------
 // a warp's walk over its range: one tile of tokens after the other
@@ -1010,27 +1020,42 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   __shared__ float red_m[kThreads / 32], red_l[kThreads / 32];
   const float kNegInf = __int_as_float(0xff800000);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // This grid is put in place once every CTA of the walk has begun, that is after all that was before the
-  // walk: the lengths may be read, the parts not yet.  The kernel after this one may start when this
-  // grid has ended, and many of its CTAs end early: one waits for the walk whatever it has to do, so that
-  // the grid cannot end before the walk.
+  // Which parts there are follows from the lengths, and these are read before the walk is waited for: this grid is
+  // put in place once every CTA of the walk has said let_next_start, that is when whatever wrote the lengths
+  // has ended and its results are in global memory (the walk waited for that).  What this SM's L1 holds of them
+  // may be older, so they are read past it (ld.relaxed.gpu).  The parts may be read after the wait only.
+  // The kernel after this one may start when this grid has ended, and many of its CTAs end early, without a
+  // wait: one waits for the walk whatever it has to do, so that the grid cannot end before the walk.
+  // One warp reads the lengths for its CTA.  256 sequences of 1..600: 29.4 us; each warp for itself, queued at a
+  // few lines of L2, 32.7; every CTA waiting before it reads them, 32.9 (and 84 of 1..3200 17.1 against 15.7).
+  using Early = WindowOf<true>;
   let_next_start();
   if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) wait_for_earlier();
-  const Line ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
-  int b = blockIdx.x, first, next;
-  if (by_seq) {
-    first = p.cu[b], next = p.cu[b + 1];
-  } else {
+  __shared__ int seen[4];  // cu_seqlens at n_seqs, the sequence (-1: no such border), its start and end
+  if (warp == 0) {
+    const int tokens = Early::cu_at(p, p.n_seqs);
+    const Line ln = line_of(tokens, p.n_seqs, p.ranges);
     const uint32_t rb = blockIdx.x + 1;
-    if (rb >= ln.ranges) return;
-    Window win;
-    win.look(p, lane);
-    b = win.find(p, ln.start(rb), lane);
-    win.need(p, b, lane);
-    first = win.at(b), next = win.at(b + 1);
-    const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
-    if (rb > 1 && ln.start(rb - 1) >= at) return;  // an earlier border has this sequence
+    int b = blockIdx.x, first = 0, next = 0;
+    if (by_seq) {
+      first = Early::cu_at(p, b), next = Early::cu_at(p, b + 1);
+    } else if (rb >= ln.ranges) {
+      b = -1;
+    } else {
+      Early win;
+      win.look(p, lane);
+      b = win.find(p, ln.start(rb), lane);
+      win.need(p, b, lane);
+      first = win.at(b), next = win.at(b + 1);
+      const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
+      if (rb > 1 && ln.start(rb - 1) >= at) b = -1;  // an earlier border has this sequence
+    }
+    if (lane == 0) seen[0] = tokens, seen[1] = b, seen[2] = first, seen[3] = next;
   }
+  __syncthreads();
+  const Line ln = line_of(seen[0], p.n_seqs, p.ranges);
+  const int b = seen[1], first = seen[2], next = seen[3];
+  if (b < 0) return;
   const int len = max(next - first, 0);
   if (len == 0) return;
   const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;

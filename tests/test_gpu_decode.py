@@ -887,6 +887,32 @@ def test_attention_right_behind_its_plan(cuda, dtype, width, bound):
         assert torch.equal(run(lambda: None), want)
 
 
+@pytest.mark.parametrize("n", [4, 300])
+def test_joins_of_lengths_that_the_plan_just_wrote(cuda, n):
+    """Other lengths every step, in memory that the steps before held theirs in; long sequences cut into parts."""
+    rng = random.Random(n)
+    longest = 12000 // n ** 0.5
+    c = Cache([4000], 1, 64, 16, BF, cuda)
+    q = torch.randn(n, 8, 64, device=cuda).to(BF)
+    width = -(-12000 // 16)
+    tables = torch.randint(0, c.k.shape[0] - 3, (n, width), dtype=torch.int32, device=cuda)
+    steps = [torch.tensor([rng.randrange(int(longest)) for _ in range(n)], dtype=torch.int32, device=cuda) for _ in range(12)]
+
+    def run(wait):
+        outs = []
+        for lens in steps:
+            step = dkv.plan_paged_step(lens, tables, 16, rows=0, max_seq_len=12000, new_lengths=torch.zeros_like(lens))
+            wait()
+            outs.append(dkv.paged_decode_attention(q, c.k, c.v, step.seqs))
+            wait()
+            del step
+        return torch.stack(outs)
+
+    want = run(torch.cuda.synchronize)
+    for _ in range(10):
+        assert torch.equal(run(lambda: None), want)
+
+
 @pytest.mark.parametrize("lens", [[300, 40], [9000, 40]])
 def test_calls_behind_one_another(cuda, lens):
     """Each call reads what the one before it wrote; nothing waits in between."""
