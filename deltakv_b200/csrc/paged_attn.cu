@@ -1061,7 +1061,9 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
   // the ranges with a part: a range is at least two tiles wide, so only those at the ends of the
   // sequence and of its virtual tokens can have none
-  uint32_t r0 = ln.owner(at), r1 = ln.owner(at + len + kSeqCost - 1);
+  // (the bound changes nothing for lengths that are prefix sums; it keeps any others within the parts)
+  const uint32_t last = ln.ranges - 1;
+  uint32_t r0 = min(ln.owner(at), last), r1 = min(ln.owner(at + len + kSeqCost - 1), last);
   while (r0 < r1 && border(ln.start(r0 + 1), at, len) == 0) ++r0;
   while (r0 < r1 && border(ln.start(r1), at, len) == len) --r1;
   if (r1 == r0) return;  // not cut: written by its warp

@@ -356,6 +356,22 @@ def test_attention_short_table(cuda):
     ops.status_word(cuda).t.zero_()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cu", [[0, 700, 100], [0, 2000000, 40], [900, 100, 500], [0, 5, 5]])
+def test_attention_of_lengths_that_are_no_prefix_sums(cuda, dtype, cu):
+    """No answer is promised for them, but every access stays in bounds and the call after is right."""
+    c = Cache([3000, 900], 2, 64, 16, dtype, cuda)
+    q = torch.randn(2, 8, 64, device=cuda).to(dtype)
+    want = dkv.paged_decode_attention(q, c.k, c.v, c.seqs())
+    for bound in (40, 3000):
+        seqs = dkv.SeqBatchTensors(cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=cuda), block_tables=c.tables,
+                                   max_seq_len=bound)
+        dkv.paged_decode_attention(q, c.k, c.v, seqs)
+        torch.cuda.synchronize()
+    ops.status_word(cuda).t.zero_()
+    assert torch.equal(dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), check=True), want)
+
+
 def test_attention_empty_batch_and_understated_bound(cuda):
     c = Cache([900, 20], 2, 64, 16, BF, cuda)
     q = torch.randn(2, 4, 64, device=cuda).to(BF)
