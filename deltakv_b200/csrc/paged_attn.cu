@@ -718,8 +718,9 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
 // (16 times the padding, operands through tensor memory) would buy nothing.
 // Weights enter the product as two 16-bit terms (value and rest: 2^-17 relative for bf16) -
 // one term would add an error as large as the output's own rounding.  In f16 they are scaled by
-// 2^14, which l shares, so that weights down to 2^-28 of the largest keep all their bits.  (The rest
-// of a weight may be 0, so an infinite V value gives NaN where one term would give infinity.)
+// 2^14, which l shares, so that weights down to 2^-28 of the largest keep all their bits.
+// The rest of a weight may be 0 or negative, so an infinite V element gives NaN where its weight as one
+// number gives infinity: columns that end as NaN are looked through, see infinite_columns.
 template <int DT>
 struct Half;
 template <>
@@ -755,6 +756,49 @@ struct Mma {
   using S = Stream<T, HD, kStages, kTile>;
   static constexpr int kWarp = S::kBytes;
 };
+
+// After a piece of sequence b (tokens i0 to i1, its tiles `step` apart) left something in O that is not finite: the
+// columns that are NaN though no weight is, as their V elements have them, infinite where these are infinite with
+// one sign.  (Whatever the weights: they are positive.)  A lane has columns 16 k + g and 16 k + 8 + g and looks
+// at every fourth token.  Rare, so it reads V again; the test for it at the end of a piece costs 0.1-0.2 us a call.
+template <int DT, int kSteps>
+__device__ __forceinline__ void infinite_columns(const Params &p, float (&o)[kSteps][4], const float (&sum)[2], int u, int b,
+                                                 int i0, int i1, int step, int g, int t) {
+  constexpr uint32_t kExp = DT == DKV_BF16 ? 0x7f80 : 0x7c00;
+  uint32_t up = 0, down = 0, nan = 0;  // a bit per column of the lane
+  const int64_t tlen = p.table_lens ? p.table_lens[b] : p.table_stride;
+  for (int i = i0; i < i1; i += step) {
+    for (int token = i + t; token < min(i + kTile, i1); token += 4) {
+      const int blk = token / p.block_size;
+      const int id = blk < tlen ? p.tables[b * p.table_stride + blk] : -1;
+      if (id < 0 || id >= p.num_blocks) continue;
+      const unsigned short *row = reinterpret_cast<const unsigned short *>(
+          p.v + u * p.v_head + id * p.v_block + (token - blk * p.block_size) * p.v_slot);
+#pragma unroll
+      for (int c = 0; c < 2 * kSteps; ++c) {
+        const int d = c * 8 + g;
+        const uint32_t x = d < p.hd ? row[d] : 0, size = x & 0x7fff;
+        nan |= static_cast<uint32_t>(size > kExp) << c;
+        up |= static_cast<uint32_t>(x == kExp) << c;
+        down |= static_cast<uint32_t>(x == (kExp | 0x8000)) << c;
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 1; k < 4; k <<= 1) {
+    nan |= __shfl_xor_sync(0xffffffffu, nan, k);
+    up |= __shfl_xor_sync(0xffffffffu, up, k);
+    down |= __shfl_xor_sync(0xffffffffu, down, k);
+  }
+  up &= ~nan, down &= ~nan;
+#pragma unroll
+  for (int c = 0; c < 2 * kSteps; ++c)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float &x = o[c / 2][c % 2 * 2 + h];
+      if (x != x && sum[h] == sum[h] && ((up ^ down) >> c & 1)) x = __int_as_float((up >> c & 1) ? 0x7f800000 : 0xff800000);
+    }
+}
 
 template <int DT, int HD, int W, int kStages>
 __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ Params p) {
@@ -802,6 +846,14 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
     x += __shfl_xor_sync(0xffffffffu, x, 4);
     x += __shfl_xor_sync(0xffffffffu, x, 8);
     return x + __shfl_xor_sync(0xffffffffu, x, 16);
+  };
+  auto all_finite = [&]() {  // of O: 0 times anything else is NaN
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = fmaf(o[k][e], 0.f, z[e]);
+    return __all_sync(0xffffffffu, (z[0] + z[1]) + (z[2] + z[3]) == 0.f);
   };
   clear();
 
@@ -898,6 +950,11 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
       const bool whole = (mt.y & kFromStart) && (mt.y & kToEnd);
       const int64_t part = (static_cast<int64_t>(r) * p.units + unit) * 2 + (mt.y & kFromStart ? 1 : 0);
       const float sum[2] = {sum_of(0), sum_of(1)};
+      if (!all_finite()) {
+        const int first = p.cu[b], len = max(p.cu[b + 1] - first, 0);
+        const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
+        infinite_columns<DT>(p, o, sum, u, b, border(ln.start(r), at, len), border(ln.start(r + 1), at, len), kTile, g, t);
+      }
       if (whole) {
         // heads to rows, so that a lane stores two neighbouring columns of one head
         const float inv0 = sum[0] == 0.f ? 0.f : 1.f / sum[0], inv1 = sum[1] == 0.f ? 0.f : 1.f / sum[1];
@@ -949,11 +1006,13 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
     __syncwarp();
     LocalState<HD, 8> *mine_out = reinterpret_cast<LocalState<HD, 8> *>(mine);
     static_assert(sizeof(LocalState<HD, 8>) <= kStages * C::S::kStage, "the state fits the ring");
+    const float sum[2] = {sum_of(0), sum_of(1)};
+    if (!all_finite())
+      infinite_columns<DT>(p, o, sum, u, r, warp * kTile, max(p.cu[r + 1] - p.cu[r], 0), p.local * kTile, g, t);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const float sum = sum_of(c);
       const int in = t * 2 + c;
-      if (g == 0) mine_out->m[in] = m[c], mine_out->l[in] = sum;
+      if (g == 0) mine_out->m[in] = m[c], mine_out->l[in] = sum[c];
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
         mine_out->o[in][k * 16 + g] = o[k][c];

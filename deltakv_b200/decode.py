@@ -142,7 +142,9 @@ def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: op
     gives zeros and ``-inf``.  Any head_dim up to 256 and any strides; rows that start on 16
     bytes and are a multiple of 16 bytes long are read fastest.
 
-    Slots behind a sequence's length are not read into the result, whatever they hold.  Tokens
+    Slots behind a sequence's length are not read into the result, whatever they hold.  An infinite
+    V element of a token that counts makes its column infinite (NaN where both signs meet; perhaps
+    also where the token's weight is below 2^-126 of the largest and so 0 in fp32).  Tokens
     in blocks outside the cache or beyond the table are left out and recorded (``check=True``
     raises).
     """

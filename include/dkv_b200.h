@@ -642,7 +642,9 @@ int dkv_append_paged(const dkv_append_args *args, dkv_stream_t stream);
  *   lse[b,h] = ln sum_i exp(s_i)   (fp32, optional).
  * A sequence without tokens gives out = 0 and lse = -inf.  Tokens whose block lies outside the
  * cache (PAGE_RANGE) or beyond the table row (BLOCK_TABLE_SHORT) are left out of both sums.
- * Slots past a sequence's length are never read into the result, whatever they hold.
+ * Slots past a sequence's length are never read into the result, whatever they hold.  An infinite V
+ * element of a token that counts makes its column infinite (NaN where both signs meet; perhaps also
+ * where the token's weight is below 2^-126 of the largest and so 0 in fp32).
  * q, K, V and out have one dtype; scores, the running maximum and sum and the output
  * accumulate in fp32.  head_dim <= 256, n_q_heads a multiple of the pages' n_heads.
  * seqs.max_seq_len sizes the split of long sequences; a length above it costs speed only.

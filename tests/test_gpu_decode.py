@@ -210,6 +210,42 @@ def test_attention_never_reads_what_no_token_owns(cuda, dtype, fill):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [32, 50, 64, 128, 256])
+@pytest.mark.parametrize("lens,bound", [([1, 40, 300, 0, 17, 75], 300), ([1, 40, 300, 0, 17, 75], 9000), ([9000, 20], 9000)])
+@pytest.mark.parametrize("scale", [0.1, 0.4])
+def test_attention_infinite_values(cuda, dtype, hd, lens, bound, scale):
+    """Infinite and NaN V elements in tokens that count: +-inf or NaN in their columns as by the definition in 64
+    bits, every other column as without them.  Scores spread by 40 at most, so no weight is 0 in fp32."""
+    c = Cache(lens, 2, hd, 16, dtype, cuda)
+    g = torch.Generator().manual_seed(hd)
+    q = (8 * torch.randn(len(lens), 8, hd, generator=g) / hd ** 0.5).to(dtype).to(cuda)
+    seqs = dkv.SeqBatchTensors(cu_seqlens=c.cu, block_tables=c.tables, max_seq_len=bound)
+    plain = dkv.paged_decode_attention(q, c.k, c.v, seqs, scale=scale, check=True)
+    for b, n in enumerate(lens):
+        for j in range(0 if n == 0 else hd // 4):  # about a quarter of the columns, one to three elements each
+            for _ in range(1 + j % 3):
+                t, x = int(torch.randint(n, (1,), generator=g)), (math.inf, -math.inf, math.inf, math.nan)[j % 4]
+                x = -x if j % 7 == 0 and _ else x
+                c.v[int(c.tables[b, t // 16]), t % 16, j % 2, int(torch.randint(hd, (1,), generator=g))] = x
+    got, lse = dkv.paged_decode_attention(q, c.k, c.v, seqs, scale=scale, return_lse=True, check=True)
+    ref = torch.zeros(got.shape, dtype=torch.float64, device=cuda)
+    for b, n in enumerate(lens):
+        if n:
+            k, v = (t.double() for t in c.tokens(b))
+            s = torch.einsum("ugd,nud->ugn", q[b].double().view(2, 4, hd), k) * scale
+            assert float(s.amax() - s.amin()) < 40
+            p = torch.softmax(s, -1)  # [2, 4, n] against [n, 2, hd]
+            ref[b] = (p[..., None] * v.permute(1, 0, 2)[:, None]).sum(2).reshape(8, hd)
+    odd = ~torch.isfinite(ref)
+    assert odd.any() and torch.equal(got[odd].double().nan_to_num(nan=7.0, posinf=math.inf, neginf=-math.inf),
+                                     ref[odd].nan_to_num(nan=7.0, posinf=math.inf, neginf=-math.inf))
+    clean = lambda b: tuple(t.nan_to_num(nan=0.0, posinf=0.0, neginf=0.0) for t in c.tokens(b))  # noqa: E731
+    assert torch.equal(got[~odd], plain[~odd])
+    check_attention(torch.where(odd, 0, got), lse, q, lambda b: (clean(b)[0], torch.where(
+        torch.isfinite(c.tokens(b)[1]).all(0), clean(b)[1], 0)), scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lens", [[20011], [9000, 1, 0, 7000], [1] * 300, [0] * 40, [3, 2049] * 20, list(range(130))])
 def test_attention_long_and_ragged(cuda, dtype, lens):
     run_attention(Cache(lens, 2, 64, 16, dtype, cuda), 8, 64, dtype, cuda)
