@@ -143,6 +143,25 @@ def test_attention_one_launch_of_fewer_warps(cuda, dtype, n_seq):
     assert float((out.double() - other.double()).abs().max()) <= 2 * (torch.finfo(dtype).eps + 2.0 ** -15) * float(c.v.double().abs().max())
 
 
+def test_attention_one_launch_of_every_number_of_warps(cuda):
+    """As many pairs of sequence and KV head as leave each number of warps a CTA, down to one, and one more pair than
+    has a warp each (that batch is split).  The sizes follow from the number of SMs."""
+    sms = torch.cuda.get_device_properties(cuda).multi_processor_count
+    g = torch.Generator().manual_seed(11)
+    for dtype, warps in ((BF, 12), (F16, 12), (F32, 8)):  # head_dim 64; fp32: up to 4 heads a KV head
+        seen = []
+        for per_sm in (1, 2, 3, 4, warps // 2, warps, warps + 1):
+            n = sms * per_sm - 3  # one KV head: a pair a sequence
+            seen.append(warps // per_sm)
+            rng = random.Random(per_sm)
+            c = Cache([rng.choice([0, 1, 16, 17, rng.randrange(40)]) for _ in range(n)], 1, 64, 16, dtype, cuda)
+            q = torch.randn(n, 3, 64, generator=g).to(dtype).to(cuda)
+            out, lse = dkv.paged_decode_attention(q, c.k, c.v, c.seqs(), return_lse=True, check=True)
+            for b in [n - 1, 0] + rng.sample(range(n), 12):
+                check_attention(out[b:b + 1], lse[b:b + 1], q[b:b + 1], lambda _, b=b: c.tokens(b), 64 ** -0.5)
+        assert {warps, warps // 2, 3 if warps == 12 else 4, 1, 0} <= set(seen)
+
+
 LENS = [0, 1, 2, 15, 16, 17, 33, 100, 0, 333, 64]
 
 
@@ -430,6 +449,40 @@ def test_attention_parts_join_by_lse(cuda, dtype):
         got.append(dkv.paged_decode_attention(q, c.k, c.v, seqs, return_lse=True))
     joined = torch.logaddexp(got[0][1].double(), got[1][1].double())
     assert float((joined - lse.double()).abs().max()) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,cut", [([600], 25), ([5000, 40, 16], 1), ([333, 9000], 7)])
+def test_attention_outputs_of_parts_join_by_lse(cuda, dtype, lens, cut):
+    """A prefix of `cut` blocks and the rest attended apart: out = sum_i exp(lse_i - lse) out_i is the whole's.
+
+    Each part is off by its own tolerance of check_attention, which is what the weights scale; the join in 64 bits adds
+    the parts' lse errors, again below the 2^-20 and n 2^-24 of that bound, hence twice the bound of a whole."""
+    c = Cache(lens, 2, 64, 16, dtype, cuda)
+    q, whole, lse = run_attention(c, 8, 64, dtype, cuda)
+    outs, lses = [], []
+    for part in (0, 1):
+        n = [min(x, cut * 16) if part == 0 else max(x - cut * 16, 0) for x in lens]
+        cu = torch.tensor([0] + n, dtype=torch.int32, device=cuda).cumsum(0).to(torch.int32)
+        table = c.tables[:, :cut] if part == 0 else c.tables[:, cut:]
+        if table.shape[1] == 0:
+            table = c.tables[:, :1]
+        seqs = dkv.SeqBatchTensors(cu_seqlens=cu, block_tables=table.contiguous(), max_seq_len=max(n))
+        out, part_lse = dkv.paged_decode_attention(q, c.k, c.v, seqs, return_lse=True, check=True)
+        outs.append(out.double()), lses.append(part_lse.double())
+    total = torch.logaddexp(*lses)
+    joined = sum(torch.exp(x - total)[..., None] * o for x, o in zip(lses, outs))
+    for b in range(len(lens)):
+        k, v = (t.double() for t in c.tokens(b))
+        s = torch.einsum("ugd,nud->ugn", q[b].double().view(2, 4, 64), k) * 64 ** -0.5
+        ds = (64 + 8) * 2.0 ** -23 * (torch.einsum("ugd,nud->ugn", q[b].double().abs().view(2, 4, 64), k.abs()) * 64 ** -0.5).amax(-1)
+        p = torch.softmax(s, -1)
+        ref, spread = torch.einsum("ugn,nud->ugd", p, v), torch.einsum("ugn,nud->ugd", p, v.abs())
+        # each part's rounding to its type is relative to its own output: at most spread after weighting
+        bound = spread * (torch.finfo(dtype).eps / 2 + 2 * (2 * ds[..., None] + 2.0 ** -20 + len(k) * 2.0 ** -24
+                                                            + (2.0 ** -16 if dtype != F32 else 0)))
+        bound = bound + 2 * torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        assert torch.all((joined[b].view(2, 4, 64) - ref).abs() <= bound), b
 
 
 def test_attention_is_deterministic_and_reads_the_right_stream(cuda):
@@ -736,6 +789,25 @@ def test_append_layouts(cuda, dtype, layout):
 @pytest.mark.parametrize("hd", [1, 7, 64, 100])
 def test_append_without_rope(cuda, dtype, hd):
     check_append(cuda, Cache([300], 2, hd, 16, dtype, cuda), dtype, 2, 2, hd, 90, rope=False, with_q=False)
+
+
+@pytest.mark.parametrize("hd", [2, 64, 100, 128])
+def test_append_in_fp32_equals_tensor_operations(cuda, hd):
+    """Products and sums rounded one by one, so every bit is that of the reference's rotate-half in fp32."""
+    c = Cache([300], 2, hd, 16, F32, cuda)
+    rows, slots = 200, torch.randperm(300, generator=torch.Generator().manual_seed(1))[:200].to(cuda)
+    q, k = torch.randn(rows, 4, hd, device=cuda), torch.randn(rows, 2, hd, device=cuda)
+    pos = torch.randint(0, 500, (rows,), device=cuda, dtype=torch.int32)
+    rope, cos, sin = rope_tables(hd, 500, cuda)
+
+    def turn(x):
+        cs, sn = (torch.cat([t, t], -1)[pos.long()][:, None] for t in (cos, sin))
+        lo, hi = x.chunk(2, -1)
+        return x * cs + torch.cat([-hi, lo], -1) * sn
+
+    got = dkv.append_into_paged(k, k, c.k, c.v, slots, q=q, positions=pos, rope=rope, check=True)
+    assert torch.equal(got, turn(q))
+    assert torch.equal(c.k[slots // 16, slots % 16], turn(k)) and torch.equal(c.v[slots // 16, slots % 16], k)
 
 
 def test_append_ranges(cuda):
