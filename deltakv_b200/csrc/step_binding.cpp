@@ -237,6 +237,10 @@ PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t count) {
     if (block_size <= 0 || block_size > INT32_MAX || rows < 0 || rows > INT32_MAX || max_seq_len < 0 ||
         max_seq_len > INT32_MAX || width > INT32_MAX || n > INT32_MAX)
       value_error("block_size must be positive, rows and max_seq_len not negative, all below 2**31");
+    apart(tables, "block_tables", lengths, "lengths");
+    if (fresh) apart(tables, "block_tables", *fresh, "new_lengths");
+    if (held) apart(tables, "block_tables", *held, "table_lens");
+    if (free_blocks) apart(tables, "block_tables", *free_blocks, "free_blocks");
     const Place at_("plan_paged_step", lengths);
     at_.also(&tables), at_.also(fresh), at_.also(held), at_.also(free_blocks);
     const c10::DeviceGuard guard(at_.device);

@@ -81,7 +81,8 @@ def plan_paged_step(lengths: Tensor, block_tables: Tensor, block_size: int, *, r
     ``lengths`` int32 ``[n_seqs]`` counts each sequence's tokens after the step, the last
     ``new_lengths`` of them new (``None``: all, a prefill).  ``block_tables`` int32
     ``[n_seqs, width]`` holds ``table_lens`` valid blocks a row (``None``: ``width``) and is
-    extended in place from the front of ``free_blocks``, sequence by sequence.  ``rows`` is the
+    extended in place from the front of ``free_blocks``, sequence by sequence; it shares no memory
+    with the other inputs.  ``rows`` is the
     capacity of the row outputs (the sum of the new lengths, or more in a padded batch: rows
     past the last sequence get slot -1 and position 0); ``max_seq_len`` bounds the lengths and
     goes into the returned ``seqs``.

@@ -42,6 +42,16 @@ def test_plan_refuses(change, error, text):
         _plan(**change)
 
 
+@pytest.mark.parametrize("name", ["lengths", "new_lengths", "table_lens", "free_blocks"])
+def test_plan_refuses_a_table_over_its_inputs(name):
+    """The table is written while other CTAs read them."""
+    whole = torch.zeros(10, dtype=I32)
+    with pytest.raises(ValueError, match=f"block_tables and {name} share memory"):
+        _plan(block_tables=whole[:8].view(2, 4), **{name: whole[7:9]})
+    with pytest.raises(ValueError, match="CUDA"):  # beside it: on to the next check
+        _plan(block_tables=whole[:8].view(2, 4), **{name: whole[8:10]})
+
+
 def _append(**change):
     a = dict(k=torch.zeros(3, 2, 8, dtype=BF), v=torch.zeros(3, 2, 8, dtype=BF),
              k_pages=torch.zeros(4, 4, 2, 8, dtype=BF), v_pages=torch.zeros(4, 4, 2, 8, dtype=BF),
