@@ -14,8 +14,9 @@ deployment swaps them in (see :func:`install`):
 * ``apply_probe_to_cache`` / ``select_probes`` / ``weight_axis_scores`` / ``residual_gate``
   (deltakv.patches.probe), ``lora_activation_scores`` (deltakv.patches.exact)
 
-and what a serving loop does with the same pages between two patches (``plan_paged_step``,
-``append_into_paged``, ``paged_decode_attention``: one prefill or decode step),
+and what a serving loop does with the same pages between two patches: a decode step
+(``plan_paged_step``, ``append_into_paged``, ``paged_decode_attention``) and the first two of
+these for prompt chunks,
 plus the fused batched forms the engine and connector use: :class:`ExactPatcher` (LoRA
 deltas) and :class:`DensePatcher` (full-rank dW of an RL step, a tensor-core GEMM).
 All computation runs in ``libdkv_b200.so``; a missing library raises (no CPU path).

@@ -1,4 +1,4 @@
-"""One prefill or decode step of a paged cache: plan, append, attend.
+"""One decode step of a paged cache: plan, append, attend.
 
 The patch routes of this package change the K/V of tokens that are already cached; these three
 operators are what a serving loop does between two patches, on the same pages, block tables
@@ -8,8 +8,13 @@ and :class:`~deltakv_b200.ops.SeqBatchTensors`:
 * :func:`append_into_paged`      rotate-half RoPE of the new q and k, K and V into their slots
 * :func:`paged_decode_attention` attention of one new token per sequence over its pages
 
+The first two take any number of new tokens a sequence, so they also serve prompt chunks; the
+attention of a chunk's rows, several a sequence, is not here.
+
 None of them reads anything back to the host (``check=True`` does, to raise what the kernels
-recorded), so a step can be captured into a CUDA graph and replayed with other lengths.  They
+recorded), so a step can be captured into a CUDA graph and replayed with other lengths, up to the
+capacities of its capture.  The first call may be inside the capture, but for a rope that is not on
+the GPU: its tables are made by a call before (see :func:`deltakv_b200.rope.half_tables`).  They
 run on the current stream of the tensors' device, which need not be the current device.  They are
 forms for serving: their outputs carry no gradient.  The cache layouts are the ones of
 :func:`~deltakv_b200.paged.scatter_into_paged`; for its 5-D forms pass the K and V views
@@ -140,7 +145,10 @@ def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: op
     ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``out [n_seqs, n_q, head_dim]`` and with
     ``return_lse`` also ``ln sum exp`` of the scores (fp32 ``[n_seqs, n_q]``), with which parts
     of a cache attended separately (a shared prefix) can be joined.  A sequence without tokens
-    gives zeros and ``-inf``.  Any head_dim up to 256 and any strides; rows that start on 16
+    gives zeros and ``-inf``.  The form of the launch goes by the batch and by ``seqs.max_seq_len``,
+    which may be any bound: with one of a few hundred tokens short sequences take one launch, about
+    half the time of the form that cuts long ones.  A captured step keeps the form of its
+    capture, so a serving loop is faster with a graph for each class of lengths.  Any head_dim up to 256 and any strides; rows that start on 16
     bytes and are a multiple of 16 bytes long are read fastest.
 
     Slots behind a sequence's length are not read into the result, whatever they hold.  An infinite

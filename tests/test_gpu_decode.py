@@ -1226,6 +1226,21 @@ q = torch.ones(1, 4, 64, device=dev, dtype=torch.bfloat16)
 k = torch.ones(4, 16, 2, 64, device=dev, dtype=torch.bfloat16)
 v = torch.ones_like(k)
 ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+class Rope: cos_cached, sin_cached = torch.zeros(2, 50, 64, device=dev)  # a quarter turn
+Rope.sin_cached += 1
+step_graph, rope, lens, table = torch.cuda.CUDAGraph(), Rope(), ints([20]), ints([[1, 0]])
+x = torch.randn(1, 2, 64, device=dev, dtype=torch.bfloat16)
+held, free, new = ints([1]), ints([3]), ints([1])
+torch.cuda.synchronize()
+with torch.cuda.graph(step_graph):
+    step = dkv.plan_paged_step(lens, table, 16, rows=1, max_seq_len=20, new_lengths=new, table_lens=held, free_blocks=free)
+    turned = dkv.append_into_paged(x, x, k, v, step.slots, q=x, positions=step.positions, rope=rope)
+step_graph.replay()
+quarter = torch.cat([-x[..., 32:], x[..., :32]], -1)
+assert table.tolist() == [[1, 3]] and step.slots.tolist() == [3 * 16 + 3] and torch.equal(turned, quarter)
+assert torch.equal(k[3, 3], quarter[0]) and torch.equal(v[3, 3], x[0])
+assert torch.equal(dkv.append_into_paged(x, x, k, v, step.slots, q=x, positions=step.positions, rope=rope), quarter)
+k.fill_(1), v.fill_(1)
 seqs = dkv.SeqBatchTensors(cu_seqlens=ints([0, 20]), block_tables=ints([[1, 9]]), max_seq_len=20)  # no block 9
 graph = torch.cuda.CUDAGraph()
 torch.cuda.synchronize()
@@ -1256,7 +1271,7 @@ print("captured first")
 
 
 def test_first_use_inside_a_capture(cuda):
-    """The status word of a process whose first call is captured: eager calls and replays share one that is valid."""
+    """A process whose first calls are captured; eager calls and replays share a status word that is valid."""
     root = Path(__file__).resolve().parent.parent
     got = subprocess.run([sys.executable, "-c", _CAPTURE_FIRST], cwd=root, capture_output=True, text=True, timeout=300)
     assert got.returncode == 0 and got.stdout.strip() == "captured first", got.stderr[-2000:]
