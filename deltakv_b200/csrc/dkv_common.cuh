@@ -444,3 +444,19 @@ cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, int threads,
       return DKV_ERR_CUDA;                        \
     }                                             \
   } while (0)
+
+namespace dkv {
+// SMs of the current device, asked for once
+inline int sm_count(int *out) {
+  static int cached[64];
+  int dev = 0, n = 0;
+  DKV_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 64) n = __atomic_load_n(&cached[dev], __ATOMIC_RELAXED);
+  if (n == 0) {
+    DKV_CUDA_CHECK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) __atomic_store_n(&cached[dev], n, __ATOMIC_RELAXED);
+  }
+  *out = n;
+  return DKV_OK;
+}
+}  // namespace dkv

@@ -1251,6 +1251,7 @@ struct Shape {
   int local;             // warps of a CTA per (sequence, unit), or 0: ranges
   int ranges;            // upper bound of the ranges in use
   int64_t parts;         // part slots
+  int sms;
   int64_t o_bytes, bytes;
 };
 
@@ -1275,21 +1276,6 @@ constexpr Variant variant(bool f32, int hd, int g) {
   return hd == 128 ? Variant{12, 2, 16} : hd == 64 ? Variant{12, 4, 16} : Variant{16, 4, 16};
 }
 
-int sm_count(int *out) {
-  static int cached[64];
-  int dev = 0;
-  DKV_CUDA_CHECK(cudaGetDevice(&dev));
-  if (dev < 64 && cached[dev] > 0) {
-    *out = cached[dev];
-    return DKV_OK;
-  }
-  int n = 0;
-  DKV_CUDA_CHECK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-  if (dev < 64) cached[dev] = n;
-  *out = n;
-  return DKV_OK;
-}
-
 bool float_dtype(int dt) { return dt == DKV_F32 || dt == DKV_F16 || dt == DKV_BF16; }
 
 int check(const dkv_paged_decode_args *a) {
@@ -1307,9 +1293,9 @@ int check(const dkv_paged_decode_args *a) {
 }
 
 int shape_of(const dkv_paged_decode_args *a, Shape *s) {
-  int sms;
-  const int rc = sm_count(&sms);
+  const int rc = sm_count(&s->sms);
   if (rc != DKV_OK) return rc;
+  const int64_t sms = s->sms;
   const int hd = a->k_pages.head_dim, group = a->n_q_heads / a->k_pages.n_heads;
   s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
   const bool f32 = a->k_pages.dtype == DKV_F32;
@@ -1320,9 +1306,9 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   s->units = a->k_pages.n_heads * s->chunks;
   const int64_t pairs = static_cast<int64_t>(a->seqs.n_seqs) * s->units;
   s->local = s->warps;
-  while (s->local > 0 && pairs > static_cast<int64_t>(sms) * (s->warps / s->local)) --s->local;
+  while (s->local > 0 && pairs > sms * (s->warps / s->local)) --s->local;
   if (a->seqs.max_seq_len > static_cast<int64_t>(kLocalTiles) * s->tokens * s->local) s->local = 0;
-  const int64_t most = static_cast<int64_t>(sms) * s->warps / s->units;
+  const int64_t most = sms * s->warps / s->units;
   const int64_t line = static_cast<int64_t>(a->seqs.n_seqs) * (static_cast<int64_t>(a->seqs.max_seq_len) + kSeqCost);
   const int64_t want = line / kMinRange;
   s->ranges = static_cast<int>(s->local || most < 1 || want < 1 ? 1 : (want < most ? want : most));
@@ -1407,16 +1393,22 @@ int launch(const Params &p, const Shape &s, cudaStream_t st) {
   if (rc != DKV_OK || s.ranges == 1) return rc;
   const int by_seq = p.n_seqs <= s.ranges - 1;
   const int cut = by_seq ? p.n_seqs : s.ranges - 1;
-  // few cut sequences: a CTA for each head (they may have many parts); else a warp each
-  const int hpc = static_cast<int64_t>(cut) * p.heads <= 148 * 8 ? 1 : kJoinThreads / 32;
-  // very few: several CTAs for each head
-  const int split = static_cast<int64_t>(cut) * p.heads <= 148 && p.hd >= 64 ? 4 : 1;
+  // A CTA for each head, or a warp where more CTAs than run at once would come of it (CTA / warp, us, bf16: 9
+  // sequences of 30000 x 16 heads x 64 38.2 / 42.5, 20 of 3000 x 32 heads x 128 51.5 / 52.4; at the border, 36 of
+  // 2000 x 32 heads 61.3 / 60.6, 74 of 1..6000 x 16 heads 111.7 / 113.1; 74 of 1000 x 32 heads 65.1 / 62.1)
+  const int64_t heads = static_cast<int64_t>(cut) * p.heads;  // to join at most
+  const int hpc = heads <= s.sms * 8 ? 1 : kJoinThreads / 32;
+  // Few heads: several CTAs for each, as long as an SM has one of them (1 / 2 / 4 CTAs a head, us, bf16: one sequence
+  // of 4000 x 32 heads x 128 15.8 / 14.0 / 13.0, of 30000 x 8 heads x 32 14.6 / 12.8 / 12.5, 6 of 6000 x 8 x 256 24.9 /
+  // 23.6 / 22.6; 12 of 8000 x 8 x 64 18.1 / 18.0 / 21.4, 4 of 8000 x 32 x 128 33.0 / 33.0 / 36.5; 5 of them 38.5 / 41.6
+  // / 45.0)
+  const int split = p.hd < 32 ? 1 : heads <= s.sms / 2 ? 4 : heads <= s.sms ? 2 : 1;
   const dim3 grid(cut, (p.heads + hpc - 1) / hpc, split);
   // heads of which some may have more parts than a CTA has threads: more threads (one sequence of 131071, 8 KV heads:
   // 99.5 -> 97.5 us; three of up to 13687, 2 KV heads: 17.4 -> 14.8; 5 of 15930, 40 heads: 54 -> 52), which cost time
   // where there are fewer parts (one of 47238, 16 KV heads of 7 query heads each, 111 ranges: 72.9 -> 75.5) and
   // where not all CTAs run at once (62 of 6119, 6 heads: 72.8 -> 74.3; 84 of 1..3200, 12 heads: 11.6 -> 15.5)
-  const bool wide = static_cast<int64_t>(cut) * p.heads <= 148 * 2 && s.ranges > kJoinThreads;
+  const bool wide = heads <= s.sms * 2 && s.ranges > kJoinThreads;
   const auto kernel = wide ? (p.hd % 4 == 0 ? join_kernel<DT, 4, kJoinWide> : join_kernel<DT, 1, kJoinWide>)
                            : (p.hd % 4 == 0 ? join_kernel<DT, 4, kJoinThreads> : join_kernel<DT, 1, kJoinThreads>);
   DKV_CUDA_CHECK(launch_overlapped(kernel, grid, wide ? kJoinWide : kJoinThreads, s.ranges * 8, st, p, s.g, by_seq, hpc));

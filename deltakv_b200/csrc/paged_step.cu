@@ -326,7 +326,12 @@ extern "C" int dkv_plan_paged_step(const dkv_step_plan_args *args, dkv_stream_t 
     DKV_CUDA_CHECK(cudaFuncSetAttribute(step::plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         2 * (step::kMaxSeqs + 1) * static_cast<int>(sizeof(int))));
   const int64_t want = (static_cast<int64_t>(a.n_rows) + 2 * step::kPlanThreads - 1) / (2 * step::kPlanThreads);
-  const int grid = static_cast<int>(want < 1 ? 1 : (want > 148 ? 148 : want));
+  int grid = 1;
+  if (want > 1) {
+    const int rc = sm_count(&grid);
+    if (rc != DKV_OK) return rc;
+    if (want < grid) grid = static_cast<int>(want);
+  }
   DKV_CUDA_CHECK(launch_overlapped(step::plan_kernel, dim3(grid), step::kPlanThreads, smem,
                                    reinterpret_cast<cudaStream_t>(stream), a));
   return DKV_OK;
