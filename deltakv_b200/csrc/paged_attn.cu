@@ -760,7 +760,8 @@ struct Mma {
 // After a piece of sequence b (tokens i0 to i1, its tiles `step` apart) left something in O that is not finite: the
 // columns that are NaN though no weight is, as their V elements have them, infinite where these are infinite with
 // one sign.  (Whatever the weights: they are positive.)  A lane has columns 16 k + g and 16 k + 8 + g and looks
-// at every fourth token.  Rare, so it reads V again; the test for it at the end of a piece costs 0.1-0.2 us a call.
+// at every fourth token.  Rare, so it reads V again, and is given what the walk holds anyway: with values of its own
+// kept for it, the walk was 1 % slower, now 0.5 %.
 template <int DT, int kSteps>
 __device__ __forceinline__ void infinite_columns(const Params &p, float (&o)[kSteps][4], const float (&sum)[2], int u, int b,
                                                  int i0, int i1, int step, int g, int t) {
@@ -953,7 +954,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
       if (!all_finite()) {
         const int first = p.cu[b], len = max(p.cu[b + 1] - first, 0);
         const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
-        infinite_columns<DT>(p, o, sum, u, b, border(ln.start(r), at, len), border(ln.start(r + 1), at, len), kTile, g, t);
+        infinite_columns<DT>(p, o, sum, h0 / p.group, b, border(stream.w.x0, at, len), border(stream.w.x1, at, len), kTile, g, t);
       }
       if (whole) {
         // heads to rows, so that a lane stores two neighbouring columns of one head
@@ -1008,7 +1009,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
     static_assert(sizeof(LocalState<HD, 8>) <= kStages * C::S::kStage, "the state fits the ring");
     const float sum[2] = {sum_of(0), sum_of(1)};
     if (!all_finite())
-      infinite_columns<DT>(p, o, sum, u, r, warp * kTile, max(p.cu[r + 1] - p.cu[r], 0), p.local * kTile, g, t);
+      infinite_columns<DT>(p, o, sum, h0 / p.group, r, warp * kTile, max(p.cu[r + 1] - p.cu[r], 0), p.local * kTile, g, t);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int in = t * 2 + c;
