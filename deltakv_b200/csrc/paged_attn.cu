@@ -8,7 +8,7 @@
 // Every K and V element is used for the query heads of its group, 2 to 16 of them mostly: 2 to 16
 // flops a byte, far below the ridge, so the kernel is built as a stream of the pages.  Work is
 // cut without regard to sequences: the tokens of all sequences are laid end to end (cu_seqlens
-// is that layout), with kSeqCost virtual tokens of overhead in front of each sequence, and the
+// is that layout), with kSeqCost virtual tokens of overhead behind those of each sequence, and the
 // line is cut into equal ranges.  One warp walks one range of one KV head, so a batch of any
 // raggedness keeps all warps equally busy and the host needs no lengths.  A sequence inside
 // one range is finished by its warp; a sequence cut by a range border leaves (m, l, O) of its
@@ -17,8 +17,8 @@
 // each sequence and KV head, its warps' parts joined in shared memory.
 //
 // Measured on a B200 (calls back to back; HBM floor at the measured 6535 GB/s): 32 sequences of
-// 20000..32768, 8 KV heads x 128, bf16: 559-591 us by the box's power (floor 529); one of 131071: 97-102 us
-// (82); 64 of 1..8192: 62-65 us (46); 256 of 1..600, f16: 28.6 us (17); fp32, 16 of 4096: 97 us (82).  About
+// 20000..32768, 8 KV heads x 128, bf16: 551-591 us by the box's power (floor 529); one of 131071: 98-103 us
+// (82); 64 of 1..8192: 63-65 us (46); 256 of 1..600, f16: 29.4 us (17); fp32, 16 of 4096: 98 us (82).  About
 // 12 us of each are the launch, the dependent loads before the first copy, the last warps and the join; the
 // rest streams at 0.93-0.97 of the peak.
 #include "dkv_common.cuh"
@@ -1262,9 +1262,11 @@ struct Shape {
 // fp32 walks, which do more arithmetic a byte, want whole sets of four warps (one a scheduler), and tiles
 // of 8 tokens to have them at 128 columns: at 8 KV heads x 128, 64 sequences of 1..8192, 4 / 8 heads a KV
 // head take 115 / 170 us with 6 / 5 warps of 16 tokens, 119 / 154 with 11 / 10 of 8, 110 / 145 with 8 of 8.
-// Groups of more than 8 heads are several units, whose warps read the pages one after the other out of
-// L2: 16 heads a warp need more registers than 12 warps leave, and 8 warps of 16 heads were slower (16
-// heads a KV head: 78 against 73 us at head_dim 128, 37 / 31 at 64, 137 / 109 at 256; 36 / 41 at 32).
+// Groups of more than 8 heads are several units, whose warps read the pages one after the other out of L2; a warp
+// of 16 heads takes more registers than 12 warps leave (8 of them an SM at head_dim 128) and a kernel of its own.
+// 16 sequences, 8 KV heads of 16 query heads, bf16, us, two units / 16 heads a warp (floor): 2048
+// tokens x 256 77 / 98 (41), 4096 x 128 65 / 63 (41), 8192 x 64 77 / 66 (41), 8192 x 32 60 / 48 (20.5): one form, which is
+// the better one at the largest heads.
 struct Variant {
   int warps, stages, tokens;
 };

@@ -224,6 +224,8 @@ struct Raw<DT, 1> {
 // neighbouring heads.  Bound by memory: every q, k and v element is read once and written once.  Measured
 // on a B200: 16384 rows of 32 + 8 + 8 heads x 128, bf16 68-70 us = 5.9-6.0 TB/s, 0.90-0.92 of the measured HBM rate
 // (an element pair a thread: 312 us; two heads a thread 75 us; a thread's heads adjacent 71 us); 64 rows 3.0 us.
+// fp32, the same rows: 120 us, at the floor of 123.  Rows whose halves are not 16-byte pieces go an element pair a
+// thread, with four heads' loads in flight still: head_dim 72 / 100, bf16, 120 / 166 us (floors 35 / 48), fp32 100 167 (96).
 constexpr int kHeads = 4;
 
 template <int SDT, int PDT, int VEC>
