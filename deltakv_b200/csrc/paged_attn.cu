@@ -766,15 +766,29 @@ template <int DT, int kSteps>
 __device__ __forceinline__ void infinite_columns(const Params &p, float (&o)[kSteps][4], const float (&sum)[2], int u, int b,
                                                  int i0, int i1, int step, int g, int t) {
   constexpr uint32_t kExp = DT == DKV_BF16 ? 0x7f80 : 0x7c00;
-  uint32_t up = 0, down = 0, nan = 0;  // a bit per column of the lane
+  auto of_row = [](uint32_t x) {  // over the four lanes that share columns
+    x |= __shfl_xor_sync(0xffffffffu, x, 1);
+    return x | __shfl_xor_sync(0xffffffffu, x, 2);
+  };
+  uint32_t asked = 0, up = 0, down = 0, nan = 0;  // a bit per column of the lane
+#pragma unroll
+  for (int c = 0; c < 2 * kSteps; ++c)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float x = o[c / 2][c % 2 * 2 + h];
+      asked |= static_cast<uint32_t>(x != x && sum[h] == sum[h]) << c;
+    }
+  asked = of_row(asked);
   const int64_t tlen = p.table_lens ? p.table_lens[b] : p.table_stride;
-  for (int i = i0; i < i1; i += step) {
-    for (int token = i + t; token < min(i + kTile, i1); token += 4) {
-      const int blk = token / p.block_size;
+  // (until every column asked for is known to be NaN; i + kTile and i + step may pass 2^31 and are not formed before the end)
+  for (int i = i0; i < i1 && __any_sync(0xffffffffu, (asked & ~(nan | (up & down))) != 0); i += step) {
+    const int n = min(i1 - i, kTile);
+    for (int j = t; j < n; j += 4) {
+      const int blk = (i + j) / p.block_size;
       const int id = blk < tlen ? p.tables[b * p.table_stride + blk] : -1;
       if (id < 0 || id >= p.num_blocks) continue;
       const unsigned short *row = reinterpret_cast<const unsigned short *>(
-          p.v + u * p.v_head + id * p.v_block + (token - blk * p.block_size) * p.v_slot);
+          p.v + u * p.v_head + id * p.v_block + (i + j - blk * p.block_size) * p.v_slot);
 #pragma unroll
       for (int c = 0; c < 2 * kSteps; ++c) {
         const int d = c * 8 + g;
@@ -784,12 +798,8 @@ __device__ __forceinline__ void infinite_columns(const Params &p, float (&o)[kSt
         down |= static_cast<uint32_t>(x == (kExp | 0x8000)) << c;
       }
     }
-  }
-#pragma unroll
-  for (int k = 1; k < 4; k <<= 1) {
-    nan |= __shfl_xor_sync(0xffffffffu, nan, k);
-    up |= __shfl_xor_sync(0xffffffffu, up, k);
-    down |= __shfl_xor_sync(0xffffffffu, down, k);
+    nan = of_row(nan), up = of_row(up), down = of_row(down);
+    if (i1 - i <= step) break;
   }
   up &= ~nan, down &= ~nan;
 #pragma unroll

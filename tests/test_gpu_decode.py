@@ -264,6 +264,25 @@ def test_attention_infinite_values(cuda, dtype, hd, lens, bound, scale):
         torch.isfinite(c.tokens(b)[1]).all(0), clean(b)[1], 0)), scale)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_attention_infinite_value_at_the_end_of_the_longest_sequence(cuda, dtype):
+    """2^31 - 1 tokens, the last of them infinite in one column: one block of equal tokens, over and over."""
+    n, block = (1 << 31) - 1, 1 << 20
+    last = (n - 1) // block
+    k = torch.zeros(2, block, 1, 32, dtype=dtype, device=cuda)
+    v = torch.ones_like(k)
+    v[1, (n - 1) % block, 0, 5] = -math.inf
+    tables = torch.zeros(1, last + 1, dtype=torch.int32, device=cuda)
+    tables[0, last] = 1
+    seqs = dkv.SeqBatchTensors(cu_seqlens=torch.tensor([0, n], dtype=torch.int32, device=cuda), block_tables=tables,
+                               max_seq_len=n)
+    got = dkv.paged_decode_attention(torch.ones(1, 2, 32, dtype=dtype, device=cuda), k, v, seqs, check=True)
+    assert torch.all(got[..., 5] == -math.inf)
+    got[..., 5] = 1
+    # sums of up to 2^31 equal fp32 terms stop growing at 2^24 of them, alike in numerator and denominator
+    assert torch.all((got.float() - 1).abs() <= torch.finfo(dtype).eps + 2.0 ** -16)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lens", [[20011], [9000, 1, 0, 7000], [1] * 300, [0] * 40, [3, 2049] * 20, list(range(130))])
 def test_attention_long_and_ragged(cuda, dtype, lens):
