@@ -780,7 +780,7 @@ __device__ __forceinline__ void infinite_columns(const Params &p, float (&o)[kSt
     }
   asked = of_row(asked);
   const int64_t tlen = p.table_lens ? p.table_lens[b] : p.table_stride;
-  // (until every column asked for is known to be NaN; i + kTile and i + step may pass 2^31 and are not formed before the end)
+  // until every column asked for is known to be NaN (i + kTile and i + step are not formed where they could pass 2^31)
   for (int i = i0; i < i1 && __any_sync(0xffffffffu, (asked & ~(nan | (up & down))) != 0); i += step) {
     const int n = min(i1 - i, kTile);
     for (int j = t; j < n; j += 4) {
@@ -964,7 +964,8 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
       if (!all_finite()) {
         const int first = p.cu[b], len = max(p.cu[b + 1] - first, 0);
         const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
-        infinite_columns<DT>(p, o, sum, h0 / p.group, b, border(stream.w.x0, at, len), border(stream.w.x1, at, len), kTile, g, t);
+        infinite_columns<DT>(p, o, sum, h0 / p.group, b, border(stream.w.x0, at, len), border(stream.w.x1, at, len), kTile,
+                             g, t);
       }
       if (whole) {
         // heads to rows, so that a lane stores two neighbouring columns of one head

@@ -148,8 +148,9 @@ def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: op
     gives zeros and ``-inf``.  The form of the launch goes by the batch and by ``seqs.max_seq_len``,
     which may be any bound: with one of a few hundred tokens short sequences take one launch, about
     half the time of the form that cuts long ones.  A captured step keeps the form of its
-    capture, so a serving loop is faster with a graph for each class of lengths.  Any head_dim up to 256 and any strides; rows that start on 16
-    bytes and are a multiple of 16 bytes long are read fastest.
+    capture, so a serving loop is faster with a graph for each class of lengths.  Any head_dim up to
+    256 and any strides; rows that start on 16 bytes and are a multiple of 16 bytes long are read
+    fastest.
 
     Slots behind a sequence's length are not read into the result, whatever they hold.  An infinite
     V element of a token that counts makes its column infinite (NaN where both signs meet; perhaps
