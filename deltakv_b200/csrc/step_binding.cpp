@@ -391,6 +391,9 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t count) {
     if (tables.dim() == 2 && tables.size(0) < n)
       value_error("block_tables has " + std::to_string(tables.size(0)) + " rows for " + std::to_string(n) +
                   " sequences");
+    // without table_lens a row has as many entries as lie between two rows (SeqBatchTensors lays its tables out so)
+    if (!lens && tables.dim() == 2 && tables.numel() > 0 && tables.stride(0) != tables.size(1))
+      value_error("block_tables without table_lens must have rows that follow one another");
     if (lens && (lens->numel() < n || !lens->is_contiguous()))
       value_error("table_lens must be a contiguous vector of " + std::to_string(n));
     if (!cu.is_contiguous()) value_error("cu_seqlens must be a contiguous vector");

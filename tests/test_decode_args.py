@@ -145,6 +145,21 @@ def test_append_refuses_rope_tables_without_positions():
             _append(rope=tables, positions=_ROPE["positions"])
 
 
+@pytest.mark.parametrize("tables", [torch.zeros(2, 9, dtype=I32)[:, 3:], torch.zeros(1, 4, dtype=I32).expand(2, 4)])
+def test_attention_refuses_tables_put_into_a_batch_without_lengths(tables):
+    """SeqBatchTensors copies such tables when it is made; one put into it later would be read past its rows."""
+    seqs = dkv.SeqBatchTensors(cu_seqlens=torch.tensor([0, 3, 5], dtype=I32), block_tables=tables, max_seq_len=3)
+    x = torch.zeros(2, 4, 8, dtype=BF), torch.zeros(4, 4, 2, 8, dtype=BF), torch.zeros(4, 4, 2, 8, dtype=BF)
+    with pytest.raises(ValueError, match="CUDA"):  # as it was made: on to the next check
+        dkv.paged_decode_attention(*x, seqs)
+    seqs.block_tables = tables
+    with pytest.raises(ValueError, match="follow one another"):
+        dkv.paged_decode_attention(*x, seqs)
+    seqs.table_lens = torch.ones(2, dtype=I32)
+    with pytest.raises(ValueError, match="CUDA"):
+        dkv.paged_decode_attention(*x, seqs)
+
+
 def test_attention_passes_on_a_truth_that_raises():
     with pytest.raises(RuntimeError, match="ambiguous"):
         _attend(return_lse=torch.zeros(2))  # used to go on, with the error pending
