@@ -330,7 +330,7 @@ def run(state):
 
             q = dkv.append_into_paged(state["k"], state["v"], k_pages, v_pages, state["slots"], q=state["q"],
                                       positions=state["positions"], rope=(state["cos"], state["sin"]),
-                                      interleaved=case["interleaved"],
+                                      rotary_dim=case["rot"], interleaved=case["interleaved"],
                                       kv_scales=None if k_scales is None else (k_scales, v_scales))
         else:
             q = _plain_append(state)
