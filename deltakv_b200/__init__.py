@@ -16,7 +16,8 @@ deployment swaps them in (see :func:`install`):
 
 and what a serving loop does with the same pages between two patches: a decode step
 (``plan_paged_step``, ``append_into_paged``, ``paged_decode_attention``) and the first two of
-these for prompt chunks,
+these for prompt chunks; also on pages of 8 bits (e4m3 or int8, with a scale for each block and head), which
+``scatter_into_paged_batched`` patches and ``gather_from_paged_batched`` reads back,
 plus the fused batched forms the engine and connector use: :class:`ExactPatcher` (LoRA
 deltas) and :class:`DensePatcher` (full-rank dW of an RL step, a tensor-core GEMM).
 All computation runs in ``libdkv_b200.so``; a missing library raises (no CPU path).
@@ -46,7 +47,12 @@ from deltakv_b200.probe import (
     select_probes,
     weight_axis_scores,
 )
-from deltakv_b200.paged import gather_from_paged, scatter_into_paged, scatter_into_paged_batched
+from deltakv_b200.paged import (
+    gather_from_paged,
+    gather_from_paged_batched,
+    scatter_into_paged,
+    scatter_into_paged_batched,
+)
 from deltakv_b200.rope import RotaryEmbedding
 from deltakv_b200.subspace import subspace_correct, subspace_correct_batched, svd_basis
 from deltakv_b200.types import KVCache, LayerDelta, LowRankFactors, LowRankKVPatch
@@ -72,6 +78,7 @@ __all__ = [
     "compare_kv",
     "exact_kv_patch",
     "gather_from_paged",
+    "gather_from_paged_batched",
     "install",
     "kivi",
     "lora_activation_scores",

@@ -28,7 +28,7 @@ DKV_ERR_WORKSPACE = -11
 DKV_ERR_NO_BLOCKS = -12
 
 # element types
-DKV_F32, DKV_F16, DKV_BF16, DKV_E4M3, DKV_I32, DKV_U8 = 0, 1, 2, 3, 4, 5
+DKV_F32, DKV_F16, DKV_BF16, DKV_E4M3, DKV_I32, DKV_U8, DKV_I8 = 0, 1, 2, 3, 4, 5, 6
 DKV_MAX_LAYERS = 128
 
 EXPORTED = (
@@ -74,6 +74,12 @@ EXPORTED = (
     "dkv_append_paged",
     "dkv_paged_decode_workspace_bytes",
     "dkv_paged_decode_attention",
+    "dkv_append_paged_rotary",
+    "dkv_append_paged_quant",
+    "dkv_scatter_paged_quant",
+    "dkv_gather_paged_quant",
+    "dkv_paged_decode_quant_workspace_bytes",
+    "dkv_paged_decode_attention_quant",
 )
 
 
@@ -344,6 +350,14 @@ class PagedDecodeArgs(C.Structure):
     ]
 
 
+class Rotary(C.Structure):
+    _fields_ = [("dim", C.c_int32), ("interleaved", C.c_int32)]
+
+
+class PageScales(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("stride_block", C.c_int64), ("stride_head", C.c_int64)]
+
+
 _lib: C.CDLL | None = None
 
 
@@ -436,6 +450,20 @@ def _declare(lib: C.CDLL) -> None:
     lib.dkv_paged_decode_workspace_bytes.argtypes = [C.POINTER(PagedDecodeArgs), C.POINTER(C.c_int64)]
     lib.dkv_paged_decode_attention.restype = C.c_int
     lib.dkv_paged_decode_attention.argtypes = [C.POINTER(PagedDecodeArgs), P]
+    scales = C.POINTER(PageScales)
+    lib.dkv_append_paged_rotary.restype = C.c_int
+    lib.dkv_append_paged_rotary.argtypes = [C.POINTER(AppendArgs), C.POINTER(Rotary), P]
+    lib.dkv_append_paged_quant.restype = C.c_int
+    lib.dkv_append_paged_quant.argtypes = [C.POINTER(AppendArgs), C.POINTER(Rotary), scales, scales, P]
+    lib.dkv_scatter_paged_quant.restype = C.c_int
+    lib.dkv_scatter_paged_quant.argtypes = [P, I32, I64, I64, I64, C.POINTER(PagedCache), scales, C.POINTER(SeqBatch), P, P]
+    lib.dkv_gather_paged_quant.restype = C.c_int
+    lib.dkv_gather_paged_quant.argtypes = [C.POINTER(PagedCache), scales, C.POINTER(SeqBatch), P, I32, I64, I64, I64, I32, P,
+                                           P]
+    lib.dkv_paged_decode_quant_workspace_bytes.restype = C.c_int
+    lib.dkv_paged_decode_quant_workspace_bytes.argtypes = [C.POINTER(PagedDecodeArgs), I32, C.POINTER(C.c_int64)]
+    lib.dkv_paged_decode_attention_quant.restype = C.c_int
+    lib.dkv_paged_decode_attention_quant.argtypes = [C.POINTER(PagedDecodeArgs), I32, scales, scales, P]
 
 
 def lib() -> C.CDLL:

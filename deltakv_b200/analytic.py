@@ -104,6 +104,7 @@ def _rope_(x: Tensor, rope) -> None:
     if n == 0:
         return
     cos, sin = half_tables(rope, x.device)
+    ops._check_rope(cos, sin, hd)
     rc = L.lib().dkv_rope_rows(x.data_ptr(), n, heads, hd, x.stride(0), cos.data_ptr(), sin.data_ptr(),
                                min(max_positions(rope), cos.shape[0]), ops.stream_ptr())
     L.check(rc, "dkv_rope_rows")

@@ -3,7 +3,7 @@
 //   dkv_append_paged     RoPE of the new q and k rows, K and V stored in their slots
 // They extend the layouts of the paged scatter / gather (src/deltakv/paged.py:8-70); the
 // rotation is the reference's rotate-half RoPE (src/deltakv/rope.py:9-63).
-#include "dkv_common.cuh"
+#include "paged_rows.cuh"
 
 namespace dkv {
 namespace step {
@@ -154,70 +154,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(dkv_step_plan_args a
 // ---------------------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------------------
-constexpr int kAppThreads = 128;
-
-struct Append {
-  const void *src[3];  // q, k, v
-  void *dst[3];        // q_out, K pages, V pages
-  int64_t src_row[3], src_head[3];
-  int64_t dst_row[3], dst_head[3];  // dst_row: q_out's row stride, the pages' slot stride
-  int64_t dst_block[3];
-  const int64_t *slots;
-  const int32_t *positions;
-  const float *cos_t, *sin_t;
-  int64_t n_rows, n_slots;
-  int32_t *status;
-  int heads[3];
-  int hd, half, block_size, rope_max_pos;
-  int wide;  // more than 2^32 threads
-};
-
-// VEC consecutive elements of a type as they lie in memory, in 16-byte pieces (one: as it is)
-template <int DT, int VEC>
-struct Raw {
-  static constexpr int kPieces = VEC * static_cast<int>(sizeof(typename Elem<DT>::T)) / 16;
-  uint4 v[kPieces];
-  __device__ __forceinline__ void load(const typename Elem<DT>::T *src) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) v[i] = reinterpret_cast<const uint4 *>(src)[i];
-  }
-  __device__ __forceinline__ void store(typename Elem<DT>::T *dst) const {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4 *>(dst)[i] = v[i];
-  }
-  __device__ __forceinline__ float get(int i) const {
-    const int per = VEC / kPieces;
-    const uint4 u = v[i / per];
-    const int e = i % per;
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    if (DT == DKV_F32) return __uint_as_float(w[e & 3]);
-    const uint32_t x = w[(e / 2) & 3];
-    return DT == DKV_BF16 ? (e & 1 ? bf16hi(x) : bf16lo(x)) : (e & 1 ? f16hi(x) : f16lo(x));
-  }
-  __device__ __forceinline__ void set(const float (&x)[VEC]) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const float *y = x + i * (VEC / kPieces);
-      if constexpr (DT == DKV_F32)
-        v[i] = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
-      else if constexpr (DT == DKV_BF16)
-        v[i] = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                          pack_bf16x2(y[6], y[7]));
-      else
-        v[i] = make_uint4(pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]), pack_f16x2(y[4], y[5]),
-                          pack_f16x2(y[6], y[7]));
-    }
-  }
-};
-template <int DT>
-struct Raw<DT, 1> {
-  typename Elem<DT>::T v;
-  __device__ __forceinline__ void load(const typename Elem<DT>::T *src) { v = src[0]; }
-  __device__ __forceinline__ void store(typename Elem<DT>::T *dst) const { dst[0] = v; }
-  __device__ __forceinline__ float get(int) const { return Elem<DT>::to_f(v); }
-  __device__ __forceinline__ void set(const float (&x)[1]) { v = Elem<DT>::from_f(x[0]); }
-};
-
 // A thread has VEC columns i and their partners i + half of up to kHeads heads of a row, so that
 // the row's slot, position and cos / sin are read once for all of them and 2 kHeads 16-byte loads
 // are in flight; the heads of a thread are `groups` apart, so that neighbouring threads read
@@ -226,78 +162,10 @@ struct Raw<DT, 1> {
 // (an element pair a thread: 312 us; two heads a thread 75 us; a thread's heads adjacent 71 us); 64 rows 3.0 us.
 // fp32, the same rows: 120 us, at the floor of 123.  Rows whose halves are not 16-byte pieces go an element pair a
 // thread, with four heads' loads in flight still: head_dim 72 / 100, bf16, 120 / 166 us (floors 35 / 48), fp32 100 167 (96).
-constexpr int kHeads = 4;
-
-template <int SDT, int PDT, int VEC>
+template <int SDT, int PDT, int VEC, bool kForms>
 __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_constant__ Append a) {
-  using ST = typename Elem<SDT>::T;
-  using PT = typename Elem<PDT>::T;
   begin_overlapped();
-  const int all = a.heads[0] + a.heads[1] + a.heads[2];
-  const int cols = a.half / VEC, groups = (all + kHeads - 1) / kHeads, per_row = cols * groups;
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * kAppThreads + threadIdx.x;
-  const int64_t row = a.wide ? e / per_row : static_cast<uint32_t>(e) / static_cast<uint32_t>(per_row);
-  if (row >= a.n_rows) return;
-  const int in = static_cast<int>(e - row * per_row);
-  const int hg = in / cols, j = (in - hg * cols) * VEC;
-  const bool pair = j + a.half < a.hd;  // false only for the middle of an odd head without RoPE
-
-  const int64_t slot = a.slots[row];
-  const int pos = a.cos_t ? a.positions[row] : 0;
-  Raw<SDT, VEC> x[kHeads][2];
-#pragma unroll
-  for (int k = 0; k < kHeads; ++k) {
-    int h = hg + k * groups;
-    if (h >= all) break;
-    const int w = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
-    h -= w == 0 ? 0 : w == 1 ? a.heads[0] : a.heads[0] + a.heads[1];
-    const ST *src = static_cast<const ST *>(a.src[w]) + row * a.src_row[w] + h * a.src_head[w] + j;
-    x[k][0].load(src);
-    if (pair) x[k][1].load(src + a.half);
-  }
-  if (a.cos_t && (pos < 0 || pos >= a.rope_max_pos)) {
-    record_error(a.status, DKV_ERR_ROPE_RANGE);
-    return;
-  }
-  if (slot >= a.n_slots) record_error(a.status, DKV_ERR_PAGE_RANGE);
-  const bool kept = slot >= 0 && slot < a.n_slots;
-  Raw<DKV_F32, VEC> c, s;
-  if (a.cos_t) {
-    c.load(a.cos_t + static_cast<int64_t>(pos) * a.half + j);
-    s.load(a.sin_t + static_cast<int64_t>(pos) * a.half + j);
-  }
-  const int64_t block = kept ? slot / a.block_size : 0;
-  const int64_t off = kept ? slot - block * a.block_size : 0;
-#pragma unroll
-  for (int k = 0; k < kHeads; ++k) {
-    int h = hg + k * groups;
-    if (h >= all) break;
-    const int w = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
-    h -= w == 0 ? 0 : w == 1 ? a.heads[0] : a.heads[0] + a.heads[1];
-    if (w && !kept) continue;
-    float lo[VEC], hi[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) lo[i] = x[k][0].get(i), hi[i] = pair ? x[k][1].get(i) : 0.f;
-    if (a.cos_t && w < 2) {  // products and sum each rounded, as the reference's tensor operations do
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float u = lo[i], v = hi[i];
-        lo[i] = __fsub_rn(__fmul_rn(u, c.get(i)), __fmul_rn(v, s.get(i)));
-        hi[i] = __fadd_rn(__fmul_rn(v, c.get(i)), __fmul_rn(u, s.get(i)));
-      }
-    }
-    if (w == 0) {
-      ST *dst = static_cast<ST *>(a.dst[0]) + row * a.dst_row[0] + h * a.dst_head[0] + j;
-      Raw<SDT, VEC> y;
-      y.set(lo), y.store(dst);
-      if (pair) y.set(hi), y.store(dst + a.half);
-    } else {
-      PT *dst = static_cast<PT *>(a.dst[w]) + block * a.dst_block[w] + off * a.dst_row[w] + h * a.dst_head[w] + j;
-      Raw<PDT, VEC> y;
-      y.set(lo), y.store(dst);
-      if (pair) y.set(hi), y.store(dst + a.half);
-    }
-  }
+  append_rows<SDT, PDT, VEC, kForms>(a, static_cast<int64_t>(blockIdx.x) * kAppThreads + threadIdx.x);
 }
 
 bool float_dtype(int dt) { return dt == DKV_F32 || dt == DKV_F16 || dt == DKV_BF16; }
@@ -340,6 +208,10 @@ extern "C" int dkv_plan_paged_step(const dkv_step_plan_args *args, dkv_stream_t 
 }
 
 extern "C" int dkv_append_paged(const dkv_append_args *args, dkv_stream_t stream) {
+  return dkv_append_paged_rotary(args, nullptr, stream);
+}
+
+extern "C" int dkv_append_paged_rotary(const dkv_append_args *args, const dkv_rotary *rotary, dkv_stream_t stream) {
   if (args == nullptr) return DKV_ERR_INVALID_ARGUMENT;
   const dkv_append_args &g = *args;
   const dkv_paged_cache &kp = g.k_pages, &vp = g.v_pages;
@@ -350,7 +222,9 @@ extern "C" int dkv_append_paged(const dkv_append_args *args, dkv_stream_t stream
     return DKV_ERR_LAYOUT;
   if (g.n_rows < 0 || (g.q != nullptr && g.n_q_heads <= 0)) return DKV_ERR_INVALID_ARGUMENT;
   if ((g.rope_cos == nullptr) != (g.rope_sin == nullptr)) return DKV_ERR_INVALID_ARGUMENT;
-  if (g.rope_cos != nullptr && (kp.head_dim & 1)) return DKV_ERR_UNSUPPORTED;
+  step::Rotary rot;
+  const int form = step::rotary_of(g.rope_cos != nullptr, rotary, kp.head_dim, &rot);
+  if (form < 0) return DKV_ERR_UNSUPPORTED;
   if (g.n_rows == 0) return DKV_OK;
   if (g.k == nullptr || g.v == nullptr || g.slots == nullptr) return DKV_ERR_INVALID_ARGUMENT;
   if (g.rope_cos != nullptr && g.positions == nullptr) return DKV_ERR_INVALID_ARGUMENT;
@@ -358,19 +232,8 @@ extern "C" int dkv_append_paged(const dkv_append_args *args, dkv_stream_t stream
   if ((kp.base == nullptr && kp.num_blocks > 0) || (vp.base == nullptr && vp.num_blocks > 0))
     return DKV_ERR_INVALID_ARGUMENT;
   step::Append a;
-  a.src[0] = g.q, a.src[1] = g.k, a.src[2] = g.v;
-  a.dst[0] = g.q_out, a.dst[1] = kp.base, a.dst[2] = vp.base;
-  a.src_row[0] = g.q_stride_row, a.src_row[1] = g.k_stride_row, a.src_row[2] = g.v_stride_row;
-  a.src_head[0] = g.q_stride_head, a.src_head[1] = g.k_stride_head, a.src_head[2] = g.v_stride_head;
-  a.dst_row[0] = g.q_out_stride_row, a.dst_row[1] = kp.stride_slot, a.dst_row[2] = vp.stride_slot;
-  a.dst_head[0] = g.q_out_stride_head, a.dst_head[1] = kp.stride_head, a.dst_head[2] = vp.stride_head;
-  a.dst_block[0] = 0, a.dst_block[1] = kp.stride_block, a.dst_block[2] = vp.stride_block;
-  a.slots = g.slots, a.positions = g.positions, a.cos_t = g.rope_cos, a.sin_t = g.rope_sin;
-  a.n_rows = g.n_rows;
-  a.n_slots = (kp.num_blocks < vp.num_blocks ? kp.num_blocks : vp.num_blocks) * kp.block_size;
-  a.status = g.status;
-  a.heads[0] = g.q != nullptr ? g.n_q_heads : 0, a.heads[1] = a.heads[2] = kp.n_heads;
-  a.hd = kp.head_dim, a.half = (kp.head_dim + 1) / 2, a.block_size = kp.block_size, a.rope_max_pos = g.rope_max_pos;
+  step::describe(g, rot, &a);
+  a.heads[1] = a.heads[2] = kp.n_heads;
   // 16-byte accesses where every half row of a head starts on 16 bytes 
   const int64_t ssz = g.in_dtype == DKV_F32 ? 4 : 2, psz = kp.dtype == DKV_F32 ? 4 : 2;
   const int vec = static_cast<int>(16 / psz);
@@ -383,9 +246,10 @@ extern "C" int dkv_append_paged(const dkv_append_args *args, dkv_stream_t stream
       page_bits |= reinterpret_cast<intptr_t>(a.dst[w]) | a.dst_row[w] * psz | a.dst_head[w] * psz | a.dst_block[w] * psz;
   }
   in_bits |= reinterpret_cast<intptr_t>(a.cos_t) | reinterpret_cast<intptr_t>(a.sin_t);
-  const bool wide = kp.head_dim % (2 * vec) == 0 && (in_bits | page_bits) % 16 == 0;
+  const bool wide = step::whole_pieces(rot, kp.head_dim, vec) && (in_bits | page_bits) % 16 == 0;
   const int all = a.heads[0] + a.heads[1] + a.heads[2];
-  const int64_t total = a.n_rows * ((all + step::kHeads - 1) / step::kHeads) * (a.half / (wide ? vec : 1));
+  const int64_t total = a.n_rows * ((all + step::kHeads - 1) / step::kHeads) *
+                        (form ? step::pieces_of(rot, kp.head_dim, wide ? vec : 1) : a.half / (wide ? vec : 1));
   a.wide = total > UINT32_MAX;
   const int64_t ctas = (total + step::kAppThreads - 1) / step::kAppThreads;
   if (ctas > INT32_MAX) return DKV_ERR_UNSUPPORTED;
@@ -393,7 +257,9 @@ extern "C" int dkv_append_paged(const dkv_append_args *args, dkv_stream_t stream
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 #define DKV_APPEND_CASE(S, P)                                                                              \
   if (g.in_dtype == S && kp.dtype == P) {                                                                  \
-    const auto kernel = wide ? step::append_kernel<S, P, P == DKV_F32 ? 4 : 8> : step::append_kernel<S, P, 1>; \
+    constexpr int kVec = P == DKV_F32 ? 4 : 8;                                                             \
+    const auto kernel = form ? (wide ? step::append_kernel<S, P, kVec, true> : step::append_kernel<S, P, 1, true>)     \
+                             : (wide ? step::append_kernel<S, P, kVec, false> : step::append_kernel<S, P, 1, false>);  \
     DKV_CUDA_CHECK(launch_overlapped(kernel, dim3(grid), step::kAppThreads, 0, st, a));                    \
     return DKV_OK;                                                                                         \
   }

@@ -29,9 +29,18 @@ namespace {
 using at::Tensor;
 
 int (*g_plan)(const dkv_step_plan_args *, dkv_stream_t);
-int (*g_append)(const dkv_append_args *, dkv_stream_t);
+int (*g_append)(const dkv_append_args *, const dkv_rotary *, dkv_stream_t);
 int (*g_workspace)(const dkv_paged_decode_args *, int64_t *);
 int (*g_attend)(const dkv_paged_decode_args *, dkv_stream_t);
+// 8-bit pages
+int (*g_append_quant)(const dkv_append_args *, const dkv_rotary *, const dkv_page_scales *, const dkv_page_scales *,
+                      dkv_stream_t);
+int (*g_scatter_quant)(const void *, int32_t, int64_t, int64_t, int64_t, const dkv_paged_cache *, const dkv_page_scales *,
+                       const dkv_seq_batch *, int32_t *, dkv_stream_t);
+int (*g_gather_quant)(const dkv_paged_cache *, const dkv_page_scales *, const dkv_seq_batch *, void *, int32_t, int64_t, int64_t,
+                      int64_t, int32_t, int32_t *, dkv_stream_t);
+int (*g_workspace_quant)(const dkv_paged_decode_args *, int32_t, int64_t *);
+int (*g_attend_quant)(const dkv_paged_decode_args *, int32_t, const dkv_page_scales *, const dkv_page_scales *, dkv_stream_t);
 PyObject *g_raise;        // raises the package's error for a status code
 PyObject *g_status_word;  // device index -> address of its status word
 constexpr int kMaxDevices = 64;
@@ -92,6 +101,8 @@ int dtype_code(at::ScalarType t) {
     default: type_error(std::string("dtype ") + dtype_name(t) + " is not supported by the B200 kernels");
   }
 }
+bool is_code(at::ScalarType t) { return t == at::kFloat8_e4m3fn || t == at::kChar; }
+int code_of(at::ScalarType t) { return t == at::kFloat8_e4m3fn ? DKV_E4M3 : DKV_I8; }
 std::string shape_text(const Tensor &t) {
   std::string s = "(";
   for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
@@ -187,20 +198,86 @@ dkv_paged_cache describe(const Tensor &t, int code) {
   c.stride_block = t.stride(0), c.stride_slot = t.stride(1), c.stride_head = t.stride(2);
   return c;
 }
-// checks the K and V pages, and describes them once they are known to be on the GPU
+// checks the K and V pages, and describes them once they are known to be on the GPU; 8 bits: where scales come with them
 struct Pages {
   const Tensor &k, &v;
   int code;
   int64_t heads, hd;
-  Pages(const Tensor &k_, const Tensor &v_) : k(k_), v(v_) {
+  Pages(const Tensor &k_, const Tensor &v_, bool scaled = false) : k(k_), v(v_) {
     if (k.dim() != 4 || v.dim() != 4)
       value_error("unsupported paged KV layout " + shape_text(k) + ", " + shape_text(v));
     if (k.scalar_type() != v.scalar_type() || k.size(1) != v.size(1) || k.size(2) != v.size(2) || k.size(3) != v.size(3))
       value_error("k_pages and v_pages must share dtype, block size, heads and head_dim");
-    code = dtype_code(k.scalar_type());
+    if (is_code(k.scalar_type()) && !scaled) type_error(std::string(dtype_name(k.scalar_type())) + " pages need kv_scales");
+    if (scaled && !is_code(k.scalar_type()))
+      type_error(std::string("kv_scales go with 8-bit pages (float8_e4m3fn or int8), not ") + dtype_name(k.scalar_type()));
+    code = scaled ? code_of(k.scalar_type()) : dtype_code(k.scalar_type());
     heads = k.size(2), hd = k.size(3);
     if ((k.stride(3) != 1 || v.stride(3) != 1) && hd > 1) value_error("paged cache head_dim must be contiguous");
     if (k.size(1) > INT32_MAX || heads > INT32_MAX || hd > INT32_MAX) value_error("paged cache too large");
+  }
+};
+
+// The scales of 8-bit pages: fp32 [num_blocks, heads], any strides.
+void scales_of(const Tensor &t, const char *name, const Tensor &pages) {
+  if (t.scalar_type() != at::kFloat) type_error(std::string(name) + " must be float32");
+  if (t.dim() != 2 || t.size(0) != pages.size(0) || t.size(1) != pages.size(2))
+    value_error(std::string(name) + " " + shape_text(t) + " must be [num_blocks, heads] = [" + std::to_string(pages.size(0)) +
+                ", " + std::to_string(pages.size(2)) + "]");
+}
+dkv_page_scales describe_scales(const Tensor &t) { return {t.data_ptr<float>(), t.stride(0), t.stride(1)}; }
+
+// kv_scales: None or a (K, V) pair of tensors
+struct PairOfScales {
+  const Tensor *k = nullptr, *v = nullptr;
+  explicit PairOfScales(PyObject *o) {
+    if (o == Py_None) return;
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) type_error("kv_scales must be a (k_scales, v_scales) tuple");
+    k = &tensor(PyTuple_GET_ITEM(o, 0), "k_scales"), v = &tensor(PyTuple_GET_ITEM(o, 1), "v_scales");
+  }
+  explicit operator bool() const { return k != nullptr; }
+  void check(const Pages &pages) const {
+    if (k == nullptr) return;
+    scales_of(*k, "k_scales", pages.k), scales_of(*v, "v_scales", pages.v);
+  }
+};
+
+// a batch of sequences, as SeqBatchTensors holds it
+struct Sequences {
+  const Tensor &cu, &tables;
+  const Tensor *lens;
+  int64_t n, max_seq_len;
+  Sequences(PyObject *cu_, PyObject *tables_, PyObject *lens_, PyObject *longest)
+      : cu(tensor(cu_, "cu_seqlens")), tables(tensor(tables_, "block_tables")), lens(maybe(lens_, "table_lens")),
+        n(cu.numel() - 1), max_seq_len(integer(longest)) {}
+  void check_shapes() const {
+    if (tables.dim() == 2 && tables.size(0) < n)
+      value_error("block_tables has " + std::to_string(tables.size(0)) + " rows for " + std::to_string(n) +
+                  " sequences");
+    // without table_lens a row has as many entries as lie between two rows (SeqBatchTensors lays its tables out so)
+    if (!lens && tables.dim() == 2 && tables.numel() > 0 && tables.stride(0) != tables.size(1))
+      value_error("block_tables without table_lens must have rows that follow one another");
+    if (lens && (lens->numel() < n || !lens->is_contiguous()))
+      value_error("table_lens must be a contiguous vector of " + std::to_string(n));
+    if (n < 0 || !cu.is_contiguous()) value_error("cu_seqlens must be a contiguous vector");
+    if (max_seq_len < 0 || max_seq_len > INT32_MAX) value_error("max_seq_len must be in [0, 2**31)");
+  }
+  void check_types() const {
+    if (cu.scalar_type() != at::kInt || tables.scalar_type() != at::kInt || (lens && lens->scalar_type() != at::kInt))
+      type_error("sequence metadata must be int32");
+    if (tables.dim() != 2 || (tables.stride(1) != 1 && tables.size(1) > 1))
+      value_error("block_tables must be a row-major [n_seqs, max_blocks] int32 tensor");
+  }
+  dkv_seq_batch describe() const {
+    dkv_seq_batch q;
+    q.cu_seqlens = cu.data_ptr<int32_t>();
+    q.block_tables = tables.data_ptr<int32_t>();
+    q.table_lens = static_cast<int32_t *>(ptr(lens));
+    q.positions = nullptr;
+    q.table_stride = tables.stride(0);
+    q.n_seqs = static_cast<int32_t>(n);
+    q.max_seq_len = static_cast<int32_t>(max_seq_len);
+    return q;
   }
 };
 
@@ -288,30 +365,44 @@ PyObject *rope_ready(PyObject *, PyObject *const *a, Py_ssize_t count) {
   });
 }
 
-// append(k, v, k_pages, v_pages, slots, q, positions, cos, sin, q_out) -> q_out or None
+// append(k, v, k_pages, v_pages, slots, q, positions, cos, sin, q_out, rotary_dim, interleaved, kv_scales)
+//   -> q_out or None; rotary_dim None: the whole head
 PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
   return guarded([&]() -> PyObject * {
-    if (count != 10) type_error("append takes 10 arguments");
+    if (count != 13) type_error("append takes 13 arguments");
     const Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v");
-    const Pages pages(tensor(a[2], "k_pages"), tensor(a[3], "v_pages"));
+    const PairOfScales scales(a[12]);
+    const Pages pages(tensor(a[2], "k_pages"), tensor(a[3], "v_pages"), static_cast<bool>(scales));
     const Tensor &slots = tensor(a[4], "slots");
     const Tensor *q = maybe(a[5], "q"), *positions = maybe(a[6], "positions"), *cos = maybe(a[7], "rope cos"),
                  *sin = maybe(a[8], "rope sin"), *q_out = maybe(a[9], "q_out");
-    const int64_t rows = slots.numel();
+    const int64_t rows = slots.numel(), rotary_dim = a[10] == Py_None ? pages.hd : integer(a[10]);
+    const int crossed = PyObject_IsTrue(a[11]);
+    if (crossed < 0) throw Raised{nullptr, ""};
+    if ((a[10] != Py_None || crossed) && !cos) value_error("rotary_dim and interleaved say how rope turns: pass rope with them");
     if (slots.scalar_type() != at::kLong) type_error("slots must be int64");
     if (slots.dim() != 1 || !slots.is_contiguous()) value_error("slots must be a contiguous vector");
     written(pages.k, "k_pages", nullptr, ""), written(pages.v, "v_pages", nullptr, "");
     apart(pages.k, "k_pages", pages.v, "v_pages");
+    if (scales) {
+      scales.check(pages);
+      written(*scales.k, "k_scales", nullptr, ""), written(*scales.v, "v_scales", nullptr, "");
+      apart(*scales.k, "k_scales", *scales.v, "v_scales");
+      if (pages.k.size(1) > 1024) value_error("8-bit pages have at most 1024 slots a block");
+      dtype_code(k.scalar_type());  // any that the kernels read
+    }
     rows_of(k, "k", rows, pages.heads, pages.hd);
     rows_of(v, "v", rows, pages.heads, pages.hd);
     if (v.scalar_type() != k.scalar_type() || (q && q->scalar_type() != k.scalar_type()))
       type_error("q, k and v must share a dtype");
-    if (k.scalar_type() != pages.k.scalar_type() && k.scalar_type() != at::kFloat)
+    if (!scales && k.scalar_type() != pages.k.scalar_type() && k.scalar_type() != at::kFloat)
       type_error(std::string(dtype_name(k.scalar_type())) + " rows do not go into " +
                  dtype_name(pages.k.scalar_type()) + " pages (pass the pages' dtype or fp32)");
     if (cos) {
       if (!positions) value_error("rope needs positions");
       if (cos->dim() == 2 && cos->size(0) == 0) value_error("rope tables without positions");
+      if (a[10] != Py_None && (rotary_dim <= 0 || rotary_dim > pages.hd || rotary_dim % 2))
+        value_error("rotary_dim " + std::to_string(rotary_dim) + " must be even and in (0, head_dim]");
       int32_vector(*positions, "positions", rows);
     }
     if (!q && q_out) value_error("q_out without q");
@@ -328,10 +419,11 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
     }
     const Place at_("append_into_paged", k);
     at_.also(&v), at_.also(&pages.k), at_.also(&pages.v), at_.also(&slots), at_.also(q), at_.also(positions);
-    at_.also(q_out), at_.also(cos), at_.also(sin);
+    at_.also(q_out), at_.also(cos), at_.also(sin), at_.also(scales.k), at_.also(scales.v);
     if (cos) {
-      if (cos->dim() != 2 || cos->sizes() != sin->sizes() || 2 * cos->size(1) != pages.hd)
-        value_error("rope tables " + shape_text(*cos) + " do not cover head_dim " + std::to_string(pages.hd));
+      if (cos->dim() != 2 || cos->sizes() != sin->sizes() || 2 * cos->size(1) != rotary_dim)
+        value_error("rope tables " + shape_text(*cos) + " do not cover " +
+                    (a[10] == Py_None ? "head_dim " : "rotary_dim ") + std::to_string(rotary_dim));
       if (cos->size(0) > INT32_MAX) value_error("rope tables too long");
     }
     const c10::DeviceGuard guard(at_.device);
@@ -353,27 +445,35 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
     p.rope_max_pos = cos ? static_cast<int32_t>(cos->size(0)) : 0;
     p.k_pages = describe(pages.k, pages.code), p.v_pages = describe(pages.v, pages.code);
     p.status = at_.status();
-    check(g_append(&p, at_.stream()), "dkv_append_paged");
+    dkv_rotary rotary;
+    rotary.dim = static_cast<int32_t>(rotary_dim), rotary.interleaved = crossed;
+    if (scales) {
+      const dkv_page_scales ks = describe_scales(*scales.k), vs = describe_scales(*scales.v);
+      check(g_append_quant(&p, &rotary, &ks, &vs, at_.stream()), "dkv_append_paged_quant");
+    } else {
+      check(g_append(&p, &rotary, at_.stream()), "dkv_append_paged");
+    }
     if (made.defined()) return THPVariable_Wrap(made);
     Py_INCREF(a[9]);  // the caller's q_out, or None
     return a[9];
   });
 }
 
-// attend(q, k_pages, v_pages, cu_seqlens, block_tables, table_lens, max_seq_len, scale, out, return_lse)
+// attend(q, k_pages, v_pages, cu_seqlens, block_tables, table_lens, max_seq_len, scale, out, return_lse,
+//        kv_scales)
 //   -> out, or (out, lse)
 PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t count) {
   return guarded([&]() -> PyObject * {
-    if (count != 10) type_error("attend takes 10 arguments");
+    if (count != 11) type_error("attend takes 11 arguments");
     const Tensor &q = tensor(a[0], "q");
-    const Pages pages(tensor(a[1], "k_pages"), tensor(a[2], "v_pages"));
-    const Tensor &cu = tensor(a[3], "cu_seqlens"), &tables = tensor(a[4], "block_tables");
-    const Tensor *lens = maybe(a[5], "table_lens"), *out = maybe(a[8], "out");
-    const int64_t max_seq_len = integer(a[6]);
+    const PairOfScales scales(a[10]);
+    const Pages pages(tensor(a[1], "k_pages"), tensor(a[2], "v_pages"), static_cast<bool>(scales));
+    const Sequences seqs(a[3], a[4], a[5], a[6]);
+    const Tensor *out = maybe(a[8], "out");
     const int wanted = PyObject_IsTrue(a[9]);
     if (wanted < 0) throw Raised{nullptr, ""};
     const bool return_lse = wanted == 1;
-    const int64_t n = cu.numel() - 1, hd = pages.hd;
+    const int64_t n = seqs.n, hd = pages.hd;
     double scale = 1.0 / std::sqrt(static_cast<double>(hd > 0 ? hd : 1));
     if (a[7] != Py_None) {
       scale = PyFloat_AsDouble(a[7]);
@@ -381,34 +481,25 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t count) {
     }
     rows_of(q, "q", n, -1, hd);
     const int64_t heads = q.size(1);
-    if (q.scalar_type() != pages.k.scalar_type())
+    scales.check(pages);
+    const int q_code = dtype_code(q.scalar_type());
+    if (!scales && q.scalar_type() != pages.k.scalar_type())
       type_error(std::string("q is ") + dtype_name(q.scalar_type()) + ", the pages are " +
                  dtype_name(pages.k.scalar_type()));
     if (hd > 256) value_error("head_dim " + std::to_string(hd) + " is above 256");
     if (heads == 0 || pages.heads == 0 || heads % pages.heads || heads > INT32_MAX)
       value_error(std::to_string(heads) + " query heads do not share " + std::to_string(pages.heads) +
                   " KV heads evenly");
-    if (tables.dim() == 2 && tables.size(0) < n)
-      value_error("block_tables has " + std::to_string(tables.size(0)) + " rows for " + std::to_string(n) +
-                  " sequences");
-    // without table_lens a row has as many entries as lie between two rows (SeqBatchTensors lays its tables out so)
-    if (!lens && tables.dim() == 2 && tables.numel() > 0 && tables.stride(0) != tables.size(1))
-      value_error("block_tables without table_lens must have rows that follow one another");
-    if (lens && (lens->numel() < n || !lens->is_contiguous()))
-      value_error("table_lens must be a contiguous vector of " + std::to_string(n));
-    if (!cu.is_contiguous()) value_error("cu_seqlens must be a contiguous vector");
-    if (max_seq_len < 0 || max_seq_len > INT32_MAX) value_error("max_seq_len must be in [0, 2**31)");
+    seqs.check_shapes();
     if (out) {
       rows_of(*out, "out", n, heads, hd);
       if (out->scalar_type() != q.scalar_type()) type_error("out must have q's dtype");
       written(*out, "out", &q, "q");
     }
     const Place at_("paged_decode_attention", q);
-    at_.also(&pages.k), at_.also(&pages.v), at_.also(&cu), at_.also(&tables), at_.also(lens), at_.also(out);
-    if (cu.scalar_type() != at::kInt || tables.scalar_type() != at::kInt || (lens && lens->scalar_type() != at::kInt))
-      type_error("sequence metadata must be int32");
-    if (tables.dim() != 2 || (tables.stride(1) != 1 && tables.size(1) > 1))
-      value_error("block_tables must be a row-major [n_seqs, max_blocks] int32 tensor");
+    at_.also(&pages.k), at_.also(&pages.v), at_.also(&seqs.cu), at_.also(&seqs.tables), at_.also(seqs.lens), at_.also(out);
+    at_.also(scales.k), at_.also(scales.v);
+    seqs.check_types();
     const c10::DeviceGuard guard(at_.device);
     Tensor made, lse, workspace;
     if (!out) made = fresh_like(q), out = &made;
@@ -418,13 +509,7 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t count) {
     p.q_stride_seq = q.stride(0), p.q_stride_head = q.stride(1);
     p.n_q_heads = static_cast<int32_t>(heads);
     p.scale = static_cast<float>(scale);
-    p.seqs.cu_seqlens = cu.data_ptr<int32_t>();
-    p.seqs.block_tables = tables.data_ptr<int32_t>();
-    p.seqs.table_lens = static_cast<int32_t *>(ptr(lens));
-    p.seqs.positions = nullptr;
-    p.seqs.table_stride = tables.stride(0);
-    p.seqs.n_seqs = static_cast<int32_t>(n);
-    p.seqs.max_seq_len = static_cast<int32_t>(max_seq_len);
+    p.seqs = seqs.describe();
     p.k_pages = describe(pages.k, pages.code), p.v_pages = describe(pages.v, pages.code);
     p.out = out->data_ptr();
     p.out_stride_seq = out->stride(0), p.out_stride_head = out->stride(1);
@@ -432,12 +517,20 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t count) {
     p.workspace = nullptr, p.workspace_bytes = 0;
     p.status = at_.status();
     int64_t bytes = 0;
-    check(g_workspace(&p, &bytes), "dkv_paged_decode_workspace_bytes");
+    if (scales)
+      check(g_workspace_quant(&p, q_code, &bytes), "dkv_paged_decode_quant_workspace_bytes");
+    else
+      check(g_workspace(&p, &bytes), "dkv_paged_decode_workspace_bytes");
     if (bytes > 0) {  // in stream order the allocator may give it away once the launches are queued
       workspace = fresh_tensor({bytes}, at::kByte, at_.device);
       p.workspace = workspace.data_ptr(), p.workspace_bytes = bytes;
     }
-    check(g_attend(&p, at_.stream()), "dkv_paged_decode_attention");
+    if (scales) {
+      const dkv_page_scales ks = describe_scales(*scales.k), vs = describe_scales(*scales.v);
+      check(g_attend_quant(&p, q_code, &ks, &vs, at_.stream()), "dkv_paged_decode_attention_quant");
+    } else {
+      check(g_attend(&p, at_.stream()), "dkv_paged_decode_attention");
+    }
     PyObject *first;
     if (made.defined()) {
       first = THPVariable_Wrap(made);
@@ -450,12 +543,86 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t count) {
   });
 }
 
-// bind(plan, append, workspace, attend, raise_error, status_word): entry addresses and callbacks
+// 8-bit pages of K or V, [num_blocks, block_size, heads, head_dim], and their scales
+void check_coded(const Tensor &pages, const Tensor &scales) {
+  if (pages.dim() != 4) value_error("unsupported paged KV layout " + shape_text(pages));
+  if (!is_code(pages.scalar_type()))
+    type_error(std::string("page_scales go with 8-bit pages (float8_e4m3fn or int8), not ") + dtype_name(pages.scalar_type()));
+  if (pages.stride(3) != 1 && pages.size(3) > 1) value_error("paged cache head_dim must be contiguous");
+  if (pages.size(1) > 1024) value_error("8-bit pages have at most 1024 slots a block");
+  if (pages.size(2) > INT32_MAX || pages.size(3) > INT32_MAX) value_error("paged cache too large");
+  scales_of(scales, "page_scales", pages);
+}
+
+// scatter(delta, pages, page_scales, cu_seqlens, block_tables, table_lens, max_seq_len)
+PyObject *scatter(PyObject *, PyObject *const *a, Py_ssize_t count) {
+  return guarded([&]() -> PyObject * {
+    if (count != 7) type_error("scatter takes 7 arguments");
+    const Tensor &delta = tensor(a[0], "delta"), &pages = tensor(a[1], "pages"), &scales = tensor(a[2], "page_scales");
+    const Sequences seqs(a[3], a[4], a[5], a[6]);
+    check_coded(pages, scales);
+    if (delta.dim() != 3) value_error("delta " + shape_text(delta) + " must be [rows, heads, head_dim]");
+    rows_of(delta, "delta", delta.size(0), pages.size(2), pages.size(3));
+    const int code = dtype_code(delta.scalar_type());
+    seqs.check_shapes();
+    written(pages, "pages", nullptr, ""), written(scales, "page_scales", nullptr, "");
+    const Place at_("scatter_into_paged_batched", pages);
+    at_.also(&delta), at_.also(&scales), at_.also(&seqs.cu), at_.also(&seqs.tables), at_.also(seqs.lens);
+    seqs.check_types();
+    const c10::DeviceGuard guard(at_.device);
+    const dkv_paged_cache cache = describe(pages, code_of(pages.scalar_type()));
+    const dkv_page_scales s = describe_scales(scales);
+    const dkv_seq_batch q = seqs.describe();
+    check(g_scatter_quant(delta.data_ptr(), code, delta.size(0), delta.stride(0), delta.stride(1), &cache, &s, &q,
+                          at_.status(), at_.stream()),
+          "dkv_scatter_paged_quant");
+    Py_RETURN_NONE;
+  });
+}
+
+// gather(pages, page_scales, cu_seqlens, block_tables, table_lens, max_seq_len, rows, like, out) -> out
+// like: a tensor of the type that a new out gets
+PyObject *gather(PyObject *, PyObject *const *a, Py_ssize_t count) {
+  return guarded([&]() -> PyObject * {
+    if (count != 9) type_error("gather takes 9 arguments");
+    const Tensor &pages = tensor(a[0], "pages"), &scales = tensor(a[1], "page_scales");
+    const Sequences seqs(a[2], a[3], a[4], a[5]);
+    const int64_t rows = integer(a[6]);
+    const Tensor *out = maybe(a[8], "out");
+    check_coded(pages, scales);
+    if (rows < 0) value_error("rows must not be negative");
+    if (out) {
+      rows_of(*out, "out", rows, pages.size(2), pages.size(3));
+      written(*out, "out", nullptr, "");
+    }
+    const at::ScalarType type = out ? out->scalar_type() : tensor(a[7], "like").scalar_type();
+    const int code = dtype_code(type);
+    seqs.check_shapes();
+    const Place at_("gather_from_paged_batched", pages);
+    at_.also(&scales), at_.also(&seqs.cu), at_.also(&seqs.tables), at_.also(seqs.lens), at_.also(out);
+    seqs.check_types();
+    const c10::DeviceGuard guard(at_.device);
+    Tensor made;
+    if (!out) made = fresh_tensor({rows, pages.size(2), pages.size(3)}, type, at_.device), out = &made;
+    const dkv_paged_cache cache = describe(pages, code_of(pages.scalar_type()));
+    const dkv_page_scales s = describe_scales(scales);
+    const dkv_seq_batch q = seqs.describe();
+    check(g_gather_quant(&cache, &s, &q, out->data_ptr(), code, rows, out->stride(0), out->stride(1), made.defined(),
+                         at_.status(), at_.stream()),
+          "dkv_gather_paged_quant");
+    if (made.defined()) return THPVariable_Wrap(made);
+    Py_INCREF(a[8]);
+    return a[8];
+  });
+}
+
+// bind(plan, append, workspace, attend, append_quant, scatter_quant, gather_quant, workspace_quant, attend_quant, raise_error,
+//      status_word): entry addresses and callbacks
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t count) {
   return guarded([&]() -> PyObject * {
-    if (count != 6) type_error("bind takes 6 arguments");
-    void *entry[4];
-    for (int i = 0; i < 4; ++i) {
+    if (count != 11) type_error("bind takes 11 arguments");
+    void *entry[9];
+    for (int i = 0; i < 9; ++i) {
       entry[i] = PyLong_AsVoidPtr(a[i]);
       if (entry[i] == nullptr) {
         if (PyErr_Occurred()) throw Raised{nullptr, ""};
@@ -466,10 +633,15 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t count) {
     g_append = reinterpret_cast<decltype(g_append)>(entry[1]);
     g_workspace = reinterpret_cast<decltype(g_workspace)>(entry[2]);
     g_attend = reinterpret_cast<decltype(g_attend)>(entry[3]);
-    Py_INCREF(a[4]);
-    Py_XSETREF(g_raise, a[4]);
-    Py_INCREF(a[5]);
-    Py_XSETREF(g_status_word, a[5]);
+    g_append_quant = reinterpret_cast<decltype(g_append_quant)>(entry[4]);
+    g_scatter_quant = reinterpret_cast<decltype(g_scatter_quant)>(entry[5]);
+    g_gather_quant = reinterpret_cast<decltype(g_gather_quant)>(entry[6]);
+    g_workspace_quant = reinterpret_cast<decltype(g_workspace_quant)>(entry[7]);
+    g_attend_quant = reinterpret_cast<decltype(g_attend_quant)>(entry[8]);
+    Py_INCREF(a[9]);
+    Py_XSETREF(g_raise, a[9]);
+    Py_INCREF(a[10]);
+    Py_XSETREF(g_status_word, a[10]);
     Py_RETURN_NONE;
   });
 }
@@ -480,6 +652,8 @@ PyMethodDef kMethods[] = {
     {"rope_ready", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope_ready)), METH_FASTCALL, nullptr},
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
     {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend)), METH_FASTCALL, nullptr},
+    {"scatter", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(scatter)), METH_FASTCALL, nullptr},
+    {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gather)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_step", "Host side of the paged step operators.", -1, kMethods};
 

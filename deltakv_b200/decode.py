@@ -33,7 +33,7 @@ from torch import Tensor
 
 from deltakv_b200 import _lib as L
 from deltakv_b200 import ops
-from deltakv_b200.rope import half_tables
+from deltakv_b200.rope import RotaryEmbedding, half_tables
 
 _native_module = None
 
@@ -60,8 +60,10 @@ def _native():
             raise ImportError("_step.so is not built; run `python -m deltakv_b200.build` "
                               "(the CUDA path has no fallback)") from e
         lib = L.lib()
-        entries = (lib.dkv_plan_paged_step, lib.dkv_append_paged, lib.dkv_paged_decode_workspace_bytes,
-                   lib.dkv_paged_decode_attention)
+        entries = (lib.dkv_plan_paged_step, lib.dkv_append_paged_rotary, lib.dkv_paged_decode_workspace_bytes,
+                   lib.dkv_paged_decode_attention, lib.dkv_append_paged_quant, lib.dkv_scatter_paged_quant,
+                   lib.dkv_gather_paged_quant, lib.dkv_paged_decode_quant_workspace_bytes,
+                   lib.dkv_paged_decode_attention_quant)
         module.bind(*(C.cast(f, C.c_void_p).value for f in entries), _raise_error, _status_address)
         _native_module = module
     return _native_module
@@ -106,7 +108,8 @@ def plan_paged_step(lengths: Tensor, block_tables: Tensor, block_size: int, *, r
 
 def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slots: Tensor, *,
                       q: Tensor | None = None, positions: Tensor | None = None, rope=None,
-                      q_out: Tensor | None = None, check: bool = False) -> Tensor | None:
+                      q_out: Tensor | None = None, check: bool = False, rotary_dim: int | None = None,
+                      interleaved: bool | None = None, kv_scales: tuple[Tensor, Tensor] | None = None) -> Tensor | None:
     """Store this step's ``k`` and ``v [rows, n_kv, head_dim]`` in their ``slots``, rotated.
 
     ``slots`` (int64) and ``positions`` (int32) are a :class:`PagedStep`'s; a negative slot
@@ -120,6 +123,20 @@ def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, sl
     distinct, and the K pages, the V pages, ``q_out`` and the inputs other than ``q`` apart in memory.
     ``check=True`` raises recorded range errors (a slot beyond the pages, a position
     beyond the tables: those rows store nothing).
+
+    ``rotary_dim`` turns only the first columns of each head (tables of half that width), and
+    ``interleaved`` the pairs ``(2i, 2i + 1)`` instead of ``(i, i + rotary_dim / 2)``.  A
+    :class:`~deltakv_b200.rope.RotaryEmbedding` made with them brings its own; they are for pairs of tables.
+
+    **8-bit pages** (``torch.float8_e4m3fn`` or ``torch.int8``, at most 1024 slots a block) come with
+    ``kv_scales = (k_scales, v_scales)``, fp32 ``[num_blocks, n_kv]``: a slot's value is its code times its block's and
+    head's scale.  The operator keeps them: storing a block's slot 0 begins the block with the scale that this call's
+    values need (e4m3: the least power of two; int8: the largest magnitude / 127), and nothing the block held
+    is kept; later values that do not fit make the scale grow by powers of two, and what the block holds is rounded to the
+    new one (int8: by less than one step in all; e4m3: not at all above its subnormals).  So codes and scales may start as any memory.
+    Rows may be fp32, fp16 or bf16, and the rows of one block follow one another
+    (as :func:`plan_paged_step` lays them out).  A value that is not finite makes the block's head read as NaN until
+    the block is begun anew.
     """
     native = _native_module or _native()
     cos = sin = None
@@ -127,8 +144,11 @@ def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, sl
         if type(rope) is tuple and native.rope_ready(*rope, k):
             cos, sin = rope
         else:
-            cos, sin = half_tables(rope, k.device)
-    q_out = native.append(k, v, k_pages, v_pages, slots, q, positions, cos, sin, q_out)
+            cos, sin = half_tables(rope, k.device, forms=True)
+            if isinstance(rope, RotaryEmbedding):
+                rotary_dim, interleaved = rope.form(k.shape[-1], rotary_dim, interleaved)
+    q_out = native.append(k, v, k_pages, v_pages, slots, q, positions, cos, sin, q_out, rotary_dim,
+                          interleaved or False, kv_scales)
     if check:
         ops.status_word(k.device).raise_if_set("append_into_paged")
     return q_out
@@ -136,7 +156,8 @@ def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, sl
 
 def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: ops.SeqBatchTensors, *,
                            scale: float | None = None, out: Tensor | None = None, return_lse: bool = False,
-                           check: bool = False) -> Tensor | tuple[Tensor, Tensor]:
+                           check: bool = False,
+                           kv_scales: tuple[Tensor, Tensor] | None = None) -> Tensor | tuple[Tensor, Tensor]:
     """``softmax(scale * q K^T) V`` of one query token per sequence over its cached tokens.
 
     ``q [n_seqs, n_q, head_dim]`` in the pages' dtype; query head ``h`` reads KV head
@@ -157,9 +178,15 @@ def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: op
     also where the token's weight is below 2^-126 of the largest and so 0 in fp32).  Tokens
     in blocks outside the cache or beyond the table are left out and recorded (``check=True``
     raises).
+
+    **8-bit pages** (``torch.float8_e4m3fn`` or ``torch.int8``) come with ``kv_scales = (k_scales, v_scales)``, fp32
+    ``[num_blocks, n_kv]``, one factor for each block and KV head — those that :func:`append_into_paged` keeps, or any.  ``q``
+    then is bf16, fp16 or fp32 and ``out`` has its type; products are fp16 with fp32 sums, in which the codes and a 16-bit ``q``
+    are exact; fp32 ``q`` and the weights enter as two terms each (the weights of bf16 ``q`` as one, rounded to 2^-11).
+    A NaN code or scale of a token that counts gives NaN.
     """
     got = (_native_module or _native()).attend(q, k_pages, v_pages, seqs.cu_seqlens, seqs.block_tables, seqs.table_lens,
-                                               seqs.max_seq_len, scale, out, return_lse)
+                                               seqs.max_seq_len, scale, out, return_lse, kv_scales)
     if check:
         ops.status_word(q.device).raise_if_set("paged_decode_attention")
     return got

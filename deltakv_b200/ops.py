@@ -297,6 +297,12 @@ def pack_factors(geom: L.ExactGeometry, a_k: torch.Tensor | None, b_k: torch.Ten
     return out
 
 
+def _check_rope(cos: torch.Tensor | None, sin: torch.Tensor | None, head_dim: int) -> None:
+    """Whole heads in halves: the kernels read head_dim / 2 angles a position."""
+    if cos is not None and (cos.ndim != 2 or cos.shape != sin.shape or 2 * cos.shape[1] != head_dim):
+        raise ValueError(f"rope tables {tuple(cos.shape)} do not cover head_dim {head_dim}")
+
+
 def exact_patch_paged(geom: L.ExactGeometry, x: torch.Tensor, packed: torch.Tensor,
                       k_pages: Sequence[torch.Tensor], v_pages: Sequence[torch.Tensor],
                       seqs: SeqBatchTensors, *, x_scale: torch.Tensor | None = None,
@@ -324,6 +330,7 @@ def exact_patch_paged(geom: L.ExactGeometry, x: torch.Tensor, packed: torch.Tens
     _require_cuda(x3, packed, x_scale, rope_cos, rope_sin, x_sumsq)
     if x3.stride(2) != 1:
         raise ValueError("x rows must be contiguous")
+    _check_rope(rope_cos, rope_sin, geom.head_dim)
     xs = None
     if x_scale is not None:
         xs = x_scale if x_scale.ndim == 2 else x_scale.unsqueeze(0)
@@ -451,6 +458,7 @@ def dense_patch_paged(geom: L.DenseGeometry, x: torch.Tensor, packed: torch.Tens
     _require_cuda(x3, p3, x_scale, rope_cos, rope_sin)
     if x3.stride(2) != 1 or p3.stride(2) != 1:
         raise ValueError("x and packed rows must be contiguous")
+    _check_rope(rope_cos, rope_sin, geom.head_dim)
     xs = None
     if x_scale is not None:
         xs = x_scale if x_scale.ndim == 2 else x_scale.unsqueeze(0)

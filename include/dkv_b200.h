@@ -61,6 +61,7 @@ typedef struct CUstream_st *dkv_stream_t;
 #define DKV_E4M3 3 /* float8 e4m3fn */
 #define DKV_I32 4
 #define DKV_U8 5
+#define DKV_I8 6
 
 /* Upper bound on layers covered by one dkv_exact_patch_paged launch. */
 #define DKV_MAX_LAYERS 128
@@ -668,6 +669,69 @@ typedef struct dkv_paged_decode_args {
 
 int dkv_paged_decode_workspace_bytes(const dkv_paged_decode_args *args, int64_t *bytes);
 int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv_stream_t stream);
+
+/*
+ * Other rotary forms of dkv_append_paged: the first dim columns of a head turn (even, up to head_dim; the tables are
+ * [rope_max_pos, dim/2]), in pairs (i, i + dim/2), or (2i, 2i + 1) where interleaved; the rest stays.  rotary NULL:
+ * dim = head_dim, pairs (i, i + dim/2).
+ */
+typedef struct dkv_rotary {
+  int32_t dim;
+  int32_t interleaved;
+} dkv_rotary;
+
+int dkv_append_paged_rotary(const dkv_append_args *args, const dkv_rotary *rotary, dkv_stream_t stream);
+
+/* ---- an 8-bit paged cache ----------------------------------------------------------- */
+
+/*
+ * The scales of K or V pages of 8-bit codes (dtype DKV_E4M3 or DKV_I8, block_size at most 1024): the value of a slot
+ * is its code times base[block * stride_block + head * stride_head] (fp32, strides in elements).  What reads takes any scales; what writes
+ * chooses them.  Of a block and head of which nothing is kept, with amax the largest magnitude stored:
+ *   e4m3: the least power of two s with amax <= 448 s;  int8: s = amax / 127;  not below 2^-126, 0 for amax = 0.
+ * Of one that holds others: s 2^j with the least j >= 0 that gives amax <= 448 s 2^j (e4m3) or 127.5 s 2^j (int8); where j > 0 the
+ * codes kept are rounded again.  Codes are the nearest to value * (1 / s), ties to even.  A value that is not finite makes the scale
+ * NaN, so that all of the block's head reads as NaN until it is begun anew.
+ */
+typedef struct dkv_page_scales {
+  float *base;
+  int64_t stride_block, stride_head;
+} dkv_page_scales;
+
+/*
+ * dkv_append_paged_rotary into 8-bit pages: in_dtype is F32, F16 or BF16 whatever the pages.  Storing a block's slot 0
+ * begins the block: nothing that it held is kept.  The rows of one block follow one another (as
+ * dkv_plan_paged_step lays them out); slots are distinct.
+ */
+int dkv_append_paged_quant(const dkv_append_args *args, const dkv_rotary *rotary, const dkv_page_scales *k_scales,
+                           const dkv_page_scales *v_scales, dkv_stream_t stream);
+
+/*
+ * Row r of delta [n_rows, heads, head_dim] (rows follow cu_seqlens) is added to the value of its slot, in fp32 and rounded
+ * after the product and after the sum, and the blocks are quantised again: one that is covered whole with a scale of its own,
+ * of another the slots behind the sequence's end are kept.  No block belongs to two sequences.  Rows past n_rows are left out (INVALID_ARGUMENT in
+ * *status), as are those without a block (BLOCK_TABLE_SHORT, PAGE_RANGE).
+ */
+int dkv_scatter_paged_quant(const void *delta, int32_t delta_dtype, int64_t n_rows, int64_t delta_stride_row,
+                            int64_t delta_stride_head, const dkv_paged_cache *cache, const dkv_page_scales *scales,
+                            const dkv_seq_batch *seqs, int32_t *status, dkv_stream_t stream);
+
+/*
+ * The values of every sequence's rows into out [n_rows, heads, head_dim] (F32, F16 or BF16, rounded once).  Rows without
+ * a block become zero (and are recorded); rows behind the last sequence become zero where zero_rest, else they are left.
+ */
+int dkv_gather_paged_quant(const dkv_paged_cache *cache, const dkv_page_scales *scales, const dkv_seq_batch *seqs, void *out,
+                           int32_t out_dtype, int64_t n_rows, int64_t out_stride_row, int64_t out_stride_head,
+                           int32_t zero_rest, int32_t *status, dkv_stream_t stream);
+
+/*
+ * dkv_paged_decode_attention over 8-bit pages (any block_size), q and out of q_dtype (F32, F16 or BF16).  Scores and weights go through
+ * the tensor cores as f16 products with fp32 sums: q of 16 bits exactly (scaled by a power of two), fp32 q as two f16 terms; a
+ * weight as two f16 terms, as one (rounded, at most 2^-11 of it) for bf16 q.  A code or a scale that is NaN gives NaN.
+ */
+int dkv_paged_decode_quant_workspace_bytes(const dkv_paged_decode_args *args, int32_t q_dtype, int64_t *bytes);
+int dkv_paged_decode_attention_quant(const dkv_paged_decode_args *args, int32_t q_dtype, const dkv_page_scales *k_scales,
+                                     const dkv_page_scales *v_scales, dkv_stream_t stream);
 
 #ifdef __cplusplus
 } /* extern "C" */
