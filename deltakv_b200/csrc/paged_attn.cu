@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(W * 32, 1) simt_kernel(const __grid_constant__
   Window win;
   if (!p.local) {
     win.look(p, lane);
-    ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
+    ln = line_of(p, p.cu[p.n_seqs]);
     if (r >= static_cast<int>(ln.ranges)) return;
   }
   const int u = unit / p.chunks, chunk = unit - u * p.chunks;
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
   Window win;
   if (!p.local) {
     win.look(p, lane);
-    ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
+    ln = line_of(p, p.cu[p.n_seqs]);
     if (r >= static_cast<int>(ln.ranges)) return;
   }
   const int u = unit / p.chunks, chunk = unit - u * p.chunks;
@@ -517,8 +517,8 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
       const float sum[2] = {sum_of(0), sum_of(1)};
       if (!all_finite()) {
         const int first = p.cu[b], len = max(p.cu[b + 1] - first, 0);
-        const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
-        infinite_columns<DT>(p, o, sum, h0 / p.group, b, border(stream.w.x0, at, len), border(stream.w.x1, at, len), kTile,
+        const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(p.seq_cost) * b;
+        infinite_columns<DT>(p, o, sum, h0 / p.group, b, border(p, stream.w.x0, at, len), border(p, stream.w.x1, at, len), kTile,
                              g, t);
       }
       if (whole) {
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   __shared__ int seen[4];  // cu_seqlens at n_seqs, the sequence (-1: no such border), its start and end
   if (warp == 0) {
     const int tokens = Early::cu_at(p, p.n_seqs);
-    const Line ln = line_of(tokens, p.n_seqs, p.ranges);
+    const Line ln = line_of(p, tokens);
     const uint32_t rb = blockIdx.x + 1;
     int b = blockIdx.x, first = 0, next = 0;
     if (by_seq) {
@@ -670,25 +670,25 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
       b = win.find(p, ln.start(rb), lane);
       win.need(p, b, lane);
       first = win.at(b), next = win.at(b + 1);
-      const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
+      const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(p.seq_cost) * b;
       if (rb > 1 && ln.start(rb - 1) >= at) b = -1;  // an earlier border has this sequence
     }
     if (lane == 0) seen[0] = tokens, seen[1] = b, seen[2] = first, seen[3] = next;
   }
   __syncthreads();
-  const Line ln = line_of(seen[0], p.n_seqs, p.ranges);
+  const Line ln = line_of(p, seen[0]);
   const int b = seen[1], first = seen[2], next = seen[3];
   if (b < 0) return;
   const int len = max(next - first, 0);
   if (len == 0) return;
-  const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * b;
+  const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(p.seq_cost) * b;
   // the ranges with a part: a range is at least two tiles wide, so only those at the ends of the
   // sequence and of its virtual tokens can have none
   // (the bound changes nothing for lengths that are prefix sums; it keeps any others within the parts)
   const uint32_t last = ln.ranges - 1;
-  uint32_t r0 = min(ln.owner(at), last), r1 = min(ln.owner(at + len + kSeqCost - 1), last);
-  while (r0 < r1 && border(ln.start(r0 + 1), at, len) == 0) ++r0;
-  while (r0 < r1 && border(ln.start(r1), at, len) == len) --r1;
+  uint32_t r0 = min(ln.owner(at), last), r1 = min(ln.owner(at + len + p.seq_cost - 1), last);
+  while (r0 < r1 && border(p, ln.start(r0 + 1), at, len) == 0) ++r0;
+  while (r0 < r1 && border(p, ln.start(r1), at, len) == len) --r1;
   if (r1 == r0) return;  // not cut: written by its warp
   const int n = r1 - r0 + 1;
   // part i of head h: slots as the walk numbers them, [range][unit][0, or 1 for the first part][head]
@@ -839,7 +839,7 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   const bool f32 = a->k_pages.dtype == DKV_F32;
   s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
   s->g = f32 && group <= 4 ? 4 : 8;
-  return cut_up(*a, variant(f32, s->hd_pad, s->g), s);
+  return cut_up(*a, variant(f32, s->hd_pad, s->g), kSeqCost, s);
 }
 
 template <int HD, int G, int W, int kStages, int kTok>

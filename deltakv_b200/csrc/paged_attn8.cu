@@ -13,8 +13,9 @@ int check8(const dkv_paged_decode_args *a, int q_dtype) {
 int shape8(const dkv_paged_decode_args *a, int q_dtype, Shape *s) {
   const int hd = a->k_pages.head_dim;
   s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-  s->g = 8;
-  return cut_up(*a, variant8(q_dtype == DKV_F32, s->hd_pad), s);
+  const bool f32 = q_dtype == DKV_F32;
+  s->g = heads8(f32, s->hd_pad, a->n_q_heads / a->k_pages.n_heads);
+  return cut_up(*a, variant8(f32, s->hd_pad, s->g), kSeqCost8, s);
 }
 
 }  // namespace pattn
@@ -54,7 +55,19 @@ extern "C" int dkv_paged_decode_attention_quant(const dkv_paged_decode_args *arg
   pattn::Params p;
   pattn::fill_params(a, s, 1, q_dtype == DKV_F32 ? 4 : 2, &p);
   p.k_scale = k_scales->base, p.ks_block = k_scales->stride_block, p.ks_head = k_scales->stride_head;
+  // a tile's halves are copied as pages where each lies in one block
+  if (p.copy == pattn::kRows && k.block_size % pattn::kTile == 0) p.copy = pattn::kPages;
+  // copies of pages step through a block's rows with 32-bit strides, and reach blocks by 32 bits of 16 bytes; scales go by 32
+  // bits as well
+  auto reach = [](int64_t blocks, int64_t block, int64_t slots, int64_t slot) {
+    return block >= 0 && slot >= 0 && (blocks == 0 || (blocks - 1) * block + (slots - 1) * slot < (int64_t{1} << 36));
+  };
+  if (p.copy == pattn::kPages &&
+      (p.k_slot > INT32_MAX || p.v_slot > INT32_MAX || !reach(p.num_blocks, p.k_block, k.block_size, p.k_slot) ||
+       !reach(p.num_blocks, p.v_block, k.block_size, p.v_slot)))
+    p.copy = pattn::kRows;
   p.v_scale = v_scales->base, p.vs_block = v_scales->stride_block, p.vs_head = v_scales->stride_head;
+  if (p.ks_block < 0 || p.vs_block < 0 || p.ks_block > UINT32_MAX || p.vs_block > UINT32_MAX) return DKV_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return k.dtype == DKV_I8 ? pattn::launch8_int8(q_dtype, p, s, st) : pattn::launch8<DKV_E4M3>(q_dtype, p, s, st);
 }

@@ -6,9 +6,11 @@
 // over the codes themselves: every e4m3 and int8 code is an f16 number, and
 //   S^T [16 tokens x 8 heads] = C . Q^T,   O^T [16 columns x 8 heads] += D^T . W^T,   W_i = exp(s_i - m) v_i
 // are mma.m16n8k16 in f16 with the tokens (columns) on the wide side, as in the 16-bit walk.  The weights W take V's
-// scales, which differ from block to block, so they have a running maximum of their own: M = max_i (s_i + log2 of v_i's
-// power of two) keeps the largest W between 1 and 2, as m keeps the largest exp(s_i - m) at 1; O is in units of
-// 2^M and l of 2^m until a piece ends.
+// scales, which differ from block to block, so they have a factor 2^up of their own that keeps the largest of them not far
+// below 2^8 and all below 2^15 (f16 ends at 2^16): it moves, and O with it, when a scale could lift a weight past that, as m
+// does when a score passes it.  m is set 4 above the largest score (a factor of 16), and 2^up so that scales of four times those
+// of the heaviest tokens fit: otherwise half of the tiles of a range of a few hundred tokens had one to move.  What an
+// f16 weight loses at least is then 2^-25 of 2^8, 2^-33 of the largest weight.
 //
 // Bytes to fragments: a lane's ldmatrix register holds four codes of one token's row, which become the k-indices
 // (2t, 2t + 1) and (2t + 8, 2t + 9) of one product (any order of the head's columns gives the same score, as long as
@@ -39,7 +41,9 @@ template <>
 struct Pairs<DKV_E4M3> {
   // bytes 0, 1 and bytes 2, 3
   static __device__ __forceinline__ void in_order(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    lo = e4m3x2_to_f16x2(w), hi = e4m3x2_to_f16x2(w >> 16);
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
   }
   // bytes 0, 2 and bytes 1, 3
   static __device__ __forceinline__ void crossed(uint32_t w, uint32_t &even, uint32_t &odd) {
@@ -58,30 +62,209 @@ struct Pairs<DKV_I8> {  // a byte b behind 0x64 is the f16 number 1024 + b; with
   }
 };
 
+// (no side effects: left to the compiler's scheduler, not volatile)
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 
-// Weights carry 2^13: they reach down to 2^-27 of the largest with all 11 bits, and stay below 2^15 in f16.
-constexpr float kWeightBias = 13.f;
+// One warp's stream of tiles of 32 tokens into its ring: a stage holds 32 rows of K, as many of V (16 bytes more than a row
+// apart: no bank conflicts), their scales and its description.  Two ways to copy:
+//   kPages  block_size a multiple of 16: each half of a tile lies in one block (borders fall on multiples of 16), its rows a
+//           fixed stride apart.  A lane holds the addresses of one of the next 32 halves, so that the table is waited
+//           for, and addresses are worked out, once in 16 tiles;
+//   kRows, kPlain  a lane for each token's block and slot, a tile ahead; rows in pieces of 16 bytes, or smaller ones.
+template <int HD, int kStages, typename O>
+struct Stream8 {
+  static constexpr int kTok = 32;
+  static constexpr int kRow = HD + 16;
+  static constexpr int kSide = kTok * kRow;
+  static constexpr int kStage = 2 * kSide + 2 * kTok * 4;  // K, V, K's scales, V's
+  static constexpr int kBytes = kStages * (kStage + 16);   // the stages' descriptions behind them
+  static constexpr int kPieces = HD / 16;                  // 16-byte pieces of a row
+  static constexpr int kAtOnce = 32 / kPieces;             // rows a copy instruction covers
 
-template <int DT, int HD, int kStages>
-struct Walk8 {
-  using O = typename Elem<DT>::T;
-  using S = Stream<uint8_t, HD, kStages, kTile, O, true>;
+  const Params &p;
+  Walk w;
+  char *ring;
+  uint4 *meta;  // per stage: sequence, flags, bit per token that takes part, end of the stream
+  const char *k, *v;    // kPages: this lane's row and piece of slot 0 of block 0; else the side's base
+  const float *ks, *vs;
+  uint32_t to;          // kPages: where this lane's first piece goes in stage 0
+  bool inside;          // this lane's piece is not past head_dim
+  int h0, n_h, lane;
+  uint64_t k_at, v_at;  // the row of this lane's token (0: none); kPages: the half it looked up, in units of 16 bytes from k, v
+  int id;               // its block, negative: none
+  int tile;             // kPages: of the 16 tiles that the lanes hold, the next
+  static constexpr int kNoRow = -1, kShort = INT32_MIN;
+
+  __device__ __forceinline__ Stream8(const Params &p_, char *mine, int u, int h0_, int n_h_, int lane_)
+      : p(p_), ring(mine), meta(reinterpret_cast<uint4 *>(mine + kStages * kStage)), k(p_.k + u * p_.k_head),
+        v(p_.v + u * p_.v_head), ks(p_.k_scale + u * p_.ks_head), vs(p_.v_scale + u * p_.vs_head), h0(h0_), n_h(n_h_),
+        lane(lane_), k_at(0), v_at(0), id(kNoRow), tile(0) {
+    const int row = lane / kPieces, piece = lane % kPieces;
+    to = smem_u32(ring) + row * kRow + piece * 16;
+    inside = piece * 16 < p.hd;
+    if (p.copy == kPages) k += row * p.k_slot + piece * 16, v += row * p.v_slot + piece * 16;
+    if (p.hd < HD) {  // columns past head_dim stay zero in every stage: only zeros are written there again
+      for (int i = lane; i < kStages * kStage / 16; i += 32) reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+    }
+  }
+  __device__ __forceinline__ float *scales(int s) const { return reinterpret_cast<float *>(ring + s * kStage + 2 * kSide); }
+  __device__ __forceinline__ void look_up() {
+    if (!w.live) return;
+    int ahead = lane;
+    if (p.copy == kPages) {
+      if (++tile < 16 && !(w.flags & kFirst)) return;
+      tile = 0;
+      ahead = (lane >> 1) * w.step + (lane & 1) * 16;
+    }
+    k_at = v_at = 0, id = kNoRow;
+    if (ahead >= w.end - w.i) return;
+    const int i = w.i + ahead;
+    const int blk = static_cast<int>((static_cast<uint64_t>(i) * p.div_mul) >> p.div_shift);
+    id = blk < w.tlen ? max(p.tables[w.b * p.table_stride + blk], kNoRow) : kShort;
+    if (id < 0 || id >= p.num_blocks) {
+      record_error(p.status, id == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
+      id = kNoRow;
+      return;
+    }
+    const int slot = i - blk * p.block_size;
+    const int64_t k_off = id * p.k_block + slot * p.k_slot, v_off = id * p.v_block + slot * p.v_slot;
+    if (p.copy == kPages)
+      k_at = static_cast<uint32_t>(k_off >> 4), v_at = static_cast<uint32_t>(v_off >> 4);
+    else
+      k_at = reinterpret_cast<uint64_t>(k + k_off), v_at = reinterpret_cast<uint64_t>(v + v_off);
+  }
+  __device__ __forceinline__ void start(const Walk &from) {
+    w = from;
+    if (!p.local) walk_seq<O>(p, w, h0, n_h, lane);
+    look_up();
+  }
+  // 16 rows from `off` on; kAll: else `rows` of them (the others zero)
+  template <bool kAll>
+  __device__ __forceinline__ void copy_half(uint32_t dst, const char *base, uint32_t off, uint32_t slot_bytes, int rows) {
+    const char *src = base + static_cast<uint64_t>(off) * 16;
+#pragma unroll
+    for (int r = 0; r < 16; r += kAtOnce) {
+      const char *from = src + static_cast<uint64_t>(slot_bytes) * static_cast<uint32_t>(r);
+      if (kAll) {  // (a register for the size costs several instructions)
+        if (inside)
+          asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst + r * kRow), "l"(from) : "memory");
+      } else {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * kRow), "l"(from),
+                     "r"(inside && r + lane / kPieces < rows ? 16 : 0)
+                     : "memory");
+      }
+    }
+  }
+  // rows whose addresses the lanes hold (0: zeros)
+  __device__ __forceinline__ void copy_rows(char *to, uint64_t addr, const char *any) {
+    if (p.copy == kRows) {
+#pragma unroll
+      for (int c = lane; c < kTok * kPieces; c += 32) {
+        const int row = c / kPieces, piece = c % kPieces;
+        const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
+        if (piece * 16 < p.hd)
+          cp_async16(to + row * kRow + piece * 16, a ? reinterpret_cast<const char *>(a) + piece * 16 : any, a ? 16 : 0);
+      }
+    } else if (p.piece >= 4) {
+      for (int row = 0; row < kTok; ++row) {
+        const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
+        const char *src = a ? reinterpret_cast<const char *>(a) : any;
+        for (int at = lane * p.piece; at < p.hd; at += 32 * p.piece) {
+          if (p.piece == 8)
+            cp_async8(to + row * kRow + at, src + at, a ? 8 : 0);
+          else
+            cp_async4(to + row * kRow + at, src + at, a ? 4 : 0);
+        }
+      }
+    } else {
+      for (int d = lane; d < (p.hd + 31) / 32 * 32; d += 32) {
+        for (int row = 0; row < kTok; row += 8) {  // eight rows' loads in flight
+          uint8_t x[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const uint64_t a = __shfl_sync(0xffffffffu, addr, row + r);
+            x[r] = a && d < p.hd ? reinterpret_cast<const uint8_t *>(a)[d] : 0;
+          }
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (d < p.hd) to[(row + r) * kRow + d] = static_cast<char>(x[r]);
+        }
+      }
+    }
+  }
+  // issues the next tile's copies into stage s (one cp.async group, empty past the end)
+  __device__ __forceinline__ void fill(int s) {
+    if (w.live) {
+      const int left = w.end - w.i;
+      uint32_t there;
+      int block;  // of this lane's token, negative: none
+      if (p.copy == kPages) {
+        block = __shfl_sync(0xffffffffu, id, 2 * tile + lane / 16);
+        if (lane >= left) block = kNoRow;
+        there = __ballot_sync(0xffffffffu, block >= 0);
+        const uint32_t k_step = static_cast<uint32_t>(p.k_slot), v_step = static_cast<uint32_t>(p.v_slot);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t k_off = __shfl_sync(0xffffffffu, static_cast<uint32_t>(k_at), 2 * tile + h);
+          const uint32_t v_off = __shfl_sync(0xffffffffu, static_cast<uint32_t>(v_at), 2 * tile + h);
+          const uint32_t dst = to + s * kStage + 16 * h * kRow;
+          if (there == 0xffffffffu) {
+            copy_half<true>(dst, k, k_off, k_step, 16);
+            copy_half<true>(dst + kSide, v, v_off, v_step, 16);
+          } else {  // (where nothing is there the offsets are 0, and nothing is read)
+            const int rows = __popc(there >> (16 * h) & 0xffffu);
+            copy_half<false>(dst, k, k_off, k_step, rows);
+            copy_half<false>(dst + kSide, v, v_off, v_step, rows);
+          }
+        }
+      } else {
+        block = id;
+        there = __ballot_sync(0xffffffffu, block >= 0);
+        copy_rows(ring + s * kStage, k_at, p.k);
+        copy_rows(ring + s * kStage + kSide, v_at, p.v);
+      }
+      if (p.num_blocks > 0) {
+        const uint32_t n = block < 0 ? 0 : 4, at = max(block, 0);
+        cp_async4(scales(s) + lane, ks + static_cast<uint64_t>(at) * static_cast<uint32_t>(p.ks_block), n);
+        cp_async4(scales(s) + kTok + lane, vs + static_cast<uint64_t>(at) * static_cast<uint32_t>(p.vs_block), n);
+      } else {
+        scales(s)[lane] = scales(s)[kTok + lane] = 0.f;
+      }
+      const bool last = !p.local && left <= kTok;
+      if (lane == 0) meta[s] = make_uint4(w.b, w.flags | (last ? kLast : 0), there, 0);
+      walk_next<O>(p, w, h0, n_h, lane);
+      look_up();
+    } else if (lane == 0) {
+      meta[s] = make_uint4(0, 0, 0, 1);  // the end
+    }
+    cp_async_commit();
+  }
 };
 
-template <int PT, int DT, int HD, int W, int kStages>
+constexpr float kSlack = 4.f;  // m above the largest score when it is set, in base 2
+
+// PT: the codes, DT: q and out, NB: blocks of 8 query heads of a unit (a K or V byte becomes an f16 once for all of them).
+template <int PT, int DT, int HD, int NB, int W, int kStages>
 __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant__ Params p) {
-  using S = typename Walk8<DT, HD, kStages>::S;
   using T = typename Elem<DT>::T;
+  using S = Stream8<HD, kStages, T>;
+  constexpr int kTok = S::kTok;
   constexpr int kTerms = DT == DKV_F32 ? 2 : 1;    // of q
   constexpr int kWTerms = DT == DKV_BF16 ? 1 : 2;  // of a weight
   constexpr int kGroups = HD / 32;  // of 32 columns: one ldmatrix
+  constexpr int kBatch = kGroups < 4 ? kGroups : 4;
   constexpr int kSteps = HD / 16;
-  const float kNegInf = __int_as_float(0xff800000);
+  constexpr int kHeadsOf = 8 * NB;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   begin_overlapped();
@@ -91,42 +274,48 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
   Window win;
   if (!p.local) {
     win.look(p, lane);
-    ln = line_of(p.cu[p.n_seqs], p.n_seqs, p.ranges);
+    ln = line_of(p, p.cu[p.n_seqs]);
     if (r >= static_cast<int>(ln.ranges)) return;
   }
   const int u = unit / p.chunks, chunk = unit - u * p.chunks;
-  const int n_h = min(8, p.group - chunk * 8), h0 = u * p.group + chunk * 8;
+  const int n_h = min(kHeadsOf, p.group - chunk * kHeadsOf), h0 = u * p.group + chunk * kHeadsOf;
 
   char *mine = smem + warp * S::kBytes;
   S stream(p, mine, u, h0, n_h, lane);
-  stream.start(p.local ? local_walk(p, r, kTile, warp, p.local) : range_walk(p, win, ln, r, kTile, lane));
+  stream.start(p.local ? local_walk(p, r, kTok, warp, p.local) : range_walk(p, win, ln, r, kTok, lane));
 
   const int g = lane >> 2, t = lane & 3;
   // ldmatrix rows: K as (token, half of 32 columns), V as (token half, 16 columns) of a 16 x 32 block
   const uint32_t k_at = smem_u32(mine) + (lane & 15) * S::kRow + (lane >> 4) * 16;
-  const uint32_t v_at = k_at + kTile * S::kRow;
-  uint32_t qf[kTerms][kGroups][2][2];
-  float unit_q[2];  // what a score of heads 2t, 2t + 1 is in base 2, but for the token's scale
-  float o[kSteps][4], m[2], l[2], top_w[2];
+  uint32_t qf[NB][kTerms][kGroups][2][2];
+  float unit_q[NB][2];  // what a score of heads 2t, 2t + 1 is in base 2, but for the token's scale
+  float o[NB][kSteps][4], m[NB][2], l[NB][2], top_z[NB][2];
+  int up[NB][2];  // O is in units of 2^-up
+  float v_cap;    // V's scales up to which no weight passes 2^15
   auto clear = [&]() {
-    m[0] = m[1] = top_w[0] = top_w[1] = kNegInf;
-    l[0] = l[1] = 0.f;
+    v_cap = 32768.f;
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k)
+    for (int n = 0; n < NB; ++n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[k][e] = 0.f;
+      for (int c = 0; c < 2; ++c) {
+        m[n][c] = -3e38f;  // below any score, and finite: no case of its own
+        l[n][c] = top_z[n][c] = 0.f, up[n][c] = 0;
+      }
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][k][e] = 0.f;
+    }
   };
-  auto sum_of = [&](int c) {  // l over the lanes that share a head
-    float x = l[c];
-    x += __shfl_xor_sync(0xffffffffu, x, 4);
-    x += __shfl_xor_sync(0xffffffffu, x, 8);
-    return x + __shfl_xor_sync(0xffffffffu, x, 16);
+  auto over_tokens = [&](float x, auto f) {  // over the lanes that share a head
+    x = f(x, __shfl_xor_sync(0xffffffffu, x, 4));
+    x = f(x, __shfl_xor_sync(0xffffffffu, x, 8));
+    return f(x, __shfl_xor_sync(0xffffffffu, x, 16));
   };
-  auto unit_of = [&](int c) {  // O in units of 2^m (O is 0 where no weight was)
-    return top_w[c] == kNegInf ? 0.f : ex2(top_w[c] - m[c] - kWeightBias);
-  };
-  auto load_q = [&](int b) {  // (lanes past the unit's heads repeat the last one; their results are not stored)
-    const T *qr = reinterpret_cast<const T *>(p.q + b * p.q_seq + (h0 + min(g, n_h - 1)) * p.q_head);
+  const auto larger = [](float a, float b) { return fmaxf(a, b); };
+  auto sum_of = [&](int n, int c) { return over_tokens(l[n][c], [](float a, float b) { return a + b; }); };
+  auto load_q = [&](int b, int nb) {  // (lanes past the unit's heads repeat the last one; their results are not stored)
+    const T *qr = reinterpret_cast<const T *>(p.q + b * p.q_seq + (h0 + min(8 * nb + g, n_h - 1)) * p.q_head);
     float x[kGroups][2][4];
     float top = 0.f;
     if (DT != DKV_F32 && p.pairs) {  // outside the loops: a branch between the loads would have each waited for
@@ -170,8 +359,8 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // the head's largest element to [2^13, 2^14) (an f16 q stays as it is): 27 binary places below it before an f16
     // subnormal loses any of 11 bits, and 448 x 2^14 x 256 columns far within fp32
-    const int up = DT == DKV_F16 ? 0 : min(140 - static_cast<int>(__float_as_uint(top) >> 23), 126);
-    const float by = exp2i(up);
+    const int by_two = DT == DKV_F16 ? 0 : min(140 - static_cast<int>(__float_as_uint(top) >> 23), 126);
+    const float by = exp2i(by_two);
 #pragma unroll
     for (int k = 0; k < kGroups; ++k)
 #pragma unroll
@@ -180,11 +369,11 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
         for (int i = 0; i < 2; ++i) {
           const float a = x[k][e][2 * i] * by, c = x[k][e][2 * i + 1] * by;
           const uint32_t w = pack_f16x2(a, c);
-          qf[0][k][e][i] = w;
-          if (kTerms == 2) qf[kTerms - 1][k][e][i] = pack_f16x2(a - f16lo(w), c - f16hi(w));
+          qf[nb][0][k][e][i] = w;
+          if (kTerms == 2) qf[nb][kTerms - 1][k][e][i] = pack_f16x2(a - f16lo(w), c - f16hi(w));
         }
-    const float back = exp2i(-up) * p.scale_log2;
-    unit_q[0] = __shfl_sync(0xffffffffu, back, t * 8), unit_q[1] = __shfl_sync(0xffffffffu, back, t * 8 + 4);
+    const float back = exp2i(-by_two) * p.scale_log2;
+    unit_q[nb][0] = __shfl_sync(0xffffffffu, back, t * 8), unit_q[nb][1] = __shfl_sync(0xffffffffu, back, t * 8 + 4);
   };
   clear();
 
@@ -195,133 +384,200 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
     if (mt.w) break;
     const int b = mt.x;
     if (mt.y & kFirst) {
-      load_q(b);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) load_q(b, n);
       clear();
     }
     cp_async_wait<kStages - 1>();  // after a first tile's q is on its way
     __syncwarp();
-    float sc[2][4];  // two chains over the head
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sc[0][e] = sc[1][e] = 0.f;
-#pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      uint32_t c[4];
-      ldmatrix_x4(c[0], c[1], c[2], c[3], k_at + s * S::kStage + k * 32);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {  // tokens g and g + 8 of 16 columns
-        uint32_t a[4];
-        Pairs<PT>::in_order(c[2 * e], a[0], a[2]);
-        Pairs<PT>::in_order(c[2 * e + 1], a[1], a[3]);
-#pragma unroll
-        for (int i = 0; i < kTerms; ++i)
-          mma16816(sc[e], a[0], a[1], a[2], a[3], qf[i][k][e][0], qf[i][k][e][1]);
-      }
-    }
-    // x: {token g, token g + 8} x {head 2t, head 2t + 1}
+    const uint32_t at = k_at + s * S::kStage;
     const float *scales = stream.scales(s);
-    const float ks[2] = {scales[g], scales[g + 8]}, vs[2] = {scales[kTile + g], scales[kTile + g + 8]};
-    float x[4], y[4], v_rest[2];
+    // {tokens 16 i + g, 16 i + g + 8} x {heads 2t, 2t + 1}: the codes' products
+    float sc[NB][2][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = (sc[0][e] + sc[1][e]) * ks[e >> 1] * unit_q[e & 1];
-    if (mt.z != 0xffffu) {
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (!((mt.z >> (g + (e & 2) * 4)) & 1)) x[e] = kNegInf;
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[n][i][e] = 0.f;
+#pragma unroll
+    for (int k0 = 0; k0 < kGroups; k0 += kBatch) {
+      uint32_t c[2][kBatch][4];  // all loads first: none waits for a product before it
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          ldmatrix_x4(c[i][k][0], c[i][k][1], c[i][k][2], c[i][k][3], at + 16 * i * S::kRow + (k0 + k) * 32);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {  // tokens g and g + 8 of 16 columns
+            uint32_t a[4];
+            Pairs<PT>::in_order(c[i][k][2 * e], a[0], a[2]);
+            Pairs<PT>::in_order(c[i][k][2 * e + 1], a[1], a[3]);
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+              for (int x = 0; x < kTerms; ++x) mma_f16(sc[n][i], a, qf[n][x][k0 + k][e]);
+          }
     }
-    // V's scales as a power of two and the rest, in [1, 2) (0 and subnormals below it, the very largest in [2, 4))
+    float k_scale[2][2], v_scale[2][2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const uint32_t bits = min(max((__float_as_uint(vs[e]) >> 23) & 0xffu, 1u), 253u);
-      v_rest[e] = vs[e] * __uint_as_float((254u - bits) << 23);
-      const float power = __uint_as_float(0x4b000000u | bits) - 8388735.f;
-      y[2 * e] = x[2 * e] + power, y[2 * e + 1] = x[2 * e + 1] + power;
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        k_scale[i][e] = scales[16 * i + g + 8 * e], v_scale[i][e] = scales[kTok + 16 * i + g + 8 * e];
+    const float kNegInf = __int_as_float(0xff800000);
+    auto absent = [&](int i, int e) { return !((mt.z >> (16 * i + g + (e & 2) * 4)) & 1); };
+    const float most = fmaxf(fmaxf(fabsf(v_scale[0][0]), fabsf(v_scale[0][1])), fmaxf(fabsf(v_scale[1][0]), fabsf(v_scale[1][1])));
+    float wt[NB][2][4];  // how far a score is above m, then its weight
+    bool moves = most > v_cap;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wt[n][i][e] = fmaf(sc[n][i][e], k_scale[i][e >> 1] * unit_q[n][e & 1], -m[n][e & 1]);
+      if (mt.z != 0xffffffffu) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (absent(i, e)) wt[n][i][e] = kNegInf;
+      }
+      const float(&x)[2][4] = wt[n];
+      moves |= fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                     fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3]))) > 0.f;
     }
-    // m and top_w are any values not far below the largest so far: they move (and l, O with them) only when
-    // one passes them, which after the first tiles is rare
-    const float top0 = fmaxf(x[0], x[2]), top1 = fmaxf(x[1], x[3]);
-    const float tw0 = fmaxf(y[0], y[2]), tw1 = fmaxf(y[1], y[3]);
-    if (__any_sync(0xffffffffu, top0 > m[0] || top1 > m[1] || tw0 > top_w[0] || tw1 > top_w[1])) {
+    // m is any value not far from the largest score so far, 2^up any factor that keeps the weights of V's codes below
+    // 2^15 and the largest of them not far below 2^8: they move (and l, O with them) only when a score passes m or a scale
+    // of V's could lift a weight too high, which after the first tile is rare
+    if (__any_sync(0xffffffffu, moves)) {
+      int highest = -126;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float top = c ? top1 : top0, tw = c ? tw1 : tw0;
+      for (int n = 0; n < NB; ++n) {
 #pragma unroll
-        for (int k = 4; k < 32; k <<= 1) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-          tw = fmaxf(tw, __shfl_xor_sync(0xffffffffu, tw, k));
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            wt[n][i][e] = absent(i, e) ? kNegInf : sc[n][i][e] * (k_scale[i][e >> 1] * unit_q[n][e & 1]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float(&x)[2][4] = wt[n];
+          const float best = over_tokens(fmaxf(fmaxf(x[0][c], x[0][c + 2]), fmaxf(x[1][c], x[1][c + 2])), larger);
+          const float next_m = best > m[n][c] ? best + kSlack : m[n][c];
+          float z = 0.f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              x[i][c + 2 * e] -= next_m;
+              z = fmaxf(z, fabsf(ex2(x[i][c + 2 * e]) * v_scale[i][e]));
+            }
+          const float keep = ex2(m[n][c] - next_m);
+          top_z[n][c] = fmaxf(top_z[n][c] * keep, over_tokens(z, larger));
+          // the largest weight to [2^8, 2^9)
+          const int next = top_z[n][c] > 0.f
+                               ? max(min(135 - static_cast<int>(__float_as_uint(top_z[n][c]) >> 23), 126), -111)
+                               : up[n][c];
+          const float keep_o = ex2(m[n][c] - next_m + static_cast<float>(next - up[n][c]));
+          l[n][c] *= keep;
+          m[n][c] = next_m, up[n][c] = next;
+          highest = max(highest, next);
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) o[n][k][c] *= keep_o, o[n][k][2 + c] *= keep_o;
         }
-        top = fmaxf(top, m[c]), tw = fmaxf(tw, top_w[c]);
-        l[c] *= ex2(m[c] - (top == kNegInf ? 0.f : top));
-        const float keep = ex2(top_w[c] - (tw == kNegInf ? 0.f : tw));
-        m[c] = top, top_w[c] = tw;
+      }
+      v_cap = exp2i(15 - highest);
+    }
+    uint32_t w[NB][2][kWTerms][2];
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) o[k][c] *= keep, o[k][2 + c] *= keep;
+    for (int n = 0; n < NB; ++n) {
+      const float lift[2] = {exp2i(up[n][0]), exp2i(up[n][1])};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = ex2(wt[n][i][e]);
+          l[n][e & 1] += y;
+          wt[n][i][e] = y * (v_scale[i][e >> 1] * lift[e & 1]);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float *y = wt[n][i] + 2 * c;
+          const uint32_t v = pack_f16x2(y[0], y[1]);
+          w[n][i][0][c] = transpose_8x8(v);
+          if (kWTerms == 2) w[n][i][kWTerms - 1][c] = transpose_8x8(pack_f16x2(y[0] - f16lo(v), y[1] - f16hi(v)));
+        }
       }
     }
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const float base = m[c] == kNegInf ? 0.f : m[c];  // nothing seen yet: any finite base
-      const float base_w = (top_w[c] == kNegInf ? 0.f : top_w[c]) - kWeightBias;
-      l[c] += ex2(x[c] - base) + ex2(x[c + 2] - base);
-      y[c] = ex2(y[c] - base_w) * v_rest[0];
-      y[c + 2] = ex2(y[c + 2] - base_w) * v_rest[1];
-    }
-    uint32_t w[kWTerms][2];
+    for (int k0 = 0; k0 < kGroups; k0 += kBatch) {
+      uint32_t c[2][kBatch][4];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const uint32_t v = pack_f16x2(y[2 * c], y[2 * c + 1]);
-      w[0][c] = transpose_8x8(v);
-      if (kWTerms == 2) w[kWTerms - 1][c] = transpose_8x8(pack_f16x2(y[2 * c] - f16lo(v), y[2 * c + 1] - f16hi(v)));
-    }
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      uint32_t c[4];
-      ldmatrix_x4_trans(c[0], c[1], c[2], c[3], v_at + s * S::kStage + k * 32);
+        for (int k = 0; k < kBatch; ++k)
+          ldmatrix_x4_trans(c[i][k][0], c[i][k][1], c[i][k][2], c[i][k][3],
+                            at + S::kSide + 16 * i * S::kRow + (k0 + k) * 32);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {  // columns 32 k + 16 e + 2 g and + 1, tokens 2t, 2t + 1 and 2t + 8, 2t + 9
-        uint32_t a[4];
-        Pairs<PT>::crossed(c[2 * e], a[0], a[1]);
-        Pairs<PT>::crossed(c[2 * e + 1], a[2], a[3]);
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < kWTerms; ++i) mma16816(o[2 * k + e], a[0], a[1], a[2], a[3], w[i][0], w[i][1]);
-      }
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {  // columns 32 k + 16 e + 2 g and + 1, tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+            uint32_t a[4];
+            Pairs<PT>::crossed(c[i][k][2 * e], a[0], a[1]);
+            Pairs<PT>::crossed(c[i][k][2 * e + 1], a[2], a[3]);
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+              for (int x = 0; x < kWTerms; ++x) mma_f16(o[n][2 * (k0 + k) + e], a, w[n][i][x]);
+          }
     }
     if (mt.y & kLast) {
       const bool whole = (mt.y & kFromStart) && (mt.y & kToEnd);
       const int64_t part = (static_cast<int64_t>(r) * p.units + unit) * 2 + (mt.y & kFromStart ? 1 : 0);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int in = t * 2 + c;
-        const float sum = sum_of(c), by = unit_of(c);
-        if (in >= n_h) continue;
-        if (whole) {
-          const float inv = sum == 0.f ? 0.f : by / sum;
-          T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + (h0 + in) * p.out_head);
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k) {
-            const int d = k * 16 + 2 * g;
-            const float lo = o[k][c] * inv, hi = o[k][2 + c] * inv;
-            if (DT != DKV_F32 && p.pairs) {
-              if (d < p.hd) *reinterpret_cast<uint32_t *>(dst + d) = DT == DKV_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
-            } else {
-              if (d < p.hd) dst[d] = Elem<DT>::from_f(lo);
-              if (d + 1 < p.hd) dst[d + 1] = Elem<DT>::from_f(hi);
+        for (int c = 0; c < 2; ++c) {
+          const int in = 8 * n + t * 2 + c;
+          const float sum = sum_of(n, c), by = exp2i(-up[n][c]);
+          if (in >= n_h) continue;
+          if (whole) {
+            const float inv = sum == 0.f ? 0.f : by / sum;
+            T *dst = reinterpret_cast<T *>(p.out + b * p.out_seq + (h0 + in) * p.out_head);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+              const int d = k * 16 + 2 * g;
+              const float lo = o[n][k][c] * inv, hi = o[n][k][2 + c] * inv;
+              if (DT != DKV_F32 && p.pairs) {
+                if (d < p.hd)
+                  *reinterpret_cast<uint32_t *>(dst + d) = DT == DKV_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+              } else {
+                if (d < p.hd) dst[d] = Elem<DT>::from_f(lo);
+                if (d + 1 < p.hd) dst[d + 1] = Elem<DT>::from_f(hi);
+              }
+            }
+            if (p.lse && g == 0)
+              p.lse[static_cast<int64_t>(b) * p.heads + h0 + in] = (m[n][c] + log2f(sum)) * 0.6931471805599453f;
+          } else {
+            float *dst = p.part_o + (part * kHeadsOf + in) * p.hd;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+              const int d = k * 16 + 2 * g;
+              if (d < p.hd) dst[d] = o[n][k][c] * by;
+              if (d + 1 < p.hd) dst[d + 1] = o[n][k][2 + c] * by;
+            }
+            if (g == 0) {
+              p.part_ml[(part * kHeadsOf + in) * 2] = m[n][c];
+              p.part_ml[(part * kHeadsOf + in) * 2 + 1] = sum;
             }
           }
-          if (p.lse && g == 0) p.lse[static_cast<int64_t>(b) * p.heads + h0 + in] = (m[c] + log2f(sum)) * 0.6931471805599453f;
-        } else {
-          float *dst = p.part_o + (part * 8 + in) * p.hd;
-#pragma unroll
-          for (int k = 0; k < kSteps; ++k) {
-            const int d = k * 16 + 2 * g;
-            if (d < p.hd) dst[d] = o[k][c] * by;
-            if (d + 1 < p.hd) dst[d + 1] = o[k][2 + c] * by;
-          }
-          if (g == 0) {
-            p.part_ml[(part * 8 + in) * 2] = m[c];
-            p.part_ml[(part * 8 + in) * 2 + 1] = sum;
-          }
         }
-      }
     }
     __syncwarp();
     stream.fill(s);
@@ -329,54 +585,68 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
   cp_async_wait<0>();
   if (p.local) {
     __syncwarp();
-    LocalState<HD, 8> *mine_out = reinterpret_cast<LocalState<HD, 8> *>(mine);
-    static_assert(sizeof(LocalState<HD, 8>) <= kStages * S::kStage, "the state fits the ring");
+    using State = LocalState<HD, kHeadsOf>;
+    State *mine_out = reinterpret_cast<State *>(mine);
+    static_assert(sizeof(State) <= kStages * S::kStage, "the state fits the ring");
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int in = t * 2 + c;
-      const float sum = sum_of(c), by = unit_of(c);
-      if (g == 0) mine_out->m[in] = m[c], mine_out->l[in] = sum;
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        mine_out->o[in][k * 16 + 2 * g] = o[k][c] * by;
-        mine_out->o[in][k * 16 + 2 * g + 1] = o[k][2 + c] * by;
+      for (int c = 0; c < 2; ++c) {
+        const int in = 8 * n + t * 2 + c;
+        const float sum = sum_of(n, c), by = exp2i(-up[n][c]);
+        if (g == 0) mine_out->m[in] = m[n][c], mine_out->l[in] = sum;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          mine_out->o[in][k * 16 + 2 * g] = o[n][k][c] * by;
+          mine_out->o[in][k * 16 + 2 * g + 1] = o[n][k][2 + c] * by;
+        }
       }
-    }
-    local_join<DT, HD, 8>(p, smem, S::kBytes, p.local, r, h0, n_h);
+    local_join<DT, HD, kHeadsOf>(p, smem, S::kBytes, p.local, r, h0, n_h);
   }
 }
 
 // ---------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------
-// as many warps and stages as registers and shared memory allow
-constexpr Variant variant8(bool f32, int hd) {
-  if (hd == 256) return f32 ? Variant{8, 3, 16} : Variant{12, 2, 16};
-  if (hd == 128) return f32 ? Variant{12, 4, 16} : Variant{16, 3, 16};
-  return hd == 64 ? Variant{16, 5, 16} : Variant{16, 8, 16};
+// warps and stages
+constexpr Variant variant8(bool f32, int hd, int heads) {
+  if (hd == 256) return {6, 2, 32};
+  if (hd == 128) return {8, 3, 32};
+  if (heads == 16) return hd == 64 ? Variant{12, 3, 32} : Variant{12, 4, 32};
+  return hd == 64 ? Variant{f32 ? 12 : 14, 3, 32} : Variant{16, 4, 32};
+}
+// query heads of a unit: 16 where a KV head has more than eight and registers allow it
+constexpr int heads8(bool f32, int hd, int group) { return !f32 && hd <= 128 && group > 8 ? 16 : 8; }
+constexpr int kSeqCost8 = 96;
+
+template <int PT, int DT, int HD, int NB>
+int launch_walk8(const Params &p, const Shape &s, cudaStream_t st) {
+  constexpr Variant v = variant8(DT == DKV_F32, HD, 8 * NB);
+  constexpr int kWarp = Stream8<HD, v.stages, typename Elem<DT>::T>::kBytes;
+  static_assert(v.warps * kWarp <= 227 * 1024, "shared memory of the walk");
+  const auto kernel = walk8_kernel<PT, DT, HD, NB, v.warps, v.stages>;
+  const int rc = allow_smem<walk8_kernel<PT, DT, HD, NB, v.warps, v.stages>>(v.warps * kWarp);
+  if (rc != DKV_OK) return rc;
+  const int64_t all = static_cast<int64_t>(s.ranges) * s.units;
+  const int64_t ctas = s.local ? static_cast<int64_t>(p.n_seqs) * s.units : (all + v.warps - 1) / v.warps;
+  const int warps = p.local ? p.local : v.warps;
+  DKV_CUDA_CHECK(launch_overlapped(kernel, dim3(static_cast<unsigned>(ctas)), warps * 32, warps * kWarp, st, p));
+  return DKV_OK;
 }
 
 template <int PT, int DT, int HD>
-int launch_walk8(const Params &p, const Shape &s, int grid, cudaStream_t st) {
-  constexpr Variant v = variant8(DT == DKV_F32, HD);
-  constexpr int kWarp = Walk8<DT, HD, v.stages>::S::kBytes;
-  static_assert(v.warps * kWarp <= 227 * 1024, "shared memory of the walk");
-  const auto kernel = walk8_kernel<PT, DT, HD, v.warps, v.stages>;
-  const int rc = allow_smem<walk8_kernel<PT, DT, HD, v.warps, v.stages>>(v.warps * kWarp);
-  if (rc != DKV_OK) return rc;
-  const int warps = p.local ? p.local : v.warps;
-  DKV_CUDA_CHECK(launch_overlapped(kernel, dim3(grid), warps * 32, warps * kWarp, st, p));
-  return DKV_OK;
+int launch_walk8(const Params &p, const Shape &s, cudaStream_t st) {
+  if constexpr (heads8(DT == DKV_F32, HD, 16) == 16)
+    if (s.g == 16) return launch_walk8<PT, DT, HD, 2>(p, s, st);
+  return launch_walk8<PT, DT, HD, 1>(p, s, st);
 }
 
 template <int PT, int DT>
 int launch8(const Params &p, const Shape &s, cudaStream_t st) {
-  const int64_t warps = static_cast<int64_t>(s.ranges) * s.units;
-  const int grid = static_cast<int>(s.local ? static_cast<int64_t>(p.n_seqs) * s.units : (warps + s.warps - 1) / s.warps);
-  const int rc = s.hd_pad == 32    ? launch_walk8<PT, DT, 32>(p, s, grid, st)
-                 : s.hd_pad == 64  ? launch_walk8<PT, DT, 64>(p, s, grid, st)
-                 : s.hd_pad == 128 ? launch_walk8<PT, DT, 128>(p, s, grid, st)
-                                   : launch_walk8<PT, DT, 256>(p, s, grid, st);
+  const int rc = s.hd_pad == 32    ? launch_walk8<PT, DT, 32>(p, s, st)
+                 : s.hd_pad == 64  ? launch_walk8<PT, DT, 64>(p, s, st)
+                 : s.hd_pad == 128 ? launch_walk8<PT, DT, 128>(p, s, st)
+                                   : launch_walk8<PT, DT, 256>(p, s, st);
   return rc != DKV_OK ? rc : launch_join(DT, p, s, st);
 }
 

@@ -9,8 +9,8 @@ namespace dkv {
 namespace pattn {
 
 constexpr int kTile = 16;  // borders fall on multiples of it; a pipeline stage has 16 or 8 tokens
-// Virtual tokens per sequence: what starting and finishing one costs a warp.  Walk of 256 sequences
-// of 1..600 tokens at 16 / 32 / 48 / 64 / 96: 38 / 34 / 31 / 34 / 39 us; of 64 of 1..8192:
+// Virtual tokens per sequence: what starting and finishing one costs a warp (Params::seq_cost).  16-bit walk of 256
+// sequences of 1..600 tokens at 16 / 32 / 48 / 64 / 96: 38 / 34 / 31 / 34 / 39 us; of 64 of 1..8192:
 // 73 / 61 / 59 / 60 / 61 us; long sequences do not notice.
 constexpr int kSeqCost = 48;
 // Up to so many tiles a warp, a batch runs as one launch, a CTA for each sequence and unit, of as many warps
@@ -41,6 +41,7 @@ struct Params {
   float bias;        // l and O of the parts carry 2^bias
   float scale_log2;  // scale * log2(e): scores are kept in base 2
   int n_seqs, n_kv, heads, group, chunks, units, ranges;
+  int seq_cost;
   int hd, block_size;
   uint32_t div_mul, div_shift;  // i / block_size = i div_mul >> div_shift
   int local;  // not 0: a CTA of so many warps per (sequence, unit), no ranges, no parts
@@ -65,18 +66,18 @@ struct Line {
     return x < big ? x / (each + 1) : more + (x - big) / each;
   }
 };
-__device__ __forceinline__ Line line_of(uint32_t tokens, int n_seqs, int most) {
+__device__ __forceinline__ Line line_of(const Params &p, uint32_t tokens) {
   Line ln;
-  ln.total = tokens + static_cast<uint32_t>(kSeqCost) * n_seqs;
-  ln.ranges = min(max(ln.total / kMinRange, 1u), static_cast<uint32_t>(most));
+  ln.total = tokens + static_cast<uint32_t>(p.seq_cost) * p.n_seqs;
+  ln.ranges = min(max(ln.total / kMinRange, 1u), static_cast<uint32_t>(p.ranges));
   ln.each = ln.total / ln.ranges;
   ln.more = ln.total - ln.each * ln.ranges;
   return ln;
 }
 // the token of sequence [at, at + len) that a range border at x falls on: a multiple of the tile
-__device__ __forceinline__ int border(uint32_t x, uint32_t at, int len) {
+__device__ __forceinline__ int border(const Params &p, uint32_t x, uint32_t at, int len) {
   if (x <= at) return 0;
-  if (x - at >= static_cast<uint32_t>(len) + kSeqCost) return len;
+  if (x - at >= static_cast<uint32_t>(len) + p.seq_cost) return len;
   return static_cast<int>(min((x - at) & ~static_cast<uint32_t>(kTile - 1), static_cast<uint32_t>(len)));
 }
 
@@ -112,20 +113,20 @@ struct WindowOf {
     else
       load(p, 0, lane);
   }
-  // the largest b with cu[b] + kSeqCost b <= x, and a window that starts at or before it
+  // the largest b with cu[b] + seq_cost b <= x, and a window that starts at or before it
   __device__ __forceinline__ int find(const Params &p, uint32_t x, int lane) {
     int lo = 0, hi = p.n_seqs;
     while (hi - lo > 31) {
       const int step = (hi - lo + 31) / 32;
       const int b = lo + lane * step;
       if (lo > 0 || hi < p.n_seqs) cu = cu_at(p, min(b, p.n_seqs));
-      const bool in = b < hi && static_cast<uint32_t>(cu) + static_cast<uint32_t>(kSeqCost) * b <= x;
+      const bool in = b < hi && static_cast<uint32_t>(cu) + static_cast<uint32_t>(p.seq_cost) * b <= x;
       const int k = __popc(__ballot_sync(0xffffffffu, in));
       if (k > 1) lo += (k - 1) * step;
       hi = min(hi, lo + step);
     }
     if (p.n_seqs > 31) load(p, lo, lane);
-    const bool in = lo + lane < hi && static_cast<uint32_t>(cu) + static_cast<uint32_t>(kSeqCost) * (lo + lane) <= x;
+    const bool in = lo + lane < hi && static_cast<uint32_t>(cu) + static_cast<uint32_t>(p.seq_cost) * (lo + lane) <= x;
     return lo + max(__popc(__ballot_sync(0xffffffffu, in)) - 1, 0);
   }
 };
@@ -164,10 +165,10 @@ __device__ __forceinline__ void walk_seq(const Params &p, Walk &w, int h0, int n
   for (; w.b < p.n_seqs; ++w.b) {
     w.win.need(p, w.b, lane);
     const int first = w.win.at(w.b);
-    const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(kSeqCost) * w.b;
+    const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(p.seq_cost) * w.b;
     if (at >= w.x1) return;
     const int len = max(w.win.at(w.b + 1) - first, 0);
-    const int i0 = border(w.x0, at, len), i1 = border(w.x1, at, len);
+    const int i0 = border(p, w.x0, at, len), i1 = border(p, w.x1, at, len);
     if (i1 > i0) {
       w.i = i0, w.end = i1;
       w.flags = kFirst | (i0 == 0 ? kFromStart : 0) | (i1 == len ? kToEnd : 0);
@@ -231,17 +232,12 @@ __device__ __forceinline__ Walk local_walk(const Params &p, int b, int tokens, i
 // 3.5 GB of 32 long sequences).
 enum { kPlain = 0, kRows = 1, kPages = 2 };
 
-//
-// Pages of 8 bits (kScaled): behind the descriptions lie each stage's scales, one for each of its rows, so
-// that tiles across blocks are no case of their own; O: the type of the output.
-template <typename T, int HD, int kStages, int kTok, typename O = T, bool kScaled = false>
+template <typename T, int HD, int kStages, int kTok>
 struct Stream {
   static constexpr int kSize = static_cast<int>(sizeof(T));
   static constexpr int kRow = HD * kSize + 16;
   static constexpr int kStage = 2 * kTok * kRow;
-  static constexpr int kScales = kScaled ? 2 * kTok * 4 : 0;
-  static constexpr int kBytes = kStages * (kStage + 16 + kScales);  // the stages' descriptions behind them
-  static_assert(!kScaled || kTok == 16, "a lane for each row's scale");
+  static constexpr int kBytes = kStages * (kStage + 16);  // the stages' descriptions behind them
   static constexpr int kPieces = HD * kSize / 16;         // 16-byte pieces of a row
   static constexpr int kRowLanes = kPieces < 32 ? kPieces : 32;
   static constexpr int kAtOnce = 32 / kRowLanes;          // rows a copy instruction covers
@@ -251,8 +247,6 @@ struct Stream {
   char *ring;
   uint4 *meta;  // per stage: sequence, flags, bit per token that takes part, end of the stream
   const char *k, *v;  // kPages: this lane's first piece of slot 0 of block 0; else its side's base
-  const float *scale;  // kScaled: of this lane's side (K: lanes below kTok) and the unit's head, block 0
-  int64_t scale_block;
   int h0, n_h, lane;
   int id, slot;  // block and slot of this lane's row of the next tile; kPages: block of the tile
   int tile;      // kPages: of the 32 tiles that the lanes hold ids of, the next
@@ -266,10 +260,6 @@ struct Stream {
     if (p.copy == kPages) {
       k += row * p.k_slot + piece * 16;
       v += row * p.v_slot + piece * 16;
-    }
-    if constexpr (kScaled) {
-      scale = lane < kTok ? p.k_scale + u * p.ks_head : p.v_scale + u * p.vs_head;
-      scale_block = lane < kTok ? p.ks_block : p.vs_block;
     }
     if (p.hd < HD) {  // columns past head_dim stay zero in every stage: nothing writes them again
       for (int i = lane; i < kStages * kStage / 16; i += 32)
@@ -302,7 +292,7 @@ struct Stream {
   }
   __device__ __forceinline__ void start(const Walk &from) {
     w = from;
-    if (!p.local) walk_seq<O>(p, w, h0, n_h, lane);
+    if (!p.local) walk_seq<T>(p, w, h0, n_h, lane);
     look_up();
   }
   // the rows of one side of a tile in one block, `rows` of them (the others zero)
@@ -360,17 +350,6 @@ struct Stream {
       }
     }
   }
-  __device__ __forceinline__ float *scales(int s) const {
-    return reinterpret_cast<float *>(ring + kStages * (kStage + 16) + s * kScales);
-  }
-  __device__ __forceinline__ void copy_scale(int s, bool there, int64_t block) {  // of this lane's row
-    if constexpr (kScaled) {
-      if (p.num_blocks > 0)
-        cp_async4(scales(s) + lane, scale + (there ? block : 0) * scale_block, there ? 4 : 0);
-      else
-        scales(s)[lane] = 0.f;
-    }
-  }
   // issues the next tile's copies into stage s (one cp.async group, empty past the end)
   __device__ __forceinline__ void fill(int s) {
     if (w.live) {
@@ -394,7 +373,6 @@ struct Stream {
           copy_side(dst, ks, p.k_slot, rows);
           copy_side(dst + kTok * kRow, vs, p.v_slot, rows);
         }
-        copy_scale(s, lane % kTok < rows, at);
       } else {
         const bool wanted = lane < 2 * kTok && lane % kTok < w.end - w.i;
         const bool good = wanted && id >= 0 && id < p.num_blocks;
@@ -414,11 +392,10 @@ struct Stream {
         } else {
           copy_plain(stage, addr);
         }
-        copy_scale(s, good, id);
       }
       const bool last = !p.local && w.end - w.i <= kTok;
       if (lane == 0) meta[s] = make_uint4(w.b, w.flags | (last ? kLast : 0), there, 0);
-      walk_next<O>(p, w, h0, n_h, lane);
+      walk_next<T>(p, w, h0, n_h, lane);
       look_up();
     } else if (lane == 0) {
       meta[s] = make_uint4(0, 0, 0, 1);  // the end
@@ -492,6 +469,7 @@ struct Shape {
   int local;             // warps of a CTA per (sequence, unit), or 0: ranges
   int ranges;            // upper bound of the ranges in use
   int64_t parts;         // part slots
+  int seq_cost;
   int sms;
   int64_t o_bytes, bytes;
 };
@@ -518,7 +496,7 @@ inline int check_args(const dkv_paged_decode_args &a) {
 constexpr int kMaxRanges = 2048;
 
 // how a batch is cut, given the kernel variant: s->hd_pad and s->g are set
-inline int cut_up(const dkv_paged_decode_args &a, const Variant &v, Shape *s) {
+inline int cut_up(const dkv_paged_decode_args &a, const Variant &v, int seq_cost, Shape *s) {
   const int rc = sm_count(&s->sms);
   if (rc != DKV_OK) return rc;
   const int64_t sms = s->sms;
@@ -531,13 +509,14 @@ inline int cut_up(const dkv_paged_decode_args &a, const Variant &v, Shape *s) {
   while (s->local > 0 && pairs > sms * (s->warps / s->local)) --s->local;
   if (a.seqs.max_seq_len > static_cast<int64_t>(kLocalTiles) * s->tokens * s->local) s->local = 0;
   const int64_t most = sms * s->warps / s->units;
-  const int64_t line = static_cast<int64_t>(a.seqs.n_seqs) * (static_cast<int64_t>(a.seqs.max_seq_len) + kSeqCost);
+  const int64_t line = static_cast<int64_t>(a.seqs.n_seqs) * (static_cast<int64_t>(a.seqs.max_seq_len) + seq_cost);
   const int64_t want = line / kMinRange;
   s->ranges = static_cast<int>(s->local || most < 1 || want < 1 ? 1 : (want < most ? want : most));
   if (s->ranges > kMaxRanges) s->ranges = kMaxRanges;
   s->parts = s->ranges > 1 ? static_cast<int64_t>(s->ranges) * s->units * 2 * s->g : 0;
   s->o_bytes = (s->parts * hd * 4 + 15) / 16 * 16;
   s->bytes = s->o_bytes + s->parts * 8;
+  s->seq_cost = seq_cost;
   return DKV_OK;
 }
 
@@ -563,6 +542,7 @@ inline void fill_params(const dkv_paged_decode_args &a, const Shape &s, int64_t 
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.n_seqs = a.seqs.n_seqs, p.n_kv = k.n_heads, p.heads = a.n_q_heads, p.group = a.n_q_heads / k.n_heads;
   p.chunks = s.chunks, p.units = s.units, p.ranges = s.ranges;
+  p.seq_cost = s.seq_cost;
   p.local = s.local;
   p.hd = k.head_dim, p.block_size = k.block_size;
   // for i < 2^31 and 2^(s - 1) < block_size <= 2^s: mul = floor(2^(31 + s) / block_size) + 1 is off by at

@@ -11,9 +11,9 @@ The attention: a score is a product sum of head_dim terms times two scales, off 
 =: ds (tensor cores may truncate, hence 2^-23; fp32 q as two f16 terms adds 2^-21), which moves every weight by a relative
 2 ds.  Weights enter to 2^-21 as two f16 terms and to 2^-11 as one (bf16); exp and the running sums add 2^-20 and n 2^-24.
 All relative to A = sum p |v| / sum p; out is rounded once.  And a floor: a weight W = p (V's scale) enters as an f16 number in
-units of 2^-13 of a power of two that is at most the largest W.  f16 steps are never below 2^-24, so a weight is
-off by at least 2^-25 2^-13 = 2^-38 of the largest W, whatever its size (a column where the heavy tokens' codes are 0 shows it): n
-tokens with codes of up to c add n c 2^-38 max W.
+units of 2^-8 of a power of two that is at most the largest W (headroom for larger scores and scales of V's to come).  f16 steps
+are never below 2^-24, so a weight is off by up to 2^-25 2^-8 = 2^-33 of the largest W, whatever its size (a column where the
+heavy tokens' codes are 0 shows it): n tokens with codes of up to c add n c 2^-33 max W.
 """
 
 from __future__ import annotations
@@ -536,7 +536,7 @@ def check_attention(got, lse, q, tokens_of, scale):
         spread = torch.einsum("ugn,nud->ugd", p, v.abs())
         tol = torch.finfo(q.dtype).eps / 2 * ref.abs() + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
         tol = tol + spread * (2 * ds[..., None] + 2.0 ** -19 + k.shape[0] * 2.0 ** -24 + (2.0 ** -11 if q.dtype == BF else 2.0 ** -21))
-        tol = tol + k.shape[0] * 2.0 ** -38 * (p * big.T[:, None]).amax(-1)[..., None]
+        tol = tol + k.shape[0] * 2.0 ** -33 * (p * big.T[:, None]).amax(-1)[..., None]
         off = (got[b].double().view(kv, heads // kv, hd) - ref).abs()
         assert torch.all(off <= tol), (b, k.shape[0], float((off / tol).max()))
         if lse is not None:
