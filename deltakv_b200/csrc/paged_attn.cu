@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(W * 32, 1) mma_kernel(const __grid_constant__ 
 // A CTA has `hpc` query heads (1 or a warp each) of a cut sequence.  blockIdx.x is a sequence
 // where by_seq, else a range border (at most ranges - 1 sequences are cut); gridDim.z CTAs share a
 // head's columns.  Which parts there are follows from the lengths alone and is worked out before
-// the walk's end is waited for.  Up to 32 parts a warp joins alone, a lane per part's weight; more are
+// the walk's end is waited for.  Up to 32 parts (of the 8-bit walk, whose ranges are shorter, 64) a warp joins alone, a lane per part's weight; more are
 // joined by the CTA: a thread per part's weight, then VW columns a thread, a group of threads for
 // every so many-th part.  The parts' addresses are an arithmetic sequence, so that several parts'
 // loads are in flight: with a test in front of each load, the 222 parts of one long sequence took
@@ -706,21 +706,26 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   const int cols = min(p.hd / VW, col0 + share);
   const int h0 = blockIdx.y * hpc, h1 = min(h0 + hpc, p.heads);
 
-  if (n <= 32) {
+  if (n <= p.alone) {
     const int h = h0 + warp;
     if (h >= h1) return;
     const int64_t part0 = part_at(h);
     wait_for_earlier();
-    float m = kNegInf, l = 0.f;
+    float m = kNegInf, l = 0.f, m2 = kNegInf, l2 = 0.f;
     if (lane < n) {
       const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (part0 + lane * stride + (lane ? 0 : g_unit)));
       m = ml.x, l = ml.y;
     }
-    float top = m;
+    if (lane + 32 < n) {
+      const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (part0 + (lane + 32) * stride));
+      m2 = ml.x, l2 = ml.y;
+    }
+    float top = fmaxf(m, m2);
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-    const float w = exp2f(m - (top == kNegInf ? 0.f : top));
-    float total = l * w;
+    const float base = top == kNegInf ? 0.f : top;
+    const float w = exp2f(m - base), w2 = exp2f(m2 - base);
+    float total = fmaf(l2, w2, l * w);  // (l2 is 0 where there are no more than 32 parts)
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
     const float inv = total == 0.f ? 0.f : 1.f / total;
@@ -730,7 +735,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
 #pragma unroll
       for (int e = 0; e < VW; ++e) acc[e] = 0.f;
       add_parts<VW>(acc, p.part_o + part0 * p.hd + c * VW, stride * p.hd, g_unit * p.hd, 0, 1, n,
-                    [&](int i) { return __shfl_sync(0xffffffffu, w, i); });
+                    [&](int i) { return __shfl_sync(0xffffffffu, i < 32 ? w : w2, i & 31); });
       if (c0 + lane < cols) store(h, c, acc, inv);
     }
     if (p.lse && lane == 0 && blockIdx.z == 0)
@@ -971,6 +976,7 @@ extern "C" int dkv_paged_decode_attention(const dkv_paged_decode_args *args, dkv
   const int64_t sz = k.dtype == DKV_F32 ? 4 : 2;
   pattn::Params p;
   pattn::fill_params(a, s, sz, sz, &p);
+  p.alone = 32;
   if (k.dtype == DKV_F16) p.bias = pattn::Half<DKV_F16>::kBias;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (k.dtype) {

@@ -57,15 +57,14 @@ extern "C" int dkv_paged_decode_attention_quant(const dkv_paged_decode_args *arg
   p.k_scale = k_scales->base, p.ks_block = k_scales->stride_block, p.ks_head = k_scales->stride_head;
   // a tile's halves are copied as pages where each lies in one block
   if (p.copy == pattn::kRows && k.block_size % pattn::kTile == 0) p.copy = pattn::kPages;
-  // copies of pages step through a block's rows with 32-bit strides, and reach blocks by 32 bits of 16 bytes; scales go by 32
-  // bits as well
+  // places in the pages are 32 bits of 16 bytes, strides of rows and of scales 32 bits
   auto reach = [](int64_t blocks, int64_t block, int64_t slots, int64_t slot) {
-    return block >= 0 && slot >= 0 && (blocks == 0 || (blocks - 1) * block + (slots - 1) * slot < (int64_t{1} << 36));
+    return block >= 0 && slot >= 0 && slot <= INT32_MAX &&
+           (blocks == 0 || (blocks - 1) * block + (slots - 1) * slot < (int64_t{1} << 36));
   };
-  if (p.copy == pattn::kPages &&
-      (p.k_slot > INT32_MAX || p.v_slot > INT32_MAX || !reach(p.num_blocks, p.k_block, k.block_size, p.k_slot) ||
-       !reach(p.num_blocks, p.v_block, k.block_size, p.v_slot)))
-    p.copy = pattn::kRows;
+  if (p.copy != pattn::kPlain && (!reach(p.num_blocks, p.k_block, k.block_size, p.k_slot) ||
+                                  !reach(p.num_blocks, p.v_block, k.block_size, p.v_slot)))
+    p.copy = pattn::kPlain;
   p.v_scale = v_scales->base, p.vs_block = v_scales->stride_block, p.vs_head = v_scales->stride_head;
   if (p.ks_block < 0 || p.vs_block < 0 || p.ks_block > UINT32_MAX || p.vs_block > UINT32_MAX) return DKV_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -74,12 +74,19 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   return r;
 }
 
+// 16 bytes into shared memory; L2 takes 256 with them, for a row of the next head lies behind most rows and is read by a
+// neighbouring warp (32 long sequences, 8 heads x 128: 320 us without, 310 with)
+__device__ __forceinline__ void copy16(uint32_t to, const void *from) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
 // One warp's stream of tiles of 32 tokens into its ring: a stage holds 32 rows of K, as many of V (16 bytes more than a row
 // apart: no bank conflicts), their scales and its description.  Two ways to copy:
 //   kPages  block_size a multiple of 16: each half of a tile lies in one block (borders fall on multiples of 16), its rows a
 //           fixed stride apart.  A lane holds the addresses of one of the next 32 halves, so that the table is waited
 //           for, and addresses are worked out, once in 16 tiles;
 //   kRows, kPlain  a lane for each token's block and slot, a tile ahead; rows in pieces of 16 bytes, or smaller ones.
+// Places in pages and rows are kept in units of 16 bytes, 32 bits for 64 GB (caches beyond that go the kPlain way).
 template <int HD, int kStages, typename O>
 struct Stream8 {
   static constexpr int kTok = 32;
@@ -94,30 +101,33 @@ struct Stream8 {
   Walk w;
   char *ring;
   uint4 *meta;  // per stage: sequence, flags, bit per token that takes part, end of the stream
-  const char *k, *v;    // kPages: this lane's row and piece of slot 0 of block 0; else the side's base
+  const char *k, *v;    // of slot 0 of block 0; kPages: this lane's row and piece behind it, kRows: its piece
   const float *ks, *vs;
-  uint32_t to;          // kPages: where this lane's first piece goes in stage 0
+  uint32_t to;          // where this lane's first piece goes in stage 0
   bool inside;          // this lane's piece is not past head_dim
   int h0, n_h, lane;
-  uint64_t k_at, v_at;  // the row of this lane's token (0: none); kPages: the half it looked up, in units of 16 bytes from k, v
-  int id;               // its block, negative: none
+  uint64_t k_at, v_at;  // kPlain: the row of this lane's token (0: none); else the row (kPages: half) it looked up, from k, v
+  int id, slot;         // its block and slot in it, negative: none
   int tile;             // kPages: of the 16 tiles that the lanes hold, the next
   static constexpr int kNoRow = -1, kShort = INT32_MIN;
 
   __device__ __forceinline__ Stream8(const Params &p_, char *mine, int u, int h0_, int n_h_, int lane_)
       : p(p_), ring(mine), meta(reinterpret_cast<uint4 *>(mine + kStages * kStage)), k(p_.k + u * p_.k_head),
         v(p_.v + u * p_.v_head), ks(p_.k_scale + u * p_.ks_head), vs(p_.v_scale + u * p_.vs_head), h0(h0_), n_h(n_h_),
-        lane(lane_), k_at(0), v_at(0), id(kNoRow), tile(0) {
+        lane(lane_), k_at(0), v_at(0), id(kNoRow), slot(-1), tile(0) {
     const int row = lane / kPieces, piece = lane % kPieces;
     to = smem_u32(ring) + row * kRow + piece * 16;
     inside = piece * 16 < p.hd;
-    if (p.copy == kPages) k += row * p.k_slot + piece * 16, v += row * p.v_slot + piece * 16;
+    if (p.copy == kPages) k += row * p.k_slot, v += row * p.v_slot;
+    if (p.copy != kPlain) k += piece * 16, v += piece * 16;
     if (p.hd < HD) {  // columns past head_dim stay zero in every stage: only zeros are written there again
       for (int i = lane; i < kStages * kStage / 16; i += 32) reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0, 0, 0, 0);
       __syncwarp();
     }
   }
   __device__ __forceinline__ float *scales(int s) const { return reinterpret_cast<float *>(ring + s * kStage + 2 * kSide); }
+  // Loads a table entry for this lane; what follows from it is worked out (resolve) when the next tile is filled, so that
+  // nothing waits for the load here.
   __device__ __forceinline__ void look_up() {
     if (!w.live) return;
     int ahead = lane;
@@ -126,19 +136,24 @@ struct Stream8 {
       tile = 0;
       ahead = (lane >> 1) * w.step + (lane & 1) * 16;
     }
-    k_at = v_at = 0, id = kNoRow;
+    id = kNoRow, slot = -1;
     if (ahead >= w.end - w.i) return;
     const int i = w.i + ahead;
     const int blk = static_cast<int>((static_cast<uint64_t>(i) * p.div_mul) >> p.div_shift);
+    slot = i - blk * p.block_size;
     id = blk < w.tlen ? max(p.tables[w.b * p.table_stride + blk], kNoRow) : kShort;
+  }
+  __device__ __forceinline__ void resolve() {
+    if (p.copy == kPages && tile != 0) return;
+    k_at = v_at = 0;
+    if (slot < 0) return;
     if (id < 0 || id >= p.num_blocks) {
       record_error(p.status, id == kShort ? DKV_ERR_BLOCK_TABLE_SHORT : DKV_ERR_PAGE_RANGE);
       id = kNoRow;
       return;
     }
-    const int slot = i - blk * p.block_size;
     const int64_t k_off = id * p.k_block + slot * p.k_slot, v_off = id * p.v_block + slot * p.v_slot;
-    if (p.copy == kPages)
+    if (p.copy != kPlain)
       k_at = static_cast<uint32_t>(k_off >> 4), v_at = static_cast<uint32_t>(v_off >> 4);
     else
       k_at = reinterpret_cast<uint64_t>(k + k_off), v_at = reinterpret_cast<uint64_t>(v + v_off);
@@ -156,8 +171,7 @@ struct Stream8 {
     for (int r = 0; r < 16; r += kAtOnce) {
       const char *from = src + static_cast<uint64_t>(slot_bytes) * static_cast<uint32_t>(r);
       if (kAll) {  // (a register for the size costs several instructions)
-        if (inside)
-          asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst + r * kRow), "l"(from) : "memory");
+        if (inside) copy16(dst + r * kRow, from);
       } else {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * kRow), "l"(from),
                      "r"(inside && r + lane / kPieces < rows ? 16 : 0)
@@ -165,25 +179,31 @@ struct Stream8 {
       }
     }
   }
-  // rows whose addresses the lanes hold (0: zeros)
-  __device__ __forceinline__ void copy_rows(char *to, uint64_t addr, const char *any) {
+  // the rows that the lanes looked up; those not in `there` zero
+  __device__ __forceinline__ void copy_rows(char *to_rows, uint64_t addr, const char *base, uint32_t there) {
     if (p.copy == kRows) {
+      const uint32_t dst = smem_u32(to_rows) + lane / kPieces * kRow + lane % kPieces * 16;
 #pragma unroll
-      for (int c = lane; c < kTok * kPieces; c += 32) {
-        const int row = c / kPieces, piece = c % kPieces;
-        const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
-        if (piece * 16 < p.hd)
-          cp_async16(to + row * kRow + piece * 16, a ? reinterpret_cast<const char *>(a) + piece * 16 : any, a ? 16 : 0);
+      for (int r = 0; r < kTok; r += kAtOnce) {
+        const int row = r + lane / kPieces;
+        const char *from = base + static_cast<uint64_t>(__shfl_sync(0xffffffffu, static_cast<uint32_t>(addr), row)) * 16;
+        if (there == 0xffffffffu) {
+          if (inside) copy16(dst + r * kRow, from);
+        } else {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * kRow), "l"(from),
+                       "r"(inside && (there >> row & 1) ? 16 : 0)
+                       : "memory");
+        }
       }
     } else if (p.piece >= 4) {
       for (int row = 0; row < kTok; ++row) {
         const uint64_t a = __shfl_sync(0xffffffffu, addr, row);
-        const char *src = a ? reinterpret_cast<const char *>(a) : any;
+        const char *src = a ? reinterpret_cast<const char *>(a) : base;
         for (int at = lane * p.piece; at < p.hd; at += 32 * p.piece) {
           if (p.piece == 8)
-            cp_async8(to + row * kRow + at, src + at, a ? 8 : 0);
+            cp_async8(to_rows + row * kRow + at, src + at, a ? 8 : 0);
           else
-            cp_async4(to + row * kRow + at, src + at, a ? 4 : 0);
+            cp_async4(to_rows + row * kRow + at, src + at, a ? 4 : 0);
         }
       }
     } else {
@@ -197,7 +217,7 @@ struct Stream8 {
           }
 #pragma unroll
           for (int r = 0; r < 8; ++r)
-            if (d < p.hd) to[(row + r) * kRow + d] = static_cast<char>(x[r]);
+            if (d < p.hd) to_rows[(row + r) * kRow + d] = static_cast<char>(x[r]);
         }
       }
     }
@@ -206,6 +226,7 @@ struct Stream8 {
   __device__ __forceinline__ void fill(int s) {
     if (w.live) {
       const int left = w.end - w.i;
+      resolve();
       uint32_t there;
       int block;  // of this lane's token, negative: none
       if (p.copy == kPages) {
@@ -230,8 +251,8 @@ struct Stream8 {
       } else {
         block = id;
         there = __ballot_sync(0xffffffffu, block >= 0);
-        copy_rows(ring + s * kStage, k_at, p.k);
-        copy_rows(ring + s * kStage + kSide, v_at, p.v);
+        copy_rows(ring + s * kStage, k_at, k, there);
+        copy_rows(ring + s * kStage + kSide, v_at, v, there);
       }
       if (p.num_blocks > 0) {
         const uint32_t n = block < 0 ? 0 : 4, at = max(block, 0);
@@ -613,11 +634,11 @@ constexpr Variant variant8(bool f32, int hd, int heads) {
   if (hd == 256) return {6, 2, 32};
   if (hd == 128) return {8, 3, 32};
   if (heads == 16) return hd == 64 ? Variant{12, 3, 32} : Variant{12, 4, 32};
-  return hd == 64 ? Variant{f32 ? 12 : 14, 3, 32} : Variant{16, 4, 32};
+  return hd == 64 ? (f32 ? Variant{12, 3, 32} : Variant{16, 2, 32}) : Variant{16, 4, 32};
 }
 // query heads of a unit: 16 where a KV head has more than eight and registers allow it
 constexpr int heads8(bool f32, int hd, int group) { return !f32 && hd <= 128 && group > 8 ? 16 : 8; }
-constexpr int kSeqCost8 = 96;
+constexpr int kSeqCost8 = 80;
 
 template <int PT, int DT, int HD, int NB>
 int launch_walk8(const Params &p, const Shape &s, cudaStream_t st) {

@@ -42,6 +42,7 @@ struct Params {
   float scale_log2;  // scale * log2(e): scores are kept in base 2
   int n_seqs, n_kv, heads, group, chunks, units, ranges;
   int seq_cost;
+  int alone;  // parts that a warp joins by itself, at most 64
   int hd, block_size;
   uint32_t div_mul, div_shift;  // i / block_size = i div_mul >> div_shift
   int local;  // not 0: a CTA of so many warps per (sequence, unit), no ranges, no parts
@@ -543,6 +544,7 @@ inline void fill_params(const dkv_paged_decode_args &a, const Shape &s, int64_t 
   p.n_seqs = a.seqs.n_seqs, p.n_kv = k.n_heads, p.heads = a.n_q_heads, p.group = a.n_q_heads / k.n_heads;
   p.chunks = s.chunks, p.units = s.units, p.ranges = s.ranges;
   p.seq_cost = s.seq_cost;
+  p.alone = 64;
   p.local = s.local;
   p.hd = k.head_dim, p.block_size = k.block_size;
   // for i < 2^31 and 2^(s - 1) < block_size <= 2^s: mul = floor(2^(31 + s) / block_size) + 1 is off by at
