@@ -3,6 +3,8 @@
 //   dkv_scatter_paged_quant  value + delta for the rows of every sequence, quantised again
 //   dkv_gather_paged_quant   the values of every sequence's rows
 // The layouts and the page arithmetic are those of the paged scatter / gather (src/deltakv/paged.py:8-70).
+#include <type_traits>
+
 #include "code8.cuh"
 #include "paged_rows.cuh"
 
@@ -25,8 +27,9 @@ struct Side {
   int64_t scale_block, scale_head;
 };
 
-// Rows of one call.  A run is the rows that follow one another in one block; a warp has a run's K or V of one
-// head, and with it alone the head's scale in that block.
+// Rows of one call.  A run is the rows that follow one another in one block.  A CTA looks through a window of rows for
+// the runs that begin there; each of its warps takes the K or V of a run's head, and with it alone the head's scale in that
+// block.  (grid: the chunks of heads and sides of a window are neighbours.)
 struct Store {
   Side side[2];
   int64_t n_rows, n_blocks, n_slots;
@@ -38,13 +41,32 @@ struct Store {
   int32_t *status;
   int heads, hd, block_size;
   Rotary rot;
-  int window;   // rows that a warp looks through for the first ones of runs
+  int window;   // rows that a CTA looks through for the first ones of runs
   int narrow;   // the cache's slots fit 32 bits
-  int64_t ctas; // of the store; behind them q's
+  int pairs;    // heads times sides
+  int chunks;   // CTAs of a window, with `each` pairs
+  int each;
+  int64_t ctas; // of the store
+  uint32_t spread;  // every so many-th CTA is one of them, the others are q's
 };
 
 constexpr int kThreads = 128;
-constexpr int kItems = 4;  // pieces of two times VEC columns that a lane holds at once
+constexpr int kItems = 2;   // pieces of two times VEC columns that a lane holds at once
+constexpr int kStaged = 4;  // and that wait in shared memory
+constexpr int kResident = 5;  // CTAs of an SM at least: leaves a thread 96 registers
+
+// the larger magnitude; NaN stays
+__device__ __forceinline__ float larger(float top, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(x)));
+  return r;
+}
+// strides that pieces of 8 columns take are below 2^31 (the host checks)
+template <int VEC>
+__device__ __forceinline__ int64_t times(int n, int64_t stride) {
+  return VEC > 1 ? static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * static_cast<uint32_t>(stride))
+                 : n * stride;
+}
 
 // block of a row's slot, -1 for none
 __device__ __forceinline__ int64_t row_block(const Store &s, int64_t row) {
@@ -99,186 +121,339 @@ struct Codes<1> {
 };
 static_assert(sizeof(Codes<8>) == 8, "eight columns are one load");
 
+// What stays of a block whose head's scale moves from held to scale, by the lanes of a warp.  mine: bit i of lane l says
+// that slot 32 l + i is being stored.
+template <int PDT, int VEC>
+__device__ __forceinline__ void scale_again(const Store &s, const Side &side, uint8_t *pages, float held, float by, uint32_t mine,
+                                            int lane) {
+  constexpr int kAtOnce = 4;
+  const int units = (s.hd + VEC - 1) / VEC, all = s.block_size * units;
+  for (int i0 = 0; i0 < all; i0 += 32 * kAtOnce) {
+    Codes<VEC> c[kAtOnce];
+    int o[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int i = i0 + k * 32 + lane;
+      const int u = min(i, all - 1) / units;
+      const bool stored = __shfl_sync(0xffffffffu, mine, u >> 5) >> (u & 31) & 1;
+      o[k] = i < all && !stored ? u : -1;
+      if (o[k] >= 0) c[k].load(pages + times<VEC>(u, side.slot) + (i - u * units) * VEC);
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (o[k] < 0) continue;
+      float y[VEC];
+      c[k].template get<PDT>(y);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y[e] = __fmul_rn(y[e], held);
+      c[k].template set<PDT>(y, by);
+      c[k].store(pages + times<VEC>(o[k], side.slot) + (i0 + k * 32 + lane - o[k] * units) * VEC);
+    }
+  }
+}
+
+// A lane's piece of a row: as read, and its values.
+template <int SDT, int PDT, int VEC>
+struct Piece {
+  Raw<SDT, VEC> raw[2];
+  Codes<VEC> old[2];
+  int slot, pos;  // slot in the block; -1: nothing to store
+  template <bool kPatch>
+  __device__ __forceinline__ void load(const Store &s, const Side &side, const typename Elem<SDT>::T *src, const uint8_t *pages,
+                                       const Columns &at, int64_t row, int r, int64_t block) {
+    src += times<VEC>(r, side.src_row);
+    raw[0].load(src + at.one);
+    if (at.pair) raw[1].load(src + at.two);
+    pos = 0;
+    if (kPatch) {
+      slot = r;
+      old[0].load(pages + times<VEC>(r, side.slot) + at.one);
+      if (at.pair) old[1].load(pages + times<VEC>(r, side.slot) + at.two);
+    } else {
+      slot = slot_in(s, row + r, block);
+      if (s.cos_t) pos = s.positions[row + r];
+    }
+  }
+  __device__ __forceinline__ void check(const Store &s) {  // a position outside the tables: the row stores nothing
+    if (slot >= 0 && s.cos_t && (pos < 0 || pos >= s.rope_max_pos)) {
+      record_error(s.status, DKV_ERR_ROPE_RANGE);
+      slot = -1;
+    }
+  }
+  template <bool kPatch>
+  __device__ __forceinline__ void values(const Store &s, const Rotary &rot, const Columns &at, float held, float(&lo)[VEC],
+                                         float(&hi)[VEC]) const {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) lo[e] = raw[0].get(e), hi[e] = at.pair ? raw[1].get(e) : 0.f;
+    if (kPatch) {
+      float y[VEC];
+      old[0].template get<PDT>(y);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) lo[e] = __fadd_rn(__fmul_rn(y[e], held), lo[e]);
+      if (at.pair) {
+        old[1].template get<PDT>(y);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) hi[e] = __fadd_rn(__fmul_rn(y[e], held), hi[e]);
+      }
+    } else if (at.turn) {
+      Raw<DKV_F32, VEC> c, sn;
+      const int64_t angle = static_cast<int64_t>(pos) * (rot.dim / 2) + at.angle;
+      c.load(s.cos_t + angle), sn.load(s.sin_t + angle);
+      step::turn<VEC>(lo, hi, c, sn, rot.interleaved);
+    }
+  }
+};
+
+template <int PDT, int VEC>
+__device__ __forceinline__ void store_piece(uint8_t *dst, const Columns &at, const float(&lo)[VEC], const float(&hi)[VEC],
+                                            float by) {
+  Codes<VEC> c;
+  c.template set<PDT>(lo, by), c.store(dst + at.one);
+  if (at.pair) c.template set<PDT>(hi, by), c.store(dst + at.two);
+}
+
+// Values of a warp between the two passes over a run: pieces of the lanes, in 16-byte parts of which neighbouring lanes have
+// neighbouring ones, and their slots.
+template <int VEC>
+struct Stage {
+  static constexpr int kParts = VEC == 1 ? 1 : VEC / 4;  // of each of a piece's two halves
+  using Part = typename std::conditional<VEC == 1, float, float4>::type;
+  Part part[kStaged][2][kParts][32];
+  int slot[kStaged][32];  // -1: nothing to store
+  __device__ __forceinline__ void put(int k, int half, int lane, const float(&x)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i)
+      if constexpr (VEC == 1)
+        part[k][half][i][lane] = x[0];
+      else
+        part[k][half][i][lane] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  }
+  __device__ __forceinline__ void get(int k, int half, int lane, float(&x)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i)
+      if constexpr (VEC == 1) {
+        x[0] = part[k][half][i][lane];
+      } else {
+        const float4 v = part[k][half][i][lane];
+        x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+      }
+  }
+};
+
 // A run of n rows from `row` on, in `block`; kPatch: the block's first n slots, whose values the rows are added to.
+// A lane has one piece of two times VEC columns of every so many-th row.  A run that fits the warp's kStaged pieces a lane (16
+// rows of 128 columns) is read once, its values wait in shared memory for the scale; longer runs are read again, out of L1
+// or L2, and worked out twice.
 template <int SDT, int PDT, int VEC, bool kPatch>
 __device__ __forceinline__ void store_run(const Store &s, const Side &side, int h, bool turns, int64_t row, int n,
-                                          int64_t block, int lane) {
+                                          int64_t block, Stage<VEC> &stage, int lane) {
   using ST = typename Elem<SDT>::T;
   uint8_t *pages = side.pages + block * side.block + h * side.head;
   float *scale_at = side.scale + block * side.scale_block + h * side.scale_head;
   const ST *src = static_cast<const ST *>(side.src) + row * side.src_row + h * side.src_head;
   const Rotary rot = turns ? s.rot : Rotary{0, 0};
   const int pieces = step::pieces_of(rot, s.hd, VEC);
-  const int items = n * pieces;
+  const int wide = min(pieces, 32), rows_at_once = 32 / wide;  // lanes of a row
+  const int my_row = lane / wide, my_piece = lane - my_row * wide;
+  const int chunk_rows = rows_at_once * kItems;
+  const bool once = pieces <= 32 && n <= rows_at_once * kStaged;
   const float held = *scale_at;
 
-  float x[kItems][2][VEC];
-  int at_slot[kItems];  // -1: nothing to store
-  Columns at[kItems];
-  // the values of items i0 + lane, i0 + 32 + lane, ...
-  auto load = [&](int i0) {
-    Raw<SDT, VEC> raw[kItems][2];
-    Codes<VEC> old[kItems][2];
-    int r[kItems], pos[kItems];
-#pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const int i = i0 + k * 32 + lane;
-      at_slot[k] = -1, pos[k] = 0, r[k] = i / pieces;
-      if (i >= items) continue;
-      at[k] = step::columns_of<VEC>(rot, s.hd, i - r[k] * pieces);
-      const ST *p = src + r[k] * side.src_row;
-      raw[k][0].load(p + at[k].one);
-      if (at[k].pair) raw[k][1].load(p + at[k].two);
-      if (kPatch) {
-        at_slot[k] = r[k];
-        old[k][0].load(pages + r[k] * side.slot + at[k].one);
-        if (at[k].pair) old[k][1].load(pages + r[k] * side.slot + at[k].two);
-      } else {
-        at_slot[k] = slot_in(s, row + r[k], block);
-        if (s.cos_t) pos[k] = s.positions[row + r[k]];
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      if (at_slot[k] >= 0) {
-        if (!kPatch && s.cos_t && (pos[k] < 0 || pos[k] >= s.rope_max_pos)) {
-          record_error(s.status, DKV_ERR_ROPE_RANGE);
-          at_slot[k] = -1;
-        }
-      }
-      if (at_slot[k] < 0) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) x[k][0][e] = x[k][1][e] = 0.f;
-        continue;
-      }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) x[k][0][e] = raw[k][0].get(e), x[k][1][e] = at[k].pair ? raw[k][1].get(e) : 0.f;
-      if (kPatch) {
-        float y[VEC];
-        old[k][0].template get<PDT>(y);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) x[k][0][e] = __fadd_rn(__fmul_rn(y[e], held), x[k][0][e]);
-        if (at[k].pair) {
-          old[k][1].template get<PDT>(y);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) x[k][1][e] = __fadd_rn(__fmul_rn(y[e], held), x[k][1][e]);
-        }
-      } else if (at[k].turn) {
-        Raw<DKV_F32, VEC> c, sn;
-        const int64_t angle = static_cast<int64_t>(pos[k]) * (rot.dim / 2) + at[k].angle;
-        c.load(s.cos_t + angle), sn.load(s.sin_t + angle);
-        step::turn<VEC>(x[k][0], x[k][1], c, sn, rot.interleaved);
-      }
-    }
-  };
-  uint32_t top = 0;
+  float top = 0.f, by = 0.f, scale = 0.f;
   bool begun = false;
-  for (int i0 = 0; i0 < items; i0 += 32 * kItems) {
-    load(i0);
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {  // the largest value; then the codes
+    int at_stage = 0;
+#pragma unroll 1
+    for (int p0 = 0; p0 < pieces; p0 += 32) {
+      const bool inside = my_row < rows_at_once && p0 + my_piece < pieces;
+      const Columns at = step::columns_of<VEC>(rot, s.hd, min(p0 + my_piece, pieces - 1));
+#pragma unroll 1
+      for (int r0 = 0; r0 < n; r0 += chunk_rows) {
+        if (pass == 0 || !once) {
+          Piece<SDT, PDT, VEC> piece[kItems];
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      begun |= at_slot[k] == 0;
+          for (int k = 0; k < kItems; ++k) {
+            const int r = r0 + k * rows_at_once + my_row;
+            piece[k].slot = -1;
+            if (inside && r < n) piece[k].template load<kPatch>(s, side, src, pages, at, row, r, block);
+          }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        top = max(top, max(__float_as_uint(x[k][0][e]) & 0x7fffffffu, __float_as_uint(x[k][1][e]) & 0x7fffffffu));
-    }
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  // nothing is kept: a block that a token begins, or one that is patched whole
-  begun = kPatch ? n == s.block_size : __any_sync(0xffffffffu, begun);
-  const float scale = code8::scale_for<PDT>(top, begun ? 0.f : held);
-  const float by = code8::inverse_of(scale);
-
-  if (!begun && !(scale == held)) {  // what stays of the block, in the new scale
-    uint32_t mine = 0;  // bit i of lane l: slot 32 l + i is stored by this run
-    if (kPatch) {
-      const int past = n - lane * 32;
-      mine = past >= 32 ? 0xffffffffu : past > 0 ? (1u << past) - 1 : 0u;
-    } else {
-      for (int i = 0; i < n; ++i) {
-        const int o = slot_in(s, row + i, block);
-        if (o >> 5 == lane) mine |= 1u << (o & 31);
+          for (int k = 0; k < kItems; ++k) {
+            if (!kPatch) piece[k].check(s);
+            stage.slot[at_stage + k][lane] = piece[k].slot;
+            if (piece[k].slot < 0) continue;
+            begun |= piece[k].slot == 0;
+            float lo[VEC], hi[VEC];
+            piece[k].template values<kPatch>(s, rot, at, held, lo, hi);
+            stage.put(at_stage + k, 0, lane, lo), stage.put(at_stage + k, 1, lane, hi);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) top = larger(larger(top, lo[e]), hi[e]);
+          }
+        }
+        if (pass == 1) {
+#pragma unroll
+          for (int k = 0; k < kItems; ++k) {
+            const int slot = stage.slot[at_stage + k][lane];
+            if (slot < 0) continue;
+            float lo[VEC], hi[VEC];
+            stage.get(at_stage + k, 0, lane, lo), stage.get(at_stage + k, 1, lane, hi);
+            store_piece<PDT, VEC>(pages + times<VEC>(slot, side.slot), at, lo, hi, by);
+          }
+        }
+        if (once) at_stage += kItems;
       }
     }
-    const int units = (s.hd + VEC - 1) / VEC, all = s.block_size * units;
-    for (int i0 = 0; i0 < all; i0 += 32 * 8) {
-      Codes<VEC> c[8];
-      int o[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int i = i0 + k * 32 + lane;
-        const int u = min(i, all - 1) / units;
-        const bool stored = __shfl_sync(0xffffffffu, mine, u >> 5) >> (u & 31) & 1;
-        o[k] = i < all && !stored ? u : -1;
-        if (o[k] >= 0) c[k].load(pages + u * side.slot + (i - u * units) * VEC);
+    if (pass == 1) break;
+    // (magnitudes compare as their bits do; NaN is above all)
+    const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    // nothing is kept: a block that a token begins, or one that is patched whole
+    begun = kPatch ? n == s.block_size : __any_sync(0xffffffffu, begun) != 0;
+    scale = code8::scale_for<PDT>(top_bits, begun ? 0.f : held);
+    by = code8::inverse_of(scale);
+    if (!begun && !(scale == held)) {
+      uint32_t mine = 0;
+      if (kPatch) {
+        const int past = n - lane * 32;
+        mine = past >= 32 ? 0xffffffffu : past > 0 ? (1u << past) - 1 : 0u;
+      } else {
+        for (int i = 0; i < n; ++i) {
+          const int o = slot_in(s, row + i, block);
+          if (o >> 5 == lane) mine |= 1u << (o & 31);
+        }
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (o[k] < 0) continue;
-        float y[VEC];
-        c[k].template get<PDT>(y);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) y[e] = __fmul_rn(y[e], held);
-        c[k].template set<PDT>(y, by);
-        c[k].store(pages + o[k] * side.slot + (i0 + k * 32 + lane - o[k] * units) * VEC);
-      }
-    }
-  }
-  for (int i0 = 0; i0 < items; i0 += 32 * kItems) {
-    if (items > 32 * kItems) load(i0);
-#pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      if (at_slot[k] < 0) continue;
-      uint8_t *dst = pages + at_slot[k] * side.slot;
-      Codes<VEC> c;
-      c.template set<PDT>(x[k][0], by), c.store(dst + at[k].one);
-      if (at[k].pair) c.template set<PDT>(x[k][1], by), c.store(dst + at[k].two);
+      scale_again<PDT, VEC>(s, side, pages, held, by, mine, lane);
     }
   }
   if (lane == 0) *scale_at = scale;
 }
 
-// Bound by memory: k, v and q are read once, codes and q written once.
-template <int SDT, int PDT, int VEC>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ Store s, const __grid_constant__ Append q) {
-  begin_overlapped();
-  if (blockIdx.x >= s.ctas) {
-    step::append_rows<SDT, SDT, VEC, true>(q, (static_cast<int64_t>(blockIdx.x) - s.ctas) * kThreads + threadIdx.x);
-    return;
-  }
-  const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int per = 2 * s.heads;
-  const int64_t r0 = item / per * s.window;
-  if (r0 >= s.n_rows) return;
-  const int in = static_cast<int>(item % per), which = in >= s.heads, h = which ? in - s.heads : in;
-  const int64_t row = r0 + lane;
-  int64_t block = -1;
-  if (lane < s.window && row < s.n_rows) {
-    block = row_block(s, row);
-    if (block < 0 && in == 0 && s.slots[row] >= 0) record_error(s.status, DKV_ERR_PAGE_RANGE);
-  }
-  int64_t before = __shfl_up_sync(0xffffffffu, block, 1);
-  if (lane == 0) before = r0 > 0 ? row_block(s, r0 - 1) : -1;
-  uint32_t first = __ballot_sync(0xffffffffu, block >= 0 && block != before);
+// The runs of a CTA's window and its pairs of head and side, dealt to its warps: f(i, n, block, pair) for the run that begins
+// at the window's row i.  `first` has a bit for each such row, lane i their n and block.
+template <typename F>
+__device__ __forceinline__ void each_run(const Store &s, int chunk, uint32_t first, int n, int64_t block, F f) {
+  const int pair0 = chunk * s.each, pairs = min(s.each, s.pairs - pair0);
+  int left = static_cast<int>(threadIdx.x >> 5);  // this warp's next pair, counted from the current run's first
   while (first) {
     const int i = __ffs(first) - 1;
     first &= first - 1;
-    const int64_t mine = __shfl_sync(0xffffffffu, block, i);
-    int64_t end = r0 + i + 1;  // the rows after it in the same block
-    while (true) {
+    const int rows = __shfl_sync(0xffffffffu, n, i);
+    const int64_t at = __shfl_sync(0xffffffffu, block, i);
+    for (; left < pairs; left += kThreads / 32) f(i, rows, at, pair0 + left);
+    left -= pairs;
+  }
+}
+
+// The runs of a window that all have one row (a decode step's): a few lanes have each, so that a warp has several at once.
+template <int SDT, int PDT, int VEC>
+__device__ __forceinline__ void store_single_rows(const Store &s, int chunk, uint32_t first, int64_t block, int64_t r0, int lane) {
+  using ST = typename Elem<SDT>::T;
+  const int pair0 = chunk * s.each, pairs = min(s.each, s.pairs - pair0);
+  const int all = __popc(first) * pairs;
+  const int most = max(step::pieces_of(s.rot, s.hd, VEC), step::pieces_of(Rotary{0, 0}, s.hd, VEC));
+  const int wide = most <= 1 ? 1 : 1 << (32 - __clz(most - 1));  // lanes of a row
+  const int groups = 32 / wide, mine_in = lane & (wide - 1);
+  const int nth = __fns(first, 0, lane + 1);  // the window's row with the lane-th run
+  for (int base = static_cast<int>(threadIdx.x >> 5) * groups; base < all; base += kThreads / 32 * groups) {
+    const int item = min(base + lane / wide, all - 1);
+    const int run = item / pairs, pair = pair0 + item - run * pairs;
+    const int i = __shfl_sync(0xffffffffu, nth, run);
+    const int64_t at_block = __shfl_sync(0xffffffffu, block, i);
+    const int which = pair >= s.heads, h = which ? pair - s.heads : pair;
+    const Side &side = s.side[which];
+    const Rotary rot = which == 0 ? s.rot : Rotary{0, 0};
+    const int pieces = step::pieces_of(rot, s.hd, VEC);
+    const Columns at = step::columns_of<VEC>(rot, s.hd, min(mine_in, pieces - 1));
+    uint8_t *pages = side.pages + at_block * side.block + h * side.head;
+    float *scale_at = side.scale + at_block * side.scale_block + h * side.scale_head;
+    const float held = *scale_at;
+    Piece<SDT, PDT, VEC> piece;
+    piece.template load<false>(s, side, static_cast<const ST *>(side.src) + (r0 + i) * side.src_row + h * side.src_head, pages, at,
+                               r0 + i, 0, at_block);
+    piece.check(s);
+    const bool there = base + lane / wide < all && piece.slot >= 0;
+    float lo[VEC], hi[VEC], top = 0.f;
+    if (there) {
+      piece.template values<false>(s, rot, at, held, lo, hi);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) top = larger(larger(top, lo[e]), hi[e]);
+    }
+    uint32_t top_bits = __float_as_uint(top);
+    for (int k = wide / 2; k > 0; k >>= 1) top_bits = max(top_bits, __shfl_xor_sync(0xffffffffu, top_bits, k));
+    const bool begun = piece.slot == 0;
+    const float scale = code8::scale_for<PDT>(top_bits, begun ? 0.f : held);
+    const float by = code8::inverse_of(scale);
+    uint32_t moved = __ballot_sync(0xffffffffu, there && mine_in == 0 && !begun && !(scale == held));
+    while (moved) {  // the warp scales again what the block of one row holds, after the other
+      const int from = __ffs(moved) - 1;
+      moved &= moved - 1;
+      const int its_pair = __shfl_sync(0xffffffffu, pair, from), its_slot = __shfl_sync(0xffffffffu, piece.slot, from);
+      const int64_t its_block = __shfl_sync(0xffffffffu, at_block, from);
+      const Side &its = s.side[its_pair >= s.heads];
+      scale_again<PDT, VEC>(s, its, its.pages + its_block * its.block + (its_pair >= s.heads ? its_pair - s.heads : its_pair) * its.head,
+                            __shfl_sync(0xffffffffu, held, from), __shfl_sync(0xffffffffu, by, from),
+                            its_slot >> 5 == lane ? 1u << (its_slot & 31) : 0u, lane);
+    }
+    if (there && mine_in < pieces) {
+      store_piece<PDT, VEC>(pages + times<VEC>(piece.slot, side.slot), at, lo, hi, by);
+      if (mine_in == 0) *scale_at = scale;
+    }
+  }
+}
+
+// Bound by memory: k, v and q are read once, codes and q written once.  The store's CTAs, which wait for memory several
+// times, lie evenly among those of q, which only stream.
+template <int SDT, int PDT, int VEC>
+__global__ void __launch_bounds__(kThreads, kResident) append_kernel(const __grid_constant__ Store s,
+                                                                     const __grid_constant__ Append q) {
+  __shared__ Stage<VEC> stage[kThreads / 32];
+  begin_overlapped();
+  const uint32_t turn = blockIdx.x / s.spread;
+  const bool stores = turn < s.ctas && blockIdx.x == turn * s.spread;
+  if (!stores) {
+    const int64_t cta = static_cast<int64_t>(blockIdx.x) - min(static_cast<int64_t>(turn) + 1, s.ctas);
+    step::append_rows<SDT, SDT, VEC, true>(q, cta * kThreads + threadIdx.x);
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  const int64_t r0 = static_cast<int64_t>(turn / s.chunks) * s.window;
+  const int chunk = static_cast<int>(turn % s.chunks);
+  const int64_t row = r0 + lane;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(s.window), s.n_rows - r0));
+  int64_t block = -1;
+  if (lane < rows) {
+    block = row_block(s, row);
+    if (block < 0 && chunk == 0 && threadIdx.x < 32 && s.slots[row] >= 0) record_error(s.status, DKV_ERR_PAGE_RANGE);
+  }
+  int64_t before = __shfl_up_sync(0xffffffffu, block, 1);
+  if (lane == 0) before = r0 > 0 ? row_block(s, r0 - 1) : -1;
+  const uint32_t first = __ballot_sync(0xffffffffu, block >= 0 && block != before);
+  if (first == 0) return;
+  const uint32_t more = __ballot_sync(0xffffffffu, block >= 0 && block == before);  // rows that go on with a run
+  int n = __ffs(~(lane == 31 ? 0u : more >> (lane + 1)));
+  const int last = 31 - __clz(first);  // the run that may go on behind the window
+  if (last + __shfl_sync(0xffffffffu, n, last) == rows) {
+    const int64_t mine = __shfl_sync(0xffffffffu, block, last);
+    int64_t end = r0 + rows;
+    while (end - (r0 + last) < s.block_size) {
       const int64_t at = end + lane;
       const uint32_t same = __ballot_sync(0xffffffffu, at < s.n_rows && row_block(s, at) == mine);
-      if (same != 0xffffffffu) {
-        end += __ffs(~same) - 1;
-        break;
-      }
-      end += 32;
+      end += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+      if (same != 0xffffffffu) break;
     }
-    const int64_t n = min(end - (r0 + i), static_cast<int64_t>(s.block_size));  // more: a slot came twice
-    store_run<SDT, PDT, VEC, false>(s, s.side[which], h, which == 0 && s.cos_t != nullptr, r0 + i, static_cast<int>(n), mine,
-                                    lane);
+    if (lane == last) n = static_cast<int>(end - (r0 + last));
   }
+  n = min(n, s.block_size);  // more: a slot came twice
+  if (more == 0 && __shfl_sync(0xffffffffu, n, last) == 1 &&
+      max(step::pieces_of(s.rot, s.hd, VEC), step::pieces_of(Rotary{0, 0}, s.hd, VEC)) <= 32) {
+    store_single_rows<SDT, PDT, VEC>(s, chunk, first, block, r0, lane);
+    return;
+  }
+  each_run(s, chunk, first, n, block, [&](int i, int rows_of, int64_t at, int pair) {
+    const int which = pair >= s.heads;
+    store_run<SDT, PDT, VEC, false>(s, s.side[which], which ? pair - s.heads : pair, which == 0 && s.cos_t != nullptr, r0 + i,
+                                    rows_of, at, stage[threadIdx.x >> 5], lane);
+  });
 }
 
 // the sequence of row r (its last one where empty ones begin there too), or n_seqs for a row behind the last
@@ -305,14 +480,14 @@ __device__ __forceinline__ int64_t page_of(const dkv_seq_batch &q, int64_t n_blo
   return id;
 }
 
+// Bound by memory: the rows and the codes are read once, codes written once.
 template <int SDT, int PDT, int VEC>
-__global__ void __launch_bounds__(kThreads) patch_kernel(const __grid_constant__ Store s) {
+__global__ void __launch_bounds__(kThreads, kResident) patch_kernel(const __grid_constant__ Store s) {
+  __shared__ Stage<VEC> stage[kThreads / 32];
   begin_overlapped();
   const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t r0 = item / s.heads * s.window;
-  if (r0 >= s.n_rows) return;
-  const int h = static_cast<int>(item % s.heads);
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x / s.chunks) * s.window;
+  const int chunk = static_cast<int>(blockIdx.x % s.chunks);
   const int64_t row = r0 + lane;
   int64_t block = -1;
   int n = 0;
@@ -326,16 +501,13 @@ __global__ void __launch_bounds__(kThreads) patch_kernel(const __grid_constant__
         block = page_of(s.seqs, s.n_blocks, b, i / s.block_size, s.status);
       }
     }
-    if (row == s.n_rows - 1 && h == 0 && s.seqs.cu_seqlens[s.seqs.n_seqs] > s.n_rows)
+    if (row == s.n_rows - 1 && chunk == 0 && s.seqs.cu_seqlens[s.seqs.n_seqs] > s.n_rows)
       record_error(s.status, DKV_ERR_INVALID_ARGUMENT);
   }
-  uint32_t first = __ballot_sync(0xffffffffu, block >= 0);
-  while (first) {
-    const int i = __ffs(first) - 1;
-    first &= first - 1;
-    store_run<SDT, PDT, VEC, true>(s, s.side[0], h, false, r0 + i, __shfl_sync(0xffffffffu, n, i),
-                                   __shfl_sync(0xffffffffu, block, i), lane);
-  }
+  const uint32_t first = __ballot_sync(0xffffffffu, block >= 0);
+  each_run(s, chunk, first, n, block, [&](int i, int rows_of, int64_t at, int head) {
+    store_run<SDT, PDT, VEC, true>(s, s.side[0], head, false, r0 + i, rows_of, at, stage[threadIdx.x >> 5], lane);
+  });
 }
 
 // ---------------------------------------------------------------------------------------
@@ -459,14 +631,22 @@ Side side_of(const dkv_paged_cache &c, const dkv_page_scales &s, const void *src
 int64_t source_bits(const Side &x, int64_t size) {
   return reinterpret_cast<intptr_t>(x.src) | x.src_row * size | x.src_head * size;
 }
+bool short_strides(const Side &x) { return x.src_row >= 0 && x.src_row <= INT32_MAX && x.slot >= 0 && x.slot <= INT32_MAX; }
 int64_t page_bits(const Side &x) { return reinterpret_cast<intptr_t>(x.pages) | x.block | x.slot | x.head; }
 
-// Rows that a warp looks through: a row each as long as all warps that come of it run about at once (64 an SM), else up to
-// 16, so that prefill rows, of which one in a block's worth begins a run, do not launch a warp each.
-int window_of(int64_t rows, int64_t warps_a_row, int sms) {
-  int w = 1;
-  while (w < 16 && rows * warps_a_row > static_cast<int64_t>(sms) * 64 * w) w *= 2;
-  return w;
+// How rows and pairs of head and side are dealt: as many rows a CTA (up to 16: one in a block's worth begins a run of a
+// prefill) and as few CTAs a window as still give 8 CTAs an SM.
+void deal(int64_t rows, int pairs, int sms, Store *s) {
+  constexpr int kWarps = kThreads / 32;
+  const int64_t want = static_cast<int64_t>(sms) * 8;
+  s->pairs = pairs;
+  s->window = 1;
+  while (s->window < 16 && rows / (2 * s->window) * ((pairs + kWarps - 1) / kWarps) >= want) s->window *= 2;
+  const int64_t windows = (rows + s->window - 1) / s->window;
+  const int64_t most = (pairs + kWarps - 1) / kWarps, chunks = (want + windows - 1) / windows;
+  s->each = static_cast<int>((pairs + (chunks < most ? chunks : most) - 1) / (chunks < most ? chunks : most));
+  s->chunks = (pairs + s->each - 1) / s->each;
+  s->ctas = windows * s->chunks;
 }
 
 }  // namespace quant
@@ -516,15 +696,15 @@ extern "C" int dkv_append_paged_quant(const dkv_append_args *args, const dkv_rot
     bits |= reinterpret_cast<intptr_t>(g.q) | reinterpret_cast<intptr_t>(g.q_out) |
             (q.src_row[0] | q.src_head[0] | q.dst_row[0] | q.dst_head[0]) * size;
   const bool wide = step::whole_pieces(rot, kp.head_dim, 8) && kp.head_dim % 16 == 0 && bits % 16 == 0 &&
-                    (quant::page_bits(s.side[0]) | quant::page_bits(s.side[1])) % 8 == 0;
-  s.window = quant::window_of(g.n_rows, 2 * kp.n_heads, sms);
-  const int64_t warps = (g.n_rows + s.window - 1) / s.window * 2 * kp.n_heads;
-  s.ctas = (warps * 32 + quant::kThreads - 1) / quant::kThreads;
+                    (quant::page_bits(s.side[0]) | quant::page_bits(s.side[1])) % 8 == 0 && quant::short_strides(s.side[0]) &&
+                    quant::short_strides(s.side[1]);
+  quant::deal(g.n_rows, 2 * kp.n_heads, sms, &s);
   const int64_t threads = q.heads[0] == 0 ? 0 : g.n_rows * ((q.heads[0] + step::kHeads - 1) / step::kHeads) *
                                                     step::pieces_of(rot, kp.head_dim, wide ? 8 : 1);
   q.wide = threads > UINT32_MAX;
   const int64_t ctas = s.ctas + (threads + quant::kThreads - 1) / quant::kThreads;
   if (ctas > INT32_MAX) return DKV_ERR_UNSUPPORTED;
+  s.spread = static_cast<uint32_t>(ctas / s.ctas);
   static_assert(quant::kThreads == step::kAppThreads, "one launch for both");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 #define DKV_QUANT_CASE(S, P)                                                                                  \
@@ -566,10 +746,9 @@ extern "C" int dkv_scatter_paged_quant(const void *delta, int32_t delta_dtype, i
   s.heads = cache->n_heads, s.hd = cache->head_dim, s.block_size = cache->block_size;
   const int64_t size = delta_dtype == DKV_F32 ? 4 : 2;
   const bool wide = cache->head_dim % 16 == 0 && quant::source_bits(s.side[0], size) % 16 == 0 &&
-                    quant::page_bits(s.side[0]) % 8 == 0;
-  s.window = quant::window_of(n_rows, cache->n_heads, sms);
-  const int64_t warps = (n_rows + s.window - 1) / s.window * cache->n_heads;
-  const int64_t ctas = (warps * 32 + quant::kThreads - 1) / quant::kThreads;
+                    quant::page_bits(s.side[0]) % 8 == 0 && quant::short_strides(s.side[0]);
+  quant::deal(n_rows, cache->n_heads, sms, &s);
+  const int64_t ctas = s.ctas;
   if (ctas > INT32_MAX) return DKV_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 #define DKV_QUANT_CASE(S, P)                                                                               \
