@@ -26,14 +26,20 @@ struct Code<DKV_E4M3> {
   }
   // four values to four codes; they fit, NaN stays NaN
   static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {
-    uint16_t lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-    return static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
+    uint32_t w;
+    asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+        "mov.b32 %0, {l, h};\n\t}"
+        : "=r"(w)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+    return w;
   }
   static __device__ __forceinline__ void unpack(uint32_t w, float (&x)[4]) {
-    const uint32_t lo = e4m3x2_to_f16x2(w), hi = e4m3x2_to_f16x2(w >> 16);
-    x[0] = f16lo(lo), x[1] = f16hi(lo), x[2] = f16lo(hi), x[3] = f16hi(hi);
+    asm("{\n\t.reg .b16 l, h, a, b;\n\t.reg .b32 u, v;\n\tmov.b32 {l, h}, %4;\n\t"
+        "cvt.rn.f16x2.e4m3x2 u, l;\n\tcvt.rn.f16x2.e4m3x2 v, h;\n\t"
+        "mov.b32 {a, b}, u;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t"
+        "mov.b32 {a, b}, v;\n\tcvt.f32.f16 %2, a;\n\tcvt.f32.f16 %3, b;\n\t}"
+        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+        : "r"(w));
   }
 };
 template <>

@@ -3,8 +3,6 @@
 //   dkv_scatter_paged_quant  value + delta for the rows of every sequence, quantised again
 //   dkv_gather_paged_quant   the values of every sequence's rows
 // The layouts and the page arithmetic are those of the paged scatter / gather (src/deltakv/paged.py:8-70).
-#include <type_traits>
-
 #include "code8.cuh"
 #include "paged_rows.cuh"
 
@@ -55,11 +53,26 @@ constexpr int kItems = 2;   // pieces of two times VEC columns that a lane holds
 constexpr int kStaged = 4;  // and that wait in shared memory
 constexpr int kResident = 5;  // CTAs of an SM at least: leaves a thread 96 registers
 
-// the larger magnitude; NaN stays
-__device__ __forceinline__ float larger(float top, float x) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(x)));
-  return r;
+// The largest magnitude of several values, and whether all are finite (0 times anything else is NaN).
+struct Largest {
+  float top = 0.f;
+  uint64_t zero = 0;
+  __device__ __forceinline__ void add(uint64_t pair) {
+    float x, y;
+    f2unpack(pair, x, y);
+    top = fmaxf(fmaxf(top, fabsf(x)), fabsf(y));
+    zero = fma2(pair, 0ull, zero);
+  }
+  __device__ __forceinline__ uint32_t bits() const {  // of the magnitude; not finite: above all finite ones
+    float x, y;
+    f2unpack(zero, x, y);
+    return x + y == 0.f ? __float_as_uint(top) : 0x7fffffffu;
+  }
+};
+// pieces of 8 columns are always two
+template <int VEC>
+__device__ __forceinline__ bool paired(const Columns &at) {
+  return VEC > 1 || at.pair;
 }
 // strides that pieces of 8 columns take are below 2^31 (the host checks)
 template <int VEC>
@@ -78,6 +91,14 @@ __device__ __forceinline__ int slot_in(const Store &s, int64_t row, int64_t bloc
   return static_cast<int>(s.slots[row] - block * s.block_size);
 }
 
+// VEC values in pairs, as the packed fp32 operations of sm_100 take them (each rounds as the single one does); one value has a
+// zero beside it
+template <int VEC>
+struct Values {
+  static constexpr int kPairs = VEC == 1 ? 1 : VEC / 2;
+  uint64_t pair[kPairs];
+};
+
 // codes of VEC consecutive columns
 template <int VEC>
 struct Codes {
@@ -88,21 +109,26 @@ struct Codes {
   }
   __device__ __forceinline__ void store(uint8_t *dst) const { *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]); }
   template <int PT>
-  __device__ __forceinline__ void get(float (&x)[VEC]) const {
+  __device__ __forceinline__ Values<VEC> get() const {
+    Values<VEC> v;
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {
       float y[4];
       Code<PT>::unpack(w[i], y);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[4 * i + k] = y[k];
+      v.pair[2 * i] = f2pack(y[0], y[1]), v.pair[2 * i + 1] = f2pack(y[2], y[3]);
     }
+    return v;
   }
   template <int PT>
-  __device__ __forceinline__ void set(const float (&x)[VEC], float by) {
+  __device__ __forceinline__ void set(const Values<VEC> &v, float by) {
+    const uint64_t two = f2pack(by, by);
 #pragma unroll
-    for (int i = 0; i < VEC / 4; ++i)
-      w[i] = Code<PT>::pack(__fmul_rn(x[4 * i], by), __fmul_rn(x[4 * i + 1], by), __fmul_rn(x[4 * i + 2], by),
-                            __fmul_rn(x[4 * i + 3], by));
+    for (int i = 0; i < VEC / 4; ++i) {
+      float y[4];
+      f2unpack(mul2(v.pair[2 * i], two), y[0], y[1]);
+      f2unpack(mul2(v.pair[2 * i + 1], two), y[2], y[3]);
+      w[i] = Code<PT>::pack(y[0], y[1], y[2], y[3]);
+    }
   }
 };
 template <>
@@ -111,13 +137,17 @@ struct Codes<1> {
   __device__ __forceinline__ void load(const uint8_t *src) { w = *src; }
   __device__ __forceinline__ void store(uint8_t *dst) const { *dst = static_cast<uint8_t>(w); }
   template <int PT>
-  __device__ __forceinline__ void get(float (&x)[1]) const {
+  __device__ __forceinline__ Values<1> get() const {
     float y[4];
     Code<PT>::unpack(w, y);
-    x[0] = y[0];
+    return {{f2pack(y[0], 0.f)}};
   }
   template <int PT>
-  __device__ __forceinline__ void set(const float (&x)[1], float by) { w = Code<PT>::pack(__fmul_rn(x[0], by), 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void set(const Values<1> &v, float by) {
+    float x, y;
+    f2unpack(v.pair[0], x, y);
+    w = Code<PT>::pack(__fmul_rn(x, by), 0.f, 0.f, 0.f);
+  }
 };
 static_assert(sizeof(Codes<8>) == 8, "eight columns are one load");
 
@@ -142,11 +172,10 @@ __device__ __forceinline__ void scale_again(const Store &s, const Side &side, ui
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
       if (o[k] < 0) continue;
-      float y[VEC];
-      c[k].template get<PDT>(y);
+      Values<VEC> v = c[k].template get<PDT>();
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) y[e] = __fmul_rn(y[e], held);
-      c[k].template set<PDT>(y, by);
+      for (int e = 0; e < Values<VEC>::kPairs; ++e) v.pair[e] = mul2(v.pair[e], f2pack(held, held));
+      c[k].template set<PDT>(v, by);
       c[k].store(pages + times<VEC>(o[k], side.slot) + (i0 + k * 32 + lane - o[k] * units) * VEC);
     }
   }
@@ -158,20 +187,20 @@ struct Piece {
   Raw<SDT, VEC> raw[2];
   Codes<VEC> old[2];
   int slot, pos;  // slot in the block; -1: nothing to store
+  // src: the row's head, held: its slot (kPatch)
   template <bool kPatch>
-  __device__ __forceinline__ void load(const Store &s, const Side &side, const typename Elem<SDT>::T *src, const uint8_t *pages,
-                                       const Columns &at, int64_t row, int r, int64_t block) {
-    src += times<VEC>(r, side.src_row);
+  __device__ __forceinline__ void load(const Store &s, const typename Elem<SDT>::T *src, const uint8_t *held, const Columns &at,
+                                       int64_t row, int r, int64_t block) {
     raw[0].load(src + at.one);
-    if (at.pair) raw[1].load(src + at.two);
+    if (paired<VEC>(at)) raw[1].load(src + at.two);
     pos = 0;
     if (kPatch) {
       slot = r;
-      old[0].load(pages + times<VEC>(r, side.slot) + at.one);
-      if (at.pair) old[1].load(pages + times<VEC>(r, side.slot) + at.two);
+      old[0].load(held + at.one);
+      if (paired<VEC>(at)) old[1].load(held + at.two);
     } else {
-      slot = slot_in(s, row + r, block);
-      if (s.cos_t) pos = s.positions[row + r];
+      slot = slot_in(s, row, block);
+      if (s.cos_t) pos = s.positions[row];
     }
   }
   __device__ __forceinline__ void check(const Store &s) {  // a position outside the tables: the row stores nothing
@@ -181,62 +210,93 @@ struct Piece {
     }
   }
   template <bool kPatch>
-  __device__ __forceinline__ void values(const Store &s, const Rotary &rot, const Columns &at, float held, float(&lo)[VEC],
-                                         float(&hi)[VEC]) const {
+  __device__ __forceinline__ void values(const Store &s, const Rotary &rot, const Columns &at, float held, Values<VEC> &lo,
+                                         Values<VEC> &hi) const {
+    constexpr int kPairs = Values<VEC>::kPairs;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) lo[e] = raw[0].get(e), hi[e] = at.pair ? raw[1].get(e) : 0.f;
+    for (int e = 0; e < kPairs; ++e) {
+      lo.pair[e] = VEC == 1 ? f2pack(raw[0].get(0), 0.f) : f2pack(raw[0].get(2 * e), raw[0].get((2 * e + 1) % VEC));
+      hi.pair[e] = !paired<VEC>(at) ? 0
+                   : VEC == 1 ? f2pack(raw[1].get(0), 0.f)
+                              : f2pack(raw[1].get(2 * e), raw[1].get((2 * e + 1) % VEC));
+    }
     if (kPatch) {
-      float y[VEC];
-      old[0].template get<PDT>(y);
+      const uint64_t two = f2pack(held, held);
+      Values<VEC> y = old[0].template get<PDT>();
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) lo[e] = __fadd_rn(__fmul_rn(y[e], held), lo[e]);
-      if (at.pair) {
-        old[1].template get<PDT>(y);
+      for (int e = 0; e < kPairs; ++e) lo.pair[e] = add2(mul2(y.pair[e], two), lo.pair[e]);
+      if (paired<VEC>(at)) {
+        y = old[1].template get<PDT>();
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) hi[e] = __fadd_rn(__fmul_rn(y[e], held), hi[e]);
+        for (int e = 0; e < kPairs; ++e) hi.pair[e] = add2(mul2(y.pair[e], two), hi.pair[e]);
       }
     } else if (at.turn) {
       Raw<DKV_F32, VEC> c, sn;
       const int64_t angle = static_cast<int64_t>(pos) * (rot.dim / 2) + at.angle;
       c.load(s.cos_t + angle), sn.load(s.sin_t + angle);
-      step::turn<VEC>(lo, hi, c, sn, rot.interleaved);
+      if (VEC > 1 && rot.interleaved) {
+        float x[VEC], y[VEC];
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+          f2unpack(lo.pair[e], x[2 * e % VEC], x[(2 * e + 1) % VEC]);
+          f2unpack(hi.pair[e], y[2 * e % VEC], y[(2 * e + 1) % VEC]);
+        }
+        step::turn<VEC>(x, y, c, sn, true);
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+          lo.pair[e] = f2pack(x[2 * e % VEC], x[(2 * e + 1) % VEC]);
+          hi.pair[e] = f2pack(y[2 * e % VEC], y[(2 * e + 1) % VEC]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+          const uint64_t cc = f2pack(c.get(2 * e % VEC), c.get((2 * e + 1) % VEC));
+          const uint64_t ss = f2pack(sn.get(2 * e % VEC), sn.get((2 * e + 1) % VEC));
+          const uint64_t x = lo.pair[e], y = hi.pair[e];
+          lo.pair[e] = sub2(mul2(x, cc), mul2(y, ss));
+          hi.pair[e] = add2(mul2(y, cc), mul2(x, ss));
+        }
+      }
     }
   }
 };
 
 template <int PDT, int VEC>
-__device__ __forceinline__ void store_piece(uint8_t *dst, const Columns &at, const float(&lo)[VEC], const float(&hi)[VEC],
+__device__ __forceinline__ void store_piece(uint8_t *dst, const Columns &at, const Values<VEC> &lo, const Values<VEC> &hi,
                                             float by) {
   Codes<VEC> c;
   c.template set<PDT>(lo, by), c.store(dst + at.one);
-  if (at.pair) c.template set<PDT>(hi, by), c.store(dst + at.two);
+  if (paired<VEC>(at)) c.template set<PDT>(hi, by), c.store(dst + at.two);
 }
+
+// How a warp's lanes share rows: `wide` lanes a row (the pieces of a head, at most 32), several rows at once.
+struct Lanes {
+  int pieces, wide, rows, my_row, my_piece;
+  __device__ __forceinline__ Lanes(int pieces_, int lane) : pieces(pieces_), wide(min(pieces_, 32)) {
+    rows = 32 / wide;
+    my_row = lane / wide, my_piece = lane - my_row * wide;
+  }
+};
 
 // Values of a warp between the two passes over a run: pieces of the lanes, in 16-byte parts of which neighbouring lanes have
 // neighbouring ones, and their slots.
 template <int VEC>
 struct Stage {
   static constexpr int kParts = VEC == 1 ? 1 : VEC / 4;  // of each of a piece's two halves
-  using Part = typename std::conditional<VEC == 1, float, float4>::type;
-  Part part[kStaged][2][kParts][32];
+  ulonglong2 part[kStaged][2][kParts][32];
   int slot[kStaged][32];  // -1: nothing to store
-  __device__ __forceinline__ void put(int k, int half, int lane, const float(&x)[VEC]) {
+  __device__ __forceinline__ void put(int k, int half, int lane, const Values<VEC> &v) {
 #pragma unroll
     for (int i = 0; i < kParts; ++i)
-      if constexpr (VEC == 1)
-        part[k][half][i][lane] = x[0];
-      else
-        part[k][half][i][lane] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      part[k][half][i][lane] = make_ulonglong2(v.pair[2 * i], v.pair[(2 * i + 1) % Values<VEC>::kPairs]);
   }
-  __device__ __forceinline__ void get(int k, int half, int lane, float(&x)[VEC]) const {
+  __device__ __forceinline__ void get(int k, int half, int lane, Values<VEC> &v) const {
 #pragma unroll
-    for (int i = 0; i < kParts; ++i)
-      if constexpr (VEC == 1) {
-        x[0] = part[k][half][i][lane];
-      } else {
-        const float4 v = part[k][half][i][lane];
-        x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-      }
+    for (int i = 0; i < kParts; ++i) {
+      const ulonglong2 x = part[k][half][i][lane];
+      v.pair[2 * i] = x.x;
+      if (VEC > 1) v.pair[(2 * i + 1) % Values<VEC>::kPairs] = x.y;
+    }
   }
 };
 
@@ -245,38 +305,39 @@ struct Stage {
 // rows of 128 columns) is read once, its values wait in shared memory for the scale; longer runs are read again, out of L1
 // or L2, and worked out twice.
 template <int SDT, int PDT, int VEC, bool kPatch>
-__device__ __forceinline__ void store_run(const Store &s, const Side &side, int h, bool turns, int64_t row, int n,
-                                          int64_t block, Stage<VEC> &stage, int lane) {
+__device__ __forceinline__ void store_run(const Store &s, const Side &side, int h, const Rotary &rot, const Lanes &lanes, int64_t row,
+                                          int n, int64_t block, Stage<VEC> &stage, int lane) {
   using ST = typename Elem<SDT>::T;
   uint8_t *pages = side.pages + block * side.block + h * side.head;
   float *scale_at = side.scale + block * side.scale_block + h * side.scale_head;
   const ST *src = static_cast<const ST *>(side.src) + row * side.src_row + h * side.src_head;
-  const Rotary rot = turns ? s.rot : Rotary{0, 0};
-  const int pieces = step::pieces_of(rot, s.hd, VEC);
-  const int wide = min(pieces, 32), rows_at_once = 32 / wide;  // lanes of a row
-  const int my_row = lane / wide, my_piece = lane - my_row * wide;
-  const int chunk_rows = rows_at_once * kItems;
-  const bool once = pieces <= 32 && n <= rows_at_once * kStaged;
+  const int64_t src_step = times<VEC>(lanes.rows, side.src_row), slot_step = times<VEC>(lanes.rows, side.slot);
+  const bool once = lanes.pieces <= 32 && n <= lanes.rows * kStaged;
   const float held = *scale_at;
 
-  float top = 0.f, by = 0.f, scale = 0.f;
+  Largest largest;
+  float by = 0.f, scale = 0.f;
   bool begun = false;
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {  // the largest value; then the codes
     int at_stage = 0;
 #pragma unroll 1
-    for (int p0 = 0; p0 < pieces; p0 += 32) {
-      const bool inside = my_row < rows_at_once && p0 + my_piece < pieces;
-      const Columns at = step::columns_of<VEC>(rot, s.hd, min(p0 + my_piece, pieces - 1));
+    for (int p0 = 0; p0 < lanes.pieces; p0 += 32) {
+      const bool inside = lanes.my_row < lanes.rows && p0 + lanes.my_piece < lanes.pieces;
+      const Columns at = step::columns_of<VEC>(rot, s.hd, min(p0 + lanes.my_piece, lanes.pieces - 1));
+      int r = lanes.my_row;
+      const ST *from = src + times<VEC>(r, side.src_row);
+      const uint8_t *was = kPatch ? pages + times<VEC>(r, side.slot) : nullptr;
 #pragma unroll 1
-      for (int r0 = 0; r0 < n; r0 += chunk_rows) {
+      for (int r0 = 0; r0 < n; r0 += lanes.rows * kItems) {
         if (pass == 0 || !once) {
           Piece<SDT, PDT, VEC> piece[kItems];
 #pragma unroll
           for (int k = 0; k < kItems; ++k) {
-            const int r = r0 + k * rows_at_once + my_row;
             piece[k].slot = -1;
-            if (inside && r < n) piece[k].template load<kPatch>(s, side, src, pages, at, row, r, block);
+            if (inside && r < n) piece[k].template load<kPatch>(s, from, was, at, row + r, r, block);
+            r += lanes.rows, from += src_step;
+            if (kPatch) was += slot_step;
           }
 #pragma unroll
           for (int k = 0; k < kItems; ++k) {
@@ -284,11 +345,11 @@ __device__ __forceinline__ void store_run(const Store &s, const Side &side, int 
             stage.slot[at_stage + k][lane] = piece[k].slot;
             if (piece[k].slot < 0) continue;
             begun |= piece[k].slot == 0;
-            float lo[VEC], hi[VEC];
+            Values<VEC> lo, hi;
             piece[k].template values<kPatch>(s, rot, at, held, lo, hi);
             stage.put(at_stage + k, 0, lane, lo), stage.put(at_stage + k, 1, lane, hi);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) top = larger(larger(top, lo[e]), hi[e]);
+            for (int e = 0; e < Values<VEC>::kPairs; ++e) largest.add(lo.pair[e]), largest.add(hi.pair[e]);
           }
         }
         if (pass == 1) {
@@ -296,7 +357,7 @@ __device__ __forceinline__ void store_run(const Store &s, const Side &side, int 
           for (int k = 0; k < kItems; ++k) {
             const int slot = stage.slot[at_stage + k][lane];
             if (slot < 0) continue;
-            float lo[VEC], hi[VEC];
+            Values<VEC> lo, hi;
             stage.get(at_stage + k, 0, lane, lo), stage.get(at_stage + k, 1, lane, hi);
             store_piece<PDT, VEC>(pages + times<VEC>(slot, side.slot), at, lo, hi, by);
           }
@@ -305,8 +366,7 @@ __device__ __forceinline__ void store_run(const Store &s, const Side &side, int 
       }
     }
     if (pass == 1) break;
-    // (magnitudes compare as their bits do; NaN is above all)
-    const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    const uint32_t top_bits = __reduce_max_sync(0xffffffffu, largest.bits());  // (magnitudes compare as their bits do)
     // nothing is kept: a block that a token begins, or one that is patched whole
     begun = kPatch ? n == s.block_size : __any_sync(0xffffffffu, begun) != 0;
     scale = code8::scale_for<PDT>(top_bits, begun ? 0.f : held);
@@ -350,8 +410,8 @@ __device__ __forceinline__ void store_single_rows(const Store &s, int chunk, uin
   using ST = typename Elem<SDT>::T;
   const int pair0 = chunk * s.each, pairs = min(s.each, s.pairs - pair0);
   const int all = __popc(first) * pairs;
-  const int most = max(step::pieces_of(s.rot, s.hd, VEC), step::pieces_of(Rotary{0, 0}, s.hd, VEC));
-  const int wide = most <= 1 ? 1 : 1 << (32 - __clz(most - 1));  // lanes of a row
+  const int pieces = step::pieces_of(s.rot, s.hd, VEC);
+  const int wide = pieces <= 1 ? 1 : 1 << (32 - __clz(pieces - 1));  // lanes of a row
   const int groups = 32 / wide, mine_in = lane & (wide - 1);
   const int nth = __fns(first, 0, lane + 1);  // the window's row with the lane-th run
   for (int base = static_cast<int>(threadIdx.x >> 5) * groups; base < all; base += kThreads / 32 * groups) {
@@ -362,23 +422,23 @@ __device__ __forceinline__ void store_single_rows(const Store &s, int chunk, uin
     const int which = pair >= s.heads, h = which ? pair - s.heads : pair;
     const Side &side = s.side[which];
     const Rotary rot = which == 0 ? s.rot : Rotary{0, 0};
-    const int pieces = step::pieces_of(rot, s.hd, VEC);
     const Columns at = step::columns_of<VEC>(rot, s.hd, min(mine_in, pieces - 1));
     uint8_t *pages = side.pages + at_block * side.block + h * side.head;
     float *scale_at = side.scale + at_block * side.scale_block + h * side.scale_head;
     const float held = *scale_at;
     Piece<SDT, PDT, VEC> piece;
-    piece.template load<false>(s, side, static_cast<const ST *>(side.src) + (r0 + i) * side.src_row + h * side.src_head, pages, at,
+    piece.template load<false>(s, static_cast<const ST *>(side.src) + (r0 + i) * side.src_row + h * side.src_head, nullptr, at,
                                r0 + i, 0, at_block);
     piece.check(s);
     const bool there = base + lane / wide < all && piece.slot >= 0;
-    float lo[VEC], hi[VEC], top = 0.f;
+    Values<VEC> lo, hi;
+    Largest largest;
     if (there) {
       piece.template values<false>(s, rot, at, held, lo, hi);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) top = larger(larger(top, lo[e]), hi[e]);
+      for (int e = 0; e < Values<VEC>::kPairs; ++e) largest.add(lo.pair[e]), largest.add(hi.pair[e]);
     }
-    uint32_t top_bits = __float_as_uint(top);
+    uint32_t top_bits = largest.bits();
     for (int k = wide / 2; k > 0; k >>= 1) top_bits = max(top_bits, __shfl_xor_sync(0xffffffffu, top_bits, k));
     const bool begun = piece.slot == 0;
     const float scale = code8::scale_for<PDT>(top_bits, begun ? 0.f : held);
@@ -445,13 +505,14 @@ __global__ void __launch_bounds__(kThreads, kResident) append_kernel(const __gri
   }
   n = min(n, s.block_size);  // more: a slot came twice
   if (more == 0 && __shfl_sync(0xffffffffu, n, last) == 1 &&
-      max(step::pieces_of(s.rot, s.hd, VEC), step::pieces_of(Rotary{0, 0}, s.hd, VEC)) <= 32) {
+      step::pieces_of(s.rot, s.hd, VEC) <= 32) {
     store_single_rows<SDT, PDT, VEC>(s, chunk, first, block, r0, lane);
     return;
   }
+  const Lanes lanes(step::pieces_of(s.rot, s.hd, VEC), lane);  // (the same for V: dim is even)
   each_run(s, chunk, first, n, block, [&](int i, int rows_of, int64_t at, int pair) {
     const int which = pair >= s.heads;
-    store_run<SDT, PDT, VEC, false>(s, s.side[which], which ? pair - s.heads : pair, which == 0 && s.cos_t != nullptr, r0 + i,
+    store_run<SDT, PDT, VEC, false>(s, s.side[which], which ? pair - s.heads : pair, which ? Rotary{0, 0} : s.rot, lanes, r0 + i,
                                     rows_of, at, stage[threadIdx.x >> 5], lane);
   });
 }
@@ -505,8 +566,9 @@ __global__ void __launch_bounds__(kThreads, kResident) patch_kernel(const __grid
       record_error(s.status, DKV_ERR_INVALID_ARGUMENT);
   }
   const uint32_t first = __ballot_sync(0xffffffffu, block >= 0);
+  const Lanes lanes(step::pieces_of(Rotary{0, 0}, s.hd, VEC), lane);
   each_run(s, chunk, first, n, block, [&](int i, int rows_of, int64_t at, int head) {
-    store_run<SDT, PDT, VEC, true>(s, s.side[0], head, false, r0 + i, rows_of, at, stage[threadIdx.x >> 5], lane);
+    store_run<SDT, PDT, VEC, true>(s, s.side[0], head, Rotary{0, 0}, lanes, r0 + i, rows_of, at, stage[threadIdx.x >> 5], lane);
   });
 }
 
