@@ -49,9 +49,12 @@ struct Store {
 };
 
 constexpr int kThreads = 128;
-constexpr int kItems = 2;   // pieces of two times VEC columns that a lane holds at once
-constexpr int kStaged = 4;  // and that wait in shared memory
-constexpr int kResident = 5;  // CTAs of an SM at least: leaves a thread 96 registers
+constexpr int kStaged = 4;  // pieces of two times VEC columns of a lane that wait in shared memory
+// Pieces that a lane reads at once, and CTAs of an SM (which leave a thread 96 or 128 registers).  16384 rows of 32 + 8 + 8 heads
+// x 128 appended / 73000 rows of 8 x 128 patched, us: 1 piece, 6 CTAs 107 / 92; 2, 5 97 / 81; 2, 4 100 / 83; 4, 4 102 / 76;
+// 4, 3 113 / 85.
+constexpr int items_of(bool patch) { return patch ? 4 : 2; }
+constexpr int resident_of(bool patch) { return patch ? 4 : 5; }
 
 // The largest magnitude of several values, and whether all are finite (0 times anything else is NaN).
 struct Largest {
@@ -91,8 +94,8 @@ __device__ __forceinline__ int slot_in(const Store &s, int64_t row, int64_t bloc
   return static_cast<int>(s.slots[row] - block * s.block_size);
 }
 
-// VEC values in pairs, as the packed fp32 operations of sm_100 take them (each rounds as the single one does); one value has a
-// zero beside it
+// VEC values in pairs, as the packed fp32 operations of sm_100 take them; one value has a zero beside it.  (Where a product
+// and a sum are rounded one after the other the single operations are used: packed ones are merged into one.)
 template <int VEC>
 struct Values {
   static constexpr int kPairs = VEC == 1 ? 1 : VEC / 2;
@@ -221,41 +224,34 @@ struct Piece {
                               : f2pack(raw[1].get(2 * e), raw[1].get((2 * e + 1) % VEC));
     }
     if (kPatch) {
-      const uint64_t two = f2pack(held, held);
+      const auto add = [&](uint64_t code, uint64_t x) {  // code times held, plus x
+        float a, b, c, d;
+        f2unpack(code, a, b), f2unpack(x, c, d);
+        return f2pack(__fadd_rn(__fmul_rn(a, held), c), __fadd_rn(__fmul_rn(b, held), d));
+      };
       Values<VEC> y = old[0].template get<PDT>();
 #pragma unroll
-      for (int e = 0; e < kPairs; ++e) lo.pair[e] = add2(mul2(y.pair[e], two), lo.pair[e]);
+      for (int e = 0; e < kPairs; ++e) lo.pair[e] = add(y.pair[e], lo.pair[e]);
       if (paired<VEC>(at)) {
         y = old[1].template get<PDT>();
 #pragma unroll
-        for (int e = 0; e < kPairs; ++e) hi.pair[e] = add2(mul2(y.pair[e], two), hi.pair[e]);
+        for (int e = 0; e < kPairs; ++e) hi.pair[e] = add(y.pair[e], hi.pair[e]);
       }
     } else if (at.turn) {
       Raw<DKV_F32, VEC> c, sn;
       const int64_t angle = static_cast<int64_t>(pos) * (rot.dim / 2) + at.angle;
       c.load(s.cos_t + angle), sn.load(s.sin_t + angle);
-      if (VEC > 1 && rot.interleaved) {
-        float x[VEC], y[VEC];
+      float x[VEC], y[VEC], none;
 #pragma unroll
-        for (int e = 0; e < kPairs; ++e) {
-          f2unpack(lo.pair[e], x[2 * e % VEC], x[(2 * e + 1) % VEC]);
-          f2unpack(hi.pair[e], y[2 * e % VEC], y[(2 * e + 1) % VEC]);
-        }
-        step::turn<VEC>(x, y, c, sn, true);
+      for (int e = 0; e < kPairs; ++e) {
+        f2unpack(lo.pair[e], x[2 * e % VEC], VEC == 1 ? none : x[(2 * e + 1) % VEC]);
+        f2unpack(hi.pair[e], y[2 * e % VEC], VEC == 1 ? none : y[(2 * e + 1) % VEC]);
+      }
+      step::turn<VEC>(x, y, c, sn, rot.interleaved);
 #pragma unroll
-        for (int e = 0; e < kPairs; ++e) {
-          lo.pair[e] = f2pack(x[2 * e % VEC], x[(2 * e + 1) % VEC]);
-          hi.pair[e] = f2pack(y[2 * e % VEC], y[(2 * e + 1) % VEC]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kPairs; ++e) {
-          const uint64_t cc = f2pack(c.get(2 * e % VEC), c.get((2 * e + 1) % VEC));
-          const uint64_t ss = f2pack(sn.get(2 * e % VEC), sn.get((2 * e + 1) % VEC));
-          const uint64_t x = lo.pair[e], y = hi.pair[e];
-          lo.pair[e] = sub2(mul2(x, cc), mul2(y, ss));
-          hi.pair[e] = add2(mul2(y, cc), mul2(x, ss));
-        }
+      for (int e = 0; e < kPairs; ++e) {
+        lo.pair[e] = f2pack(x[2 * e % VEC], VEC == 1 ? 0.f : x[(2 * e + 1) % VEC]);
+        hi.pair[e] = f2pack(y[2 * e % VEC], VEC == 1 ? 0.f : y[(2 * e + 1) % VEC]);
       }
     }
   }
@@ -312,6 +308,7 @@ __device__ __forceinline__ void store_run(const Store &s, const Side &side, int 
   float *scale_at = side.scale + block * side.scale_block + h * side.scale_head;
   const ST *src = static_cast<const ST *>(side.src) + row * side.src_row + h * side.src_head;
   const int64_t src_step = times<VEC>(lanes.rows, side.src_row), slot_step = times<VEC>(lanes.rows, side.slot);
+  constexpr int kItems = items_of(kPatch);
   const bool once = lanes.pieces <= 32 && n <= lanes.rows * kStaged;
   const float held = *scale_at;
 
@@ -464,7 +461,7 @@ __device__ __forceinline__ void store_single_rows(const Store &s, int chunk, uin
 // Bound by memory: k, v and q are read once, codes and q written once.  The store's CTAs, which wait for memory several
 // times, lie evenly among those of q, which only stream.
 template <int SDT, int PDT, int VEC>
-__global__ void __launch_bounds__(kThreads, kResident) append_kernel(const __grid_constant__ Store s,
+__global__ void __launch_bounds__(kThreads, resident_of(false)) append_kernel(const __grid_constant__ Store s,
                                                                      const __grid_constant__ Append q) {
   __shared__ Stage<VEC> stage[kThreads / 32];
   begin_overlapped();
@@ -543,7 +540,7 @@ __device__ __forceinline__ int64_t page_of(const dkv_seq_batch &q, int64_t n_blo
 
 // Bound by memory: the rows and the codes are read once, codes written once.
 template <int SDT, int PDT, int VEC>
-__global__ void __launch_bounds__(kThreads, kResident) patch_kernel(const __grid_constant__ Store s) {
+__global__ void __launch_bounds__(kThreads, resident_of(true)) patch_kernel(const __grid_constant__ Store s) {
   __shared__ Stage<VEC> stage[kThreads / 32];
   begin_overlapped();
   const int lane = threadIdx.x & 31;
@@ -593,36 +590,55 @@ struct Read {
 constexpr int kReadThreads = 256;
 constexpr int kReadRows = 32;
 
+// VEC codes to values; the value's rows are written in whole 16 (8, 1) elements' worth of bytes
 template <int PDT, int ODT, int VEC>
 __device__ __forceinline__ void read_piece(const uint8_t *src, float scale, bool there, typename Elem<ODT>::T *dst) {
-  if constexpr (VEC == 16) {
-    const uint4 w = there ? *reinterpret_cast<const uint4 *>(src) : make_uint4(0, 0, 0, 0);
-    const uint32_t c[4] = {w.x, w.y, w.z, w.w};
-    float x[16];
+  if constexpr (VEC == 1) {
+    float y[4];
+    Code<PDT>::unpack(there ? *src : 0, y);
+    *dst = Elem<ODT>::from_f(there ? __fmul_rn(y[0], scale) : 0.f);
+  } else {
+    uint32_t c[VEC / 4] = {};
+    if (there) {
+      if constexpr (VEC == 16) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(src);
+        c[0] = w.x, c[1] = w.y, c[2] = w.z, c[3] = w.w;
+      } else if constexpr (VEC == 8) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(src);
+        c[0] = w.x, c[1] = w.y;
+      } else {
+        c[0] = *reinterpret_cast<const uint32_t *>(src);
+      }
+    }
+    float x[VEC];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < VEC / 4; ++i) {
       float y[4];
       Code<PDT>::unpack(c[i], y);
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[4 * i + k] = there ? __fmul_rn(y[k], scale) : 0.f;
     }
-    Raw<ODT, 16> y;
-    y.set(x), y.store(dst);
-  } else {
-    float y[4];
-    Code<PDT>::unpack(there ? *src : 0, y);
-    *dst = Elem<ODT>::from_f(there ? __fmul_rn(y[0], scale) : 0.f);
+    if constexpr (VEC * sizeof(typename Elem<ODT>::T) == 8) {
+      uint2 w;
+      if (ODT == DKV_BF16)
+        w = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+      else
+        w = make_uint2(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]));
+      *reinterpret_cast<uint2 *>(dst) = w;
+    } else {
+      Raw<ODT, VEC> y;
+      y.set(x), y.store(dst);
+    }
   }
 }
 
 // Bound by memory: each code read once, each value written once.  A CTA first finds its rows' places (one lane each),
-// then a thread has 16 columns of a head.
+// then a thread has the same columns of every so many-th row.
 template <int PDT, int ODT, int VEC>
 __global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constant__ Read a) {
   using OT = typename Elem<ODT>::T;
   begin_overlapped();
-  __shared__ int64_t block_at[kReadRows];  // -1: zeros, -2: left alone
-  __shared__ int slot_at[kReadRows];
+  __shared__ int64_t row_at[kReadRows], scale_at[kReadRows];  // scale_at -1: zeros, -2: left alone
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.rows;
   const int n = static_cast<int>(min(static_cast<int64_t>(a.rows), a.n_rows - r0));
   const int tid = threadIdx.x;
@@ -638,20 +654,26 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constan
       block = i >= 0 ? page_of(a.seqs, a.n_blocks, b, blk, a.status) : -1;
     }
     if (row == a.n_rows - 1 && a.seqs.cu_seqlens[a.seqs.n_seqs] > a.n_rows) record_error(a.status, DKV_ERR_INVALID_ARGUMENT);
-    block_at[tid] = block, slot_at[tid] = slot;
+    row_at[tid] = block < 0 ? 0 : block * a.block + slot * a.slot;
+    scale_at[tid] = block < 0 ? block : block * a.scale_block;
   }
   __syncthreads();
-  const int pieces = a.hd / VEC, per_row = a.heads * pieces, all = n * per_row;
+  const int pieces = a.hd / VEC, per_row = a.heads * pieces;
+  const int wide = min(per_row, kReadThreads), rows_at_once = kReadThreads / wide;
+  const int my_row = tid / wide;
+  if (my_row >= rows_at_once) return;
+  for (int in = tid - my_row * wide; in < per_row; in += wide) {
+    const int h = in / pieces, d = (in - h * pieces) * VEC;
+    const uint8_t *src = a.pages + h * a.head + d;
+    const float *scales = a.scale + h * a.scale_head;
+    OT *dst = static_cast<OT *>(a.out) + (r0 + my_row) * a.out_row + h * a.out_head + d;
+    const int64_t step = rows_at_once * a.out_row;
 #pragma unroll 4
-  for (int i = tid; i < all; i += kReadThreads) {
-    const int r = i / per_row, in = i - r * per_row, h = in / pieces, d = (in - h * pieces) * VEC;
-    const int64_t block = block_at[r];
-    if (block == -2) continue;
-    const bool there = block >= 0;
-    const int64_t at = there ? block : 0;
-    const uint8_t *src = a.pages + at * a.block + slot_at[r] * a.slot + h * a.head + d;
-    const float scale = there ? a.scale[at * a.scale_block + h * a.scale_head] : 0.f;
-    read_piece<PDT, ODT, VEC>(src, scale, there, static_cast<OT *>(a.out) + (r0 + r) * a.out_row + h * a.out_head + d);
+    for (int r = my_row; r < n; r += rows_at_once, dst += step) {
+      const int64_t at = scale_at[r];
+      if (at == -2) continue;
+      read_piece<PDT, ODT, VEC>(src + row_at[r], at >= 0 ? scales[at] : 0.f, at >= 0, dst);
+    }
   }
 }
 
@@ -667,6 +689,7 @@ int check_pages(const dkv_paged_cache &c, const dkv_page_scales &s) {
   if (c.block_size <= 0 || c.n_heads <= 0 || c.head_dim <= 0 || c.num_blocks < 0) return DKV_ERR_LAYOUT;
   if (c.block_size > kMaxBlock) return DKV_ERR_UNSUPPORTED;
   if (c.num_blocks > 0 && (c.base == nullptr || s.base == nullptr)) return DKV_ERR_INVALID_ARGUMENT;
+  if (s.stride_block < 0 || s.stride_head < 0) return DKV_ERR_LAYOUT;
   return DKV_OK;
 }
 int check_seqs(const dkv_seq_batch &q) {
@@ -855,16 +878,20 @@ extern "C" int dkv_gather_paged_quant(const dkv_paged_cache *cache, const dkv_pa
   a.rows = n_rows >= static_cast<int64_t>(sms) * quant::kReadRows * 2 ? quant::kReadRows : 8;
   a.zero_rest = zero_rest != 0;
   const int64_t size = out_dtype == DKV_F32 ? 4 : 2;
-  const bool wide = cache->head_dim % 16 == 0 &&
-                    (reinterpret_cast<intptr_t>(a.pages) | a.block | a.slot | a.head) % 16 == 0 &&
-                    (reinterpret_cast<intptr_t>(out) | out_stride_row * size | out_stride_head * size) % 16 == 0;
+  // codes of a thread: 32 bytes of values, or 4 codes, or one
+  const int full = static_cast<int>(32 / size);
+  const int64_t code_bits = reinterpret_cast<intptr_t>(a.pages) | a.block | a.slot | a.head | a.hd;
+  const int64_t out_bits = reinterpret_cast<intptr_t>(out) | out_stride_row * size | out_stride_head * size;
+  const int vec = code_bits % full == 0 && out_bits % 16 == 0 ? full : code_bits % 4 == 0 && out_bits % (4 * size) == 0 ? 4 : 1;
   const int64_t ctas = (n_rows + a.rows - 1) / a.rows;
   if (ctas > INT32_MAX || static_cast<int64_t>(a.heads) * a.hd > INT32_MAX / quant::kReadRows - quant::kReadThreads)
     return DKV_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 #define DKV_QUANT_CASE(P, O)                                                                                  \
   if (cache->dtype == P && out_dtype == O) {                                                                  \
-    const auto kernel = wide ? quant::read_kernel<P, O, 16> : quant::read_kernel<P, O, 1>;                    \
+    constexpr int kFull = O == DKV_F32 ? 8 : 16;                                                              \
+    const auto kernel = vec == kFull ? quant::read_kernel<P, O, kFull>                                        \
+                                     : (vec == 4 ? quant::read_kernel<P, O, 4> : quant::read_kernel<P, O, 1>); \
     DKV_CUDA_CHECK(launch_overlapped(kernel, dim3(static_cast<unsigned>(ctas)), quant::kReadThreads, 0, st, a)); \
     return DKV_OK;                                                                                            \
   }
