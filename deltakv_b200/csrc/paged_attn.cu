@@ -844,7 +844,7 @@ int shape_of(const dkv_paged_decode_args *a, Shape *s) {
   const bool f32 = a->k_pages.dtype == DKV_F32;
   s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
   s->g = f32 && group <= 4 ? 4 : 8;
-  return cut_up(*a, variant(f32, s->hd_pad, s->g), kSeqCost, s);
+  return cut_up(*a, variant(f32, s->hd_pad, s->g), kSeqCost, 1, s);
 }
 
 template <int HD, int G, int W, int kStages, int kTok>

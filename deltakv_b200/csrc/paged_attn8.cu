@@ -15,7 +15,7 @@ int shape8(const dkv_paged_decode_args *a, int q_dtype, Shape *s) {
   s->hd_pad = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
   const bool f32 = q_dtype == DKV_F32;
   s->g = heads8(f32, s->hd_pad, a->n_q_heads / a->k_pages.n_heads);
-  return cut_up(*a, variant8(f32, s->hd_pad, s->g), kSeqCost8, s);
+  return cut_up(*a, variant8(f32, s->hd_pad, s->g), kSeqCost8, kLeastLocal8, s);
 }
 
 }  // namespace pattn

@@ -629,16 +629,28 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
 // ---------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------
-// warps and stages
+// Warps of a CTA (one an SM) and stages of a warp's ring, as registers and 227 KB allow.  Three stages of eight warps stream
+// better than two of twelve (one range's eight heads on one SM, whose rows are neighbours in memory); where arithmetic or
+// many short sequences bound it, twelve are a little better.  us, 8 KV heads: head_dim 128, 8 x 3 / 12 x 2: 32 sequences of
+// 26000..30200 307 / 325, 16 of 8192 55.6 / 58.2, 64 of 1..8192 34.0 / 35.6, 256 of 1..600 24.7 / 23.1, block_size 24 (rows looked up one
+// by one) 70 / 60.  head_dim 64, 16 x 2 / 14 x 3 / 10 x 4 / 8 x 5: 16 of 16384 57.5 / 60 / 65 / 70.  32, 16 x 4 / 12 x 5 / 8 x 8: 16 of
+// 32768 85 / 91 / 115.  256, 6 x 2 / 4 x 3: 16 of 4096 59 / 58.
 constexpr Variant variant8(bool f32, int hd, int heads) {
   if (hd == 256) return {6, 2, 32};
   if (hd == 128) return {8, 3, 32};
   if (heads == 16) return hd == 64 ? Variant{12, 3, 32} : Variant{12, 4, 32};
   return hd == 64 ? (f32 ? Variant{12, 3, 32} : Variant{16, 2, 32}) : Variant{16, 4, 32};
 }
-// query heads of a unit: 16 where a KV head has more than eight and registers allow it
+// Query heads of a unit: 16 where a KV head has more than eight and registers allow it (16 sequences of 8192, 16 heads for each
+// of 8 KV heads x 128: 63 us, as two units of eight 89, with twelve warps 77).
 constexpr int heads8(bool f32, int hd, int group) { return !f32 && hd <= 128 && group > 8 ? 16 : 8; }
+// A sequence costs more tokens than in the 16-bit walk, whose tokens take longer.  At 48 / 96 / 160, us: 64 sequences of
+// 1..8192 39.5 / 33.6 / 34.1, 256 of 1..600 23.8 / 25.5 / 28.7.
 constexpr int kSeqCost8 = 80;
+// CTAs of one warp lose to ranges (148 sequences of 64 / 150 tokens: 13.7 / 20.1 us in one launch, 11.8 / 16.4 split); of two,
+// they win (60 of 300: 12.8 against 17.0), as do more (37 of 500: 11.3 against 17.8; 18 of 1000: 11.6 against 16.3, of
+// 1..1000 11.3 against 10.7).
+constexpr int kLeastLocal8 = 2;
 
 template <int PT, int DT, int HD, int NB>
 int launch_walk8(const Params &p, const Shape &s, cudaStream_t st) {

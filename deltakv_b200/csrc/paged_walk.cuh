@@ -496,8 +496,8 @@ inline int check_args(const dkv_paged_decode_args &a) {
 
 constexpr int kMaxRanges = 2048;
 
-// how a batch is cut, given the kernel variant: s->hd_pad and s->g are set
-inline int cut_up(const dkv_paged_decode_args &a, const Variant &v, int seq_cost, Shape *s) {
+// how a batch is cut, given the kernel variant: s->hd_pad and s->g are set; least_local: fewest warps of a CTA of the one-launch form
+inline int cut_up(const dkv_paged_decode_args &a, const Variant &v, int seq_cost, int least_local, Shape *s) {
   const int rc = sm_count(&s->sms);
   if (rc != DKV_OK) return rc;
   const int64_t sms = s->sms;
@@ -508,6 +508,7 @@ inline int cut_up(const dkv_paged_decode_args &a, const Variant &v, int seq_cost
   const int64_t pairs = static_cast<int64_t>(a.seqs.n_seqs) * s->units;
   s->local = s->warps;
   while (s->local > 0 && pairs > sms * (s->warps / s->local)) --s->local;
+  if (s->local < least_local) s->local = 0;
   if (a.seqs.max_seq_len > static_cast<int64_t>(kLocalTiles) * s->tokens * s->local) s->local = 0;
   const int64_t most = sms * s->warps / s->units;
   const int64_t line = static_cast<int64_t>(a.seqs.n_seqs) * (static_cast<int64_t>(a.seqs.max_seq_len) + seq_cost);
