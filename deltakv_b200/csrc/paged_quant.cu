@@ -385,6 +385,14 @@ __device__ __forceinline__ void store_run(const Store &s, const Side &side, int 
   if (lane == 0) *scale_at = scale;
 }
 
+// The runs that begin in a CTA's window, as its first warp finds them: a bit for each row where one begins, and for these
+// how many rows they have and their block.
+struct Runs {
+  uint32_t first;
+  int n[32];
+  int64_t block[32];
+};
+
 // The runs of a CTA's window and its pairs of head and side, dealt to its warps: f(i, n, block, pair) for the run that begins
 // at the window's row i.  `first` has a bit for each such row, lane i their n and block.
 template <typename F>
@@ -464,6 +472,7 @@ template <int SDT, int PDT, int VEC>
 __global__ void __launch_bounds__(kThreads, resident_of(false)) append_kernel(const __grid_constant__ Store s,
                                                                      const __grid_constant__ Append q) {
   __shared__ Stage<VEC> stage[kThreads / 32];
+  __shared__ Runs runs;
   begin_overlapped();
   const uint32_t turn = blockIdx.x / s.spread;
   const bool stores = turn < s.ctas && blockIdx.x == turn * s.spread;
@@ -475,34 +484,41 @@ __global__ void __launch_bounds__(kThreads, resident_of(false)) append_kernel(co
   const int lane = threadIdx.x & 31;
   const int64_t r0 = static_cast<int64_t>(turn / s.chunks) * s.window;
   const int chunk = static_cast<int>(turn % s.chunks);
-  const int64_t row = r0 + lane;
-  const int rows = static_cast<int>(min(static_cast<int64_t>(s.window), s.n_rows - r0));
-  int64_t block = -1;
-  if (lane < rows) {
-    block = row_block(s, row);
-    if (block < 0 && chunk == 0 && threadIdx.x < 32 && s.slots[row] >= 0) record_error(s.status, DKV_ERR_PAGE_RANGE);
-  }
-  int64_t before = __shfl_up_sync(0xffffffffu, block, 1);
-  if (lane == 0) before = r0 > 0 ? row_block(s, r0 - 1) : -1;
-  const uint32_t first = __ballot_sync(0xffffffffu, block >= 0 && block != before);
-  if (first == 0) return;
-  const uint32_t more = __ballot_sync(0xffffffffu, block >= 0 && block == before);  // rows that go on with a run
-  int n = __ffs(~(lane == 31 ? 0u : more >> (lane + 1)));
-  const int last = 31 - __clz(first);  // the run that may go on behind the window
-  if (last + __shfl_sync(0xffffffffu, n, last) == rows) {
-    const int64_t mine = __shfl_sync(0xffffffffu, block, last);
-    int64_t end = r0 + rows;
-    while (end - (r0 + last) < s.block_size) {
-      const int64_t at = end + lane;
-      const uint32_t same = __ballot_sync(0xffffffffu, at < s.n_rows && row_block(s, at) == mine);
-      end += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
-      if (same != 0xffffffffu) break;
+  if (threadIdx.x < 32) {
+    const int64_t row = r0 + lane;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(s.window), s.n_rows - r0));
+    int64_t block = -1;
+    if (lane < rows) {
+      block = row_block(s, row);
+      if (block < 0 && chunk == 0 && s.slots[row] >= 0) record_error(s.status, DKV_ERR_PAGE_RANGE);
     }
-    if (lane == last) n = static_cast<int>(end - (r0 + last));
+    int64_t before = __shfl_up_sync(0xffffffffu, block, 1);
+    if (lane == 0) before = r0 > 0 ? row_block(s, r0 - 1) : -1;
+    const uint32_t first = __ballot_sync(0xffffffffu, block >= 0 && block != before);
+    const uint32_t more = __ballot_sync(0xffffffffu, block >= 0 && block == before);  // rows that go on with a run
+    int n = __ffs(~(lane == 31 ? 0u : more >> (lane + 1)));
+    const int last = first ? 31 - __clz(first) : 0;  // the run that may go on behind the window
+    if (first && last + __shfl_sync(0xffffffffu, n, last) == rows) {
+      const int64_t mine = __shfl_sync(0xffffffffu, block, last);
+      int64_t end = r0 + rows;
+      while (end - (r0 + last) < s.block_size) {
+        const int64_t at = end + lane;
+        const uint32_t same = __ballot_sync(0xffffffffu, at < s.n_rows && row_block(s, at) == mine);
+        end += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+        if (same != 0xffffffffu) break;
+      }
+      if (lane == last) n = static_cast<int>(end - (r0 + last));
+    }
+    runs.n[lane] = min(n, s.block_size);  // more: a slot came twice
+    runs.block[lane] = block;
+    if (lane == 0) runs.first = first;
   }
-  n = min(n, s.block_size);  // more: a slot came twice
-  if (more == 0 && __shfl_sync(0xffffffffu, n, last) == 1 &&
-      step::pieces_of(s.rot, s.hd, VEC) <= 32) {
+  __syncthreads();
+  const uint32_t first = runs.first;
+  const int n = runs.n[lane];
+  const int64_t block = runs.block[lane];
+  if (first == 0) return;
+  if (__all_sync(0xffffffffu, n == 1 || !(first >> lane & 1)) && step::pieces_of(s.rot, s.hd, VEC) <= 32) {
     store_single_rows<SDT, PDT, VEC>(s, chunk, first, block, r0, lane);
     return;
   }
@@ -542,27 +558,36 @@ __device__ __forceinline__ int64_t page_of(const dkv_seq_batch &q, int64_t n_blo
 template <int SDT, int PDT, int VEC>
 __global__ void __launch_bounds__(kThreads, resident_of(true)) patch_kernel(const __grid_constant__ Store s) {
   __shared__ Stage<VEC> stage[kThreads / 32];
+  __shared__ Runs runs;
   begin_overlapped();
   const int lane = threadIdx.x & 31;
   const int64_t r0 = static_cast<int64_t>(blockIdx.x / s.chunks) * s.window;
   const int chunk = static_cast<int>(blockIdx.x % s.chunks);
-  const int64_t row = r0 + lane;
-  int64_t block = -1;
-  int n = 0;
-  if (lane < s.window && row < s.n_rows) {
-    const int b = sequence_of(s.seqs, row);
-    if (b < s.seqs.n_seqs) {
-      const int first = s.seqs.cu_seqlens[b], i = static_cast<int>(row - first);
-      const int left = s.seqs.cu_seqlens[b + 1] - static_cast<int>(row);
-      if (i >= 0 && left > 0 && i % s.block_size == 0) {  // (always so, where cu_seqlens are prefix sums)
-        n = min(min(left, s.block_size), static_cast<int>(min(s.n_rows - row, static_cast<int64_t>(INT32_MAX))));
-        block = page_of(s.seqs, s.n_blocks, b, i / s.block_size, s.status);
+  if (threadIdx.x < 32) {
+    const int64_t row = r0 + lane;
+    int64_t block = -1;
+    int n = 0;
+    if (lane < s.window && row < s.n_rows) {
+      const int b = sequence_of(s.seqs, row);
+      if (b < s.seqs.n_seqs) {
+        const int start = s.seqs.cu_seqlens[b], i = static_cast<int>(row - start);
+        const int left = s.seqs.cu_seqlens[b + 1] - static_cast<int>(row);
+        if (i >= 0 && left > 0 && i % s.block_size == 0) {  // (always so, where cu_seqlens are prefix sums)
+          n = min(min(left, s.block_size), static_cast<int>(min(s.n_rows - row, static_cast<int64_t>(INT32_MAX))));
+          block = page_of(s.seqs, s.n_blocks, b, i / s.block_size, s.status);
+        }
       }
+      if (row == s.n_rows - 1 && chunk == 0 && s.seqs.cu_seqlens[s.seqs.n_seqs] > s.n_rows)
+        record_error(s.status, DKV_ERR_INVALID_ARGUMENT);
     }
-    if (row == s.n_rows - 1 && chunk == 0 && s.seqs.cu_seqlens[s.seqs.n_seqs] > s.n_rows)
-      record_error(s.status, DKV_ERR_INVALID_ARGUMENT);
+    const uint32_t first = __ballot_sync(0xffffffffu, block >= 0);
+    runs.n[lane] = n, runs.block[lane] = block;
+    if (lane == 0) runs.first = first;
   }
-  const uint32_t first = __ballot_sync(0xffffffffu, block >= 0);
+  __syncthreads();
+  const uint32_t first = runs.first;
+  const int n = runs.n[lane];
+  const int64_t block = runs.block[lane];
   const Lanes lanes(step::pieces_of(Rotary{0, 0}, s.hd, VEC), lane);
   each_run(s, chunk, first, n, block, [&](int i, int rows_of, int64_t at, int head) {
     store_run<SDT, PDT, VEC, true>(s, s.side[0], head, Rotary{0, 0}, lanes, r0 + i, rows_of, at, stage[threadIdx.x >> 5], lane);
