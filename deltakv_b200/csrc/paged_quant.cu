@@ -466,8 +466,13 @@ __device__ __forceinline__ void store_single_rows(const Store &s, int chunk, uin
   }
 }
 
-// Bound by memory: k, v and q are read once, codes and q written once.  The store's CTAs, which wait for memory several
-// times, lie evenly among those of q, which only stream.
+// k, v and q are read once, codes and q written once, so memory would bound it (57.8 us for 16384 rows of 32 + 8 + 8 heads x 128,
+// bf16 to e4m3); it takes 96-99 us, half of the issue slots used by 18 warps an SM: a run of 16 rows of a head takes some 1200
+// instructions (the rotation, the largest, two conversions), and registers leave no room for more warps.  The store's CTAs,
+// which wait for memory several times, lie evenly among those of q, which only stream.  4096 single rows of the same heads 29 us
+// (a run a warp: 103), 64 of them 6 us of device time from cold caches.  Left out, for the 16384 rows: values kept in registers
+// 140 us (spilled), a run for the whole CTA 123, rows kept as read and rotated twice 106, L2 asked for a CTA's rows before their
+// runs are found 98.
 template <int SDT, int PDT, int VEC>
 __global__ void __launch_bounds__(kThreads, resident_of(false)) append_kernel(const __grid_constant__ Store s,
                                                                      const __grid_constant__ Append q) {
@@ -554,7 +559,8 @@ __device__ __forceinline__ int64_t page_of(const dkv_seq_batch &q, int64_t n_blo
   return id;
 }
 
-// Bound by memory: the rows and the codes are read once, codes written once.
+// The rows and the codes are read once, codes written once: memory would bound it (46 us for 73200 rows of 8 x 128, bf16 on
+// e4m3); it takes 76-78 us, 55 % of the issue slots used by 15 warps an SM (without dequantising and adding: 67).
 template <int SDT, int PDT, int VEC>
 __global__ void __launch_bounds__(kThreads, resident_of(true)) patch_kernel(const __grid_constant__ Store s) {
   __shared__ Stage<VEC> stage[kThreads / 32];
@@ -658,7 +664,8 @@ __device__ __forceinline__ void read_piece(const uint8_t *src, float scale, bool
 }
 
 // Bound by memory: each code read once, each value written once.  A CTA first finds its rows' places (one lane each),
-// then a thread has the same columns of every so many-th row.
+// then a thread has the same columns of every so many-th row.  73200 rows of 8 x 128: to bf16 43-44 us (floor 34.5; 16 bytes of
+// values a thread instead of 32: 53), to fp32 75 (57.4; 64 bytes: 98).
 template <int PDT, int ODT, int VEC>
 __global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constant__ Read a) {
   using OT = typename Elem<ODT>::T;
