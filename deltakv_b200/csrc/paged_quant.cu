@@ -94,6 +94,9 @@ __device__ __forceinline__ int slot_in(const Store &s, int64_t row, int64_t bloc
   return static_cast<int>(s.slots[row] - block * s.block_size);
 }
 
+// whether the tables have a row's position
+__device__ __forceinline__ bool turns(const Store &s, int pos) { return pos >= 0 && pos < s.rope_max_pos; }
+
 // VEC values in pairs, as the packed fp32 operations of sm_100 take them; one value has a zero beside it.  (Where a product
 // and a sum are rounded one after the other the single operations are used: packed ones are merged into one.)
 template <int VEC>
@@ -207,7 +210,7 @@ struct Piece {
     }
   }
   __device__ __forceinline__ void check(const Store &s) {  // a position outside the tables: the row stores nothing
-    if (slot >= 0 && s.cos_t && (pos < 0 || pos >= s.rope_max_pos)) {
+    if (slot >= 0 && s.cos_t && !turns(s, pos)) {
       record_error(s.status, DKV_ERR_ROPE_RANGE);
       slot = -1;
     }
@@ -376,7 +379,7 @@ __device__ __forceinline__ void store_run(const Store &s, const Side &side, int 
       } else {
         for (int i = 0; i < n; ++i) {
           const int o = slot_in(s, row + i, block);
-          if (o >> 5 == lane) mine |= 1u << (o & 31);
+          if (o >> 5 == lane && (!s.cos_t || turns(s, s.positions[row + i]))) mine |= 1u << (o & 31);
         }
       }
       scale_again<PDT, VEC>(s, side, pages, held, by, mine, lane);

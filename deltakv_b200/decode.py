@@ -134,8 +134,8 @@ def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, sl
     values need (e4m3: the least power of two; int8: the largest magnitude / 127), and nothing the block held
     is kept; later values that do not fit make the scale grow by powers of two, and what the block holds is rounded to the
     new one (int8: by less than one step in all; e4m3: not at all above its subnormals).  So codes and scales may start as any memory.
-    Rows may be fp32, fp16 or bf16, and the rows of one block follow one another
-    (as :func:`plan_paged_step` lays them out).  A value that is not finite makes the block's head read as NaN until
+    Rows may be fp32, fp16 or bf16, and the rows of one block follow one another, with no row
+    of a negative slot between them (as :func:`plan_paged_step` lays them out).  A value that is not finite makes the block's head read as NaN until
     the block is begun anew.
     """
     native = _native_module or _native()

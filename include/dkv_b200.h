@@ -700,8 +700,8 @@ typedef struct dkv_page_scales {
 
 /*
  * dkv_append_paged_rotary into 8-bit pages: in_dtype is F32, F16 or BF16 whatever the pages.  Storing a block's slot 0
- * begins the block: nothing that it held is kept.  The rows of one block follow one another (as
- * dkv_plan_paged_step lays them out); slots are distinct.
+ * begins the block: nothing that it held is kept.  The rows of one block follow one another, with no row without a slot
+ * between them (as dkv_plan_paged_step lays them out); slots are distinct.
  */
 int dkv_append_paged_quant(const dkv_append_args *args, const dkv_rotary *rotary, const dkv_page_scales *k_scales,
                            const dkv_page_scales *v_scales, dkv_stream_t stream);

@@ -369,6 +369,27 @@ def test_append_ranges(cuda, kind, dtype):
         dkv.append_into_paged(k, k, c.k, c.v, slots, positions=pos, rope=(cos, sin), rotary_dim=32, kv_scales=c.scales)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [64, 50])
+def test_append_keeps_the_slot_of_a_row_that_stores_nothing(cuda, kind, hd):
+    """A row among others of its block whose position lies beyond the tables: its slot's value stays where the scale grows."""
+    c = Cache8([20], 2, hd, 16, kind, cuda, garbage=False, layout="kv_first" if hd == 64 else "odd")
+    block = int(c.tables[0, 0])
+    slots = block * 16 + torch.tensor([6, 7, 8, 9], device=cuda)
+    pos = torch.tensor([6, 50, 8, -1], dtype=torch.int32, device=cuda)
+    angle = torch.outer(torch.arange(50.0), torch.rand(hd // 2)).to(cuda)
+    before, scales_before = c.values(), [x.clone() for x in c.scales]
+    k = 1000.0 * torch.randn(4, 2, hd, device=cuda)
+    with pytest.raises(dkv.DkvError):
+        dkv.append_into_paged(k, k, c.k, c.v, slots, positions=pos, rope=(angle.cos(), angle.sin()), kv_scales=c.scales, check=True)
+    kept = [i for i in range(16) if i not in (6, 8)]
+    for now, was, scale, old in zip(c.values(), before, c.scales, scales_before):
+        assert torch.all(scale[block] > old[block])
+        step = scale[block].double()[None, :, None] * torch.ones_like(was[block, kept])
+        again = half_step(was[block, kept], step, kind) if kind == I8 else 2.0 ** -10 * step  # (kept codes are rounded once more)
+        assert torch.all((now[block, kept] - was[block, kept]).abs() <= again * (1 + 2.0 ** -20))
+
+
 # ---------------------------------------------------------------------------------------
 # reading back and patching
 # ---------------------------------------------------------------------------------------
