@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
         for (int e = 0; e < 4; ++e) {
           const float y = ex2(wt[n][i][e]);
           l[n][e & 1] += y;
-          wt[n][i][e] = y * (v_scale[i][e >> 1] * lift[e & 1]);
+          wt[n][i][e] = y * lift[e & 1] * v_scale[i][e >> 1];  // (the other product could be infinite where y is 0)
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {

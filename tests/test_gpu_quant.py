@@ -633,6 +633,33 @@ def test_attention_scales_that_differ_widely(cuda, kind, dtype):
     run_attention(c, 8, dtype, cuda)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_small_weights_alone_meet_values(cuda, kind, dtype):
+    """The heaviest tokens' values are zero (as is their scale), tokens of weight e^-80 give the result, and the weight of a
+    token with large values is 0 in fp32.  Scores are exact products; the weight's exponent, 116 in base 2, is off by
+    four roundings of 2^-24 of it (2^-15.5 of the weight), the f16 weight by 2^-11 for bf16 out (else 2^-22)."""
+    c = Cache8([24], 2, 64, 8, kind, cuda, garbage=False)
+    blocks = c.tables[0].long()
+    codes = torch.zeros(c.k.shape, device=cuda)
+    codes[blocks[1:], :, :, 0] = -1.0
+    c.k = codes.to(kind)
+    c.v = torch.randint(-9, 10, c.v.shape, device=cuda).float().to(kind)
+    c.scales = tuple(torch.zeros_like(x) for x in c.scales)
+    c.scales[0][blocks] = torch.tensor([1.0, 80.0, 200.0], device=cuda)[:, None]
+    c.scales[1][blocks] = torch.tensor([0.0, 1.0, 1024.0], device=cuda)[:, None]
+    q = torch.ones(1, 8, 64, device=cuda).to(dtype)
+    k, v, _ = c.tokens(0)
+    want = torch.einsum("tu,tud->ud", torch.softmax(k.sum(-1), 0), v).repeat_interleave(4, 0)
+    tol = want.abs() * (torch.finfo(dtype).eps / 2 + 2.0 ** -15.5 + (2.0 ** -11 if dtype == BF else 2.0 ** -22))
+    # the sum of a column may cancel: the weights' roundings count against the sum of magnitudes
+    sizes = torch.einsum("tu,tud->ud", torch.softmax(k.sum(-1), 0), v.abs()).repeat_interleave(4, 0)
+    tol = tol + sizes * (2.0 ** -15.5 + (2.0 ** -11 if dtype == BF else 2.0 ** -22)) + (2.0 ** -25 if dtype == F16 else 0)
+    for bound in (24, 5000):
+        out = dkv.paged_decode_attention(q, c.k, c.v, c.seqs(bound), scale=1.0, kv_scales=c.scales)
+        assert torch.all((out[0].double() - want).abs() <= tol)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("amp", [1e-30, 1e-3, 40.0, 1e20])
 def test_attention_q_of_any_size(cuda, dtype, amp):
