@@ -23,8 +23,10 @@
 // once, SMs that get less of the HBM than others, the join); the rest streams at 0.90-0.96 of the peak.
 //
 // A K or V byte meets twice the arithmetic that it meets in a 16-bit page, so the issue of instructions counts here:
-// q is one f16 term where it has 16 bits (exact: scaled by a power of two, 11 bits hold it) and two where it is fp32; W is one
-// term where out is bf16 (off by 2^-11 of itself at most, where out's own rounding is 2^-8), else two (2^-22).
+// q is one f16 term where it has 16 bits (exact: scaled by a power of two, 11 bits hold it) and two where it is fp32; W is two
+// (2^-22 of itself).  One term of W would do for a bf16 out's own rounding, but not where values cancel; it saves 0-6 %: us,
+// bf16 q, one / two: 32 sequences of 26000..30200 308 / 316-320, 16 of 8192 62.5 / 63, with 16 heads a KV head 65.5 / 69.4,
+// head_dim 64 57.4 / 60.2, 32 85.9 / 89.2, 64 of 1..8192 34.9 / 35.2.
 #pragma once
 
 #include "code8.cuh"
@@ -285,8 +287,7 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
   using T = typename Elem<DT>::T;
   using S = Stream8<HD, kStages, T>;
   constexpr int kTok = S::kTok;
-  constexpr int kTerms = DT == DKV_F32 ? 2 : 1;    // of q
-  constexpr int kWTerms = DT == DKV_BF16 ? 1 : 2;  // of a weight
+  constexpr int kTerms = DT == DKV_F32 ? 2 : 1;  // of q
   constexpr int kGroups = HD / 32;  // of 32 columns: one ldmatrix
   constexpr int kBatch = kGroups < 4 ? kGroups : 4;
   constexpr int kSteps = HD / 16;
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
       }
       v_cap = exp2i(15 - highest);
     }
-    uint32_t w[NB][2][kWTerms][2];
+    uint32_t w[NB][2][2][2];  // two terms
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       const float lift[2] = {exp2i(up[n][0]), exp2i(up[n][1])};
@@ -535,7 +536,7 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
           const float *y = wt[n][i] + 2 * c;
           const uint32_t v = pack_f16x2(y[0], y[1]);
           w[n][i][0][c] = transpose_8x8(v);
-          if (kWTerms == 2) w[n][i][kWTerms - 1][c] = transpose_8x8(pack_f16x2(y[0] - f16lo(v), y[1] - f16hi(v)));
+          w[n][i][1][c] = transpose_8x8(pack_f16x2(y[0] - f16lo(v), y[1] - f16hi(v)));
         }
       }
     }
@@ -560,7 +561,7 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
-              for (int x = 0; x < kWTerms; ++x) mma_f16(o[n][2 * (k0 + k) + e], a, w[n][i][x]);
+              for (int x = 0; x < 2; ++x) mma_f16(o[n][2 * (k0 + k) + e], a, w[n][i][x]);
           }
     }
     if (mt.y & kLast) {
