@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
   float unit_q[NB][2];  // what a score of heads 2t, 2t + 1 is in base 2, but for the token's scale
   float o[NB][kSteps][4], m[NB][2], l[NB][2], top_z[NB][2];
   int up[NB][2];  // O is in units of 2^-up
-  float v_cap;    // V's scales up to which no weight passes 2^15
+  float v_cap;    // V's scales up to which no weight passes 2^15; 0 while a head has no weight that `up` could be set by
   auto clear = [&]() {
     v_cap = 32768.f;
 #pragma unroll
@@ -480,9 +480,11 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
     }
     // m is any value not far from the largest score so far, 2^up any factor that keeps the weights of V's codes below
     // 2^15 and the largest of them not far below 2^8: they move (and l, O with them) only when a score passes m or a scale
-    // of V's could lift a weight too high, which after the first tile is rare
+    // of V's could lift a weight too high, which after the first tile is rare; and with every V scale that is not 0 until
+    // there is a weight to set 2^up by (a range may begin with tokens whose values are all zero)
     if (__any_sync(0xffffffffu, moves)) {
       int highest = -126;
+      bool unset = false;
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
 #pragma unroll
@@ -509,15 +511,16 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
           const int next = top_z[n][c] > 0.f
                                ? max(min(135 - static_cast<int>(__float_as_uint(top_z[n][c]) >> 23), 126), -111)
                                : up[n][c];
-          const float keep_o = ex2(m[n][c] - next_m + static_cast<float>(next - up[n][c]));
+          // (O is 0 wherever the exponent could pass 126: it has no weight yet, or m has moved by more than 126)
+          const float keep_o = ex2(fminf(m[n][c] - next_m + static_cast<float>(next - up[n][c]), 126.f));
           l[n][c] *= keep;
           m[n][c] = next_m, up[n][c] = next;
-          highest = max(highest, next);
+          highest = max(highest, next), unset |= top_z[n][c] == 0.f;
 #pragma unroll
           for (int k = 0; k < kSteps; ++k) o[n][k][c] *= keep_o, o[n][k][2 + c] *= keep_o;
         }
       }
-      v_cap = exp2i(15 - highest);
+      v_cap = unset ? 0.f : exp2i(15 - highest);
     }
     uint32_t w[NB][2][2][2];  // two terms
 #pragma unroll

@@ -1,4 +1,5 @@
-"""The weights of the attention over 8-bit pages, against plain implementations in 64 bits: values that cancel."""
+"""The weights of the attention over 8-bit pages, against plain implementations in 64 bits: values that cancel, and V's scales that
+are zero for whole tiles."""
 
 from __future__ import annotations
 
@@ -6,7 +7,7 @@ import pytest
 import torch
 
 import deltakv_b200 as dkv
-from tests.test_gpu_quant import E4M3, KINDS, TYPES, Cache8
+from tests.test_gpu_quant import E4M3, F16, KINDS, TYPES, Cache8, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,49 @@ def test_weights_of_values_that_cancel(cuda, kind, dtype):
         out = dkv.paged_decode_attention(q, c.k, c.v, c.seqs(bound), scale=1.0, kv_scales=c.scales, check=True)
         off = (out.double() - want).abs()
         assert torch.all(off <= tol), float((off / tol).max())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("span", [32, 512])
+@pytest.mark.parametrize("later", [-6, -12, -20])
+def test_tiles_whose_v_scales_are_zero(cuda, kind, dtype, span, later):
+    """Spans of tokens with V scales of 0 (as append stores zero rows) come first, and their scores are the larger ones; what
+    counts are the small V scales behind them.  Spans of 512 tokens: the first tile of each of up to 16 warps of a CTA."""
+    c = Cache8([1000, 1100, 96, 40], 2, 64, 32, kind, cuda, seed=span)
+    k_scales, v_scales = (torch.full_like(s, x) for s, x in zip(c.scales, (2.0 ** -9, 2.0 ** later)))
+    for b, n in enumerate(c.lens):
+        for i in range(0, n, 32):
+            if i // span % 2 == 0:
+                block = int(c.tables[b, i // 32])
+                v_scales[block] = 0.0
+                k_scales[block] = 2.0 ** -8
+    c.scales = (k_scales, v_scales)
+    _, out, _ = run_attention(c, 8, dtype, cuda, amp=3.0)
+    assert torch.all(out[0].abs().amax(-1) > 0)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_small_weights_behind_a_tile_of_zero_values(cuda, kind, dtype):
+    """The heaviest 32 tokens' values are zero (as is their scale), the 32 behind them, of weight e^-80, give the result; the last
+    32 have large values and a weight of 0 in fp32.  Scores are exact products; the weight's exponent, 116 in base 2, is off by
+    four roundings of 2^-24 of it (2^-15.5 of the weight), the weight as two f16 terms by 2^-22."""
+    c = Cache8([96], 2, 64, 32, kind, cuda, garbage=False)
+    blocks = c.tables[0].long()
+    codes = torch.zeros(c.k.shape, device=cuda)
+    codes[blocks, :, :, 0] = -1.0
+    c.k = codes.to(kind)
+    c.v = torch.randint(-9, 10, c.v.shape, device=cuda).float().to(kind)
+    c.scales = tuple(torch.zeros_like(x) for x in c.scales)
+    c.scales[0][blocks] = torch.tensor([0.0, 80.0, 200.0], device=cuda)[:, None]
+    c.scales[1][blocks] = torch.tensor([0.0, 1.0, 1024.0], device=cuda)[:, None]
+    q = torch.ones(1, 8, 64, device=cuda).to(dtype)
+    k, v, _ = c.tokens(0)
+    p = torch.softmax(k.sum(-1), 0)
+    want = torch.einsum("tu,tud->ud", p, v).repeat_interleave(4, 0)
+    sizes = torch.einsum("tu,tud->ud", p, v.abs()).repeat_interleave(4, 0)
+    tol = want.abs() * torch.finfo(dtype).eps / 2 + sizes * (2.0 ** -15.5 + 2.0 ** -22) + (2.0 ** -25 if dtype == F16 else 0)
+    for bound in (96, 5000):
+        out = dkv.paged_decode_attention(q, c.k, c.v, c.seqs(bound), scale=1.0, kv_scales=c.scales)
+        assert torch.all((out[0].double() - want).abs() <= tol), float(((out[0].double() - want).abs() / tol).max())
