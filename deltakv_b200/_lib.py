@@ -26,6 +26,7 @@ DKV_ERR_TIMEOUT = -9
 DKV_ERR_PAGE_RANGE = -10
 DKV_ERR_WORKSPACE = -11
 DKV_ERR_NO_BLOCKS = -12
+DKV_ERR_BLOCK_TWICE = -13
 
 # element types
 DKV_F32, DKV_F16, DKV_BF16, DKV_E4M3, DKV_I32, DKV_U8, DKV_I8 = 0, 1, 2, 3, 4, 5, 6
@@ -76,7 +77,9 @@ EXPORTED = (
     "dkv_paged_decode_attention",
     "dkv_append_paged_rotary",
     "dkv_append_paged_quant",
+    "dkv_append_paged_quant_check",
     "dkv_scatter_paged_quant",
+    "dkv_scatter_paged_quant_check",
     "dkv_gather_paged_quant",
     "dkv_paged_decode_quant_workspace_bytes",
     "dkv_paged_decode_attention_quant",
@@ -457,6 +460,10 @@ def _declare(lib: C.CDLL) -> None:
     lib.dkv_append_paged_quant.argtypes = [C.POINTER(AppendArgs), C.POINTER(Rotary), scales, scales, P]
     lib.dkv_scatter_paged_quant.restype = C.c_int
     lib.dkv_scatter_paged_quant.argtypes = [P, I32, I64, I64, I64, C.POINTER(PagedCache), scales, C.POINTER(SeqBatch), P, P]
+    lib.dkv_append_paged_quant_check.restype = C.c_int
+    lib.dkv_append_paged_quant_check.argtypes = [C.POINTER(AppendArgs), P]
+    lib.dkv_scatter_paged_quant_check.restype = C.c_int
+    lib.dkv_scatter_paged_quant_check.argtypes = [I64, C.POINTER(PagedCache), C.POINTER(SeqBatch), P, P]
     lib.dkv_gather_paged_quant.restype = C.c_int
     lib.dkv_gather_paged_quant.argtypes = [C.POINTER(PagedCache), scales, C.POINTER(SeqBatch), P, I32, I64, I64, I64, I32, P,
                                            P]

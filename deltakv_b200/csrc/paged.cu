@@ -309,6 +309,7 @@ extern "C" const char *dkv_status_string(int status) {
     case DKV_ERR_PAGE_RANGE: return "block id outside the paged cache";
     case DKV_ERR_WORKSPACE: return "workspace too small";
     case DKV_ERR_NO_BLOCKS: return "free block list exhausted";
+    case DKV_ERR_BLOCK_TWICE: return "a block of 8-bit pages is written in two places of one call";
     default: return "unknown status";
   }
 }

@@ -2,6 +2,7 @@
 //   dkv_append_paged_quant   RoPE of the new q and k rows, K and V quantised into their slots
 //   dkv_scatter_paged_quant  value + delta for the rows of every sequence, quantised again
 //   dkv_gather_paged_quant   the values of every sequence's rows
+//   dkv_append_paged_quant_check, dkv_scatter_paged_quant_check   whether a call would write a block in two places
 // The layouts and the page arithmetic are those of the paged scatter / gather (src/deltakv/paged.py:8-70).
 #include "code8.cuh"
 #include "paged_rows.cuh"
@@ -46,6 +47,9 @@ struct Store {
   int each;
   int64_t ctas; // of the store
   uint32_t spread;  // every so many-th CTA is one of them, the others are q's
+  int watchers;     // the launch's first CTAs, which look for blocks of two runs
+  int places;       // of a watcher's table, a power of two
+  int64_t segment, segments;  // the rows that a watcher takes at once, and how many of them there are
 };
 
 constexpr int kThreads = 128;
@@ -96,6 +100,169 @@ __device__ __forceinline__ int slot_in(const Store &s, int64_t row, int64_t bloc
 
 // whether the tables have a row's position
 __device__ __forceinline__ bool turns(const Store &s, int pos) { return pos >= 0 && pos < s.rope_max_pos; }
+
+// ---------------------------------------------------------------------------------------
+// blocks of two runs
+// ---------------------------------------------------------------------------------------
+// Two runs of one block in a call would be two warps that choose its scale and round its codes again at the same time: what
+// the block holds then is anything.  (Every run would have to know all others before it stores, so a launch before this
+// one: 2 us of a decode step's 5.5.)  So the launch's first CTAs watch, beside the store's.  The rows are cut into segments; a watcher
+// has two of them (or one, with itself), puts the blocks of the first one's runs into a table in shared memory and looks up the
+// second one's: every pair of runs is some watcher's.  us without / with them: 16384 rows of 32 + 8 + 8 heads x 128 92.4 / 93.1, of one
+// KV head x 64 11.4 / 11.9 (32 with four watchers, each for a quarter of the blocks and all rows), 4096 single rows 28.5 / 29.2, 73000 rows
+// of 8 x 128 patched 75.2 / 75.5; 16 segments cost another 1 us, eight 0.5 to 1.
+constexpr int kMostPlaces = 8192;
+constexpr int kQueue = 64;  // blocks of a warp that wait to be looked up, 32 at once
+struct Watch {
+  uint32_t *table;  // block + 1, 0: free
+  uint32_t *queue;  // of the warp
+  uint32_t places, seen = 0, queued = 0;
+  int lane;
+  bool adds = true, twice = false;
+  // all threads of the CTA
+  __device__ __forceinline__ Watch(uint32_t *memory, int places_)
+      : table(memory), queue(memory + places_ + (threadIdx.x >> 5) * kQueue), places(places_), lane(threadIdx.x & 31) {
+    for (uint32_t i = threadIdx.x; i < places; i += kThreads) table[i] = 0;
+    __syncthreads();
+  }
+  // (multiplicative hashing, Knuth: the top bits of the product with an odd number near 2^32 / phi)
+  __device__ __forceinline__ void look_up(uint32_t block) {
+    uint32_t at = __umulhi(block * 0x9e3779b1u, places);
+    for (uint32_t i = 0; i < places; ++i, at = (at + 1) & (places - 1)) {
+      const uint32_t was = adds ? atomicCAS(table + at, 0u, block + 1) : table[at];
+      twice |= was == block + 1;
+      if (was == 0 || was == block + 1) return;
+    }
+  }
+  // a warp's blocks, where `there`
+  __device__ __forceinline__ void see(uint32_t block, bool there) {
+    const uint32_t who = __ballot_sync(0xffffffffu, there);
+    if (there) queue[(queued + __popc(who & ((1u << lane) - 1))) % kQueue] = block;
+    queued += __popc(who);
+    __syncwarp();
+    if (queued - seen < 32) return;
+    look_up(queue[(seen + lane) % kQueue]);
+    seen += 32;
+    __syncwarp();
+  }
+  __device__ __forceinline__ void rest() {
+    if (lane < queued - seen) look_up(queue[(seen + lane) % kQueue]);
+    seen = queued;
+    __syncwarp();
+  }
+};
+
+// Rows [from, to) of an append: a run begins where a row's block is not the one of the row before.
+__device__ __forceinline__ void watch_rows(const Store &s, Watch &w, int64_t from, int64_t to) {
+  constexpr int kAtOnce = 4;
+  constexpr uint32_t kNone = 0xffffffffu;
+  const int64_t *slots = s.slots;
+  const uint64_t n_slots = s.n_slots;
+  const uint32_t size = s.block_size, inverse = 0xffffffffu / size;
+  const bool narrow = s.narrow;
+  const auto block_of = [&](int64_t slot) -> uint32_t {
+    if (static_cast<uint64_t>(slot) >= n_slots) return kNone;
+    if (!narrow) return static_cast<uint32_t>(slot / size);
+    const uint32_t x = static_cast<uint32_t>(slot), q = __umulhi(x, inverse);  // x / size, or one less: inverse is 2^32 / size less at most 1
+    return q + (x - q * size >= size);
+  };
+  for (int64_t row0 = from + (threadIdx.x & ~31u) * kAtOnce; row0 < to; row0 += kThreads * kAtOnce) {
+    int64_t slot[kAtOnce];  // all loads first
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) slot[k] = slots[min(row0 + k * 32 + w.lane, to - 1)];
+    const int64_t before = slots[max(row0 - 1, static_cast<int64_t>(0))];
+    uint32_t last = row0 > 0 ? block_of(before) : kNone;  // of the row before a warp's 32
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const uint32_t block = row0 + k * 32 + w.lane < to ? block_of(slot[k]) : kNone;
+      const uint32_t up = __shfl_up_sync(0xffffffffu, block, 1);
+      w.see(block, block != kNone && block != (w.lane == 0 ? last : up));
+      last = __shfl_sync(0xffffffffu, block, 31);
+    }
+  }
+}
+
+// The blocks of a patch that begin in rows [from, to): a warp takes 32 sequences and their blocks one after the other, 128 at once.
+__device__ __forceinline__ void watch_blocks(const Store &s, Watch &w, int64_t from, int64_t to) {
+  constexpr int kAtOnce = 4;
+  const dkv_seq_batch &q = s.seqs;
+  const int32_t *cu = q.cu_seqlens, *tables = q.block_tables;
+  const int64_t n_blocks = s.n_blocks, stride = q.table_stride, size = s.block_size, zero = 0;
+  int first = 0, end = q.n_seqs;  // the last sequence that begins at `from` or before it is in [first, end)
+  while (end - first > 1) {
+    const int step = (end - first + 31) / 32, b = first + w.lane * step;
+    const int k = __popc(__ballot_sync(0xffffffffu, b < end && cu[min(b, end - 1)] <= from));
+    first += max(k - 1, 0) * step;
+    end = min(end, first + step);
+  }
+  for (int b0 = first + static_cast<int>(threadIdx.x & ~31u); b0 < q.n_seqs; b0 += kThreads) {
+    const int b = b0 + w.lane;
+    int begin = 0, mine = 0;  // this lane's sequence's first block here, and how many of them the table has
+    bool beyond = false;
+    if (b < q.n_seqs) {
+      const int64_t start = cu[b], stop = min(static_cast<int64_t>(cu[b + 1]), to);
+      const int64_t tlen = q.table_lens ? q.table_lens[b] : stride;
+      beyond = start >= to;
+      if (start >= 0 && stop > start) {
+        const int64_t one = max(from - start + size - 1, zero) / size, n = min((stop - start + size - 1) / size, tlen) - one;
+        begin = static_cast<int>(one);
+        mine = static_cast<int>(max(min(n, static_cast<int64_t>(1 << 25)), zero));  // (32 of them fit an int)
+      }
+    }
+    int upto = mine;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, k);
+      if (w.lane >= k) upto += y;
+    }
+    const int all = __shfl_sync(0xffffffffu, upto, 31);
+    for (int i0 = 0; i0 < all; i0 += 32 * kAtOnce) {
+      int32_t id[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int i = min(i0 + j * 32 + w.lane, all - 1);
+        int l = 0;  // the sequence of block i: as many lanes have no more than i blocks up to theirs
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1)
+          if (__shfl_sync(0xffffffffu, upto, l + k - 1) <= i) l += k;
+        const int blk = i + __shfl_sync(0xffffffffu, begin - (upto - mine), l);
+        id[j] = tables[static_cast<int64_t>(b0 + l) * stride + blk];
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        w.see(id[j], i0 + j * 32 + w.lane < all && id[j] >= 0 && id[j] < n_blocks);
+    }
+    if (__any_sync(0xffffffffu, beyond)) break;
+  }
+}
+
+// one watcher (not part of the kernels' own code, whose registers it would cost)
+template <bool kPatch>
+__device__ __noinline__ void watch_runs(const Store &s, uint32_t *memory) {
+  int64_t one = 0, two = blockIdx.x;  // its segments: the pairs one <= two in order
+  for (int64_t more = s.segments; two >= more; --more) two -= more, ++one;
+  two += one;
+  Watch w(memory, s.places);
+  const auto go = [&](int64_t i) {
+    const int64_t from = i * s.segment, to = min(from + s.segment, s.n_rows);
+    if (kPatch) watch_blocks(s, w, from, to); else watch_rows(s, w, from, to);
+    w.rest();
+  };
+  go(one);
+  if (two != one) {
+    __syncthreads();
+    w.adds = false;
+    go(two);
+  }
+  if (w.twice) record_error(s.status, DKV_ERR_BLOCK_TWICE);
+}
+// the watchers alone
+template <bool kPatch>
+__global__ void __launch_bounds__(kThreads) watch_kernel(const __grid_constant__ Store s) {
+  __shared__ uint32_t memory[kMostPlaces + kThreads / 32 * kQueue];
+  begin_overlapped();
+  watch_runs<kPatch>(s, memory);
+}
 
 // VEC values in pairs, as the packed fp32 operations of sm_100 take them; one value has a zero beside it.  (Where a product
 // and a sum are rounded one after the other the single operations are used: packed ones are merged into one.)
@@ -503,10 +670,15 @@ __global__ void __launch_bounds__(kThreads, resident_of(false, SDT)) append_kern
   __shared__ Stage<VEC> stage[kThreads / 32];
   __shared__ Runs runs;
   begin_overlapped();
-  const uint32_t turn = blockIdx.x / s.spread;
-  const bool stores = turn < s.ctas && blockIdx.x == turn * s.spread;
+  if (blockIdx.x < s.watchers) {
+    watch_runs<false>(s, reinterpret_cast<uint32_t *>(stage));
+    return;
+  }
+  const uint32_t block_id = blockIdx.x - s.watchers;
+  const uint32_t turn = block_id / s.spread;
+  const bool stores = turn < s.ctas && block_id == turn * s.spread;
   if (!stores) {
-    const int64_t cta = static_cast<int64_t>(blockIdx.x) - min(static_cast<int64_t>(turn) + 1, s.ctas);
+    const int64_t cta = static_cast<int64_t>(block_id) - min(static_cast<int64_t>(turn) + 1, s.ctas);
     step::append_rows<SDT, SDT, VEC, true>(q, cta * kThreads + threadIdx.x);
     return;
   }
@@ -597,9 +769,14 @@ __global__ void __launch_bounds__(kThreads, resident_of(true, SDT)) patch_kernel
   __shared__ Stage<VEC> stage[kThreads / 32];
   __shared__ Runs runs;
   begin_overlapped();
+  if (blockIdx.x < s.watchers) {
+    watch_runs<true>(s, reinterpret_cast<uint32_t *>(stage));
+    return;
+  }
+  const uint32_t block_id = blockIdx.x - s.watchers;
   const int lane = threadIdx.x & 31;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x / s.chunks) * s.window;
-  const int chunk = static_cast<int>(blockIdx.x % s.chunks);
+  const int64_t r0 = static_cast<int64_t>(block_id / s.chunks) * s.window;
+  const int chunk = static_cast<int>(block_id % s.chunks);
   if (threadIdx.x < 32) {
     const int64_t row = r0 + lane;
     int64_t block = -1;
@@ -794,6 +971,50 @@ void deal(int64_t rows, int pairs, int sms, Store *s) {
   s->ctas = windows * s->chunks;
 }
 
+// How the rows are cut for the watchers: into 8 segments, not below 512 rows (an append's: a load of four rows a thread) or 1024, and
+// not above what a table half full holds, given that rows have a run each or (a patch) one in each block and sequence.
+void watch(bool patch, int64_t most, Store *s) {
+  const int64_t least = patch ? 1024 : 512;
+  const auto runs = [&](int64_t rows) {
+    const int64_t n = patch ? rows / s->block_size + s->seqs.n_seqs + 1 : rows;
+    return n < rows ? n : rows;
+  };
+  s->segment = (s->n_rows + 7) / 8 > least ? (s->n_rows + 7) / 8 : least;
+  while (2 * runs(s->segment) > most) s->segment = s->segment / 2 > most / 2 ? s->segment / 2 : most / 2;
+  s->segments = (s->n_rows + s->segment - 1) / s->segment;
+  s->places = 64;
+  while (s->places < 2 * runs(s->segment) && s->places < 2 * s->n_rows) s->places *= 2;
+  // ids are 32-bit in block tables, and so are a table's entries; more rows than any call has (2 million in an append) are not watched
+  constexpr int64_t kMostSegments = 512;
+  s->watchers = s->n_blocks >= UINT32_MAX || s->segments > kMostSegments ? 0 : static_cast<int>(s->segments * (s->segments + 1) / 2);
+}
+// the bytes of a launch's stages, as places
+constexpr int64_t stage_places(bool wide) { return wide ? 8192 : 4096; }
+static_assert(sizeof(Stage<8>) >= 4 * (stage_places(true) / (kThreads / 32) + kQueue) && stage_places(true) <= kMostPlaces, "a watcher's memory");
+static_assert(sizeof(Stage<1>) >= 4 * (stage_places(false) / (kThreads / 32) + kQueue), "a watcher's memory");
+
+// What the rows of an append say of themselves, without their values.
+int check_append(const dkv_append_args &g) {
+  const dkv_paged_cache &kp = g.k_pages, &vp = g.v_pages;
+  if (!code_dtype(kp.dtype)) return DKV_ERR_UNSUPPORTED;
+  if (kp.block_size <= 0 || kp.num_blocks < 0 || vp.num_blocks < 0) return DKV_ERR_LAYOUT;
+  if (g.n_rows < 0 || (g.n_rows > 0 && g.slots == nullptr)) return DKV_ERR_INVALID_ARGUMENT;
+  return DKV_OK;
+}
+void slots_of(const dkv_append_args &g, Store *s) {
+  const dkv_paged_cache &kp = g.k_pages, &vp = g.v_pages;
+  s->n_rows = g.n_rows;
+  s->n_blocks = kp.num_blocks < vp.num_blocks ? kp.num_blocks : vp.num_blocks;
+  s->n_slots = s->n_blocks * kp.block_size, s->narrow = s->n_slots <= UINT32_MAX;
+  s->slots = g.slots, s->status = g.status, s->block_size = kp.block_size;
+}
+int launch_watch(Store *s, cudaStream_t st) {
+  watch(s->slots == nullptr, kMostPlaces, s);
+  const auto kernel = s->slots ? watch_kernel<false> : watch_kernel<true>;
+  if (s->watchers > 0) DKV_CUDA_CHECK(launch_overlapped(kernel, dim3(s->watchers), kThreads, 0, st, *s));
+  return DKV_OK;
+}
+
 }  // namespace quant
 }  // namespace dkv
 
@@ -824,13 +1045,10 @@ extern "C" int dkv_append_paged_quant(const dkv_append_args *args, const dkv_rot
   quant::Store s = {};
   s.side[0] = quant::side_of(kp, *k_scales, g.k, g.k_stride_row, g.k_stride_head);
   s.side[1] = quant::side_of(vp, *v_scales, g.v, g.v_stride_row, g.v_stride_head);
-  s.n_rows = g.n_rows;
-  s.n_blocks = kp.num_blocks < vp.num_blocks ? kp.num_blocks : vp.num_blocks;
-  s.n_slots = s.n_blocks * kp.block_size, s.narrow = s.n_slots <= UINT32_MAX;
-  s.slots = g.slots, s.positions = g.positions, s.cos_t = g.rope_cos, s.sin_t = g.rope_sin;
+  quant::slots_of(g, &s);
+  s.positions = g.positions, s.cos_t = g.rope_cos, s.sin_t = g.rope_sin;
   s.rope_max_pos = g.rope_max_pos;
-  s.status = g.status;
-  s.heads = kp.n_heads, s.hd = kp.head_dim, s.block_size = kp.block_size;
+  s.heads = kp.n_heads, s.hd = kp.head_dim;
   s.rot = rot;
   step::Append q;
   step::describe(g, rot, &q);
@@ -847,9 +1065,11 @@ extern "C" int dkv_append_paged_quant(const dkv_append_args *args, const dkv_rot
   const int64_t threads = q.heads[0] == 0 ? 0 : g.n_rows * ((q.heads[0] + step::kHeads - 1) / step::kHeads) *
                                                     step::pieces_of(rot, kp.head_dim, wide ? 8 : 1);
   q.wide = threads > UINT32_MAX;
-  const int64_t ctas = s.ctas + (threads + quant::kThreads - 1) / quant::kThreads;
+  const int64_t work = s.ctas + (threads + quant::kThreads - 1) / quant::kThreads;
+  s.spread = static_cast<uint32_t>(work / s.ctas);
+  quant::watch(false, quant::stage_places(wide), &s);
+  const int64_t ctas = work + s.watchers;
   if (ctas > INT32_MAX) return DKV_ERR_UNSUPPORTED;
-  s.spread = static_cast<uint32_t>(ctas / s.ctas);
   static_assert(quant::kThreads == step::kAppThreads, "one launch for both");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 #define DKV_QUANT_CASE(S, P)                                                                                  \
@@ -893,7 +1113,8 @@ extern "C" int dkv_scatter_paged_quant(const void *delta, int32_t delta_dtype, i
   const bool wide = cache->head_dim % 16 == 0 && cache->head_dim <= 512 && quant::source_bits(s.side[0], size) % 16 == 0 &&
                     quant::page_bits(s.side[0]) % 8 == 0 && quant::short_strides(s.side[0]);
   quant::deal(n_rows, cache->n_heads, sms, &s);
-  const int64_t ctas = s.ctas;
+  quant::watch(true, quant::stage_places(wide), &s);
+  const int64_t ctas = s.ctas + s.watchers;
   if (ctas > INT32_MAX) return DKV_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 #define DKV_QUANT_CASE(S, P)                                                                               \
@@ -910,6 +1131,28 @@ extern "C" int dkv_scatter_paged_quant(const void *delta, int32_t delta_dtype, i
   DKV_QUANT_CASE(DKV_F32, DKV_I8)
 #undef DKV_QUANT_CASE
   return DKV_ERR_UNSUPPORTED;
+}
+
+extern "C" int dkv_append_paged_quant_check(const dkv_append_args *args, dkv_stream_t stream) {
+  if (args == nullptr) return DKV_ERR_INVALID_ARGUMENT;
+  const int rc = quant::check_append(*args);
+  if (rc != DKV_OK || args->n_rows == 0) return rc;
+  quant::Store s = {};
+  quant::slots_of(*args, &s);
+  return quant::launch_watch(&s, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dkv_scatter_paged_quant_check(int64_t n_rows, const dkv_paged_cache *cache, const dkv_seq_batch *seqs, int32_t *status,
+                                             dkv_stream_t stream) {
+  if (cache == nullptr || seqs == nullptr || n_rows < 0) return DKV_ERR_INVALID_ARGUMENT;
+  if (!quant::code_dtype(cache->dtype)) return DKV_ERR_UNSUPPORTED;
+  if (cache->block_size <= 0 || cache->num_blocks < 0) return DKV_ERR_LAYOUT;
+  const int rc = quant::check_seqs(*seqs);
+  if (rc != DKV_OK || n_rows == 0 || seqs->n_seqs == 0) return rc;
+  quant::Store s = {};
+  s.n_rows = n_rows, s.n_blocks = cache->num_blocks, s.block_size = cache->block_size;
+  s.seqs = quant::readable(*seqs), s.status = status;
+  return quant::launch_watch(&s, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dkv_gather_paged_quant(const dkv_paged_cache *cache, const dkv_page_scales *scales, const dkv_seq_batch *seqs,

@@ -41,6 +41,8 @@ int (*g_gather_quant)(const dkv_paged_cache *, const dkv_page_scales *, const dk
                       int64_t, int32_t, int32_t *, dkv_stream_t);
 int (*g_workspace_quant)(const dkv_paged_decode_args *, int32_t, int64_t *);
 int (*g_attend_quant)(const dkv_paged_decode_args *, int32_t, const dkv_page_scales *, const dkv_page_scales *, dkv_stream_t);
+int (*g_append_check)(const dkv_append_args *, dkv_stream_t);
+int (*g_scatter_check)(int64_t, const dkv_paged_cache *, const dkv_seq_batch *, int32_t *, dkv_stream_t);
 PyObject *g_raise;        // raises the package's error for a status code
 PyObject *g_status_word;  // device index -> address of its status word
 constexpr int kMaxDevices = 64;
@@ -156,6 +158,14 @@ void check(int rc, const char *entry) {
   PyObject *r = PyObject_CallFunction(g_raise, "is", rc, entry);
   Py_XDECREF(r);
   throw Raised{nullptr, ""};  // the call above raised
+}
+
+// Launches a look at a call's blocks, waits for what it records and raises it: f(status word) is the launch.
+template <typename F>
+void refuse(const Place &place, const char *look, F f) {
+  Tensor word = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(place.device));
+  check(f(word.data_ptr<int32_t>()), look);
+  check(word.item<int32_t>(), place.where);
 }
 
 void int32_vector(const Tensor &t, const char *name, int64_t n) {  // n < 0: any length
@@ -365,11 +375,11 @@ PyObject *rope_ready(PyObject *, PyObject *const *a, Py_ssize_t count) {
   });
 }
 
-// append(k, v, k_pages, v_pages, slots, q, positions, cos, sin, q_out, rotary_dim, interleaved, kv_scales)
-//   -> q_out or None; rotary_dim None: the whole head
+// append(k, v, k_pages, v_pages, slots, q, positions, cos, sin, q_out, rotary_dim, interleaved, kv_scales, look)
+//   -> q_out or None; rotary_dim None: the whole head; look: whether 8-bit pages' rows follow one another is seen first
 PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
   return guarded([&]() -> PyObject * {
-    if (count != 13) type_error("append takes 13 arguments");
+    if (count != 14) type_error("append takes 14 arguments");
     const Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v");
     const PairOfScales scales(a[12]);
     const Pages pages(tensor(a[2], "k_pages"), tensor(a[3], "v_pages"), static_cast<bool>(scales));
@@ -377,8 +387,8 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
     const Tensor *q = maybe(a[5], "q"), *positions = maybe(a[6], "positions"), *cos = maybe(a[7], "rope cos"),
                  *sin = maybe(a[8], "rope sin"), *q_out = maybe(a[9], "q_out");
     const int64_t rows = slots.numel(), rotary_dim = a[10] == Py_None ? pages.hd : integer(a[10]);
-    const int crossed = PyObject_IsTrue(a[11]);
-    if (crossed < 0) throw Raised{nullptr, ""};
+    const int crossed = PyObject_IsTrue(a[11]), look = PyObject_IsTrue(a[13]);
+    if (crossed < 0 || look < 0) throw Raised{nullptr, ""};
     if ((a[10] != Py_None || crossed) && !cos) value_error("rotary_dim and interleaved say how rope turns: pass rope with them");
     if (slots.scalar_type() != at::kLong) type_error("slots must be int64");
     if (slots.dim() != 1 || !slots.is_contiguous()) value_error("slots must be a contiguous vector");
@@ -448,6 +458,12 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t count) {
     dkv_rotary rotary;
     rotary.dim = static_cast<int32_t>(rotary_dim), rotary.interleaved = crossed;
     if (scales) {
+      if (look)
+        refuse(at_, "dkv_append_paged_quant_check", [&](int32_t *word) {
+          dkv_append_args rows = p;
+          rows.status = word;
+          return g_append_check(&rows, at_.stream());
+        });
       const dkv_page_scales ks = describe_scales(*scales.k), vs = describe_scales(*scales.v);
       check(g_append_quant(&p, &rotary, &ks, &vs, at_.stream()), "dkv_append_paged_quant");
     } else {
@@ -554,10 +570,12 @@ void check_coded(const Tensor &pages, const Tensor &scales) {
   scales_of(scales, "page_scales", pages);
 }
 
-// scatter(delta, pages, page_scales, cu_seqlens, block_tables, table_lens, max_seq_len)
+// scatter(delta, pages, page_scales, cu_seqlens, block_tables, table_lens, max_seq_len, look)
 PyObject *scatter(PyObject *, PyObject *const *a, Py_ssize_t count) {
   return guarded([&]() -> PyObject * {
-    if (count != 7) type_error("scatter takes 7 arguments");
+    if (count != 8) type_error("scatter takes 8 arguments");
+    const int look = PyObject_IsTrue(a[7]);
+    if (look < 0) throw Raised{nullptr, ""};
     const Tensor &delta = tensor(a[0], "delta"), &pages = tensor(a[1], "pages"), &scales = tensor(a[2], "page_scales");
     const Sequences seqs(a[3], a[4], a[5], a[6]);
     check_coded(pages, scales);
@@ -573,6 +591,9 @@ PyObject *scatter(PyObject *, PyObject *const *a, Py_ssize_t count) {
     const dkv_paged_cache cache = describe(pages, code_of(pages.scalar_type()));
     const dkv_page_scales s = describe_scales(scales);
     const dkv_seq_batch q = seqs.describe();
+    if (look)
+      refuse(at_, "dkv_scatter_paged_quant_check",
+             [&](int32_t *word) { return g_scatter_check(delta.size(0), &cache, &q, word, at_.stream()); });
     check(g_scatter_quant(delta.data_ptr(), code, delta.size(0), delta.stride(0), delta.stride(1), &cache, &s, &q,
                           at_.status(), at_.stream()),
           "dkv_scatter_paged_quant");
@@ -616,13 +637,14 @@ PyObject *gather(PyObject *, PyObject *const *a, Py_ssize_t count) {
   });
 }
 
-// bind(plan, append, workspace, attend, append_quant, scatter_quant, gather_quant, workspace_quant, attend_quant, raise_error,
-//      status_word): entry addresses and callbacks
+// bind(plan, append, workspace, attend, append_quant, scatter_quant, gather_quant, workspace_quant, attend_quant, append_check,
+//      scatter_check, raise_error, status_word): entry addresses and callbacks
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t count) {
   return guarded([&]() -> PyObject * {
-    if (count != 11) type_error("bind takes 11 arguments");
-    void *entry[9];
-    for (int i = 0; i < 9; ++i) {
+    constexpr int kEntries = 11;
+    if (count != kEntries + 2) type_error("bind takes 13 arguments");
+    void *entry[kEntries];
+    for (int i = 0; i < kEntries; ++i) {
       entry[i] = PyLong_AsVoidPtr(a[i]);
       if (entry[i] == nullptr) {
         if (PyErr_Occurred()) throw Raised{nullptr, ""};
@@ -638,10 +660,12 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t count) {
     g_gather_quant = reinterpret_cast<decltype(g_gather_quant)>(entry[6]);
     g_workspace_quant = reinterpret_cast<decltype(g_workspace_quant)>(entry[7]);
     g_attend_quant = reinterpret_cast<decltype(g_attend_quant)>(entry[8]);
-    Py_INCREF(a[9]);
-    Py_XSETREF(g_raise, a[9]);
-    Py_INCREF(a[10]);
-    Py_XSETREF(g_status_word, a[10]);
+    g_append_check = reinterpret_cast<decltype(g_append_check)>(entry[9]);
+    g_scatter_check = reinterpret_cast<decltype(g_scatter_check)>(entry[10]);
+    Py_INCREF(a[kEntries]);
+    Py_XSETREF(g_raise, a[kEntries]);
+    Py_INCREF(a[kEntries + 1]);
+    Py_XSETREF(g_status_word, a[kEntries + 1]);
     Py_RETURN_NONE;
   });
 }

@@ -63,7 +63,7 @@ def _native():
         entries = (lib.dkv_plan_paged_step, lib.dkv_append_paged_rotary, lib.dkv_paged_decode_workspace_bytes,
                    lib.dkv_paged_decode_attention, lib.dkv_append_paged_quant, lib.dkv_scatter_paged_quant,
                    lib.dkv_gather_paged_quant, lib.dkv_paged_decode_quant_workspace_bytes,
-                   lib.dkv_paged_decode_attention_quant)
+                   lib.dkv_paged_decode_attention_quant, lib.dkv_append_paged_quant_check, lib.dkv_scatter_paged_quant_check)
         module.bind(*(C.cast(f, C.c_void_p).value for f in entries), _raise_error, _status_address)
         _native_module = module
     return _native_module
@@ -135,8 +135,9 @@ def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, sl
     is kept; later values that do not fit make the scale grow by powers of two, and what the block holds is rounded to the
     new one (int8: by less than one step in all; e4m3: not at all above its subnormals).  So codes and scales may start as any memory.
     Rows may be fp32, fp16 or bf16, and the rows of one block follow one another, with no row
-    of a negative slot between them (as :func:`plan_paged_step` lays them out).  A value that is not finite makes the block's head read as NaN until
-    the block is begun anew.
+    of a negative slot between them (as :func:`plan_paged_step` lays them out): ``check=True`` refuses a call in which they do not
+    before it stores anything; without it such a call is recorded, and the block holds anything.  A value that is not finite makes
+    the block's head read as NaN until the block is begun anew.
     """
     native = _native_module or _native()
     cos = sin = None
@@ -148,7 +149,7 @@ def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, sl
             if isinstance(rope, RotaryEmbedding):
                 rotary_dim, interleaved = rope.form(k.shape[-1], rotary_dim, interleaved)
     q_out = native.append(k, v, k_pages, v_pages, slots, q, positions, cos, sin, q_out, rotary_dim,
-                          interleaved or False, kv_scales)
+                          interleaved or False, kv_scales, check)
     if check:
         ops.status_word(k.device).raise_if_set("append_into_paged")
     return q_out

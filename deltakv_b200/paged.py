@@ -48,6 +48,8 @@ def scatter_into_paged(delta: Tensor, cache: Tensor, block_table: list[int], blo
     seqs = ops.SeqBatchTensors.single(seq, table, pages.device)
     if page_scales is not None:
         _whole_blocks(pages, block_size)
+        if len(set(table)) != len(table):
+            raise ValueError("block_table names a block of 8-bit pages twice")
         return scatter_into_paged_batched(delta, pages, seqs, page_scales=page_scales)
     # the kernel reads slot i % block_size of block i // block_size, as the reference does
     view = pages if block_size == pages.shape[1] else pages[:, :block_size]
@@ -99,11 +101,12 @@ def scatter_into_paged_batched(delta: Tensor, pages: Tensor, seqs: ops.SeqBatchT
     ``[num_blocks, heads]`` (:func:`~deltakv_b200.append_into_paged` keeps such): value + delta is formed in fp32 and
     the block quantised again.  A block that a sequence covers whole gets the scale that its new values need; in
     a sequence's last block the slots behind its end are kept, and the scale only grows.  Pages of one sequence
-    must not be another's.  ``delta`` may be fp32, fp16 or bf16; the launch runs on the current stream of the pages' device.
+    must not be another's (a shared prefix is patched by one of them): ``check=True`` refuses such a call before it stores anything, without it
+    it is recorded, and the pages hold anything.  ``delta`` may be fp32, fp16 or bf16; the launch runs on the current stream of the pages' device.
     """
     st = ops.status_word(pages.device) if pages.is_cuda else None
     if page_scales is not None:
-        _native().scatter(delta, pages, page_scales, seqs.cu_seqlens, seqs.block_tables, seqs.table_lens, seqs.max_seq_len)
+        _native().scatter(delta, pages, page_scales, seqs.cu_seqlens, seqs.block_tables, seqs.table_lens, seqs.max_seq_len, check)
     else:
         ops.scatter_paged(delta, pages, seqs, st)
     if check:

@@ -53,6 +53,7 @@ typedef struct CUstream_st *dkv_stream_t;
 #define DKV_ERR_PAGE_RANGE (-10)       /* block id outside [0, num_blocks)                */
 #define DKV_ERR_WORKSPACE (-11)        /* workspace too small                             */
 #define DKV_ERR_NO_BLOCKS (-12)        /* the list of free blocks ran out                 */
+#define DKV_ERR_BLOCK_TWICE (-13)      /* an 8-bit block written in two places of a call  */
 
 /* ---- element types ------------------------------------------------------ */
 #define DKV_F32 0
@@ -701,20 +702,27 @@ typedef struct dkv_page_scales {
 /*
  * dkv_append_paged_rotary into 8-bit pages: in_dtype is F32, F16 or BF16 whatever the pages.  Storing a block's slot 0
  * begins the block: nothing that it held is kept.  The rows of one block follow one another, with no row without a slot
- * between them (as dkv_plan_paged_step lays them out); slots are distinct.
+ * between them (as dkv_plan_paged_step lays them out); slots are distinct.  A block whose rows do not follow one another is
+ * recorded (BLOCK_TWICE in *status; calls of up to a million rows), and what it then holds is anything: two warps choose its
+ * scale.  The _check entry looks for such blocks and stores nothing (it reads n_rows, slots, the pages' descriptions and status
+ * alone).
  */
 int dkv_append_paged_quant(const dkv_append_args *args, const dkv_rotary *rotary, const dkv_page_scales *k_scales,
                            const dkv_page_scales *v_scales, dkv_stream_t stream);
+int dkv_append_paged_quant_check(const dkv_append_args *args, dkv_stream_t stream);
 
 /*
  * Row r of delta [n_rows, heads, head_dim] (rows follow cu_seqlens) is added to the value of its slot, in fp32 and rounded
  * after the product and after the sum, and the blocks are quantised again: one that is covered whole with a scale of its own,
- * of another the slots behind the sequence's end are kept.  No block belongs to two sequences.  Rows past n_rows are left out (INVALID_ARGUMENT in
+ * of another the slots behind the sequence's end are kept.  No block belongs to two sequences,
+ * or comes twice in one's table: that is recorded, and can be asked for beforehand, as in dkv_append_paged_quant.  Rows past n_rows are left out (INVALID_ARGUMENT in
  * *status), as are those without a block (BLOCK_TABLE_SHORT, PAGE_RANGE).
  */
 int dkv_scatter_paged_quant(const void *delta, int32_t delta_dtype, int64_t n_rows, int64_t delta_stride_row,
                             int64_t delta_stride_head, const dkv_paged_cache *cache, const dkv_page_scales *scales,
                             const dkv_seq_batch *seqs, int32_t *status, dkv_stream_t stream);
+int dkv_scatter_paged_quant_check(int64_t n_rows, const dkv_paged_cache *cache, const dkv_seq_batch *seqs, int32_t *status,
+                                  dkv_stream_t stream);
 
 /*
  * The values of every sequence's rows into out [n_rows, heads, head_dim] (F32, F16 or BF16, rounded once).  Rows without
