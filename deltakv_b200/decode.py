@@ -131,7 +131,7 @@ def append_into_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, sl
     **8-bit pages** (``torch.float8_e4m3fn`` or ``torch.int8``, at most 1024 slots a block) come with
     ``kv_scales = (k_scales, v_scales)``, fp32 ``[num_blocks, n_kv]``: a slot's value is its code times its block's and
     head's scale.  The operator keeps them: storing a block's slot 0 begins the block with the scale that this call's
-    values need (e4m3: the least power of two; int8: the largest magnitude / 127), and nothing the block held
+    values need (e4m3: the least power of two; int8: the largest magnitude times 1/127 in fp32), and nothing the block held
     is kept; later values that do not fit make the scale grow by powers of two, and what the block holds is rounded to the
     new one (int8: by less than one step in all; e4m3: not at all above its subnormals).  So codes and scales may start as any memory.
     Rows may be fp32, fp16 or bf16, and the rows of one block follow one another, with no row

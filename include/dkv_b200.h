@@ -689,7 +689,8 @@ int dkv_append_paged_rotary(const dkv_append_args *args, const dkv_rotary *rotar
  * The scales of K or V pages of 8-bit codes (dtype DKV_E4M3 or DKV_I8, block_size at most 1024): the value of a slot
  * is its code times base[block * stride_block + head * stride_head] (fp32, strides in elements).  What reads takes any scales; what writes
  * chooses them.  Of a block and head of which nothing is kept, with amax the largest magnitude stored:
- *   e4m3: the least power of two s with amax <= 448 s;  int8: s = amax / 127;  not below 2^-126, 0 for amax = 0.
+ *   e4m3: the least power of two s with amax <= 448 s;  int8: s = amax times 1/127, each
+ *   rounded to fp32 (so one unit of the last place off the quotient at times);  not below 2^-126, 0 for amax = 0.
  * Of one that holds others: s 2^j with the least j >= 0 that gives amax <= 448 s 2^j (e4m3) or 127.5 s 2^j (int8); where j > 0 the
  * codes kept are rounded again.  Codes are the nearest to value * (1 / s), ties to even.  A value that is not finite makes the scale
  * NaN, so that all of the block's head reads as NaN until it is begun anew.
