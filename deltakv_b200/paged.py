@@ -120,7 +120,7 @@ def gather_from_paged_batched(pages: Tensor, seqs: ops.SeqBatchTensors, rows: in
 
     ``page_scales``: as for :func:`scatter_into_paged_batched`.  ``rows`` is the capacity (the lengths live on the GPU); rows behind the last
     sequence are zero in a new tensor and left as they are in ``out``.  ``dtype`` (fp32, the default, fp16 or bf16) is
-    the new tensor's: an e4m3 code times a power of two is exact in bf16, an int8 value is rounded once.  Tokens without a block
+    the new tensor's: values are rounded to fp32 and then to it (an e4m3 code times a power of two is exact in all but fp16's range).  Tokens without a block
     are zero, recorded and raised with ``check=True``.
     """
     if out is not None and dtype not in (None, out.dtype):

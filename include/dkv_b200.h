@@ -726,8 +726,9 @@ int dkv_scatter_paged_quant_check(int64_t n_rows, const dkv_paged_cache *cache, 
                                   dkv_stream_t stream);
 
 /*
- * The values of every sequence's rows into out [n_rows, heads, head_dim] (F32, F16 or BF16, rounded once).  Rows without
- * a block become zero (and are recorded); rows behind the last sequence become zero where zero_rest, else they are left.
+ * The values of every sequence's rows into out [n_rows, heads, head_dim] (F32, F16 or BF16): code times scale, rounded to fp32 and
+ * then to out's type (which is one rounding where the product is exact in fp32, as of e4m3 codes and powers of two).  Rows
+ * without a block become zero (and are recorded); rows behind the last sequence become zero where zero_rest, else they are left.
  */
 int dkv_gather_paged_quant(const dkv_paged_cache *cache, const dkv_page_scales *scales, const dkv_seq_batch *seqs, void *out,
                            int32_t out_dtype, int64_t n_rows, int64_t out_stride_row, int64_t out_stride_head,

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import deltakv_b200 as dkv
-from tests.test_gpu_quant import E4M3, KINDS
+from tests.test_gpu_quant import BF, E4M3, F16, KINDS
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,23 @@ def test_first_scales_bit_for_bit(cuda, kind):
                                block_tables=torch.arange(blocks, dtype=torch.int32, device=cuda)[None], max_seq_len=blocks * block)
     dkv.scatter_into_paged_batched(x, pages[0], seqs, page_scales=scales[0], check=True)
     assert torch.equal(scales[0], want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_values_are_rounded_to_fp32_first(cuda, dtype):
+    """Where code times scale lies so near a tie of the 16-bit type that fp32 makes it one, the value is the fp32 number's rounding."""
+    g = torch.Generator().manual_seed(0)
+    places = 8 if dtype == BF else 11
+    code = torch.randint(-127, 128, (4_000_000,), generator=g)
+    scale = 1e-2 * (1 + torch.rand(code.shape, generator=g))
+    exact = code.double() * scale.double()
+    m, e = torch.frexp(exact)
+    once = torch.ldexp(torch.round(m * 2 ** places), e - places)  # (ties to even)
+    want = (code.float() * scale).to(dtype)
+    twice = torch.nonzero(want.double() != once)[:, 0][:64]
+    assert len(twice) > 8
+    pages = code[twice].to(torch.int8)[:, None, None, None].expand(-1, 8, 1, 32).contiguous().to(cuda)
+    seqs = dkv.SeqBatchTensors(cu_seqlens=torch.tensor([0, 8 * len(twice)], dtype=torch.int32, device=cuda),
+                               block_tables=torch.arange(len(twice), dtype=torch.int32, device=cuda)[None], max_seq_len=8 * len(twice))
+    got = dkv.gather_from_paged_batched(pages, seqs, 8 * len(twice), page_scales=scale[twice][:, None].to(cuda), dtype=dtype, check=True)
+    assert torch.equal(got.view(len(twice), 8, 32), want[twice][:, None, None].expand(-1, 8, 32).to(cuda))
