@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import deltakv_b200 as dkv
-from tests.test_gpu_quant import BF, E4M3, F16, KINDS
+from tests.test_gpu_quant import BF, E4M3, F16, F32, KINDS, append_case
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,13 @@ def test_values_are_rounded_to_fp32_first(cuda, dtype):
                                block_tables=torch.arange(len(twice), dtype=torch.int32, device=cuda)[None], max_seq_len=8 * len(twice))
     got = dkv.gather_from_paged_batched(pages, seqs, 8 * len(twice), page_scales=scale[twice][:, None].to(cuda), dtype=dtype, check=True)
     assert torch.equal(got.view(len(twice), 8, 32), want[twice][:, None, None].expand(-1, 8, 32).to(cuda))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("block,hd,layout", [(64, 128, "kv_first"), (1024, 64, "block_first"), (100, 50, "odd")])
+def test_single_rows_in_long_blocks(cuda, kind, dtype, block, hd, layout):
+    """A decode step whose rows, one a block, lie behind a block's 32nd slot, and whose scales grow: the slots of all 32-slot words
+    keep their values."""
+    chunks = [(at % block, 1) for at in (32, 33, 40, 63, 64, 95, 96, 31, 500, 992, 1023, 991, 99, 65, 5, 60)]
+    append_case(cuda, kind, dtype, hd=hd, rot=0, interleaved=False, block=block, layout=layout, n_kv=3, heads=3, chunks=chunks, seed=block)
