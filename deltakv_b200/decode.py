@@ -183,7 +183,9 @@ def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: op
     **8-bit pages** (``torch.float8_e4m3fn`` or ``torch.int8``) come with ``kv_scales = (k_scales, v_scales)``, fp32
     ``[num_blocks, n_kv]``, one factor for each block and KV head — those that :func:`append_into_paged` keeps, or any.  ``q``
     then is bf16, fp16 or fp32 and ``out`` has its type; products are fp16 with fp32 sums, in which the codes and a 16-bit ``q``
-    are exact; fp32 ``q`` and the weights enter as two terms each (2^-22).
+    are exact (bf16: elements down to 2^-27 of the head's largest, those below in steps of 2^-38 of it); fp32 ``q`` and the weights
+    enter as two terms each (2^-22).  A weight enters times its token's V scale, in steps of 2^-33 of the largest such product: beside
+    a token whose V scale is 2^33 times theirs, others vanish even from the columns in which that token's codes are 0.
     A NaN code or scale of a token that counts gives NaN.
     """
     got = (_native_module or _native()).attend(q, k_pages, v_pages, seqs.cu_seqlens, seqs.block_tables, seqs.table_lens,

@@ -736,8 +736,9 @@ int dkv_gather_paged_quant(const dkv_paged_cache *cache, const dkv_page_scales *
 
 /*
  * dkv_paged_decode_attention over 8-bit pages (any block_size), q and out of q_dtype (F32, F16 or BF16).  Scores and weights go through
- * the tensor cores as f16 products with fp32 sums: q of 16 bits exactly (scaled by a power of two), fp32 q and the weights
- * as two f16 terms each (2^-22).  A code or a scale that is NaN gives NaN.
+ * the tensor cores as f16 products with fp32 sums: q of 16 bits exactly (scaled by a power of two; of bf16 the elements down to
+ * 2^-27 of the head's largest), fp32 q and the weights as two f16 terms each (2^-22), and both not below 2^-38 of the head's
+ * largest element and 2^-33 of the largest weight times V scale.  A code or a scale that is NaN gives NaN.
  */
 int dkv_paged_decode_quant_workspace_bytes(const dkv_paged_decode_args *args, int32_t q_dtype, int64_t *bytes);
 int dkv_paged_decode_attention_quant(const dkv_paged_decode_args *args, int32_t q_dtype, const dkv_page_scales *k_scales,
