@@ -18,15 +18,15 @@
 // dealt so that a lane's rows g and g + 8 of O^T are neighbours, 16 k + 2 g and + 1, and outputs are stored in pairs.
 //
 // Measured on a B200 (calls back to back; HBM floor at the measured 6535 GB/s): 32 sequences of 20000..32768, 8 KV heads x 128,
-// e4m3: 299-330 us by the box's power (floor 265); 16 of 8192: 55-63 us (41); one of 131071: 56 (41); 64 of 1..8192, int8, f16 q
-// of 64 heads: 36-43 (23); 256 of 1..600: 25 (7.5).  12 to 15 us of each are fixed (the launch, the first tiles of all SMs at
+// e4m3: 300-330 us by the box's power (floor 265); 16 of 8192: 56-66 us (41); one of 131071: 57 (41); 64 of 1..8192, int8, f16 q
+// of 64 heads: 42-43 (23); 256 of 1..600: 25-26 (7.5).  12 to 15 us of each are fixed (the launch, the first tiles of all SMs at
 // once, SMs that get less of the HBM than others, the join); the rest streams at 0.90-0.96 of the peak.
 //
 // A K or V byte meets twice the arithmetic that it meets in a 16-bit page, so the issue of instructions counts here:
 // q is one f16 term where it has 16 bits (exact: scaled by a power of two, 11 bits hold it) and two where it is fp32; W is two
 // (2^-22 of itself).  One term of W would do for a bf16 out's own rounding, but not where values cancel; it saves 0-6 %: us,
-// bf16 q, one / two: 32 sequences of 26000..30200 308 / 316-320, 16 of 8192 62.5 / 63, with 16 heads a KV head 65.5 / 69.4,
-// head_dim 64 57.4 / 60.2, 32 85.9 / 89.2, 64 of 1..8192 34.9 / 35.2.
+// bf16 q, one / two: 32 sequences of 26000..30200 303-311 / 316-325, 16 of 8192 62.5 / 64, with 16 heads a KV head 65.5 / 69.5,
+// 16 of 16384 of head_dim 64 57.4 / 60.3, of 32768 of 32 85.9 / 89.3, 64 of 1..8192 34.9 / 35.2.
 #pragma once
 
 #include "code8.cuh"
@@ -641,9 +641,9 @@ __global__ void __launch_bounds__(W * 32, 1) walk8_kernel(const __grid_constant_
 // Warps of a CTA (one an SM) and stages of a warp's ring, as registers and 227 KB allow.  Three stages of eight warps stream
 // better than two of twelve (one range's eight heads on one SM, whose rows are neighbours in memory); where arithmetic or
 // many short sequences bound it, twelve are a little better.  us, 8 KV heads: head_dim 128, 8 x 3 / 12 x 2: 32 sequences of
-// 26000..30200 307 / 325, 16 of 8192 55.6 / 58.2, 64 of 1..8192 34.0 / 35.6, 256 of 1..600 24.7 / 23.1, block_size 24 (rows looked up one
-// by one) 70 / 60.  head_dim 64, 16 x 2 / 14 x 3 / 10 x 4 / 8 x 5: 16 of 16384 57.5 / 60 / 65 / 70.  32, 16 x 4 / 12 x 5 / 8 x 8: 16 of
-// 32768 85 / 91 / 115.  256, 6 x 2 / 4 x 3: 16 of 4096 59 / 58.
+// 26000..30200 303 / 323, 16 of 8192 61 / 61, 64 of 1..8192 35.6 / 36.5, 256 of 1..600 25.7 / 24.3, block_size 24 (rows looked up one
+// by one) 74 / 63.  head_dim 64, 16 x 2 / 14 x 3 / 8 x 5: 16 of 16384 60.7 / 64.6 / 75.2.  32, 16 x 4 / 12 x 5 / 8 x 8: 16 of
+// 32768 89.5 / 98.7 / 121.5.  256, 6 x 2 / 4 x 3: 16 of 4096 60.1 / 62.6.
 constexpr Variant variant8(bool f32, int hd, int heads) {
   if (hd == 256) return {6, 2, 32};
   if (hd == 128) return {8, 3, 32};
@@ -651,10 +651,10 @@ constexpr Variant variant8(bool f32, int hd, int heads) {
   return hd == 64 ? (f32 ? Variant{12, 3, 32} : Variant{16, 2, 32}) : Variant{16, 4, 32};
 }
 // Query heads of a unit: 16 where a KV head has more than eight and registers allow it (16 sequences of 8192, 16 heads for each
-// of 8 KV heads x 128: 63 us, as two units of eight 89, with twelve warps 77).
+// of 8 KV heads x 128: 70 us, as two units of eight 92, with twelve warps 105).
 constexpr int heads8(bool f32, int hd, int group) { return !f32 && hd <= 128 && group > 8 ? 16 : 8; }
-// A sequence costs more tokens than in the 16-bit walk, whose tokens take longer.  At 48 / 96 / 160, us: 64 sequences of
-// 1..8192 39.5 / 33.6 / 34.1, 256 of 1..600 23.8 / 25.5 / 28.7.
+// A sequence costs more tokens than in the 16-bit walk, whose tokens take longer.  At 48 / 80 / 160, us: 64 sequences of
+// 1..8192 41.0 / 35.6 / 36.7, 256 of 1..600 25.3 / 25.7 / 30.8.
 constexpr int kSeqCost8 = 80;
 // CTAs of one warp lose to ranges (148 sequences of 64 / 150 tokens: 13.7 / 20.1 us in one launch, 11.8 / 16.4 split); of two,
 // they win (60 of 300: 12.8 against 17.0), as do more (37 of 500: 11.3 against 17.8; 18 of 1000: 11.6 against 16.3, of

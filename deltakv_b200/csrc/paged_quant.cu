@@ -658,9 +658,9 @@ __device__ __forceinline__ void store_single_rows(const Store &s, int chunk, con
 }
 
 // k, v and q are read once, codes and q written once, so memory would bound it (57.8 us for 16384 rows of 32 + 8 + 8 heads x 128,
-// bf16 to e4m3); it takes 92 us (without q about 50, floor 17), half of the issue slots used by 18 warps an SM: a run of 16 rows of a head takes some 1100
+// bf16 to e4m3); it takes 93 us (without q about 50, floor 17), half of the issue slots used by 18 warps an SM: a run of 16 rows of a head takes some 1100
 // instructions (the rotation, the largest, two conversions), and registers leave no room for more warps.  The store's CTAs,
-// which wait for memory several times, lie evenly among those of q, which only stream.  4096 single rows of the same heads 28.5 us
+// which wait for memory several times, lie evenly among those of q, which only stream.  4096 single rows of the same heads 29 us
 // (a run a warp: 103), 64 of them 6 us of device time from cold caches.  Left out, for the 16384 rows: values kept in registers
 // 140 us (spilled), a run for the whole CTA 123, rows kept as read and rotated twice 106, L2 asked for a CTA's rows before their
 // runs are found 98.
@@ -763,7 +763,7 @@ __device__ __forceinline__ int64_t page_of(const dkv_seq_batch &q, int64_t n_blo
 }
 
 // The rows and the codes are read once, codes written once: memory would bound it (46 us for 73200 rows of 8 x 128, bf16 on
-// e4m3); it takes 75 us, 49 % of the issue slots used by 15 warps an SM, 1060 instructions a run of 16 rows of a head.
+// e4m3); it takes 76 us, 50 % of the issue slots used by 15 warps an SM, 1105 instructions a run of 16 rows of a head.
 template <int SDT, int PDT, int VEC>
 __global__ void __launch_bounds__(kThreads, resident_of(true, SDT)) patch_kernel(const __grid_constant__ Store s) {
   __shared__ Stage<VEC> stage[kThreads / 32];
