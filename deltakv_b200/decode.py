@@ -185,7 +185,8 @@ def paged_decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, seqs: op
     then is bf16, fp16 or fp32 and ``out`` has its type; products are fp16 with fp32 sums, in which the codes and a 16-bit ``q``
     are exact (bf16: elements down to 2^-27 of the head's largest, those below in steps of 2^-38 of it); fp32 ``q`` and the weights
     enter as two terms each (2^-22).  A weight enters times its token's V scale, in steps of 2^-33 of the largest such product: beside
-    a token whose V scale is 2^33 times theirs, others vanish even from the columns in which that token's codes are 0.
+    a token whose V scale is 2^33 times theirs, others vanish even from the columns in which that token's codes are 0.  Weights below
+    2^-122 of the largest are 0, whatever their V scale.
     A NaN code or scale of a token that counts gives NaN.
     """
     got = (_native_module or _native()).attend(q, k_pages, v_pages, seqs.cu_seqlens, seqs.block_tables, seqs.table_lens,
