@@ -110,7 +110,7 @@ __device__ __forceinline__ bool turns(const Store &s, int pos) { return pos >= 0
 // has two of them (or one, with itself), puts the blocks of the first one's runs into a table in shared memory and looks up the
 // second one's: every pair of runs is some watcher's.  us without / with them: 16384 rows of 32 + 8 + 8 heads x 128 92.4 / 93.1, of one
 // KV head x 64 11.4 / 11.9 (32 with four watchers, each for a quarter of the blocks and all rows), 4096 single rows 28.5 / 29.2, 73000 rows
-// of 8 x 128 patched 75.2 / 75.5; 16 segments cost another 1 us, eight 0.5 to 1.
+// of 8 x 128 patched 75.2 / 75.5; 100000 rows of 4 + 1 + 1 x 128, 25 segments, 103 / 113.  16 segments instead of eight cost another 1 us.
 constexpr int kMostPlaces = 8192;
 constexpr int kQueue = 64;  // blocks of a warp that wait to be looked up, 32 at once
 struct Watch {
